@@ -27,6 +27,10 @@
  *                                                              src/t5_encoder.cpp:68-73
  *   tsk_t5_*            <- ts_t5::load / encode                src/t5_encoder.cpp:28-104
  *   tsk_vae_*           <- ts_vae::load / decode               src/vae_decoder.cpp:7-124
+ *   tsk_block_norm      <- the adaLN glue of a block: x + gate * y, ggml_norm,
+ *                          x * (1 + scale) + shift             src/mmdit.cpp:55-59, :231-234
+ *   tsk_mxfp4_*         4-bit block-scaled (MXFP4) tensors, no counterpart in
+ *                       the reference's files
  *
  * Conventions (all follow ggml):
  *   - tensors are non-owning views: ne[] = extents with ne[0] fastest,
@@ -64,10 +68,17 @@ enum tsk_type {
     TSK_TYPE_Q8_0 = 8,   /* blocks of {fp16 d; int8 qs[32]} (34 bytes) along ne[0] */
     TSK_TYPE_I32  = 26,
     TSK_TYPE_BF16 = 30,
+    TSK_TYPE_MXFP4 = 39, /* blocks of {uint8 e; uint8 qs[16]} (17 bytes) along ne[0]: 32 E2M1 codes, value
+                          * i < 16 in qs[i]'s low nibble, i >= 16 in qs[i - 16]'s high one, times 2^(e - 127) */
     /* Extension (no ggml counterpart): Q8_0 weights repacked once for the GPU
      * by tsk_q8_0_repack. Same values as TSK_TYPE_Q8_0, split into two planes:
      * int8 qs[ne1][ne0] followed by fp16 d[ne1][ne0/32]; nb[] are ignored. */
-    TSK_TYPE_Q8_0_SPLIT = 0x1008
+    TSK_TYPE_Q8_0_SPLIT = 0x1008,
+    /* Extension: MXFP4 tensors as the GPU reads them, two planes over the rows
+     * r = (i3 * ne2 + i2) * ne1 + i1: codes uint8 [rows][ne0 / 2] (value 2 i in
+     * byte i's low nibble, 2 i + 1 in the high one) followed by scale bytes
+     * uint8 [rows][ne0 / 32]; nb[] are ignored. data is 16-byte aligned. */
+    TSK_TYPE_MXFP4_SPLIT = 0x1027
 };
 
 /* ggml_prec values (ggml_flash_attn_ext_set_prec). */
@@ -138,15 +149,24 @@ const char *tsk_version(void);
 
 /*
  * dst = a x b (+ bias), ggml_mul_mat semantics.
- *   a    : weight, ne = [K, M, 1, 1]; F32, F16, BF16, Q8_0 or Q8_0_SPLIT.
- *          Rows must be contiguous (nb[0] = element/block size).
+ *   a    : weight, ne = [K, M, 1, 1]; F32, F16, BF16, Q8_0, Q8_0_SPLIT, MXFP4
+ *          or MXFP4_SPLIT. Rows must be contiguous (nb[0] = element/block size).
  *   b    : activations, ne = [K, N, n2, n3]; F32 (or BF16), rows contiguous.
  *          As in ggml, b is first converted to a's vec_dot type: BF16 weights
  *          round b to bf16 (RNE); Q8_0 weights quantize b per 32-block to Q8_0
  *          (amax/127 scale, round-to-nearest-even); F16 weights round to fp16.
+ *          MXFP4 weights multiply F32 / BF16 b as BF16 weights do (b rounded to
+ *          bf16, the weights' values exact in bf16; ggml's own MXFP4 product
+ *          would round b to Q8_0, which is coarser), or b of type MXFP4_SPLIT
+ *          (ne = [K, N, n2, n3], tsk_mxfp4_quantize): both operands in 4 bits on
+ *          the block-scaled matrix instructions.
  *   bias : nullable, F32 ne = [M]; fused ggml_add broadcast over N.
  *   dst  : F32 (or BF16), ne = [M, N, n2, n3]; rows contiguous.
- * K must be a multiple of 32 for Q8_0 (ggml block) and of 8 otherwise.
+ * K must be a multiple of 32 for Q8_0 and MXFP4 (their block) and of 8 otherwise.
+ * MXFP4: products are exact and summed in fp32 (sums below fp32's normal range
+ * may be flushed to zero); a scale byte of 255 makes its block 32 NaNs; M, N and
+ * K of any size up to 2^31 - 1. MXFP4 blocks are repacked into scratch on every
+ * call, MXFP4_SPLIT weights are read in place.
  */
 int tsk_mul_mat(const tsk_tensor *a, const tsk_tensor *b, const tsk_tensor *bias,
                 tsk_tensor *dst, tsk_stream stream);
@@ -256,6 +276,68 @@ int tsk_q8_0_dequantize(const tsk_tensor *x, tsk_tensor *dst, tsk_stream stream)
 int tsk_q8_0_repack(const tsk_tensor *src, tsk_tensor *dst, tsk_stream stream);
 /* Bytes a Q8_0_SPLIT tensor of ne = [K, M] occupies. */
 size_t tsk_q8_0_split_nbytes(int64_t K, int64_t M);
+
+/* ---- MXFP4: 4-bit floating point with a power-of-two scale per 32 values ----
+ * (the OCP Microscaling Formats specification v1.0: E2M1 elements, E8M0 scales). */
+
+/*
+ * Quantize rows to MXFP4: x F32 or BF16, ne0 % 32 == 0, rows contiguous and
+ * aligned to their element; dst MXFP4 (nb[0] = 17, rows uniformly strided) or
+ * MXFP4_SPLIT of the same shape. Per block of 32 along ne[0]: amax = max |x|,
+ * e = max(floor(log2 amax) - 2, -127) (-127 for a block of zeros), scale byte
+ * e + 127; every element is x / 2^e rounded to the nearest of 0, 0.5, 1, 1.5, 2,
+ * 3, 4, 6 (ties to the even code; |x| / 2^e up to 8 saturates at 6), its sign
+ * kept, zeros included. A block that holds an infinity or a NaN gets scale byte
+ * 255 and codes 0: 32 NaNs. x and dst must not overlap.
+ */
+int tsk_mxfp4_quantize(const tsk_tensor *x, tsk_tensor *dst, tsk_stream stream);
+/* The values of an MXFP4 or MXFP4_SPLIT tensor as F32 or BF16 rows (exact; past
+ * the largest finite value, 2^128 up, infinite). */
+int tsk_mxfp4_dequantize(const tsk_tensor *x, tsk_tensor *dst, tsk_stream stream);
+/* Repack MXFP4 blocks (2-D, rows at least ne0 / 32 * 17 bytes apart) into the
+ * MXFP4_SPLIT planes (value-preserving). */
+int tsk_mxfp4_repack(const tsk_tensor *src, tsk_tensor *dst, tsk_stream stream);
+/* Bytes an MXFP4_SPLIT tensor of ne = [K, M] occupies (0 unless K % 32 == 0). */
+size_t tsk_mxfp4_split_nbytes(int64_t K, int64_t M);
+
+/* ---- norms before and after a block, its gate and residual ---------------- */
+
+enum tsk_norm_kind {
+    TSK_NORM_NONE  = 0,
+    TSK_NORM_LAYER = 1,    /* (x - mean) / sqrt(var + eps)  */
+    TSK_NORM_RMS   = 2     /* x / sqrt(mean(x^2) + eps)     */
+};
+typedef struct tsk_block_norm_params {
+    int   post_norm;             /* enum tsk_norm_kind: the norm of the branch y          */
+    float post_eps;
+    const tsk_tensor *post_w;    /* nullable, F32 [C]: weight of that norm                */
+    const tsk_tensor *gate;      /* nullable: factor of the branch, broadcast over x      */
+    float res_scale;             /* factor of x (1: the plain residual)                   */
+    int   pre_norm;              /* enum tsk_norm_kind: the norm before the next block    */
+    float pre_eps;
+    const tsk_tensor *pre_w;     /* nullable, F32 [C]: weight of that norm                */
+    const tsk_tensor *scale;     /* nullable: adaLN scale, broadcast over x               */
+    const tsk_tensor *shift;     /* nullable: adaLN shift, broadcast over x               */
+} tsk_block_norm_params;
+/*
+ * What stands between two blocks' matrices, in one pass over the rows:
+ *   r   = res_scale * x + gate * post(y)          post(y) = norm(y) * post_w
+ *   res = r in its type
+ *   dst = pre(res) * pre_w * (1 + scale) + shift
+ * per row of C = ne[0] values, statistics and arithmetic in fp32 (the second norm
+ * reads r as res holds it, or as x's type would where res is NULL).
+ *   x   : F32 or BF16, ne = [C, n1, n2, n3], rows contiguous
+ *   y   : nullable (no branch: r = res_scale * x; post_norm, post_w, gate unused
+ *         and required to be NONE / NULL); F32 or BF16 of x's shape
+ *   gate, scale, shift: F32, ne[0] = C, every other extent x's or 1; rows contiguous
+ *   res : nullable; x's type and shape. May be x itself (the same data and strides)
+ *   dst : nullable (the residual alone: pre_norm NONE, no pre_w / scale / shift);
+ *         F32, BF16, or MXFP4_SPLIT (C % 32 == 0: tsk_mxfp4_quantize's rounding of
+ *         the row, the operand of an MXFP4 product). At least one of res and dst.
+ * Outputs must not overlap each other or any input, but for res in place of x.
+ */
+int tsk_block_norm(const tsk_tensor *x, const tsk_tensor *y, const tsk_block_norm_params *p,
+                   tsk_tensor *res, tsk_tensor *dst, tsk_stream stream);
 
 /* ---- convolution and SwiGLU glue (src/mmdit.cpp:20-52) -------------------
  * The reference graph's latent / clip streams run kernel-3 convolutions

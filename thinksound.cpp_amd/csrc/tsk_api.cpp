@@ -261,6 +261,69 @@ bool rows_uniform(const tsk_tensor *t) {
            (t->ne[3] == 1 || t->nb[3] == t->nb[2] * (size_t) t->ne[2]);
 }
 
+// ---- MXFP4 tensors
+constexpr int64_t MX_MAX_EXTENT = 0x7fffffff - 63;      // (tiles past the end stay in int)
+
+// rows of ne1 x ne2 x ne3 within MX_MAX_EXTENT (the extents are >= 1)
+bool rows_fit(const tsk_tensor *t) {
+    int64_t n = 1;
+    for (int i = 1; i < 4; ++i) {
+        if (t->ne[i] > MX_MAX_EXTENT / n) return false;
+        n *= t->ne[i];
+    }
+    return true;
+}
+int64_t row_count(const tsk_tensor *t) { return t->ne[1] * t->ne[2] * t->ne[3]; }
+
+// MXFP4 blocks: 17 bytes each, whole rows that do not overlap
+int check_mx_blocks(const tsk_tensor *t, const char *name) {
+    if (t->nb[0] != 17) return fail(TSK_ERR_STRIDE, "%s: MXFP4 nb[0] must be 17 (block size)", name);
+    if (t->ne[1] > 1 && t->nb[1] < (size_t) (t->ne[0] / 32) * 17) return fail(TSK_ERR_STRIDE, "%s: MXFP4 rows overlap", name);
+    if (!rows_uniform(t)) return fail(TSK_ERR_STRIDE, "%s: MXFP4 rows must be uniformly strided", name);
+    return TSK_OK;
+}
+// either MXFP4 layout, of rows of ne0 % 32 == 0
+int check_mx(const tsk_tensor *t, const char *name) {
+    if (t->type != TSK_TYPE_MXFP4 && t->type != TSK_TYPE_MXFP4_SPLIT)
+        return fail(TSK_ERR_TYPE, "%s must be MXFP4 or MXFP4_SPLIT", name);
+    if (t->ne[0] % 32) return fail(TSK_ERR_SHAPE, "%s: ne0 %% 32 != 0", name);
+    if (t->ne[0] > MX_MAX_EXTENT || !rows_fit(t)) return fail(TSK_ERR_SHAPE, "%s is too large", name);
+    if (t->type == TSK_TYPE_MXFP4) return check_mx_blocks(t, name);
+    if (!aligned(t->data, 16)) return fail(TSK_ERR_ALIGN, "%s: MXFP4_SPLIT data must be 16-byte aligned", name);
+    return TSK_OK;
+}
+uint8_t *mx_codes(const tsk_tensor *t) { return (uint8_t *) t->data; }
+uint8_t *mx_scales(const tsk_tensor *t) { return (uint8_t *) t->data + (size_t) row_count(t) * (size_t) (t->ne[0] / 2); }
+
+// bytes of a row, and from the first byte of a tensor to past its last
+size_t row_bytes(const tsk_tensor *t) {
+    const size_t n = (size_t) t->ne[0];
+    return t->type == TSK_TYPE_MXFP4 ? n / 32 * 17 : n * (size_t) elt_size(t->type);
+}
+size_t span_bytes(const tsk_tensor *t) {
+    if (t->type == TSK_TYPE_MXFP4_SPLIT) return (size_t) row_count(t) * (size_t) (t->ne[0] / 32 * 17);
+    size_t n = row_bytes(t);
+    for (int i = 1; i < 4; ++i) n += (size_t) (t->ne[i] - 1) * t->nb[i];
+    return n;
+}
+// whether two tensors may share bytes: their spans meet, and they are not
+// columns of one array of rows (every stride a multiple of one row's) side by side
+bool may_overlap(const tsk_tensor *a, const tsk_tensor *b) {
+    const uintptr_t pa = (uintptr_t) a->data, pb = (uintptr_t) b->data;
+    if (pa + span_bytes(a) <= pb || pb + span_bytes(b) <= pa) return false;
+    if (a->type == TSK_TYPE_MXFP4_SPLIT || b->type == TSK_TYPE_MXFP4_SPLIT) return true;
+    size_t ld = 0;
+    for (const tsk_tensor *t : {a, b})
+        for (int i = 1; i < 4; ++i)
+            if (t->ne[i] > 1 && (!ld || t->nb[i] < ld)) ld = t->nb[i];
+    if (!ld) return true;
+    for (const tsk_tensor *t : {a, b})
+        for (int i = 1; i < 4; ++i)
+            if (t->ne[i] > 1 && t->nb[i] % ld) return true;
+    const size_t d = pb >= pa ? (size_t) (pb - pa) % ld : (ld - (size_t) (pa - pb) % ld) % ld;   // b's column from a's
+    return d < row_bytes(a) || d + row_bytes(b) > ld;
+}
+
 }  // namespace
 
 // ------------------------------------------------------------------ library
@@ -370,9 +433,12 @@ int validate_mul_mat(const tsk_tensor *a, const tsk_tensor *b, const tsk_tensor 
     if (b->ne[0] != K) return fail(TSK_ERR_SHAPE, "b->ne[0]=%lld != K=%lld", (long long) b->ne[0], (long long) K);
     if (dst->ne[0] != M || dst->ne[1] != b->ne[1] || dst->ne[2] != b->ne[2] || dst->ne[3] != b->ne[3])
         return fail(TSK_ERR_SHAPE, "dst must be [M=%lld, %lld, %lld, %lld]", (long long) M, (long long) b->ne[1], (long long) b->ne[2], (long long) b->ne[3]);
-    if (b->type != TSK_TYPE_F32 && b->type != TSK_TYPE_BF16) return fail(TSK_ERR_TYPE, "b must be F32 or BF16");
+    const bool mx = a->type == TSK_TYPE_MXFP4 || a->type == TSK_TYPE_MXFP4_SPLIT, mx_b = mx && b->type == TSK_TYPE_MXFP4_SPLIT;
+    if (b->type != TSK_TYPE_F32 && b->type != TSK_TYPE_BF16 && !mx_b)
+        return fail(TSK_ERR_TYPE, mx ? "b must be F32, BF16 or MXFP4_SPLIT" : "b must be F32 or BF16");
     if (dst->type != TSK_TYPE_F32 && dst->type != TSK_TYPE_BF16) return fail(TSK_ERR_TYPE, "dst must be F32 or BF16");
-    if ((rc = check_rows(b, "b", 16)) || (rc = check_rows(dst, "dst", 16))) return rc;
+    if (mx_b && !aligned(b->data, 16)) return fail(TSK_ERR_ALIGN, "MXFP4_SPLIT b must be 16-byte aligned");
+    if ((!mx_b && (rc = check_rows(b, "b", 16))) || (rc = check_rows(dst, "dst", 16))) return rc;
     if (bias) {
         if (bias->type != TSK_TYPE_F32 || bias->ne[0] != M || bias->ne[1] * bias->ne[2] * bias->ne[3] != 1)
             return fail(TSK_ERR_SHAPE, "bias must be F32 [M]");
@@ -392,6 +458,14 @@ int validate_mul_mat(const tsk_tensor *a, const tsk_tensor *b, const tsk_tensor 
         case TSK_TYPE_Q8_0_SPLIT:
             if (K % 32) return fail(TSK_ERR_SHAPE, "K=%lld must be a multiple of 32 for Q8_0", (long long) K);
             if (!aligned(a->data, 16)) return fail(TSK_ERR_ALIGN, "Q8_0_SPLIT data must be 16-byte aligned");
+            break;
+        case TSK_TYPE_MXFP4:
+        case TSK_TYPE_MXFP4_SPLIT:
+            if (K % 32) return fail(TSK_ERR_SHAPE, "K=%lld must be a multiple of 32 for MXFP4", (long long) K);
+            if (K > MX_MAX_EXTENT || M > MX_MAX_EXTENT) return fail(TSK_ERR_SHAPE, "MXFP4 weights of [%lld, %lld]", (long long) K, (long long) M);
+            if (!rows_fit(b)) return fail(TSK_ERR_SHAPE, "b has too many rows");
+            if (a->type == TSK_TYPE_MXFP4) return check_mx_blocks(a, "a");
+            if (!aligned(a->data, 16)) return fail(TSK_ERR_ALIGN, "MXFP4_SPLIT data must be 16-byte aligned");
             break;
         case TSK_TYPE_F32:
             // vec_dot type F32: the activations stay fp32
@@ -495,6 +569,7 @@ struct MulMatPlan {
     int splits;
     size_t wbytes;       // Q8_0: the weights repacked into planes
     size_t act_bytes;    // Q8_0 / Q8_0_SPLIT: the quantized activation planes
+    bool mx;             // MXFP4 weights
     size_t bytes;        // scratch the call needs
 };
 
@@ -503,9 +578,14 @@ MulMatPlan plan_mul_mat(const tsk_tensor *a, const tsk_tensor *b, const tsk_tens
     memset(&pl, 0, sizeof(pl));
     const int64_t K = a->ne[0], M = a->ne[1];
     // slices of uniformly strided rows: one launch per (i2, i3) unless rows are uniform
-    pl.uni = rows_uniform(b) && rows_uniform(dst);
+    pl.uni = (b->type == TSK_TYPE_MXFP4_SPLIT || rows_uniform(b)) && rows_uniform(dst);
     pl.nslices = pl.uni ? 1 : b->ne[2] * b->ne[3];
     pl.Nslice = pl.uni ? b->ne[1] * b->ne[2] * b->ne[3] : b->ne[1];
+    if (a->type == TSK_TYPE_MXFP4 || a->type == TSK_TYPE_MXFP4_SPLIT) {
+        pl.mx = true;
+        pl.bytes = pl.wbytes = a->type == TSK_TYPE_MXFP4 ? align256(tsk_mxfp4_split_nbytes(K, M)) : 0;
+        return pl;
+    }
     // Few rows. From 5 rows on every wave's own conversion of the activations
     // costs as much as a launch of it where there are many waves (8 rows, tiles
     // against rows: BF16 M = 1024 10.1 / 5.5 us, M = 6144 9.6 / 9.8; Q8_0 M =
@@ -526,12 +606,52 @@ MulMatPlan plan_mul_mat(const tsk_tensor *a, const tsk_tensor *b, const tsk_tens
     return pl;
 }
 
+// MXFP4 weights (gemm_mx.hip); blocks are repacked into the scratch first
+int mul_mat_mx(const tsk_tensor *a, const tsk_tensor *b, const tsk_tensor *bias, tsk_tensor *dst, const MulMatPlan &pl,
+               const Scratch &scr) {
+    const int64_t K = a->ne[0], M = a->ne[1];
+    MxGemm p;
+    memset(&p, 0, sizeof(p));
+    p.wq = mx_codes(a);
+    hipError_t e;
+    if (a->type == TSK_TYPE_MXFP4) {
+        int rc;
+        void *ws = nullptr;
+        if ((rc = scr.get(pl.bytes, &ws))) return rc;
+        e = launch_mx_repack((const uint8_t *) a->data, (int64_t) a->nb[1], M, K, (uint8_t *) ws,
+                             (uint8_t *) ws + (size_t) M * (size_t) (K / 2), scr.s);
+        if (e != hipSuccess) return hip_fail(e, "mxfp4 repack");
+        p.wq = (const uint8_t *) ws;
+    }
+    p.ws = p.wq + (size_t) M * (size_t) (K / 2);
+    p.bias = bias ? (const float *) bias->data : nullptr;
+    p.y_bf16 = dst->type == TSK_TYPE_BF16;
+    p.x_f32 = b->type == TSK_TYPE_F32;
+    p.M = (int) M; p.N = (int) pl.Nslice; p.K = (int) K;
+    const bool mx_b = b->type == TSK_TYPE_MXFP4_SPLIT;
+    p.ld_x = mx_b ? 0 : (int64_t) b->nb[1] / elt_size(b->type);
+    p.ld_y = (int64_t) dst->nb[1] / elt_size(dst->type);
+    for (int64_t sl = 0; sl < pl.nslices; ++sl) {
+        const int64_t i2 = sl % b->ne[2], i3 = sl / b->ne[2];
+        p.y = (char *) dst->data + i2 * dst->nb[2] + i3 * dst->nb[3];
+        if (mx_b) {
+            p.xq = mx_codes(b) + sl * pl.Nslice * (K / 2);
+            p.xs = mx_scales(b) + sl * pl.Nslice * (K / 32);
+        } else {
+            p.x = (const char *) b->data + i2 * b->nb[2] + i3 * b->nb[3];
+        }
+        if ((e = launch_gemm_mx(p, scr.s)) != hipSuccess) return hip_fail(e, "mul_mat launch");
+    }
+    return TSK_OK;
+}
+
 int mul_mat_impl(const tsk_tensor *a, const tsk_tensor *b, const tsk_tensor *bias, tsk_tensor *dst,
                  const Scratch &scr) {
     hipStream_t s = scr.s;
     const int64_t K = a->ne[0], M = a->ne[1];
-    const int es_b = elt_size(b->type), es_d = elt_size(dst->type);
     const MulMatPlan pl = plan_mul_mat(a, b, dst);
+    if (pl.mx) return mul_mat_mx(a, b, bias, dst, pl, scr);
+    const int es_b = elt_size(b->type), es_d = elt_size(dst->type);
     int rc;
     char *ws = nullptr;
     if (pl.gemv) {
@@ -1052,6 +1172,171 @@ extern "C" int tsk_q8_0_repack(const tsk_tensor *src, tsk_tensor *dst, tsk_strea
     if ((rc = require_init())) return rc;
     hipError_t e = launch_q8_repack(src->data, (int64_t) src->nb[1], src->ne[1], src->ne[0], dst->data, (hipStream_t) stream);
     return e == hipSuccess ? TSK_OK : hip_fail(e, "q8 repack launch");
+}
+
+// ------------------------------------------------------------------ MXFP4
+extern "C" size_t tsk_mxfp4_split_nbytes(int64_t K, int64_t M) {
+    if (K <= 0 || M <= 0 || K % 32) return 0;
+    return (size_t) M * (size_t) (K / 32) * 17;
+}
+
+extern "C" int tsk_mxfp4_quantize(const tsk_tensor *x, tsk_tensor *dst, tsk_stream stream) {
+    int rc;
+    if ((rc = check_tensor(x, "x")) || (rc = check_tensor(dst, "dst"))) return rc;
+    if (x->type != TSK_TYPE_F32 && x->type != TSK_TYPE_BF16) return fail(TSK_ERR_TYPE, "x must be F32 or BF16");
+    if ((rc = check_mx(dst, "dst"))) return rc;
+    if (!same_shape(x, dst)) return fail(TSK_ERR_SHAPE, "shapes differ");
+    if ((rc = check_rows(x, "x", elt_size(x->type)))) return rc;
+    if (may_overlap(x, dst)) return fail(TSK_ERR_INVALID_ARG, "x and dst overlap");
+    if ((rc = require_init())) return rc;
+    const bool split = dst->type == TSK_TYPE_MXFP4_SPLIT;
+    hipError_t e = launch_mx_quantize(view(x), split ? mx_codes(dst) : nullptr, split ? mx_scales(dst) : nullptr,
+                                      split ? nullptr : (uint8_t *) dst->data, (int64_t) dst->nb[1], (hipStream_t) stream);
+    return e == hipSuccess ? TSK_OK : hip_fail(e, "mxfp4 quantize launch");
+}
+
+extern "C" int tsk_mxfp4_dequantize(const tsk_tensor *x, tsk_tensor *dst, tsk_stream stream) {
+    int rc;
+    if ((rc = check_tensor(x, "x")) || (rc = check_tensor(dst, "dst"))) return rc;
+    if ((rc = check_mx(x, "x"))) return rc;
+    if (dst->type != TSK_TYPE_F32 && dst->type != TSK_TYPE_BF16) return fail(TSK_ERR_TYPE, "dst must be F32 or BF16");
+    if (!same_shape(x, dst)) return fail(TSK_ERR_SHAPE, "shapes differ");
+    if ((rc = check_rows(dst, "dst", elt_size(dst->type)))) return rc;
+    if (may_overlap(x, dst)) return fail(TSK_ERR_INVALID_ARG, "x and dst overlap");
+    if ((rc = require_init())) return rc;
+    const bool split = x->type == TSK_TYPE_MXFP4_SPLIT;
+    hipError_t e = launch_mx_dequantize(split ? mx_codes(x) : nullptr, split ? mx_scales(x) : nullptr,
+                                        split ? nullptr : (const uint8_t *) x->data, (int64_t) x->nb[1], view(dst),
+                                        (hipStream_t) stream);
+    return e == hipSuccess ? TSK_OK : hip_fail(e, "mxfp4 dequantize launch");
+}
+
+extern "C" int tsk_mxfp4_repack(const tsk_tensor *src, tsk_tensor *dst, tsk_stream stream) {
+    int rc;
+    if ((rc = check_tensor(src, "src")) || (rc = check_tensor(dst, "dst"))) return rc;
+    if (src->type != TSK_TYPE_MXFP4 || dst->type != TSK_TYPE_MXFP4_SPLIT) return fail(TSK_ERR_TYPE, "MXFP4 -> MXFP4_SPLIT");
+    if (!same_shape(src, dst) || src->ne[2] * src->ne[3] != 1) return fail(TSK_ERR_SHAPE, "2-D MXFP4 of equal shape");
+    if ((rc = check_mx(src, "src")) || (rc = check_mx(dst, "dst"))) return rc;
+    if (may_overlap(src, dst)) return fail(TSK_ERR_INVALID_ARG, "src and dst overlap");
+    if ((rc = require_init())) return rc;
+    hipError_t e = launch_mx_repack((const uint8_t *) src->data, (int64_t) src->nb[1], src->ne[1], src->ne[0], mx_codes(dst),
+                                    mx_scales(dst), (hipStream_t) stream);
+    return e == hipSuccess ? TSK_OK : hip_fail(e, "mxfp4 repack launch");
+}
+
+// ------------------------------------------------------------------ block norm
+namespace {
+
+bool norm_kind(int k) { return k == TSK_NORM_NONE || k == TSK_NORM_LAYER || k == TSK_NORM_RMS; }
+
+// a row operand of x's shape, F32 or BF16, aligned to its elements
+int check_bn_rows(const tsk_tensor *t, const char *name, const tsk_tensor *x) {
+    int rc;
+    if ((rc = check_tensor(t, name))) return rc;
+    if (t->type != TSK_TYPE_F32 && t->type != TSK_TYPE_BF16) return fail(TSK_ERR_TYPE, "%s must be F32 or BF16", name);
+    if (!same_shape(t, x)) return fail(TSK_ERR_SHAPE, "%s must have x's shape", name);
+    return check_rows(t, name, elt_size(t->type));
+}
+// a nullable F32 factor, its extents x's or 1
+int check_bn_factor(const tsk_tensor *t, const char *name, const tsk_tensor *x) {
+    int rc;
+    if (!t) return TSK_OK;
+    if ((rc = check_tensor(t, name))) return rc;
+    if (t->type != TSK_TYPE_F32) return fail(TSK_ERR_TYPE, "%s must be F32", name);
+    if (t->ne[0] != x->ne[0]) return fail(TSK_ERR_SHAPE, "%s->ne[0] must be C", name);
+    for (int i = 1; i < 4; ++i)
+        if (t->ne[i] != 1 && t->ne[i] != x->ne[i]) return fail(TSK_ERR_SHAPE, "%s->ne[%d] must be 1 or x's", name, i);
+    return check_rows(t, name, 4);
+}
+
+int validate_block_norm(const tsk_tensor *x, const tsk_tensor *y, const tsk_block_norm_params *p, const tsk_tensor *res,
+                        const tsk_tensor *dst) {
+    int rc;
+    if (!p) return fail(TSK_ERR_INVALID_ARG, "params is NULL");
+    if ((rc = check_tensor(x, "x")) || (rc = check_bn_rows(x, "x", x))) return rc;
+    if (x->ne[0] > MX_MAX_EXTENT || !rows_fit(x)) return fail(TSK_ERR_SHAPE, "x is too large");
+    if (!norm_kind(p->post_norm) || !norm_kind(p->pre_norm)) return fail(TSK_ERR_INVALID_ARG, "norm kind");
+    if (y && (rc = check_bn_rows(y, "y", x))) return rc;
+    if (!y && (p->post_norm != TSK_NORM_NONE || p->post_w || p->gate))
+        return fail(TSK_ERR_INVALID_ARG, "post_norm, post_w and gate need y");
+    if (!res && !dst) return fail(TSK_ERR_INVALID_ARG, "res and dst are both NULL");
+    if (!dst && (p->pre_norm != TSK_NORM_NONE || p->pre_w || p->scale || p->shift))
+        return fail(TSK_ERR_INVALID_ARG, "pre_norm, pre_w, scale and shift need dst");
+    if (!(p->post_eps >= 0.0f) || !(p->pre_eps >= 0.0f)) return fail(TSK_ERR_INVALID_ARG, "eps");
+    if (p->res_scale != p->res_scale) return fail(TSK_ERR_INVALID_ARG, "res_scale");
+    for (const tsk_tensor *w : {p->post_w, p->pre_w})
+        if (w && ((rc = check_w(w, x->ne[0])) || (rc = check_rows(w, "w", 4)))) return rc;
+    if ((rc = check_bn_factor(p->gate, "gate", x)) || (rc = check_bn_factor(p->scale, "scale", x)) ||
+        (rc = check_bn_factor(p->shift, "shift", x)))
+        return rc;
+    if (res) {
+        if ((rc = check_bn_rows(res, "res", x))) return rc;
+        if (res->type != x->type) return fail(TSK_ERR_TYPE, "res must have x's type");
+    }
+    if (dst) {
+        if (dst->type == TSK_TYPE_MXFP4_SPLIT) {
+            if ((rc = check_tensor(dst, "dst")) || (rc = check_mx(dst, "dst"))) return rc;
+            if (!same_shape(dst, x)) return fail(TSK_ERR_SHAPE, "dst must have x's shape");
+        } else if ((rc = check_bn_rows(dst, "dst", x))) {
+            return rc;
+        }
+    }
+    return TSK_OK;
+}
+
+// outputs that share bytes with an input or with each other (but res in place of x)
+int check_bn_overlap(const tsk_tensor *x, const tsk_tensor *y, const tsk_block_norm_params *p, const tsk_tensor *res,
+                     const tsk_tensor *dst) {
+    bool in_place = res && res->data == x->data;
+    for (int i = 1; in_place && i < 4; ++i) in_place = x->ne[i] == 1 || res->nb[i] == x->nb[i];
+    for (const tsk_tensor *o : {res, dst}) {
+        if (!o) continue;
+        for (const tsk_tensor *t : {x, y, p->post_w, p->gate, p->pre_w, p->scale, p->shift})
+            if (t && !(o == res && t == x && in_place) && may_overlap(o, t))
+                return fail(TSK_ERR_INVALID_ARG, "an output overlaps an input");
+    }
+    if (res && dst && may_overlap(res, dst)) return fail(TSK_ERR_INVALID_ARG, "res and dst overlap");
+    return TSK_OK;
+}
+
+// t's rows for x's indices (extents of 1 broadcast)
+BnView bn_view(const tsk_tensor *t) {
+    BnView v = {nullptr, 0, 0, 0};
+    if (!t) return v;
+    v.data = t->data;
+    v.nb1 = t->ne[1] > 1 ? (int64_t) t->nb[1] : 0;
+    v.nb2 = t->ne[2] > 1 ? (int64_t) t->nb[2] : 0;
+    v.nb3 = t->ne[3] > 1 ? (int64_t) t->nb[3] : 0;
+    return v;
+}
+
+}  // namespace
+
+extern "C" int tsk_block_norm(const tsk_tensor *x, const tsk_tensor *y, const tsk_block_norm_params *p, tsk_tensor *res,
+                              tsk_tensor *dst, tsk_stream stream) {
+    int rc;
+    if ((rc = validate_block_norm(x, y, p, res, dst)) || (rc = check_bn_overlap(x, y, p, res, dst))) return rc;
+    if ((rc = require_init())) return rc;
+    BlockNorm b;
+    memset(&b, 0, sizeof(b));
+    b.x = bn_view(x); b.y = bn_view(y); b.gate = bn_view(p->gate); b.scale = bn_view(p->scale); b.shift = bn_view(p->shift);
+    b.res = bn_view(res);
+    if (dst && dst->type == TSK_TYPE_MXFP4_SPLIT) {
+        b.codes = mx_codes(dst);
+        b.scales = mx_scales(dst);
+    } else {
+        b.dst = bn_view(dst);
+    }
+    b.x_bf16 = x->type == TSK_TYPE_BF16;
+    b.y_bf16 = y && y->type == TSK_TYPE_BF16;
+    b.dst_bf16 = dst && dst->type == TSK_TYPE_BF16;
+    b.post_w = p->post_w ? (const float *) p->post_w->data : nullptr;
+    b.pre_w = p->pre_w ? (const float *) p->pre_w->data : nullptr;
+    b.post_norm = p->post_norm; b.pre_norm = p->pre_norm;
+    b.post_eps = p->post_eps; b.pre_eps = p->pre_eps; b.res_scale = p->res_scale;
+    b.C = (int) x->ne[0]; b.n1 = (int) x->ne[1]; b.n2 = (int) x->ne[2]; b.n3 = (int) x->ne[3];
+    hipError_t e = launch_block_norm(b, (hipStream_t) stream);
+    return e == hipSuccess ? TSK_OK : hip_fail(e, "block_norm launch");
 }
 
 // ------------------------------------------------------------------ convolution / SwiGLU

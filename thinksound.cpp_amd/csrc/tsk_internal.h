@@ -348,6 +348,50 @@ hipError_t launch_q8_repack(const void *src, int64_t ld_src, int64_t rows, int64
                             void *dst, hipStream_t s);
 hipError_t launch_f32_to_bf16(const float *x, uint16_t *y, int64_t n, hipStream_t s);
 
+// ---------------------------------------------------------------- MXFP4
+// rows of x (f32 / bf16) -> planes (codes [rows][K / 2], scales [rows][K / 32]),
+// or blocks of 17 bytes (non-null; rows ld_blocks bytes apart); K % 32 == 0
+hipError_t launch_mx_quantize(const View4 &x, uint8_t *codes, uint8_t *scales, uint8_t *blocks, int64_t ld_blocks,
+                              hipStream_t s);
+// planes or blocks -> rows of y (f32 / bf16)
+hipError_t launch_mx_dequantize(const uint8_t *codes, const uint8_t *scales, const uint8_t *blocks, int64_t ld_blocks,
+                                const View4 &y, hipStream_t s);
+hipError_t launch_mx_repack(const uint8_t *blocks, int64_t ld_blocks, int64_t rows, int64_t K, uint8_t *codes,
+                            uint8_t *scales, hipStream_t s);
+// Y[n, m] = sum_k X[n, k] W[m, k] + bias[m] over MXFP4 planes W (gemm_mx.hip):
+// X bf16 / f32 rows (16-byte aligned, ld_x elements apart; f32 rounded to
+// bf16), or MXFP4 planes xq / xs; Y rows 16-byte aligned, K % 32 == 0
+struct MxGemm {
+    const uint8_t *wq, *ws;        // [M][K / 2], [M][K / 32]
+    const void *x;
+    int x_f32;
+    int64_t ld_x;
+    const uint8_t *xq, *xs;        // [N][K / 2], [N][K / 32]; null: x
+    const float *bias;             // [M], nullable, 16-byte aligned
+    void *y;
+    int y_bf16;
+    int64_t ld_y;
+    int M, N, K;
+};
+hipError_t launch_gemm_mx(const MxGemm &p, hipStream_t s);
+
+// ---------------------------------------------------------------- block norm
+// tsk_block_norm's operands; a stride of 0 broadcasts, data null: absent
+struct BnView {
+    const void *data;
+    int64_t nb1, nb2, nb3;
+};
+struct BlockNorm {
+    BnView x, y, gate, scale, shift, res, dst;
+    int x_bf16, y_bf16, dst_bf16;
+    const float *post_w, *pre_w;
+    uint8_t *codes, *scales;       // dst as MXFP4 planes (dst.data null)
+    int post_norm, pre_norm;       // tsk_norm_kind
+    float post_eps, pre_eps, res_scale;
+    int C, n1, n2, n3;
+};
+hipError_t launch_block_norm(const BlockNorm &p, hipStream_t s);
+
 // ---------------------------------------------------------------- DiT glue
 // Residual update + LayerNorm + modulate for up to two streams in one launch.
 // Row r of a stream (b = r / rows_per_b):

@@ -17,7 +17,8 @@ import numpy as np
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "lib", "libtsk.so")
 
-F32, F16, Q8_0, I32, BF16, Q8_0_SPLIT = 0, 1, 8, 26, 30, 0x1008
+F32, F16, Q8_0, I32, BF16, MXFP4, Q8_0_SPLIT, MXFP4_SPLIT = 0, 1, 8, 26, 30, 39, 0x1008, 0x1027
+NORM_NONE, NORM_LAYER, NORM_RMS = 0, 1, 2
 PREC_DEFAULT, PREC_F32 = 0, 10
 ROPE_NORMAL = 0
 OP_MUL_MAT, OP_FLASH_ATTN_EXT, OP_RMS_NORM_MUL, OP_ROPE_EXT, OP_NORM, OP_IM2COL, OP_CONV1D = 1, 2, 3, 4, 5, 6, 7
@@ -36,6 +37,13 @@ class TskError(RuntimeError):
 class TskTensor(ctypes.Structure):
     _fields_ = [("type", ctypes.c_int32), ("ne", ctypes.c_int64 * 4),
                 ("nb", ctypes.c_size_t * 4), ("data", ctypes.c_void_p)]
+
+
+class BlockNormParams(ctypes.Structure):
+    _fields_ = [("post_norm", ctypes.c_int), ("post_eps", ctypes.c_float), ("post_w", ctypes.POINTER(TskTensor)),
+                ("gate", ctypes.POINTER(TskTensor)), ("res_scale", ctypes.c_float), ("pre_norm", ctypes.c_int),
+                ("pre_eps", ctypes.c_float), ("pre_w", ctypes.POINTER(TskTensor)),
+                ("scale", ctypes.POINTER(TskTensor)), ("shift", ctypes.POINTER(TskTensor))]
 
 
 class T5Config(ctypes.Structure):
@@ -92,6 +100,10 @@ def load():
         "tsk_q8_0_quantize": ([P, P, vp], i), "tsk_q8_0_dequantize": ([P, P, vp], i),
         "tsk_q8_0_repack": ([P, P, vp], i),
         "tsk_q8_0_split_nbytes": ([ctypes.c_int64, ctypes.c_int64], ctypes.c_size_t),
+        "tsk_mxfp4_quantize": ([P, P, vp], i), "tsk_mxfp4_dequantize": ([P, P, vp], i),
+        "tsk_mxfp4_repack": ([P, P, vp], i),
+        "tsk_mxfp4_split_nbytes": ([ctypes.c_int64, ctypes.c_int64], ctypes.c_size_t),
+        "tsk_block_norm": ([P, P, ctypes.POINTER(BlockNormParams), P, P, vp], i),
         "tsk_supports_op": ([i, ctypes.POINTER(P), i, P], i),
         "tsk_workspace_size": ([i, ctypes.POINTER(P), i, P, ctypes.POINTER(ctypes.c_size_t)], i),
         "tsk_set_workspace": ([vp, vp, ctypes.c_size_t], i),
@@ -370,15 +382,15 @@ def bf16_to_device(bits):
 # ---------------------------------------------------------------- descriptors
 def desc(t, ttype=None):
     """tsk_tensor view of a DeviceArray: ne = reversed shape, nb = reversed byte strides.
-    A Q8_0 tensor is a u8 array of shape (rows, K/32, 34)."""
+    A Q8_0 tensor is a u8 array of shape (rows, K/32, 34), an MXFP4 one of (rows, K/32, 17)."""
     d = TskTensor()
     ttype = t.ttype if ttype is None else ttype
     d.type = ttype
-    if ttype == Q8_0:
+    if ttype in (Q8_0, MXFP4):
         rows, nblk = t.shape[0], t.shape[1]
         ne = [nblk * 32, rows]
-        nb = [34, t.stride(0)]
-    elif ttype == Q8_0_SPLIT:
+        nb = [34 if ttype == Q8_0 else 17, t.stride(0)]
+    elif ttype in (Q8_0_SPLIT, MXFP4_SPLIT):
         ne = list(t.logical_shape)
         nb = [1, ne[0]]
     else:
@@ -453,32 +465,29 @@ def _ref(x):
 
 
 # ---------------------------------------------------------------- operators
-def mul_mat(a, b, bias=None, out=None, a_type=None, out_dtype="f32", stream=None):
-    """ggml_mul_mat(a, b) (+bias): a (M, K) weights, b (..., N, K) -> (..., N, M)."""
+def _mul_mat(fn, a, b, bias, out, a_type, out_dtype, stream):
     init()
     at = a_type if a_type is not None else a.ttype
-    M = a.shape[0] if at != Q8_0_SPLIT else a.logical_shape[1]
+    M = a.logical_shape[1] if at in (Q8_0_SPLIT, MXFP4_SPLIT) else a.shape[0]
+    bt = MXFP4_SPLIT if isinstance(b, SplitMXFP4) else None
     if out is None:
-        out = DeviceArray(tuple(b.shape[:-1]) + (M,), out_dtype)
-    da, db, dd = desc(a, at), desc(b), desc(out)
+        rows = (b.logical_shape[1],) if bt else tuple(b.shape[:-1])
+        out = DeviceArray(rows + (M,), out_dtype)
+    da, db, dd = desc(a, at), desc(b, bt), desc(out)
     dbias = desc(bias) if bias is not None else None
-    check(load().tsk_mul_mat(ctypes.byref(da), ctypes.byref(db), _ref(dbias), ctypes.byref(dd),
-                             _stream(stream)))
+    check(getattr(load(), fn)(ctypes.byref(da), ctypes.byref(db), _ref(dbias), ctypes.byref(dd), _stream(stream)))
     return out
+
+
+def mul_mat(a, b, bias=None, out=None, a_type=None, out_dtype="f32", stream=None):
+    """ggml_mul_mat(a, b) (+bias): a (M, K) weights, b (..., N, K) -> (..., N, M).
+    MXFP4 weights: a u8 blocks with a_type=MXFP4 or a SplitMXFP4; b then also a SplitMXFP4 of N rows."""
+    return _mul_mat("tsk_mul_mat", a, b, bias, out, a_type, out_dtype, stream)
 
 
 def mul_mat_noalloc(a, b, bias=None, out=None, a_type=None, out_dtype="f32", stream=None):
     """mul_mat through tsk_mul_mat_noalloc (scratch in the library's fixed per-GPU array)."""
-    init()
-    at = a_type if a_type is not None else a.ttype
-    M = a.shape[0] if at != Q8_0_SPLIT else a.logical_shape[1]
-    if out is None:
-        out = DeviceArray(tuple(b.shape[:-1]) + (M,), out_dtype)
-    da, db, dd = desc(a, at), desc(b), desc(out)
-    dbias = desc(bias) if bias is not None else None
-    check(load().tsk_mul_mat_noalloc(ctypes.byref(da), ctypes.byref(db), _ref(dbias), ctypes.byref(dd),
-                                     _stream(stream)))
-    return out
+    return _mul_mat("tsk_mul_mat_noalloc", a, b, bias, out, a_type, out_dtype, stream)
 
 
 def flash_attn_ext(q, k, v, mask=None, scale=0.125, max_bias=0.0, softcap=0.0, prec=PREC_F32,
@@ -630,6 +639,81 @@ def q8_0_dequantize(x):
     dd = desc(out)
     check(load().tsk_q8_0_dequantize(ctypes.byref(dx), ctypes.byref(dd), _stream()))
     return out
+
+
+# ---------------------------------------------------------------- MXFP4
+class SplitMXFP4:
+    """A (rows, K) matrix in MXFP4 planes (TSK_TYPE_MXFP4_SPLIT): K / 2 code bytes a row, then K / 32 scale bytes a row."""
+    ttype = MXFP4_SPLIT
+
+    def __init__(self, buf, K, rows):
+        self.buf, self.logical_shape = buf, (K, rows)
+
+    def data_ptr(self):
+        return self.buf.data_ptr()
+
+
+def _split_mxfp4(K, rows):
+    return SplitMXFP4(DeviceArray((load().tsk_mxfp4_split_nbytes(K, rows),), "u8"), K, rows)
+
+
+def mxfp4_quantize(x, split=True, out=None, stream=None):
+    """(..., K) f32 / bf16 rows -> SplitMXFP4 of all rows, or (split=False) u8 blocks (rows, K/32, 17)."""
+    init()
+    K, rows = x.shape[-1], int(np.prod(x.shape[:-1]))
+    if out is None:
+        out = _split_mxfp4(K, rows) if split else DeviceArray((rows, K // 32, 17), "u8")
+    dx, dd = desc(x), desc(out, MXFP4_SPLIT if isinstance(out, SplitMXFP4) else MXFP4)
+    if isinstance(out, SplitMXFP4):                        # planes take x's extents
+        for k in range(1, 4):
+            dd.ne[k] = dx.ne[k]
+    elif len(x.shape) > 2:
+        raise ValueError("blocks are 2-D here")
+    check(load().tsk_mxfp4_quantize(ctypes.byref(dx), ctypes.byref(dd), _stream(stream)))
+    return out
+
+
+def mxfp4_dequantize(x, dtype="f32", out=None, stream=None):
+    """SplitMXFP4 or u8 blocks (rows, K/32, 17) -> (rows, K) f32 / bf16."""
+    init()
+    split = isinstance(x, SplitMXFP4)
+    dx = desc(x, MXFP4_SPLIT if split else MXFP4)
+    out = DeviceArray((dx.ne[1], dx.ne[0]), dtype) if out is None else out
+    dd = desc(out)
+    check(load().tsk_mxfp4_dequantize(ctypes.byref(dx), ctypes.byref(dd), _stream(stream)))
+    return out
+
+
+def mxfp4_repack(blocks, stream=None):
+    """u8 MXFP4 blocks (rows, K/32, 17) -> SplitMXFP4."""
+    init()
+    sp = _split_mxfp4(blocks.shape[1] * 32, blocks.shape[0])
+    ds, dd = desc(blocks, MXFP4), desc(sp, MXFP4_SPLIT)
+    check(load().tsk_mxfp4_repack(ctypes.byref(ds), ctypes.byref(dd), _stream(stream)))
+    return sp
+
+
+# ---------------------------------------------------------------- norms around a block
+def block_norm(x, y=None, gate=None, post=NORM_NONE, post_w=None, post_eps=1e-5, res_scale=1.0, pre=NORM_LAYER,
+               pre_w=None, pre_eps=1e-5, scale=None, shift=None, res=None, dst=None, stream=None):
+    """res = res_scale x + gate post(y), dst = pre(res) pre_w (1 + scale) + shift (tsk_block_norm):
+    x / y (..., C), gate / scale / shift (..., C) broadcast over x's rows; res None: not kept,
+    dst a DeviceArray or SplitMXFP4, None: the residual alone (pre=NORM_NONE). Returns (res, dst)."""
+    init()
+    ptr = lambda t: None if t is None else ctypes.pointer(desc(t))
+    p = BlockNormParams(post, post_eps, ptr(post_w), ptr(gate), res_scale, pre, pre_eps, ptr(pre_w), ptr(scale),
+                        ptr(shift))
+    dx = desc(x)
+    dd = None
+    if dst is not None:
+        split = isinstance(dst, SplitMXFP4)
+        dd = desc(dst, MXFP4_SPLIT if split else None)
+        if split:
+            for k in range(1, 4):
+                dd.ne[k] = dx.ne[k]
+    dy, dr = (desc(t) if t is not None else None for t in (y, res))
+    check(load().tsk_block_norm(ctypes.byref(dx), _ref(dy), ctypes.byref(p), _ref(dr), _ref(dd), _stream(stream)))
+    return res, dst
 
 
 # ---------------------------------------------------------------- convolution / SwiGLU
