@@ -24,6 +24,12 @@ __device__ __forceinline__ float mx_scale(uint32_t byte) {
     return __uint_as_float(byte ? byte << 23 : 0x00400000u);
 }
 
+// the largest of a group of four lanes (all of them active)
+__device__ __forceinline__ uint32_t mx_quad_max(uint32_t v) {
+    v = max(v, (uint32_t) __builtin_amdgcn_update_dpp(0, (int) v, 0xB1, 0xF, 0xF, false));   // quad [1, 0, 3, 2]
+    return max(v, (uint32_t) __builtin_amdgcn_update_dpp(0, (int) v, 0x4E, 0xF, 0xF, false));  // quad [2, 3, 0, 1]
+}
+
 // 8 values over `scale` -> 8 codes (v_cvt_scalef32_pk_fp4_f32: nearest, ties to
 // the even code, saturating at 6); values of a block whose byte is not 255
 __device__ __forceinline__ uint32_t mx_encode8(const float *v, float scale) {
