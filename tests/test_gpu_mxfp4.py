@@ -168,6 +168,43 @@ def test_products_equal_where_sums_are_exact(T, n, k, m, act):
     assert (got[:, m:] == 3.0).all()
 
 
+@pytest.fixture
+def shape(T, monkeypatch):
+    """force a launch shape of the products"""
+    def force(cfg):
+        monkeypatch.setenv("TSK_MX_CFG", str(cfg))
+        T.init(0, reread=True)
+    yield force
+    monkeypatch.delenv("TSK_MX_CFG")
+    T.init(0, reread=True)
+
+
+@pytest.mark.parametrize("cfg", [1, 2, 3, 4, 5, 11, 12, 13, 14])
+@pytest.mark.parametrize("act", ["mxfp4", "bf16", "f32"])
+def test_every_launch_shape(T, shape, cfg, act):
+    """ragged in rows, outputs and K (blocks of scales whole, by twos and odd; K shorter than a stage and longer than a
+    chunk of scales), equal to the exact sums; a NaN scale right behind the end of a row reaches only its own"""
+    shape(cfg)
+    rng = np.random.default_rng(cfg)
+    for n, k, m in ((300, 1152, 273), (257, 2176, 260), (131, 192, 130), (70, 1088, 515), (270, 160, 300), (33, 32, 65), (19, 96, 17),
+                    (140, 2592, 150)):
+        wc, wb, xc, xb = operands(rng, n, k, m, True)
+        wb[m // 2, 0] = 255
+        if act == "mxfp4":
+            xb[n // 2, 0] = 255
+            x, xd = mxref.values(xc, xb), split(T, xc, xb)
+        else:
+            x = rng.integers(-8, 9, (n, k)).astype(np.float32)
+            xd = dev(T, x, act)
+        want = (x.astype(np.float64) @ mxref.values(wc, wb).T).astype(np.float32)
+        buf, y = padded(T, n, m, "f32")
+        T.mul_mat(split(T, wc, wb), xd, out=y)
+        got = buf.numpy()
+        assert np.array_equal(got[:, :m], want, equal_nan=True), (n, k, m)
+        assert np.isnan(want).sum() == n + ((m - 1) if act == "mxfp4" else 0)
+        assert (got[:, m:] == 3.0).all()
+
+
 @pytest.mark.parametrize("n,k,m", [(1, 8192, 96), (4, 1024, 2048), (30, 4096, 200), (200, 1536, 1000), (1025, 2048, 640)])
 @pytest.mark.parametrize("act", ["mxfp4", "bf16", "f32"])
 @pytest.mark.parametrize("out", ["f32", "bf16"])

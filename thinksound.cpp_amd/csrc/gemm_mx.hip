@@ -3,30 +3,17 @@
 //   Y[n, m] = sum_k X[n, k] W[m, k] + bias[m],   W = codes * 2^(scale - 127) per 32 k,
 //
 // with X in bf16 (or f32, rounded to bf16 as it is read), or X in MXFP4 too.
+#include <algorithm>
+
 #include "mxfp4.h"
 #include "tsk_internal.h"
+#include "tsk_runtime.h"
 
 namespace tsk {
 
 namespace {
 
 typedef __attribute__((__vector_size__(8 * sizeof(int)))) int i32x8;
-
-// 8 activations at element k of a row, as bf16
-template <bool XF32>
-__device__ __forceinline__ bf16x8 load_x8(const void *row, int64_t k) {
-    if constexpr (XF32) {
-        const f32x4 a = *(const f32x4 *) ((const float *) row + k), b = *(const f32x4 *) ((const float *) row + k + 4);
-        bf16x8 r;
-        for (int j = 0; j < 4; ++j) {
-            r[j] = (__bf16) a[j];
-            r[4 + j] = (__bf16) b[j];
-        }
-        return r;
-    } else {
-        return *(const bf16x8 *) ((const uint16_t *) row + k);
-    }
-}
 
 // 4 outputs m .. m + 3 of row n (those below M)
 __device__ __forceinline__ void store4(const MxGemm &p, int n, int m, f32x4 v) {
@@ -53,53 +40,546 @@ __device__ __forceinline__ void store4(const MxGemm &p, int n, int m, f32x4 v) {
     }
 }
 
-// One wave per 16 x 16 outputs. Lane l holds row l % 16 of either operand and
-// of each 128 k the block of 32 number l / 16: the operand layout of
-// v_mfma_scale_f32_16x16x128_f8f6f4, and with the k of four
-// v_mfma_f32_16x16x32_bf16 taken in the same order on both sides, of those.
 enum : int { X_BF16 = 0, X_F32 = 1, X_MX = 2 };
 
-template <int XT>
-__global__ __launch_bounds__(64) void mx_gemm_simple_kernel(const MxGemm p) {
-    const int lane = threadIdx.x, r = lane & 15, g = lane >> 4;
-    const int tiles_m = (p.M + 15) / 16;
-    const int m0 = (int) (blockIdx.x % tiles_m) * 16, n0 = (int) (blockIdx.x / tiles_m) * 16;
-    const int KB = p.K / 32;
-    const int64_t m = min(m0 + r, p.M - 1), n = min(n0 + r, p.N - 1);
-    const uint8_t *wc = p.wq + m * (p.K / 2), *ws = p.ws + m * KB;
-    f32x4 acc = {0, 0, 0, 0};
-    for (int kb = g; kb < (KB + 3) / 4 * 4; kb += 4) {
-        const bool in = kb < KB;
-        const u32x4 w = in ? *(const u32x4 *) (wc + kb * 16) : u32x4{0, 0, 0, 0};
-        const uint32_t sb = in ? ws[kb] : 127u;
-        if constexpr (XT == X_MX) {
-            const u32x4 x = in ? *(const u32x4 *) (p.xq + n * (p.K / 2) + kb * 16) : u32x4{0, 0, 0, 0};
-            const uint32_t xb = in ? p.xs[n * KB + kb] : 127u;
-            const i32x8 a = {(int) w[0], (int) w[1], (int) w[2], (int) w[3], 0, 0, 0, 0};
-            const i32x8 b = {(int) x[0], (int) x[1], (int) x[2], (int) x[3], 0, 0, 0, 0};
-            acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4, 4, 0, (int) sb, 0, (int) xb);
-        } else {
-            const void *xr = (const char *) p.x + n * p.ld_x * (XT == X_F32 ? 4 : 2);
-            for (int j = 0; j < 4; ++j) {
-                bf16x8 b = {0, 0, 0, 0, 0, 0, 0, 0};
-                if (in) b = load_x8<XT == X_F32>(xr, (int64_t) kb * 32 + 8 * j);
-                acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mx_decode8_bf16(w[j], mx_scale(sb)), b, acc, 0, 0, 0);
+// ---------------------------------------------------------------- few rows
+// Operands straight into registers. NW waves share 16 MT x 16 NT outputs and
+// deal the K range among them in turns of 256 k; their sums meet in LDS, in
+// wave order. Lane l holds row l % 16 of either operand and of each 128 k the
+// block of 32 number l / 16: the layout of v_mfma_scale_f32_16x16x128_f8f6f4,
+// and with the k of four v_mfma_f32_16x16x32_bf16 taken in the same order on
+// both sides, of those.
+template <int XT, int MT, int NT>
+struct RowFrags {
+    static constexpr int BQ = XT == X_MX ? 1 : XT == X_BF16 ? 4 : 8;       // 16-byte pieces of an activation block
+    u32x4 a[MT][2], b[NT][2][BQ];
+    u32x2 sa[MT], sb[XT == X_MX ? NT : 1];
+};
+
+template <int XT, int MT, int NT, int NW>
+__device__ __forceinline__ void mx_gemm_rows(const MxGemm &p, int tiles_m, float *red) {
+    constexpr bool MX = XT == X_MX;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
+    const int m0 = (int) (blockIdx.x % tiles_m) * (16 * MT), n0 = (int) (blockIdx.x / tiles_m) * (16 * NT);
+    const int64_t K2 = p.K / 2, KB = p.K / 32;
+    const int nit = (int) ((KB + 7) / 8);
+    typedef RowFrags<XT, MT, NT> Frags;
+    // rows past M or N read the last one (their outputs are not stored)
+    const uint8_t *wq[MT], *ws[MT], *xq[NT], *xs[NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const int64_t m = min(m0 + 16 * i + r, p.M - 1);
+        wq[i] = p.wq + m * K2 + 16 * g;
+        ws[i] = p.ws + m * KB;
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        const int64_t n = min(n0 + 16 * j + r, p.N - 1);
+        xq[j] = MX ? p.xq + n * K2 + 16 * g : (const uint8_t *) p.x + n * p.ld_x * (XT == X_F32 ? 4 : 2) + (16 * Frags::BQ) * g;
+        xs[j] = MX ? p.xs + n * KB : nullptr;
+    }
+    auto load = [&](int it, Frags &f) {
+        const int64_t b0 = (int64_t) it * 8;
+        if (b0 + 8 <= KB) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks) f.a[i][ks] = *(const u32x4 *) (wq[i] + (b0 + 4 * ks) * 16);
+                __builtin_memcpy(&f.sa[i], ws[i] + b0, 8);
+            }
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                    for (int h = 0; h < Frags::BQ; ++h)
+                        f.b[j][ks][h] = *(const u32x4 *) (xq[j] + (b0 + 4 * ks) * (16 * Frags::BQ) + 16 * h);
+                if constexpr (MX) __builtin_memcpy(&f.sb[j], xs[j] + b0, 8);
+            }
+            return;
+        }
+        // the last turn's blocks past K: zeros
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            const int64_t blk = b0 + 4 * ks + g;
+            const bool in = blk < KB;
+            const u32x4 zero = {0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                f.a[i][ks] = in ? *(const u32x4 *) (wq[i] + (b0 + 4 * ks) * 16) : zero;
+                f.sa[i][ks] = in ? (uint32_t) ws[i][blk] << 8 * g : 0u;
+            }
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+#pragma unroll
+                for (int h = 0; h < Frags::BQ; ++h)
+                    f.b[j][ks][h] = in ? *(const u32x4 *) (xq[j] + (b0 + 4 * ks) * (16 * Frags::BQ) + 16 * h) : zero;
+                if constexpr (MX) f.sb[j][ks] = in ? (uint32_t) xs[j][blk] << 8 * g : 0u;
             }
         }
+    };
+    f32x4 acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+    auto product = [&](const Frags &f) {
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            if constexpr (MX) {
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        const i32x8 av = {(int) f.a[i][ks][0], (int) f.a[i][ks][1], (int) f.a[i][ks][2], (int) f.a[i][ks][3], 0, 0, 0, 0};
+                        const i32x8 bv = {(int) f.b[j][ks][0][0], (int) f.b[j][ks][0][1], (int) f.b[j][ks][0][2], (int) f.b[j][ks][0][3], 0, 0, 0, 0};
+                        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, acc[i][j], 4, 4, 0, (int) (f.sa[i][ks] >> 8 * g), 0,
+                                                                                     (int) (f.sb[j][ks] >> 8 * g));
+                    }
+            } else {
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    bf16x8 b[NT];
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        if constexpr (XT == X_F32) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                b[j][e] = (__bf16) __uint_as_float(f.b[j][ks][2 * h][e]);
+                                b[j][4 + e] = (__bf16) __uint_as_float(f.b[j][ks][2 * h + 1][e]);
+                            }
+                        } else {
+                            b[j] = __builtin_bit_cast(bf16x8, f.b[j][ks][h]);
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) {
+                        const bf16x8 av = mx_decode8_bf16(f.a[i][ks][h], mx_scale(f.sa[i][ks] >> 8 * g & 255u));
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, b[j], acc[i][j], 0, 0, 0);
+                    }
+                }
+            }
+        }
+    };
+    if (wave < nit) {
+        Frags f0, f1;
+        load(wave, f0);
+        int it = wave;
+        for (; it + NW < nit; it += 2 * NW) {
+            load(it + NW, f1);
+            product(f0);
+            if (it + 2 * NW < nit) load(it + 2 * NW, f0);
+            product(f1);
+        }
+        if (it < nit) product(f0);
     }
-    store4(p, n0 + r, m0 + 4 * g, acc);
+    if constexpr (NW > 1) {
+        // [wave][tile][lane] partial sums, four floats each
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) *(f32x4 *) (red + ((wave * MT * NT + i * NT + j) * 64 + lane) * 4) = acc[i][j];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                if ((i * NT + j) % NW != wave) continue;
+                f32x4 v = *(const f32x4 *) (red + ((i * NT + j) * 64 + lane) * 4);
+                for (int w = 1; w < NW; ++w) v += *(const f32x4 *) (red + ((w * MT * NT + i * NT + j) * 64 + lane) * 4);
+                store4(p, n0 + 16 * j + r, m0 + 16 * i + 4 * g, v);
+            }
+    } else {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) store4(p, n0 + 16 * j + r, m0 + 16 * i + 4 * g, acc[i][j]);
+    }
+}
+
+template <int XT, int MT, int NT, int NW>
+__global__ __launch_bounds__(NW * 64) void mx_gemm_rows_kernel(const MxGemm p, int tiles_m) {
+    __shared__ __attribute__((aligned(16))) float red[NW > 1 ? NW * MT * NT * 256 : 4];
+    mx_gemm_rows<XT, MT, NT, NW>(p, tiles_m, red);
+}
+// A launch holds fewer than 2^32 threads: products of more are cut into two by
+// their rows (16 rows at least, of M < 2^26 outputs each: 2^30 threads).
+constexpr int64_t MAX_THREADS = (int64_t) 1 << 31;
+template <class F>
+hipError_t halves(const MxGemm &p, F launch) {
+    MxGemm a = p, b = p;
+    a.N = (p.N / 2 + 15) / 16 * 16;
+    b.N = p.N - a.N;
+    if (b.N < 1) return hipErrorInvalidValue;
+    b.y = (char *) p.y + a.N * p.ld_y * (p.y_bf16 ? 2 : 4);
+    if (p.xq) {
+        b.xq = p.xq + (int64_t) a.N * (p.K / 2);
+        b.xs = p.xs + (int64_t) a.N * (p.K / 32);
+    } else {
+        b.x = (const char *) p.x + a.N * p.ld_x * (p.x_f32 ? 4 : 2);
+    }
+    const hipError_t e = launch(a);
+    return e == hipSuccess ? launch(b) : e;
+}
+
+template <int XT, int MT, int NT, int NW>
+hipError_t launch_rows(const MxGemm &p, hipStream_t s) {
+    const int tiles_m = (p.M + 16 * MT - 1) / (16 * MT), tiles_n = (p.N + 16 * NT - 1) / (16 * NT);
+    const int64_t T = (int64_t) tiles_m * tiles_n;
+    if (T * NW * 64 >= MAX_THREADS) return halves(p, [&](const MxGemm &q) { return launch_rows<XT, MT, NT, NW>(q, s); });
+    launch_kernel(mx_gemm_rows_kernel<XT, MT, NT, NW>, dim3((unsigned) T), dim3(NW * 64), 0, s, p, tiles_m);
+    return hipGetLastError();
+}
+
+// ---------------------------------------------------------------- tiles
+typedef __attribute__((address_space(3))) void lds_void;
+
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+    static_assert(N >= 0 && N < 64, "vmcnt range");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// at most `rem` stages of L loads in flight, and MOST at all
+template <int L, int MOST>
+__device__ __forceinline__ void wait_stages(int rem) {
+    if constexpr (MOST >= 1) {
+        if (rem >= MOST) wait_vm<MOST * L>();
+        else wait_stages<L, MOST - 1>(rem);
+    } else {
+        wait_vm<0>();
+    }
+}
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc_of(const void *base, int64_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), (short) 0, (int) bytes, 0x00020000);
+}
+
+// BYTES per lane, zero-extended, to LDS at dst + 4 * lane
+template <int BYTES>
+__device__ __forceinline__ void load_scales(__amdgpu_buffer_rsrc_t rsrc, uint8_t *dst, int off) {
+    if constexpr (BYTES == 2) __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void *) dst, 2, off, 0, 0, 0);
+    else __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void *) dst, 1, off, 0, 0, 0);
+}
+
+// Tiles. WM x WN waves share a BM x BN output tile, each TM x TN sub-tiles of
+// 16 x 16, over stages of SK blocks of 32 k in a ring of R stages of LDS.
+// Scales (SCB bytes a load and lane): with SCB = 16 in chunks of 1024 k beside
+// the ring (rows of scale bytes dword-aligned, K % 128 == 0), else with their stage.
+template <int XT_, int WM_, int WN_, int TM_, int TN_, int SK_, int R_, int SCB_>
+struct Cfg {
+    static constexpr int XT = XT_, WM = WM_, WN = WN_, TM = TM_, TN = TN_, SK = SK_, R = R_, SCB = SCB_;
+    static constexpr int NW = WM * WN, BM = WM * TM * 16, BN = WN * TN * 16;
+    static constexpr bool MX = XT == X_MX, CHUNK = SCB == 16;
+    static constexpr int XROW = MX ? SK * 16 : SK * 64;                    // bytes of an activation row per stage
+    static constexpr int SROW = CHUNK ? 0 : SK / SCB * 4;                  // bytes of a row's scales per stage
+    static constexpr int SROWS = BM + (MX ? BN : 0);                       // rows with scales
+    // LDS of a stage: weight codes, activations, weight scales, activation scales
+    static constexpr int A_BYTES = BM * SK * 16, B_BYTES = BN * XROW, S_BYTES = SROWS * SROW;
+    static constexpr int STAGE = A_BYTES + B_BYTES + S_BYTES;
+    // chunks: CS stages each; a ring of two stages loads a chunk whole with its
+    // first stage, a longer one a part with every stage, one chunk ahead
+    static constexpr int CS = 32 / SK, CHUNK_BYTES = CHUNK ? SROWS * 32 : 0, CHUNKS = !CHUNK ? 0 : R == 2 ? 2 : 3;
+    // loads of a wave per stage: 64 lanes x 16 bytes of codes or bf16, x 4 bytes of scales
+    static constexpr int UA = A_BYTES / 1024, UB = B_BYTES / 1024, US = CHUNK ? SROWS / 32 : S_BYTES / 256;
+    static constexpr int USP = CHUNK && R > 2 ? (US + CS - 1) / CS : US;   // scale loads with one stage
+    static constexpr int LA = UA / NW, LB = UB / NW, LS = (USP + NW - 1) / NW;
+    static constexpr int LOADS = LA + LB + LS;
+    static constexpr size_t LDS = (size_t) R * STAGE + CHUNKS * CHUNK_BYTES;
+    static_assert(NW % 4 == 0 && UA % NW == 0 && UB % NW == 0 && R >= 2 && R <= 5 && LOADS * (R - 2) < 64 && LDS <= 160 * 1024, "tile");
+};
+
+template <class C>
+__device__ __forceinline__ void mx_gemm_tile(const MxGemm &p, int tiles_m, int tiles_n, uint8_t *lds) {
+    constexpr int TM = C::TM, TN = C::TN, SK = C::SK, NW = C::NW, SCB = C::SCB, R = C::R;
+    constexpr bool MX = C::MX, CHUNK = C::CHUNK;
+    // workgroup L runs on XCD L % 8: each XCD takes a run of the tiles, eight tiles of m wide
+    int tm, tn;
+    {
+        const int T = tiles_m * tiles_n, per = (T + 7) / 8, t = (int) (blockIdx.x & 7) * per + (int) (blockIdx.x >> 3);
+        if ((int) (blockIdx.x >> 3) >= per || t >= T) return;
+        const int band = t / (8 * tiles_n), w = min(8, tiles_m - 8 * band), in = t - band * 8 * tiles_n;
+        tm = 8 * band + in % w;
+        tn = in / w;
+    }
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6);
+    const int r = lane & 15, g = lane >> 4, wm = wave % C::WM, wn = wave / C::WM;
+    const int m0 = tm * C::BM, n0 = tn * C::BN;
+    const int K2 = p.K / 2, KB = p.K / 32;
+    const int nst = (KB + SK - 1) / SK, kv = KB - (nst - 1) * SK;              // blocks of the last stage
+
+    // Rows past M or N are past the descriptors' ends by the lane's own offset:
+    // the loads put zeros there. So do blocks past K, sent FAR with the last
+    // stage; a scale past K is zeroed like its codes (it would be the next
+    // row's, and could be a NaN).
+    const int rm = min(C::BM, p.M - m0), rn = min(C::BN, p.N - n0);
+    const int64_t xrow = MX ? K2 : p.ld_x * 2;                                 // bytes between activation rows
+    const __amdgpu_buffer_rsrc_t ra = rsrc_of(p.wq + (int64_t) m0 * K2, (int64_t) rm * K2);
+    const __amdgpu_buffer_rsrc_t rsa = rsrc_of(p.ws + (int64_t) m0 * KB, (int64_t) rm * KB);
+    const __amdgpu_buffer_rsrc_t rb = MX ? rsrc_of(p.xq + (int64_t) n0 * K2, (int64_t) rn * K2)
+                                         : rsrc_of((const char *) p.x + n0 * xrow, (rn - 1) * xrow + (int64_t) p.K * 2);
+    const __amdgpu_buffer_rsrc_t rsb = MX ? rsrc_of(p.xs + (int64_t) n0 * KB, (int64_t) rn * KB) : rsa;
+    constexpr int FAR = (int) 0x80000000u;
+    // A lane's part of a load: rows of SK 16-byte chunks of codes, 64 / SK rows
+    // a load, chunk c of row t at slot c ^ key(t). An MFMA read takes one chunk
+    // of 16 rows at a time, which the keys spread over all 256 bytes of banks.
+    constexpr int AR = 64 / SK;
+    auto key = [](int row) { return SK == 8 ? row >> 1 & 7 : row >> 2 & 3; };
+    const int a_chk = (lane % SK) ^ key(wave * AR + lane / SK);                // (a wave's loads are NW, a multiple of 4, apart)
+    int a_off[C::LA];
+#pragma unroll
+    for (int q = 0; q < C::LA; ++q) a_off[q] = ((wave + NW * q) * AR + lane / SK) * K2 + a_chk * 16;
+    // bf16 rows: 16 chunks, 4 rows a load, chunk c of row t at slot c ^ (t % 16)
+    static_assert(MX || SK == 4, "bf16 rows of 256 bytes");
+    constexpr int BC = MX ? SK : 4 * SK, BR = 64 / BC;
+    const int b_row = wave * BR + lane / BC;
+    const int b_chk = (lane % BC) ^ (MX ? key(b_row) : b_row & 15), b_blk = MX ? b_chk : b_chk / 4;
+    int b_off[C::LB];
+#pragma unroll
+    for (int q = 0; q < C::LB; ++q) b_off[q] = (int) ((b_row + NW * q * BR) * xrow) + b_chk * 16;
+    // scales with their stage: SCB bytes a lane, zero-extended to a dword; chunks: 16 bytes of a row's 32
+    constexpr int SL = CHUNK ? 2 : SK / SCB, SR = 64 / SL;
+    const int s_row = lane / SL, s_blk = lane % SL * SCB, s_off = s_row * KB + s_blk;
+    uint8_t *chunks = lds + R * C::STAGE;
+
+    // scale load f (of SR rows: the weights' first, then the activations') from block blk on
+    auto scale_load = [&](int f, uint8_t *dst, int blk, bool past) {
+        constexpr int FA = C::BM / SR;
+        const bool b = MX && f >= FA;
+        const int off = past ? FAR : (b ? f - FA : f) * SR * KB + blk + s_off;
+        if constexpr (CHUNK) __builtin_amdgcn_raw_ptr_buffer_load_lds(b ? rsb : rsa, (lds_void *) (dst + f * 1024), 16, off, 0, 0, 0);
+        else load_scales<C::SCB>(b ? rsb : rsa, dst + f * 256, off);
+    };
+    auto issue = [&](int t, int slot) {
+        uint8_t *st = lds + slot * C::STAGE;
+        const bool last = t == nst - 1;
+        if (last && kv < SK) {
+#pragma unroll
+            for (int q = 0; q < C::LA; ++q) a_off[q] = a_chk >= kv ? FAR : a_off[q];
+#pragma unroll
+            for (int q = 0; q < C::LB; ++q) b_off[q] = b_blk >= kv ? FAR : b_off[q];
+        }
+#pragma unroll
+        for (int q = 0; q < C::LA; ++q)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_void *) (st + (wave + NW * q) * 1024), 16, a_off[q], t * (SK * 16), 0, 0);
+#pragma unroll
+        for (int q = 0; q < C::LB; ++q)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_void *) (st + C::A_BYTES + (wave + NW * q) * 1024), 16, b_off[q],
+                                                     t * C::XROW, 0, 0);
+        if constexpr (!CHUNK) {
+#pragma unroll
+            for (int q = 0; q < C::LS; ++q)
+                scale_load((wave + NW * q) % C::US, st + C::A_BYTES + C::B_BYTES, t * SK, last && s_blk >= kv);
+        } else if constexpr (R == 2) {
+            if (t % C::CS == 0) {
+#pragma unroll
+                for (int q = 0; q < C::LS; ++q)
+                    scale_load((wave + NW * q) % C::US, chunks + (t / C::CS & 1) * C::CHUNK_BYTES, t * SK, false);
+            }
+        } else {
+            const int c = t / C::CS + 1;
+#pragma unroll
+            for (int q = 0; q < C::LS; ++q)
+                scale_load(((t % C::CS) * C::USP + (wave + NW * q) % C::USP) % C::US, chunks + c % 3 * C::CHUNK_BYTES, c * 32, false);
+        }
+    };
+
+    f32x4 acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+
+    // step ks of a stage: lane group g takes block SK / 4 * g + ks of every row
+    const int akey = key(r);
+    // the scale bytes of this lane's blocks of a stage, byte ks for step ks
+    auto scale_at = [&](const uint8_t *base, int row) -> int {
+        const uint8_t *q = base + row * (CHUNK ? 32 : C::SROW);
+        if constexpr (CHUNK) return SK == 8 ? *(const uint16_t *) (q + 2 * g) : q[g];
+        else if constexpr (SK == 8) return SCB == 2 ? *(const int *) (q + 4 * g) : q[8 * g] | q[8 * g + 4] << 8;
+        else return SCB == 2 ? q[(g >> 1) * 4 + (g & 1)] : q[4 * g];
+    };
+    auto compute = [&](int t, int slot) {
+        const uint8_t *st = lds + slot * C::STAGE, *sb = st + C::A_BYTES;
+        const uint8_t *ss = CHUNK ? chunks + t / C::CS % C::CHUNKS * C::CHUNK_BYTES + t % C::CS * SK : sb + C::B_BYTES;
+        int sa[TM], sx[MX ? TN : 1];
+#pragma unroll
+        for (int i = 0; i < TM; ++i) sa[i] = scale_at(ss, (wm * TM + i) * 16 + r);
+        if constexpr (MX) {
+#pragma unroll
+            for (int j = 0; j < TN; ++j) sx[j] = scale_at(ss, C::BM + (wn * TN + j) * 16 + r);
+        }
+        if (CHUNK && t == nst - 1) {                              // (no scales past K)
+            const int b0 = SK / 4 * g, msk = (b0 < kv ? 0xff : 0) | (b0 + 1 < kv ? 0xff00 : 0);
+#pragma unroll
+            for (int i = 0; i < TM; ++i) sa[i] &= msk;
+            if constexpr (MX) {
+#pragma unroll
+                for (int j = 0; j < TN; ++j) sx[j] &= msk;
+            }
+        }
+#pragma unroll
+        for (int ks = 0; ks < SK / 4; ++ks) {
+            const int c = SK / 4 * g + ks;
+            u32x4 a[TM];
+#pragma unroll
+            for (int i = 0; i < TM; ++i) a[i] = *(const u32x4 *) (st + ((wm * TM + i) * 16 + r) * (SK * 16) + (c ^ akey) * 16);
+            if constexpr (MX) {
+                u32x4 b[TN];
+#pragma unroll
+                for (int j = 0; j < TN; ++j) b[j] = *(const u32x4 *) (sb + ((wn * TN + j) * 16 + r) * (SK * 16) + (c ^ akey) * 16);
+#pragma unroll
+                for (int i = 0; i < TM; ++i)
+#pragma unroll
+                    for (int j = 0; j < TN; ++j) {
+                        const i32x8 av = {(int) a[i][0], (int) a[i][1], (int) a[i][2], (int) a[i][3], 0, 0, 0, 0};
+                        const i32x8 bv = {(int) b[j][0], (int) b[j][1], (int) b[j][2], (int) b[j][3], 0, 0, 0, 0};
+                        if (ks == 1) acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, acc[i][j], 4, 4, 1, sa[i], 1, sx[j]);
+                        else acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, acc[i][j], 4, 4, 0, sa[i], 0, sx[j]);
+                    }
+            } else {
+                float s[TM];
+#pragma unroll
+                for (int i = 0; i < TM; ++i) s[i] = mx_scale((uint32_t) sa[i] & 255u);
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    bf16x8 b[TN];
+#pragma unroll
+                    for (int j = 0; j < TN; ++j)
+                        b[j] = *(const bf16x8 *) (sb + ((wn * TN + j) * 16 + r) * C::XROW + ((4 * c + h) ^ r) * 16);
+#pragma unroll
+                    for (int i = 0; i < TM; ++i) {
+                        const bf16x8 av = mx_decode8_bf16(a[i][h], s[i]);
+#pragma unroll
+                        for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, b[j], acc[i][j], 0, 0, 0);
+                    }
+                }
+            }
+        }
+    };
+
+    if constexpr (CHUNK && R > 2) {
+        for (int f = wave; f < C::US; f += NW) scale_load(f, chunks, 0, false);
+    }
+#pragma unroll
+    for (int s = 0; s < R - 1; ++s)
+        if (s < nst) issue(s, s);
+    int slot = 0;
+    for (int t = 0; t < nst; ++t) {
+        // this wave's loads of stage t have landed; past the barrier every
+        // wave's have, and every wave has read stage t - 1, whose slot is refilled
+        wait_stages<C::LOADS, R - 2>(nst - 1 - t);
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (t + R - 1 < nst) issue(t + R - 1, slot == 0 ? R - 1 : slot - 1);
+        compute(t, slot);
+        slot = slot + 1 == R ? 0 : slot + 1;
+    }
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) store4(p, n0 + (wn * TN + j) * 16 + r, m0 + (wm * TM + i) * 16 + 4 * g, acc[i][j]);
+}
+
+template <class C>
+__global__ __launch_bounds__(C::NW * 64) void mx_gemm_tile_kernel(const MxGemm p, int tiles_m, int tiles_n) {
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    mx_gemm_tile<C>(p, tiles_m, tiles_n, lds);
+}
+
+template <class C>
+hipError_t launch_tile(const MxGemm &p, hipStream_t s) {
+    const int tiles_m = (p.M + C::BM - 1) / C::BM, tiles_n = (p.N + C::BN - 1) / C::BN;
+    const int64_t T = (int64_t) tiles_m * tiles_n;
+    if ((T + 7) * C::NW * 64 >= MAX_THREADS) return halves(p, [&](const MxGemm &q) { return launch_tile<C>(q, s); });
+    lds_opt_in((const void *) mx_gemm_tile_kernel<C>, C::LDS);
+    launch_kernel(mx_gemm_tile_kernel<C>, dim3((unsigned) ((T + 7) / 8 * 8)), dim3(C::NW * 64), C::LDS, s, p, tiles_m, tiles_n);
+    return hipGetLastError();
+}
+template <int XT, int WM, int WN, int TM, int TN, int SK, int R>
+hipError_t launch_tile_k(const MxGemm &p, hipStream_t s) {
+    if (p.K % 128 == 0) return launch_tile<Cfg<XT, WM, WN, TM, TN, SK, R, 16>>(p, s);
+    if (p.K % 64 == 0) return launch_tile<Cfg<XT, WM, WN, TM, TN, SK, R, 2>>(p, s);
+    return launch_tile<Cfg<XT, WM, WN, TM, TN, SK, R - (R > 2), 1>>(p, s);
+}
+
+// Shapes, by number (TSK_MX_CFG):
+//        both operands MXFP4             bf16 activations
+//   1    256 x 256, 8 waves              -
+//   2    128 x 256, 8 waves              256 x 128, 8 waves
+//   3    128 x 128, 8 waves              the same
+//   4    64 x 128, 4 waves               the same
+//   5    64 x 32, 4 waves                the same
+//   11   rows kernel, 16 x 16 outputs (f32 activations too, as 12 to 14)
+//   12   32 x 16,  13  32 x 32,  14  64 x 32
+//
+// Tiles run in rounds of the 256 CUs (64 x 32: two a CU), so the choice is the
+// shape of the least rounds times the time of one, measured at K = 5120 (us:
+// MXFP4 45, 29, 22, 15, 11; bf16 -, 64, 45, 33, 22 for shapes 1 to 5). Some
+// pairs (us, taken / next): MXFP4, 512 x 5120, K = 2048 128 x 128 11.2 / 15.6;
+// 388 x 4096, K = 1024 64 x 128 6.2 / 7.6; 1292 x 4096, K = 1024 128 x 256 11.2 /
+// 14.3; bf16, 2047 x 2050, K = 5120 256 x 128 (144 tiles) 66 / 128 x 128 (272) 89.
+// Too few tiles of the smallest shape, or at most 32 rows: the rows kernel, the
+// largest of its shapes of which there are 200 (16 rows, M = K = 4096, 128 of 32 x
+// 16 6.3 / 4.7; 1 row, M = K = 8192, 256 of them 9.6 / 11.0). With bf16
+// activations it is the faster one up to more tiles (128 rows, K = 1024, M =
+// 4096, 256 tiles 6.5 / rows 5.8; M = K = 8192, 512 tiles 39 / 56).
+template <int XT>
+int shape_for(const MxGemm &p) {
+    if (tuning().mx_cfg) return tuning().mx_cfg;
+    auto tiles = [&](int bm, int bn) { return (int64_t) ((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
+    if constexpr (XT != X_F32) {
+        constexpr bool MX = XT == X_MX;
+        struct Shape { int bm, bn, a_round, us; };
+        constexpr Shape shapes[5] = {{256, 256, 256, MX ? 45 : 0}, {MX ? 128 : 256, MX ? 256 : 128, 256, MX ? 29 : 64},
+                                     {128, 128, 256, MX ? 22 : 45}, {64, 128, 256, MX ? 15 : 33}, {64, 32, 512, MX ? 11 : 22}};
+        if (p.N > 32 && tiles(64, 32) >= (MX ? 150 : 300)) {
+            int best = 0;
+            int64_t least = 0;
+            for (int i = MX ? 0 : 1; i < 5; ++i) {
+                const Shape &c = shapes[i];
+                const int64_t cost = (tiles(c.bm, c.bn) + c.a_round - 1) / c.a_round * c.us;
+                if (!best || cost < least) {
+                    best = i + 1;
+                    least = cost;
+                }
+            }
+            return best;
+        }
+    }
+    return tiles(64, 32) >= 200 ? 14 : tiles(32, 32) >= 200 ? 13 : tiles(32, 16) >= 200 ? 12 : 11;
+}
+
+template <int XT>
+hipError_t launch_kind(const MxGemm &p, hipStream_t s) {
+    int shape = shape_for<XT>(p);
+    if constexpr (XT != X_F32) {
+        constexpr bool MX = XT == X_MX;
+        // a tile's offsets have 31 bits (else the rows kernel, whose addresses have 64)
+        const int64_t xrow = MX ? p.K / 2 : p.ld_x * 2, most = (int64_t) 1 << 31;
+        if (256 * (int64_t) (p.K / 2) >= most || 256 * xrow + (int64_t) p.K * 2 >= most) shape = std::max(shape, 11);
+        switch (shape) {
+            case 1: if constexpr (MX) return launch_tile_k<XT, 2, 4, 8, 4, 8, 2>(p, s);
+            [[fallthrough]];
+            case 2: if constexpr (MX) return launch_tile_k<XT, 2, 4, 4, 4, 8, 2>(p, s);
+                    else return launch_tile_k<XT, 4, 2, 4, 4, 4, 2>(p, s);
+            case 3: if constexpr (MX) return launch_tile_k<XT, 2, 4, 4, 2, 8, 4>(p, s);
+                    else return launch_tile_k<XT, 4, 2, 2, 4, 4, 3>(p, s);
+            case 4: return launch_tile_k<XT, 2, 2, 2, 4, MX ? 8 : 4, MX ? 5 : 4>(p, s);
+            case 5: return launch_tile_k<XT, 4, 1, 1, 2, MX ? 8 : 4, 5>(p, s);
+        }
+    }
+    switch (shape) {
+        case 14: return launch_rows<XT, 4, 2, 4>(p, s);
+        case 13: return launch_rows<XT, 2, 2, 4>(p, s);
+        case 12: return launch_rows<XT, 2, 1, 4>(p, s);
+        default: return launch_rows<XT, 1, 1, 4>(p, s);
+    }
 }
 
 }  // namespace
 
 hipError_t launch_gemm_mx(const MxGemm &p, hipStream_t s) {
-    const int64_t tiles = (int64_t) ((p.M + 15) / 16) * ((p.N + 15) / 16);
-    if (tiles > (1 << 26) - 1) return hipErrorInvalidValue;
-    const dim3 grid((unsigned) tiles), block(64);
-    if (p.xq) launch_kernel(mx_gemm_simple_kernel<X_MX>, grid, block, 0, s, p);
-    else if (p.x_f32) launch_kernel(mx_gemm_simple_kernel<X_F32>, grid, block, 0, s, p);
-    else launch_kernel(mx_gemm_simple_kernel<X_BF16>, grid, block, 0, s, p);
-    return hipGetLastError();
+    return p.xq ? launch_kind<X_MX>(p, s) : p.x_f32 ? launch_kind<X_F32>(p, s) : launch_kind<X_BF16>(p, s);
 }
 
 }  // namespace tsk

@@ -63,6 +63,7 @@ void read_tuning() {
     t.q8_old = env_int("TSK_Q8_OLD", 0) != 0;
     t.q8_pair = env_int("TSK_Q8_PAIR", 1) != 0;
     t.coop_cfg = env_int("TSK_COOP_CFG", 0);
+    t.mx_cfg = env_int("TSK_MX_CFG", 0);
     t.attn_cfg = env_int("TSK_ATTN_CFG", 0);
     t.dit_sched = env_int("TSK_DIT_SCHED", 1) != 0;
     t.ln_block = env_int("TSK_LN_BLOCK", 0) != 0;
@@ -262,7 +263,8 @@ bool rows_uniform(const tsk_tensor *t) {
 }
 
 // ---- MXFP4 tensors
-constexpr int64_t MX_MAX_EXTENT = 0x7fffffff - 63;      // (tiles past the end stay in int)
+constexpr int64_t MX_MAX_EXTENT = 0x7fffffff - 255;     // (tiles past the end stay in int)
+constexpr int64_t MX_MAX_WEIGHT = 1 << 26;              // K and M of a product's weights
 
 // rows of ne1 x ne2 x ne3 within MX_MAX_EXTENT (the extents are >= 1)
 bool rows_fit(const tsk_tensor *t) {
@@ -462,7 +464,7 @@ int validate_mul_mat(const tsk_tensor *a, const tsk_tensor *b, const tsk_tensor 
         case TSK_TYPE_MXFP4:
         case TSK_TYPE_MXFP4_SPLIT:
             if (K % 32) return fail(TSK_ERR_SHAPE, "K=%lld must be a multiple of 32 for MXFP4", (long long) K);
-            if (K > MX_MAX_EXTENT || M > MX_MAX_EXTENT) return fail(TSK_ERR_SHAPE, "MXFP4 weights of [%lld, %lld]", (long long) K, (long long) M);
+            if (K > MX_MAX_WEIGHT || M > MX_MAX_WEIGHT) return fail(TSK_ERR_SHAPE, "MXFP4 weights of [%lld, %lld]", (long long) K, (long long) M);
             if (!rows_fit(b)) return fail(TSK_ERR_SHAPE, "b has too many rows");
             if (a->type == TSK_TYPE_MXFP4) return check_mx_blocks(a, "a");
             if (!aligned(a->data, 16)) return fail(TSK_ERR_ALIGN, "MXFP4_SPLIT data must be 16-byte aligned");
@@ -582,8 +584,15 @@ MulMatPlan plan_mul_mat(const tsk_tensor *a, const tsk_tensor *b, const tsk_tens
     pl.nslices = pl.uni ? 1 : b->ne[2] * b->ne[3];
     pl.Nslice = pl.uni ? b->ne[1] * b->ne[2] * b->ne[3] : b->ne[1];
     if (a->type == TSK_TYPE_MXFP4 || a->type == TSK_TYPE_MXFP4_SPLIT) {
+        // f32 activations: read and rounded by the rows kernel in every one of its
+        // workgroups, or once by a launch before the product (us, M = K = 4096: 16
+        // rows 10.6 / 9.6, 32 rows 12.9 / 11.3; K = 1024, M = 4096, 64 rows 6.6 /
+        // 7.2; K = M = 1024, 77 rows 4.5 / 6.2; K = M = 8192, 8 rows 17.4 / 15.1)
         pl.mx = true;
-        pl.bytes = pl.wbytes = a->type == TSK_TYPE_MXFP4 ? align256(tsk_mxfp4_split_nbytes(K, M)) : 0;
+        pl.wbytes = a->type == TSK_TYPE_MXFP4 ? align256(tsk_mxfp4_split_nbytes(K, M)) : 0;
+        if (b->type == TSK_TYPE_F32 && (double) pl.Nslice * (double) K * (double) M > (double) (1 << 28))
+            pl.cast_bytes = align256((size_t) (pl.Nslice * K) * 2);
+        pl.bytes = pl.wbytes + pl.cast_bytes;
         return pl;
     }
     // Few rows. From 5 rows on every wave's own conversion of the activations
@@ -614,10 +623,10 @@ int mul_mat_mx(const tsk_tensor *a, const tsk_tensor *b, const tsk_tensor *bias,
     memset(&p, 0, sizeof(p));
     p.wq = mx_codes(a);
     hipError_t e;
+    void *ws = nullptr;
+    int rc;
+    if (pl.bytes && (rc = scr.get(pl.bytes, &ws))) return rc;
     if (a->type == TSK_TYPE_MXFP4) {
-        int rc;
-        void *ws = nullptr;
-        if ((rc = scr.get(pl.bytes, &ws))) return rc;
         e = launch_mx_repack((const uint8_t *) a->data, (int64_t) a->nb[1], M, K, (uint8_t *) ws,
                              (uint8_t *) ws + (size_t) M * (size_t) (K / 2), scr.s);
         if (e != hipSuccess) return hip_fail(e, "mxfp4 repack");
@@ -626,11 +635,12 @@ int mul_mat_mx(const tsk_tensor *a, const tsk_tensor *b, const tsk_tensor *bias,
     p.ws = p.wq + (size_t) M * (size_t) (K / 2);
     p.bias = bias ? (const float *) bias->data : nullptr;
     p.y_bf16 = dst->type == TSK_TYPE_BF16;
-    p.x_f32 = b->type == TSK_TYPE_F32;
+    p.x_f32 = b->type == TSK_TYPE_F32;                       // (unless a launch rounds them first)
     p.M = (int) M; p.N = (int) pl.Nslice; p.K = (int) K;
     const bool mx_b = b->type == TSK_TYPE_MXFP4_SPLIT;
-    p.ld_x = mx_b ? 0 : (int64_t) b->nb[1] / elt_size(b->type);
-    p.ld_y = (int64_t) dst->nb[1] / elt_size(dst->type);
+    // (a single row's stride may be anything)
+    p.ld_x = mx_b ? 0 : p.N == 1 ? K : (int64_t) b->nb[1] / elt_size(b->type);
+    p.ld_y = p.N == 1 ? M : (int64_t) dst->nb[1] / elt_size(dst->type);
     for (int64_t sl = 0; sl < pl.nslices; ++sl) {
         const int64_t i2 = sl % b->ne[2], i3 = sl / b->ne[2];
         p.y = (char *) dst->data + i2 * dst->nb[2] + i3 * dst->nb[3];
@@ -639,6 +649,15 @@ int mul_mat_mx(const tsk_tensor *a, const tsk_tensor *b, const tsk_tensor *bias,
             p.xs = mx_scales(b) + sl * pl.Nslice * (K / 32);
         } else {
             p.x = (const char *) b->data + i2 * b->nb[2] + i3 * b->nb[3];
+            if (pl.cast_bytes) {
+                uint16_t *xb = (uint16_t *) ((char *) ws + pl.wbytes);
+                e = launch_cast_rows_bf16((const float *) p.x, pl.Nslice == 1 ? K : (int64_t) b->nb[1] / 4, 0, (int) std::min<int64_t>(pl.Nslice, 1 << 30),
+                                          pl.Nslice, (int) K, xb, scr.s);
+                if (e != hipSuccess) return hip_fail(e, "mul_mat input cast");
+                p.x = xb;
+                p.x_f32 = 0;
+                p.ld_x = K;
+            }
         }
         if ((e = launch_gemm_mx(p, scr.s)) != hipSuccess) return hip_fail(e, "mul_mat launch");
     }

@@ -30,6 +30,7 @@ bool workspace_can(hipStream_t s, size_t bytes);
 //   TSK_Q8_OLD    1: the 2 x 2-wave Q8_0 kernel for every shape
 //   TSK_Q8_PAIR   0: the Q8_0 DiT's two streams as separate launches (A/B reference)
 //   TSK_COOP_CFG  cooperative BF16 tile of the C-ABI GEMMs (0 = rule)
+//   TSK_MX_CFG    MXFP4 products: the tile or rows shape launch_gemm_mx's table numbers (0 = rule)
 //   TSK_GEMM_CFG  DiT block GEMM tiles, one character per projection
 //   TSK_ATTN_CFG  DiT attention launch shape (10 * key ranges + query blocks)
 //   TSK_DIT_SCHED 0: the sampler computes its conditioning inside every step
@@ -51,6 +52,7 @@ struct Tuning {
     bool q8_old = false;
     bool q8_pair = true;                  // a joint block's two Q8_0 projections in one launch
     int coop_cfg = 0;
+    int mx_cfg = 0;
     int gemm_cfg[4] = {0, 0, 0, 0};
     int attn_cfg = 0;
     bool dit_sched = true;
