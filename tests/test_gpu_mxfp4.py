@@ -44,7 +44,8 @@ def hard_rows(rng, rows, k):
     b[::3] = rng.integers(-32, 33, b[::3].shape) * 0.25        # ties of the scale 2^0 and its neighbours
     b[1::7] *= 2.0 ** -120                                     # (the scale stops at 2^-127)
     b[2::11] *= 2.0 ** 110
-    x = x.astype(np.float32)
+    with np.errstate(over="ignore"):                           # (some blocks become infinite)
+        x = x.astype(np.float32)
     b = x.reshape(-1, 32)
     if len(b) > 8:
         b[3] = 0.0
@@ -179,7 +180,7 @@ def shape(T, monkeypatch):
     T.init(0, reread=True)
 
 
-@pytest.mark.parametrize("cfg", [1, 2, 3, 4, 5, 11, 12, 13, 14])
+@pytest.mark.parametrize("cfg", [1, 2, 3, 4, 5, 11, 12, 13, 14, 15])
 @pytest.mark.parametrize("act", ["mxfp4", "bf16", "f32"])
 def test_every_launch_shape(T, shape, cfg, act):
     """ragged in rows, outputs and K (blocks of scales whole, by twos and odd; K shorter than a stage and longer than a

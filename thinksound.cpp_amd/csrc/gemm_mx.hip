@@ -266,8 +266,12 @@ __device__ __forceinline__ void load_scales(__amdgpu_buffer_rsrc_t rsrc, uint8_t
 // 16 x 16, over stages of SK blocks of 32 k in a ring of R stages of LDS.
 // Scales (SCB bytes a load and lane): with SCB = 16 in chunks of 1024 k beside
 // the ring (rows of scale bytes dword-aligned, K % 128 == 0), else with their stage.
-template <int XT_, int WM_, int WN_, int TM_, int TN_, int SK_, int R_, int SCB_>
+template <int XT_, int WM_, int WN_, int TM_, int TN_, int SK_, int R_, int SCB_, bool PIPE_>
 struct Cfg {
+    // PIPE: a stage's fragments are read from LDS while the stage before is
+    // multiplied. It pays where a wave holds few (64 x 32: 388 x 1024, K = 4096 8.8 ->
+    // 7.7 us); at 64 x 128 it changes nothing, and larger tiles lack the registers.
+    static constexpr bool PIPE = PIPE_;
     static constexpr int XT = XT_, WM = WM_, WN = WN_, TM = TM_, TN = TN_, SK = SK_, R = R_, SCB = SCB_;
     static constexpr int NW = WM * WN, BM = WM * TM * 16, BN = WN * TN * 16;
     static constexpr bool MX = XT == X_MX, CHUNK = SCB == 16;
@@ -286,7 +290,7 @@ struct Cfg {
     static constexpr int LA = UA / NW, LB = UB / NW, LS = (USP + NW - 1) / NW;
     static constexpr int LOADS = LA + LB + LS;
     static constexpr size_t LDS = (size_t) R * STAGE + CHUNKS * CHUNK_BYTES;
-    static_assert(NW % 4 == 0 && UA % NW == 0 && UB % NW == 0 && R >= 2 && R <= 5 && LOADS * (R - 2) < 64 && LDS <= 160 * 1024, "tile");
+    static_assert(NW % 4 == 0 && UA % NW == 0 && UB % NW == 0 && R >= 2 && R <= 5 && LOADS * (R - 1) < 64 && LDS <= 160 * 1024, "tile");
 };
 
 template <class C>
@@ -399,61 +403,73 @@ __device__ __forceinline__ void mx_gemm_tile(const MxGemm &p, int tiles_m, int t
         else if constexpr (SK == 8) return SCB == 2 ? *(const int *) (q + 4 * g) : q[8 * g] | q[8 * g + 4] << 8;
         else return SCB == 2 ? q[(g >> 1) * 4 + (g & 1)] : q[4 * g];
     };
-    auto compute = [&](int t, int slot) {
+    constexpr int KS = SK / 4;
+    struct Frags {
+        u32x4 a[KS][TM], b[KS][MX ? TN : 4 * TN];
+        int sa[TM], sx[MX ? TN : 1];
+    };
+    auto read = [&](int t, int slot, Frags &f) {
         const uint8_t *st = lds + slot * C::STAGE, *sb = st + C::A_BYTES;
         const uint8_t *ss = CHUNK ? chunks + t / C::CS % C::CHUNKS * C::CHUNK_BYTES + t % C::CS * SK : sb + C::B_BYTES;
-        int sa[TM], sx[MX ? TN : 1];
 #pragma unroll
-        for (int i = 0; i < TM; ++i) sa[i] = scale_at(ss, (wm * TM + i) * 16 + r);
+        for (int i = 0; i < TM; ++i) f.sa[i] = scale_at(ss, (wm * TM + i) * 16 + r);
         if constexpr (MX) {
 #pragma unroll
-            for (int j = 0; j < TN; ++j) sx[j] = scale_at(ss, C::BM + (wn * TN + j) * 16 + r);
+            for (int j = 0; j < TN; ++j) f.sx[j] = scale_at(ss, C::BM + (wn * TN + j) * 16 + r);
         }
         if (CHUNK && t == nst - 1) {                              // (no scales past K)
             const int b0 = SK / 4 * g, msk = (b0 < kv ? 0xff : 0) | (b0 + 1 < kv ? 0xff00 : 0);
 #pragma unroll
-            for (int i = 0; i < TM; ++i) sa[i] &= msk;
+            for (int i = 0; i < TM; ++i) f.sa[i] &= msk;
             if constexpr (MX) {
 #pragma unroll
-                for (int j = 0; j < TN; ++j) sx[j] &= msk;
+                for (int j = 0; j < TN; ++j) f.sx[j] &= msk;
             }
         }
 #pragma unroll
-        for (int ks = 0; ks < SK / 4; ++ks) {
-            const int c = SK / 4 * g + ks;
-            u32x4 a[TM];
+        for (int ks = 0; ks < KS; ++ks) {
+            const int c = KS * g + ks;
 #pragma unroll
-            for (int i = 0; i < TM; ++i) a[i] = *(const u32x4 *) (st + ((wm * TM + i) * 16 + r) * (SK * 16) + (c ^ akey) * 16);
+            for (int i = 0; i < TM; ++i) f.a[ks][i] = *(const u32x4 *) (st + ((wm * TM + i) * 16 + r) * (SK * 16) + (c ^ akey) * 16);
             if constexpr (MX) {
-                u32x4 b[TN];
 #pragma unroll
-                for (int j = 0; j < TN; ++j) b[j] = *(const u32x4 *) (sb + ((wn * TN + j) * 16 + r) * (SK * 16) + (c ^ akey) * 16);
+                for (int j = 0; j < TN; ++j) f.b[ks][j] = *(const u32x4 *) (sb + ((wn * TN + j) * 16 + r) * (SK * 16) + (c ^ akey) * 16);
+            } else {
+#pragma unroll
+                for (int h = 0; h < 4; ++h)
+#pragma unroll
+                    for (int j = 0; j < TN; ++j)
+                        f.b[ks][h * TN + j] = *(const u32x4 *) (sb + ((wn * TN + j) * 16 + r) * C::XROW + ((4 * c + h) ^ r) * 16);
+            }
+        }
+    };
+    auto multiply = [&](const Frags &f) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            if constexpr (MX) {
 #pragma unroll
                 for (int i = 0; i < TM; ++i)
 #pragma unroll
                     for (int j = 0; j < TN; ++j) {
-                        const i32x8 av = {(int) a[i][0], (int) a[i][1], (int) a[i][2], (int) a[i][3], 0, 0, 0, 0};
-                        const i32x8 bv = {(int) b[j][0], (int) b[j][1], (int) b[j][2], (int) b[j][3], 0, 0, 0, 0};
-                        if (ks == 1) acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, acc[i][j], 4, 4, 1, sa[i], 1, sx[j]);
-                        else acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, acc[i][j], 4, 4, 0, sa[i], 0, sx[j]);
+                        const u32x4 &a = f.a[ks][i], &b = f.b[ks][j];
+                        const i32x8 av = {(int) a[0], (int) a[1], (int) a[2], (int) a[3], 0, 0, 0, 0};
+                        const i32x8 bv = {(int) b[0], (int) b[1], (int) b[2], (int) b[3], 0, 0, 0, 0};
+                        if (ks == 1) acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, acc[i][j], 4, 4, 1, f.sa[i], 1, f.sx[j]);
+                        else acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, acc[i][j], 4, 4, 0, f.sa[i], 0, f.sx[j]);
                     }
             } else {
                 float s[TM];
 #pragma unroll
-                for (int i = 0; i < TM; ++i) s[i] = mx_scale((uint32_t) sa[i] & 255u);
+                for (int i = 0; i < TM; ++i) s[i] = mx_scale((uint32_t) f.sa[i] & 255u);
 #pragma unroll
-                for (int h = 0; h < 4; ++h) {
-                    bf16x8 b[TN];
-#pragma unroll
-                    for (int j = 0; j < TN; ++j)
-                        b[j] = *(const bf16x8 *) (sb + ((wn * TN + j) * 16 + r) * C::XROW + ((4 * c + h) ^ r) * 16);
+                for (int h = 0; h < 4; ++h)
 #pragma unroll
                     for (int i = 0; i < TM; ++i) {
-                        const bf16x8 av = mx_decode8_bf16(a[i][h], s[i]);
+                        const bf16x8 av = mx_decode8_bf16(f.a[ks][i][h], s[i]);
 #pragma unroll
-                        for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, b[j], acc[i][j], 0, 0, 0);
+                        for (int j = 0; j < TN; ++j)
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, __builtin_bit_cast(bf16x8, f.b[ks][h * TN + j]), acc[i][j], 0, 0, 0);
                     }
-                }
             }
         }
     };
@@ -461,18 +477,55 @@ __device__ __forceinline__ void mx_gemm_tile(const MxGemm &p, int tiles_m, int t
     if constexpr (CHUNK && R > 2) {
         for (int f = wave; f < C::US; f += NW) scale_load(f, chunks, 0, false);
     }
+    if constexpr (!C::PIPE) {
 #pragma unroll
-    for (int s = 0; s < R - 1; ++s)
-        if (s < nst) issue(s, s);
-    int slot = 0;
-    for (int t = 0; t < nst; ++t) {
-        // this wave's loads of stage t have landed; past the barrier every
-        // wave's have, and every wave has read stage t - 1, whose slot is refilled
-        wait_stages<C::LOADS, R - 2>(nst - 1 - t);
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (t + R - 1 < nst) issue(t + R - 1, slot == 0 ? R - 1 : slot - 1);
-        compute(t, slot);
-        slot = slot + 1 == R ? 0 : slot + 1;
+        for (int s = 0; s < R - 1; ++s)
+            if (s < nst) issue(s, s);
+        int slot = 0;
+        for (int t = 0; t < nst; ++t) {
+            // this wave's loads of stage t have landed; past the barrier every
+            // wave's have, and every wave has read stage t - 1, whose slot is refilled
+            wait_stages<C::LOADS, R - 2>(nst - 1 - t);
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            if (t + R - 1 < nst) issue(t + R - 1, slot == 0 ? R - 1 : slot - 1);
+            Frags f;
+            read(t, slot, f);
+            multiply(f);
+            slot = slot + 1 == R ? 0 : slot + 1;
+        }
+    } else {
+        // stage t is multiplied from registers while stage t + 1 is read from
+        // LDS into the other set
+#pragma unroll
+        for (int s = 0; s < R; ++s)
+            if (s < nst) issue(s, s);
+        Frags f0, f1;
+        wait_stages<C::LOADS, R - 1>(nst - 1);
+        asm volatile("s_barrier" ::: "memory");
+        read(0, 0, f0);
+        int slot = 0;                                          // of stage t
+        auto step = [&](int t, const Frags &now, Frags &next) {
+            // every wave has stage t in registers, whose slot is refilled, and
+            // every wave's loads of stage t + 1 have landed
+            const int s1 = slot + 1 == R ? 0 : slot + 1;
+            wait_stages<C::LOADS, R - 2>(nst - 2 - t);
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            read(t + 1, s1, next);
+            if (t + R < nst) issue(t + R, slot);
+            multiply(now);
+            slot = s1;
+        };
+        int t = 0;
+        for (; t + 2 < nst; t += 2) {
+            step(t, f0, f1);
+            step(t + 1, f1, f0);
+        }
+        if (t + 1 < nst) {
+            step(t, f0, f1);
+            multiply(f1);
+        } else {
+            multiply(f0);
+        }
     }
 #pragma unroll
     for (int i = 0; i < TM; ++i)
@@ -495,11 +548,11 @@ hipError_t launch_tile(const MxGemm &p, hipStream_t s) {
     launch_kernel(mx_gemm_tile_kernel<C>, dim3((unsigned) ((T + 7) / 8 * 8)), dim3(C::NW * 64), C::LDS, s, p, tiles_m, tiles_n);
     return hipGetLastError();
 }
-template <int XT, int WM, int WN, int TM, int TN, int SK, int R>
+template <int XT, int WM, int WN, int TM, int TN, int SK, int R, bool PIPE = false>
 hipError_t launch_tile_k(const MxGemm &p, hipStream_t s) {
-    if (p.K % 128 == 0) return launch_tile<Cfg<XT, WM, WN, TM, TN, SK, R, 16>>(p, s);
-    if (p.K % 64 == 0) return launch_tile<Cfg<XT, WM, WN, TM, TN, SK, R, 2>>(p, s);
-    return launch_tile<Cfg<XT, WM, WN, TM, TN, SK, R - (R > 2), 1>>(p, s);
+    if (p.K % 128 == 0) return launch_tile<Cfg<XT, WM, WN, TM, TN, SK, R, 16, PIPE>>(p, s);
+    if (p.K % 64 == 0) return launch_tile<Cfg<XT, WM, WN, TM, TN, SK, R, 2, PIPE>>(p, s);
+    return launch_tile<Cfg<XT, WM, WN, TM, TN, SK, R - (R > 2), 1, PIPE>>(p, s);
 }
 
 // Shapes, by number (TSK_MX_CFG):
@@ -510,19 +563,20 @@ hipError_t launch_tile_k(const MxGemm &p, hipStream_t s) {
 //   4    64 x 128, 4 waves               the same
 //   5    64 x 32, 4 waves                the same
 //   11   rows kernel, 16 x 16 outputs (f32 activations too, as 12 to 14)
-//   12   32 x 16,  13  32 x 32,  14  64 x 32
+//   12   32 x 16,  13  32 x 32,  14  64 x 32,  15  64 x 16
 //
 // Tiles run in rounds of the 256 CUs (64 x 32: two a CU), so the choice is the
 // shape of the least rounds times the time of one, measured at K = 5120 (us:
-// MXFP4 45, 29, 22, 15, 11; bf16 -, 64, 45, 33, 22 for shapes 1 to 5). Some
+// MXFP4 45, 29, 22, 15, 10; bf16 -, 64, 45, 33, 20 for shapes 1 to 5). Some
 // pairs (us, taken / next): MXFP4, 512 x 5120, K = 2048 128 x 128 11.2 / 15.6;
 // 388 x 4096, K = 1024 64 x 128 6.2 / 7.6; 1292 x 4096, K = 1024 128 x 256 11.2 /
 // 14.3; bf16, 2047 x 2050, K = 5120 256 x 128 (144 tiles) 66 / 128 x 128 (272) 89.
-// Too few tiles of the smallest shape, or at most 32 rows: the rows kernel, the
-// largest of its shapes of which there are 200 (16 rows, M = K = 4096, 128 of 32 x
-// 16 6.3 / 4.7; 1 row, M = K = 8192, 256 of them 9.6 / 11.0). With bf16
-// activations it is the faster one up to more tiles (128 rows, K = 1024, M =
-// 4096, 256 tiles 6.5 / rows 5.8; M = K = 8192, 512 tiles 39 / 56).
+// At most 32 rows, or too few tiles of the smallest shape: the rows kernel
+// (MXFP4, K = 2048, 96 x 3000, 141 tiles 5.2 / rows 6.9; K = 4096, 33 x 4096, 128
+// tiles 7.5 / 7.8, with bf16 activations 14.3 / 12.7), in the largest of its
+// shapes of which there are 200 (16 rows, M = K = 4096, 128 of 32 x 16 6.3 / 4.7;
+// 1 row, M = K = 8192, 256 of them 9.6 / 11.0; bf16, 16 rows, K = 4096, M = 16384
+// 64 x 16 12.1 / 15.1).
 template <int XT>
 int shape_for(const MxGemm &p) {
     if (tuning().mx_cfg) return tuning().mx_cfg;
@@ -531,8 +585,8 @@ int shape_for(const MxGemm &p) {
         constexpr bool MX = XT == X_MX;
         struct Shape { int bm, bn, a_round, us; };
         constexpr Shape shapes[5] = {{256, 256, 256, MX ? 45 : 0}, {MX ? 128 : 256, MX ? 256 : 128, 256, MX ? 29 : 64},
-                                     {128, 128, 256, MX ? 22 : 45}, {64, 128, 256, MX ? 15 : 33}, {64, 32, 512, MX ? 11 : 22}};
-        if (p.N > 32 && tiles(64, 32) >= (MX ? 150 : 300)) {
+                                     {128, 128, 256, MX ? 22 : 45}, {64, 128, 256, MX ? 15 : 33}, {64, 32, 512, MX ? 10 : 20}};
+        if (p.N > 32 && tiles(64, 32) >= 130) {
             int best = 0;
             int64_t least = 0;
             for (int i = MX ? 0 : 1; i < 5; ++i) {
@@ -546,6 +600,7 @@ int shape_for(const MxGemm &p) {
             return best;
         }
     }
+    if (p.N <= 16) return tiles(64, 16) >= 200 ? 15 : tiles(32, 16) >= 200 ? 12 : 11;
     return tiles(64, 32) >= 200 ? 14 : tiles(32, 32) >= 200 ? 13 : tiles(32, 16) >= 200 ? 12 : 11;
 }
 
@@ -565,11 +620,12 @@ hipError_t launch_kind(const MxGemm &p, hipStream_t s) {
             case 3: if constexpr (MX) return launch_tile_k<XT, 2, 4, 4, 2, 8, 4>(p, s);
                     else return launch_tile_k<XT, 4, 2, 2, 4, 4, 3>(p, s);
             case 4: return launch_tile_k<XT, 2, 2, 2, 4, MX ? 8 : 4, MX ? 5 : 4>(p, s);
-            case 5: return launch_tile_k<XT, 4, 1, 1, 2, MX ? 8 : 4, 5>(p, s);
+            case 5: return launch_tile_k<XT, 4, 1, 1, 2, MX ? 8 : 4, 5, true>(p, s);
         }
     }
     switch (shape) {
         case 14: return launch_rows<XT, 4, 2, 4>(p, s);
+        case 15: return launch_rows<XT, 4, 1, 4>(p, s);
         case 13: return launch_rows<XT, 2, 2, 4>(p, s);
         case 12: return launch_rows<XT, 2, 1, 4>(p, s);
         default: return launch_rows<XT, 1, 1, 4>(p, s);
