@@ -287,10 +287,11 @@ struct Cfg {
     // loads of a wave per stage: 64 lanes x 16 bytes of codes or bf16, x 4 bytes of scales
     static constexpr int UA = A_BYTES / 1024, UB = B_BYTES / 1024, US = CHUNK ? SROWS / 32 : S_BYTES / 256;
     static constexpr int USP = CHUNK && R > 2 ? (US + CS - 1) / CS : US;   // scale loads with one stage
-    static constexpr int LA = UA / NW, LB = UB / NW, LS = (USP + NW - 1) / NW;
+    // (a wave without a load of its own repeats another's: the waits count the same for all)
+    static constexpr int LA = (UA + NW - 1) / NW, LB = (UB + NW - 1) / NW, LS = (USP + NW - 1) / NW;
     static constexpr int LOADS = LA + LB + LS;
     static constexpr size_t LDS = (size_t) R * STAGE + CHUNKS * CHUNK_BYTES;
-    static_assert(NW % 4 == 0 && UA % NW == 0 && UB % NW == 0 && R >= 2 && R <= 5 && LOADS * (R - 1) < 64 && LDS <= 160 * 1024, "tile");
+    static_assert(NW % 4 == 0 && UA % 4 == 0 && UB % 4 == 0 && R >= 2 && R <= 5 && LOADS * (R - 1) < 64 && LDS <= 160 * 1024, "tile");
 };
 
 template <class C>
@@ -332,7 +333,7 @@ __device__ __forceinline__ void mx_gemm_tile(const MxGemm &p, int tiles_m, int t
     const int a_chk = (lane % SK) ^ key(wave * AR + lane / SK);                // (a wave's loads are NW, a multiple of 4, apart)
     int a_off[C::LA];
 #pragma unroll
-    for (int q = 0; q < C::LA; ++q) a_off[q] = ((wave + NW * q) * AR + lane / SK) * K2 + a_chk * 16;
+    for (int q = 0; q < C::LA; ++q) a_off[q] = ((wave + NW * q) % C::UA * AR + lane / SK) * K2 + a_chk * 16;
     // bf16 rows: 16 chunks, 4 rows a load, chunk c of row t at slot c ^ (t % 16)
     static_assert(MX || SK == 4, "bf16 rows of 256 bytes");
     constexpr int BC = MX ? SK : 4 * SK, BR = 64 / BC;
@@ -340,7 +341,7 @@ __device__ __forceinline__ void mx_gemm_tile(const MxGemm &p, int tiles_m, int t
     const int b_chk = (lane % BC) ^ (MX ? key(b_row) : b_row & 15), b_blk = MX ? b_chk : b_chk / 4;
     int b_off[C::LB];
 #pragma unroll
-    for (int q = 0; q < C::LB; ++q) b_off[q] = (int) ((b_row + NW * q * BR) * xrow) + b_chk * 16;
+    for (int q = 0; q < C::LB; ++q) b_off[q] = (int) (((wave + NW * q) % C::UB * BR + lane / BC) * xrow) + b_chk * 16;
     // scales with their stage: SCB bytes a lane, zero-extended to a dword; chunks: 16 bytes of a row's 32
     constexpr int SL = CHUNK ? 2 : SK / SCB, SR = 64 / SL;
     const int s_row = lane / SL, s_blk = lane % SL * SCB, s_off = s_row * KB + s_blk;
@@ -365,10 +366,10 @@ __device__ __forceinline__ void mx_gemm_tile(const MxGemm &p, int tiles_m, int t
         }
 #pragma unroll
         for (int q = 0; q < C::LA; ++q)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_void *) (st + (wave + NW * q) * 1024), 16, a_off[q], t * (SK * 16), 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_void *) (st + (wave + NW * q) % C::UA * 1024), 16, a_off[q], t * (SK * 16), 0, 0);
 #pragma unroll
         for (int q = 0; q < C::LB; ++q)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_void *) (st + C::A_BYTES + (wave + NW * q) * 1024), 16, b_off[q],
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_void *) (st + C::A_BYTES + (wave + NW * q) % C::UB * 1024), 16, b_off[q],
                                                      t * C::XROW, 0, 0);
         if constexpr (!CHUNK) {
 #pragma unroll
@@ -555,22 +556,26 @@ hipError_t launch_tile_k(const MxGemm &p, hipStream_t s) {
     return launch_tile<Cfg<XT, WM, WN, TM, TN, SK, R - (R > 2), 1, PIPE>>(p, s);
 }
 
-// Shapes, by number (TSK_MX_CFG):
+// Shapes, by number (TSK_MX_CFG), and the us of a round of their tiles at K = 5120:
 //        both operands MXFP4             bf16 activations
-//   1    256 x 256, 8 waves              -
-//   2    128 x 256, 8 waves              256 x 128, 8 waves
-//   3    128 x 128, 8 waves              the same
-//   4    64 x 128, 4 waves               the same
-//   5    64 x 32, 4 waves                the same
-//   11   rows kernel, 16 x 16 outputs (f32 activations too, as 12 to 14)
+//   1    256 x 256, 8 waves     45       -
+//   2    128 x 256, 8 waves     29       256 x 128, 8 waves    64
+//   3    128 x 128, 8 waves     22       the same              45
+//   4    64 x 128, 4 waves      15       the same              33
+//   5    64 x 32, 4 waves       10       the same              20
+//   6    192 x 128, 8 waves     25       the same              55
+//   7    128 x 192, 8 waves     26       the same              55
+//   8    192 x 256, 8 waves     35       -
+//   11   rows kernel, 16 x 16 outputs (f32 activations too, as 12 to 15)
 //   12   32 x 16,  13  32 x 32,  14  64 x 32,  15  64 x 16
 //
 // Tiles run in rounds of the 256 CUs (64 x 32: two a CU), so the choice is the
-// shape of the least rounds times the time of one, measured at K = 5120 (us:
-// MXFP4 45, 29, 22, 15, 10; bf16 -, 64, 45, 33, 20 for shapes 1 to 5). Some
-// pairs (us, taken / next): MXFP4, 512 x 5120, K = 2048 128 x 128 11.2 / 15.6;
-// 388 x 4096, K = 1024 64 x 128 6.2 / 7.6; 1292 x 4096, K = 1024 128 x 256 11.2 /
-// 14.3; bf16, 2047 x 2050, K = 5120 256 x 128 (144 tiles) 66 / 128 x 128 (272) 89.
+// shape of the least rounds times the time of one. Some pairs (us, taken /
+// next; outputs as rows x M): MXFP4, 512 x 5120, K = 2048 128 x 128 11.2 / 15.6;
+// 388 x 4096, K = 1024 64 x 128 6.2 / 7.6; 1292 x 4096, K = 1024 192 x 128 10.2 /
+// 128 x 256 11.2; 2047 x 2050, K = 5120 192 x 128 (176 tiles) 25.4 / 128 x 256 (144)
+// 28.7 / 128 x 128 (272) 40.7, with bf16 activations 54.9 / 63.7 / 87.4; 4096 x 4096,
+// K = 5120 256 x 256 56 / 192 x 128 75.
 // At most 32 rows, or too few tiles of the smallest shape: the rows kernel
 // (MXFP4, K = 2048, 96 x 3000, 141 tiles 5.2 / rows 6.9; K = 4096, 33 x 4096, 128
 // tiles 7.5 / 7.8, with bf16 activations 14.3 / 12.7), in the largest of its
@@ -584,12 +589,13 @@ int shape_for(const MxGemm &p) {
     if constexpr (XT != X_F32) {
         constexpr bool MX = XT == X_MX;
         struct Shape { int bm, bn, a_round, us; };
-        constexpr Shape shapes[5] = {{256, 256, 256, MX ? 45 : 0}, {MX ? 128 : 256, MX ? 256 : 128, 256, MX ? 29 : 64},
-                                     {128, 128, 256, MX ? 22 : 45}, {64, 128, 256, MX ? 15 : 33}, {64, 32, 512, MX ? 10 : 20}};
+        constexpr Shape shapes[8] = {{256, 256, 256, 45}, {MX ? 128 : 256, MX ? 256 : 128, 256, MX ? 29 : 64},
+                                     {128, 128, 256, MX ? 22 : 45}, {64, 128, 256, MX ? 15 : 33}, {64, 32, 512, MX ? 10 : 20},
+                                     {192, 128, 256, MX ? 25 : 55}, {128, 192, 256, MX ? 26 : 55}, {192, 256, 256, 35}};
         if (p.N > 32 && tiles(64, 32) >= 130) {
             int best = 0;
             int64_t least = 0;
-            for (int i = MX ? 0 : 1; i < 5; ++i) {
+            for (int i = MX ? 0 : 1; i < (MX ? 8 : 7); ++i) {
                 const Shape &c = shapes[i];
                 const int64_t cost = (tiles(c.bm, c.bn) + c.a_round - 1) / c.a_round * c.us;
                 if (!best || cost < least) {
@@ -621,6 +627,10 @@ hipError_t launch_kind(const MxGemm &p, hipStream_t s) {
                     else return launch_tile_k<XT, 4, 2, 2, 4, 4, 3>(p, s);
             case 4: return launch_tile_k<XT, 2, 2, 2, 4, MX ? 8 : 4, MX ? 5 : 4>(p, s);
             case 5: return launch_tile_k<XT, 4, 1, 1, 2, MX ? 8 : 4, 5, true>(p, s);
+            case 6: return launch_tile_k<XT, 4, 2, 3, 4, MX ? 8 : 4, MX ? 3 : 2>(p, s);
+            case 7: if constexpr (MX) return launch_tile_k<XT, 2, 4, 4, 3, 8, 3>(p, s);
+                    else return launch_tile_k<XT, 4, 2, 2, 6, 4, 2>(p, s);
+            case 8: if constexpr (MX) return launch_tile_k<XT, 2, 4, 6, 4, 8, 2>(p, s);
         }
     }
     switch (shape) {
