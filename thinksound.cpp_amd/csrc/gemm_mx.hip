@@ -3,7 +3,17 @@
 //   Y[n, m] = sum_k X[n, k] W[m, k] + bias[m],   W = codes * 2^(scale - 127) per 32 k,
 //
 // with X in bf16 (or f32, rounded to bf16 as it is read), or X in MXFP4 too.
+// Sums are f32. With bf16 X a code times its scale is a bf16 number exactly
+// (the conversion instruction takes the scale), so v_mfma_f32_16x16x32_bf16
+// adds exact products; with MXFP4 X v_mfma_scale_f32_16x16x128_f8f6f4 takes
+// codes and scale bytes as they lie in memory.
+//
+// Bound: few rows by the weights' bytes (8 x 8192, K = 8192 12.6 us, 2.8 TB/s);
+// many rows by the matrix units, LDS and power together: 8192 x 8192, K = 8192
+// 300 us with MXFP4 X (3.7 PFLOP/s; products alone, without their loads, take
+// 200), 850 us with bf16 X (1.30 PFLOP/s).
 #include <algorithm>
+#include <utility>
 
 #include "mxfp4.h"
 #include "tsk_internal.h"
@@ -48,7 +58,9 @@ enum : int { X_BF16 = 0, X_F32 = 1, X_MX = 2 };
 // wave order. Lane l holds row l % 16 of either operand and of each 128 k the
 // block of 32 number l / 16: the layout of v_mfma_scale_f32_16x16x128_f8f6f4,
 // and with the k of four v_mfma_f32_16x16x32_bf16 taken in the same order on
-// both sides, of those.
+// both sides, of those. Bound by the weights' bytes and the latency of the first
+// loads: each wave keeps the loads of its next turn in flight (8 x 8192, K = 8192
+// 12.6 us, 2.8 TB/s; 1 x 6144, K = 1024 4.0 us); 8 and 16 waves are no faster.
 template <int XT, int MT, int NT>
 struct RowFrags {
     static constexpr int BQ = XT == X_MX ? 1 : XT == X_BF16 ? 4 : 8;       // 16-byte pieces of an activation block
@@ -240,17 +252,6 @@ __device__ __forceinline__ void wait_vm() {
     static_assert(N >= 0 && N < 64, "vmcnt range");
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
-// at most `rem` stages of L loads in flight, and MOST at all
-template <int L, int MOST>
-__device__ __forceinline__ void wait_stages(int rem) {
-    if constexpr (MOST >= 1) {
-        if (rem >= MOST) wait_vm<MOST * L>();
-        else wait_stages<L, MOST - 1>(rem);
-    } else {
-        wait_vm<0>();
-    }
-}
-
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc_of(const void *base, int64_t bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), (short) 0, (int) bytes, 0x00020000);
 }
@@ -265,14 +266,26 @@ __device__ __forceinline__ void load_scales(__amdgpu_buffer_rsrc_t rsrc, uint8_t
 // Tiles. WM x WN waves share a BM x BN output tile, each TM x TN sub-tiles of
 // 16 x 16, over stages of SK blocks of 32 k in a ring of R stages of LDS.
 // Scales (SCB bytes a load and lane): with SCB = 16 in chunks of 1024 k beside
-// the ring (rows of scale bytes dword-aligned, K % 128 == 0), else with their stage.
-template <int XT_, int WM_, int WN_, int TM_, int TN_, int SK_, int R_, int SCB_, bool PIPE_>
+// the ring (rows of scale bytes dword-aligned, K % 128 == 0; a stage's own few
+// bytes cost as many L2 requests as its codes: 8192^3 357 us against 326), else
+// with their stage.
+//
+// A stage takes from LDS, per wave, TM + TN pieces of 1 KB each 128 k (128 bytes
+// a clock and CU), from L2 64 bytes a clock, from the matrix unit 16 clocks an
+// instruction. In turns these add up; so each product is followed by at most a
+// read of what the next ones take and a load of a later stage, in the program's
+// order (sched_barrier). HALVES: the first half of a stage's products reads
+// the second half's operands, the second half the next stage's first, with the
+// one barrier of a stage inside it. Otherwise (one row of sub-tiles a wave: too
+// few products a half to hide a read) a whole stage is read while the one before
+// is multiplied. Measured (us): all reads before the products, loads before the
+// reads 8192^3 320-333, 4096 x 4096, K = 5120 56; whole stages in order, 128 x 256
+// tiles 8192^3 397, halves 322; halves, 256 x 256 tiles 302 and 51; 64 x 32 tiles,
+// 1292 x 1024, K = 4096 halves 16.2, whole 14.4.
+template <int XT_, int WM_, int WN_, int TM_, int TN_, int SK_, int R_, int SCB_, bool HALVES_>
 struct Cfg {
-    // PIPE: a stage's fragments are read from LDS while the stage before is
-    // multiplied. It pays where a wave holds few (64 x 32: 388 x 1024, K = 4096 8.8 ->
-    // 7.7 us); at 64 x 128 it changes nothing, and larger tiles lack the registers.
-    static constexpr bool PIPE = PIPE_;
     static constexpr int XT = XT_, WM = WM_, WN = WN_, TM = TM_, TN = TN_, SK = SK_, R = R_, SCB = SCB_;
+    static constexpr bool HALVES = HALVES_;
     static constexpr int NW = WM * WN, BM = WM * TM * 16, BN = WN * TN * 16;
     static constexpr bool MX = XT == X_MX, CHUNK = SCB == 16;
     static constexpr int XROW = MX ? SK * 16 : SK * 64;                    // bytes of an activation row per stage
@@ -281,18 +294,24 @@ struct Cfg {
     // LDS of a stage: weight codes, activations, weight scales, activation scales
     static constexpr int A_BYTES = BM * SK * 16, B_BYTES = BN * XROW, S_BYTES = SROWS * SROW;
     static constexpr int STAGE = A_BYTES + B_BYTES + S_BYTES;
-    // chunks: CS stages each; a ring of two stages loads a chunk whole with its
-    // first stage, a longer one a part with every stage, one chunk ahead
+    // chunks: CS stages each, a part loaded with every stage: with a ring of two
+    // stages from a chunk's first stage on, when the chunk before the one that is
+    // read has been read, longer ones one stage earlier and into a third buffer
     static constexpr int CS = 32 / SK, CHUNK_BYTES = CHUNK ? SROWS * 32 : 0, CHUNKS = !CHUNK ? 0 : R == 2 ? 2 : 3;
     // loads of a wave per stage: 64 lanes x 16 bytes of codes or bf16, x 4 bytes of scales
     static constexpr int UA = A_BYTES / 1024, UB = B_BYTES / 1024, US = CHUNK ? SROWS / 32 : S_BYTES / 256;
-    static constexpr int USP = CHUNK && R > 2 ? (US + CS - 1) / CS : US;   // scale loads with one stage
+    static constexpr int USP = CHUNK ? (US + CS - 1) / CS : US;   // scale loads with one stage
     // (a wave without a load of its own repeats another's: the waits count the same for all)
     static constexpr int LA = (UA + NW - 1) / NW, LB = (UB + NW - 1) / NW, LS = (USP + NW - 1) / NW;
     static constexpr int LOADS = LA + LB + LS;
     static constexpr size_t LDS = (size_t) R * STAGE + CHUNKS * CHUNK_BYTES;
     static_assert(NW % 4 == 0 && UA % 4 == 0 && UB % 4 == 0 && R >= 2 && R <= 5 && LOADS * (R - 1) < 64 && LDS <= 160 * 1024, "tile");
 };
+
+// f(0), ..., f(N - 1), the arguments constants
+template <class F, int... I>
+__device__ __forceinline__ void each(F f, std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>{}), ...); }
+#define EACH(q, from, to, ...) each([&](auto q##_) __attribute__((always_inline)) { constexpr int q = decltype(q##_)::value + (from); __VA_ARGS__ }, std::make_integer_sequence<int, ((to) > (from) ? (to) - (from) : 0)>{})
 
 template <class C>
 __device__ __forceinline__ void mx_gemm_tile(const MxGemm &p, int tiles_m, int tiles_n, uint8_t *lds) {
@@ -311,7 +330,7 @@ __device__ __forceinline__ void mx_gemm_tile(const MxGemm &p, int tiles_m, int t
     const int r = lane & 15, g = lane >> 4, wm = wave % C::WM, wn = wave / C::WM;
     const int m0 = tm * C::BM, n0 = tn * C::BN;
     const int K2 = p.K / 2, KB = p.K / 32;
-    const int nst = (KB + SK - 1) / SK, kv = KB - (nst - 1) * SK;              // blocks of the last stage
+    const int nst = (KB + SK - 1) / SK;
 
     // Rows past M or N are past the descriptors' ends by the lane's own offset:
     // the loads put zeros there. So do blocks past K, sent FAR with the last
@@ -331,17 +350,11 @@ __device__ __forceinline__ void mx_gemm_tile(const MxGemm &p, int tiles_m, int t
     constexpr int AR = 64 / SK;
     auto key = [](int row) { return SK == 8 ? row >> 1 & 7 : row >> 2 & 3; };
     const int a_chk = (lane % SK) ^ key(wave * AR + lane / SK);                // (a wave's loads are NW, a multiple of 4, apart)
-    int a_off[C::LA];
-#pragma unroll
-    for (int q = 0; q < C::LA; ++q) a_off[q] = ((wave + NW * q) % C::UA * AR + lane / SK) * K2 + a_chk * 16;
     // bf16 rows: 16 chunks, 4 rows a load, chunk c of row t at slot c ^ (t % 16)
     static_assert(MX || SK == 4, "bf16 rows of 256 bytes");
     constexpr int BC = MX ? SK : 4 * SK, BR = 64 / BC;
     const int b_row = wave * BR + lane / BC;
     const int b_chk = (lane % BC) ^ (MX ? key(b_row) : b_row & 15), b_blk = MX ? b_chk : b_chk / 4;
-    int b_off[C::LB];
-#pragma unroll
-    for (int q = 0; q < C::LB; ++q) b_off[q] = (int) (((wave + NW * q) % C::UB * BR + lane / BC) * xrow) + b_chk * 16;
     // scales with their stage: SCB bytes a lane, zero-extended to a dword; chunks: 16 bytes of a row's 32
     constexpr int SL = CHUNK ? 2 : SK / SCB, SR = 64 / SL;
     const int s_row = lane / SL, s_blk = lane % SL * SCB, s_off = s_row * KB + s_blk;
@@ -355,38 +368,39 @@ __device__ __forceinline__ void mx_gemm_tile(const MxGemm &p, int tiles_m, int t
         if constexpr (CHUNK) __builtin_amdgcn_raw_ptr_buffer_load_lds(b ? rsb : rsa, (lds_void *) (dst + f * 1024), 16, off, 0, 0, 0);
         else load_scales<C::SCB>(b ? rsb : rsa, dst + f * 256, off);
     };
-    auto issue = [&](int t, int slot) {
+    // a lane's own parts of these offsets. The loop takes them as new in every
+    // stage, or the compiler keeps each load's whole offset in a register.
+    int a_lane = lane / SK * K2 + a_chk * 16, b_lane = (int) (lane / BC * xrow) + b_chk * 16;
+    int a_at = r * (SK * 16) + ((SK / 4 * g) ^ key(r)) * 16, s_at;
+    if constexpr (CHUNK) s_at = r * 32 + (SK == 8 ? 2 * g : g);
+    else if constexpr (SK == 8) s_at = r * C::SROW + (SCB == 2 ? 4 : 8) * g;
+    else s_at = r * C::SROW + (SCB == 2 ? (g >> 1) * 4 + (g & 1) : 4 * g);
+    // load q of this wave's for stage t (stages past the last: zeros, so that every wait counts the same)
+    auto issue_one = [&](int t, int slot, int q) __attribute__((always_inline)) {
         uint8_t *st = lds + slot * C::STAGE;
-        const bool last = t == nst - 1;
-        if (last && kv < SK) {
-#pragma unroll
-            for (int q = 0; q < C::LA; ++q) a_off[q] = a_chk >= kv ? FAR : a_off[q];
-#pragma unroll
-            for (int q = 0; q < C::LB; ++q) b_off[q] = b_blk >= kv ? FAR : b_off[q];
-        }
-#pragma unroll
-        for (int q = 0; q < C::LA; ++q)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_void *) (st + (wave + NW * q) % C::UA * 1024), 16, a_off[q], t * (SK * 16), 0, 0);
-#pragma unroll
-        for (int q = 0; q < C::LB; ++q)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_void *) (st + C::A_BYTES + (wave + NW * q) % C::UB * 1024), 16, b_off[q],
+        const int blk = t * SK;
+        if (q < C::LA) {
+            const int u = (wave + NW * q) % C::UA;
+            const int off = u * (AR * K2) + a_lane;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_void *) (st + u * 1024), 16, blk + a_chk < KB ? off : FAR, blk * 16, 0, 0);
+        } else if (q < C::LA + C::LB) {
+            const int u = (wave + NW * (q - C::LA)) % C::UB;
+            const int off = u * (int) (BR * xrow) + b_lane;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_void *) (st + C::A_BYTES + u * 1024), 16, blk + b_blk < KB ? off : FAR,
                                                      t * C::XROW, 0, 0);
-        if constexpr (!CHUNK) {
-#pragma unroll
-            for (int q = 0; q < C::LS; ++q)
-                scale_load((wave + NW * q) % C::US, st + C::A_BYTES + C::B_BYTES, t * SK, last && s_blk >= kv);
-        } else if constexpr (R == 2) {
-            if (t % C::CS == 0) {
-#pragma unroll
-                for (int q = 0; q < C::LS; ++q)
-                    scale_load((wave + NW * q) % C::US, chunks + (t / C::CS & 1) * C::CHUNK_BYTES, t * SK, false);
-            }
         } else {
-            const int c = t / C::CS + 1;
-#pragma unroll
-            for (int q = 0; q < C::LS; ++q)
-                scale_load(((t % C::CS) * C::USP + (wave + NW * q) % C::USP) % C::US, chunks + c % 3 * C::CHUNK_BYTES, c * 32, false);
+            const int u = wave + NW * (q - C::LA - C::LB);
+            if constexpr (!CHUNK) {
+                scale_load(u % C::US, st + C::A_BYTES + C::B_BYTES, blk, blk + s_blk >= KB);
+            } else {
+                const int w = t + (R == 2 ? C::CS - 1 : C::CS), c = w / C::CS;
+                scale_load(((w % C::CS) * C::USP + u % C::USP) % C::US, chunks + c % C::CHUNKS * C::CHUNK_BYTES, c * 32, false);
+            }
         }
+    };
+    auto issue = [&](int t, int slot) {
+#pragma unroll
+        for (int q = 0; q < C::LOADS; ++q) issue_one(t, slot, q);
     };
 
     f32x4 acc[TM][TN];
@@ -396,138 +410,128 @@ __device__ __forceinline__ void mx_gemm_tile(const MxGemm &p, int tiles_m, int t
         for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
 
     // step ks of a stage: lane group g takes block SK / 4 * g + ks of every row
-    const int akey = key(r);
-    // the scale bytes of this lane's blocks of a stage, byte ks for step ks
-    auto scale_at = [&](const uint8_t *base, int row) -> int {
-        const uint8_t *q = base + row * (CHUNK ? 32 : C::SROW);
-        if constexpr (CHUNK) return SK == 8 ? *(const uint16_t *) (q + 2 * g) : q[g];
-        else if constexpr (SK == 8) return SCB == 2 ? *(const int *) (q + 4 * g) : q[8 * g] | q[8 * g + 4] << 8;
-        else return SCB == 2 ? q[(g >> 1) * 4 + (g & 1)] : q[4 * g];
+    // the scale bytes of this lane's blocks of a stage, byte ks for step ks: base at its row 16 u
+    auto scale_at = [&](const uint8_t *base, int u) __attribute__((always_inline)) -> int {
+        const uint8_t *q = base + u * (CHUNK ? 512 : 16 * C::SROW) + s_at;
+        if constexpr (CHUNK) return SK == 8 ? *(const uint16_t *) q : *q;
+        else if constexpr (SK == 8) return SCB == 2 ? *(const int *) q : q[0] | q[4] << 8;
+        else return *q;
     };
     constexpr int KS = SK / 4;
     struct Frags {
         u32x4 a[KS][TM], b[KS][MX ? TN : 4 * TN];
         int sa[TM], sx[MX ? TN : 1];
     };
-    auto read = [&](int t, int slot, Frags &f) {
+    // read q of a stage's fragments
+    constexpr int NSC = TM + (MX ? TN : 0), NKS = TM + (MX ? TN : 4 * TN), NR = NSC + KS * NKS;
+    auto read_one = [&](int t, int slot, Frags &f, int q) __attribute__((always_inline)) {
         const uint8_t *st = lds + slot * C::STAGE, *sb = st + C::A_BYTES;
-        const uint8_t *ss = CHUNK ? chunks + t / C::CS % C::CHUNKS * C::CHUNK_BYTES + t % C::CS * SK : sb + C::B_BYTES;
-#pragma unroll
-        for (int i = 0; i < TM; ++i) f.sa[i] = scale_at(ss, (wm * TM + i) * 16 + r);
+        if (q < NSC) {
+            const uint8_t *ss = CHUNK ? chunks + t / C::CS % C::CHUNKS * C::CHUNK_BYTES + t % C::CS * SK : sb + C::B_BYTES;
+            const bool x = q >= TM;
+            if (x) f.sx[MX ? q - TM : 0] = scale_at(ss, C::BM / 16 + wn * TN + q - TM);
+            else f.sa[q] = scale_at(ss, wm * TM + q);
+            return;
+        }
+        // what the first half of the products takes, then the rest of the second; activations first
         if constexpr (MX) {
-#pragma unroll
-            for (int j = 0; j < TN; ++j) f.sx[j] = scale_at(ss, C::BM + (wn * TN + j) * 16 + r);
-        }
-        if (CHUNK && t == nst - 1) {                              // (no scales past K)
-            const int b0 = SK / 4 * g, msk = (b0 < kv ? 0xff : 0) | (b0 + 1 < kv ? 0xff00 : 0);
-#pragma unroll
-            for (int i = 0; i < TM; ++i) f.sa[i] &= msk;
-            if constexpr (MX) {
-#pragma unroll
-                for (int j = 0; j < TN; ++j) f.sx[j] &= msk;
-            }
-        }
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            const int c = KS * g + ks;
-#pragma unroll
-            for (int i = 0; i < TM; ++i) f.a[ks][i] = *(const u32x4 *) (st + ((wm * TM + i) * 16 + r) * (SK * 16) + (c ^ akey) * 16);
-            if constexpr (MX) {
-#pragma unroll
-                for (int j = 0; j < TN; ++j) f.b[ks][j] = *(const u32x4 *) (sb + ((wn * TN + j) * 16 + r) * (SK * 16) + (c ^ akey) * 16);
-            } else {
-#pragma unroll
-                for (int h = 0; h < 4; ++h)
-#pragma unroll
-                    for (int j = 0; j < TN; ++j)
-                        f.b[ks][h * TN + j] = *(const u32x4 *) (sb + ((wn * TN + j) * 16 + r) * C::XROW + ((4 * c + h) ^ r) * 16);
-            }
+            const int ks = (q - NSC) / NKS, u = (q - NSC) % NKS;
+            if (u < TN) f.b[ks][u] = *(const u32x4 *) (sb + (wn * TN + u) * (16 * SK * 16) + (a_at ^ 16 * ks));
+            else f.a[ks][u - TN] = *(const u32x4 *) (st + (wm * TM + u - TN) * (16 * SK * 16) + (a_at ^ 16 * ks));
+        } else {
+            const int u = q - NSC, a = u - 2 * TN, h = u < 2 * TN ? u : u - TM;
+            if (a >= 0 && a < TM) f.a[0][a] = *(const u32x4 *) (st + (wm * TM + a) * (16 * SK * 16) + a_at);
+            else f.b[0][h] = *(const u32x4 *) (sb + ((wn * TN + h % TN) * 16 + r) * C::XROW + ((4 * g + h / TN) ^ r) * 16);
         }
     };
-    auto multiply = [&](const Frags &f) {
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            if constexpr (MX) {
-#pragma unroll
-                for (int i = 0; i < TM; ++i)
-#pragma unroll
-                    for (int j = 0; j < TN; ++j) {
-                        const u32x4 &a = f.a[ks][i], &b = f.b[ks][j];
-                        const i32x8 av = {(int) a[0], (int) a[1], (int) a[2], (int) a[3], 0, 0, 0, 0};
-                        const i32x8 bv = {(int) b[0], (int) b[1], (int) b[2], (int) b[3], 0, 0, 0, 0};
-                        if (ks == 1) acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, acc[i][j], 4, 4, 1, f.sa[i], 1, f.sx[j]);
-                        else acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, acc[i][j], 4, 4, 0, f.sa[i], 0, f.sx[j]);
-                    }
-            } else {
-                float s[TM];
-#pragma unroll
-                for (int i = 0; i < TM; ++i) s[i] = mx_scale((uint32_t) f.sa[i] & 255u);
-#pragma unroll
-                for (int h = 0; h < 4; ++h)
-#pragma unroll
-                    for (int i = 0; i < TM; ++i) {
-                        const bf16x8 av = mx_decode8_bf16(f.a[ks][i][h], s[i]);
-#pragma unroll
-                        for (int j = 0; j < TN; ++j)
-                            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, __builtin_bit_cast(bf16x8, f.b[ks][h * TN + j]), acc[i][j], 0, 0, 0);
-                    }
-            }
+    constexpr int NR0 = MX ? NSC + NKS : NSC + 2 * TN + TM;               // reads of the first half
+    // chunks hold the next row's scales past K (K % 128 == 0: past K for all of a lane group's blocks or none)
+    auto scales_of = [&](int t, Frags &f) __attribute__((always_inline)) {
+        if constexpr (CHUNK) {
+            const int in = t * SK + KS * g < KB ? -1 : 0;
+            EACH(q, 0, TM, f.sa[q] &= in;);
+            if constexpr (MX) EACH(q, 0, TN, f.sx[q] &= in;);
+        }
+    };
+    // product q of a stage
+    constexpr int NM = (MX ? KS : 4) * TM * TN;
+    bf16x8 av;
+    auto multiply_one = [&](const Frags &f, int q) __attribute__((always_inline)) {
+        const int ks = q / (TM * TN), i = q / TN % TM, j = q % TN;
+        if constexpr (MX) {
+            const u32x4 &a = f.a[ks][i], &b = f.b[ks][j];
+            const i32x8 av = {(int) a[0], (int) a[1], (int) a[2], (int) a[3], 0, 0, 0, 0};
+            const i32x8 bv = {(int) b[0], (int) b[1], (int) b[2], (int) b[3], 0, 0, 0, 0};
+            if (ks == 1) acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, acc[i][j], 4, 4, 1, f.sa[i], 1, f.sx[j]);
+            else acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, acc[i][j], 4, 4, 0, f.sa[i], 0, f.sx[j]);
+        } else {
+            if (j == 0) av = mx_decode8_bf16(f.a[0][i][ks], mx_scale((uint32_t) f.sa[i] & 255u));
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, __builtin_bit_cast(bf16x8, f.b[0][ks * TN + j]), acc[i][j], 0, 0, 0);
         }
     };
 
-    if constexpr (CHUNK && R > 2) {
+    if constexpr (CHUNK) {
         for (int f = wave; f < C::US; f += NW) scale_load(f, chunks, 0, false);
     }
-    if constexpr (!C::PIPE) {
 #pragma unroll
-        for (int s = 0; s < R - 1; ++s)
-            if (s < nst) issue(s, s);
-        int slot = 0;
-        for (int t = 0; t < nst; ++t) {
-            // this wave's loads of stage t have landed; past the barrier every
-            // wave's have, and every wave has read stage t - 1, whose slot is refilled
-            wait_stages<C::LOADS, R - 2>(nst - 1 - t);
-            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            if (t + R - 1 < nst) issue(t + R - 1, slot == 0 ? R - 1 : slot - 1);
-            Frags f;
-            read(t, slot, f);
-            multiply(f);
-            slot = slot + 1 == R ? 0 : slot + 1;
+    for (int s = 0; s < R; ++s) issue(s, s);
+    Frags f0;
+    wait_vm<(R - 1) * C::LOADS>();
+    asm volatile("s_barrier" ::: "memory");
+    EACH(q, 0, (C::HALVES ? NR0 : NR), read_one(0, 0, f0, q););
+    scales_of(0, f0);
+    int slot = 0;                                                              // of stage t
+    // `fill` after it every wave has stage t in registers, whose slot is
+    // refilled, and every wave's loads of stage t + 1 have landed
+    auto fill = [&]() __attribute__((always_inline)) {
+        wait_vm<(R - 2) * C::LOADS>();
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    };
+    auto step = [&](int t, Frags &now, Frags &next) __attribute__((always_inline)) {
+        const int s1 = slot + 1 == R ? 0 : slot + 1;
+        asm volatile("" : "+v"(a_lane), "+v"(b_lane), "+v"(a_at), "+v"(s_at));
+        if constexpr (C::HALVES) {
+            constexpr int H = NM / 2, GB = TM / 4 * TN * (MX ? 1 : 2), H0 = TM < 8 ? (3 * H + 3) / 4 : H, N1 = NR - NR0, H1 = H - GB;
+            EACH(q, 0, H,
+                multiply_one(now, q);
+                EACH(u, q * N1 / H0, (q + 1) * N1 / H0 < N1 ? (q + 1) * N1 / H0 : N1, read_one(t, slot, now, NR0 + u););
+                __builtin_amdgcn_sched_barrier(0););
+            EACH(q, 0, GB, multiply_one(now, H + q););
+            __builtin_amdgcn_sched_barrier(0);
+            fill();
+            EACH(q, 0, H1,
+                multiply_one(now, H + GB + q);
+                EACH(u, q * NR0 / H1, (q + 1) * NR0 / H1, read_one(t + 1, s1, next, u););
+                EACH(u, q * C::LOADS / H1, (q + 1) * C::LOADS / H1, issue_one(t + R, slot, u););
+                __builtin_amdgcn_sched_barrier(0););
+        } else {
+            constexpr int H0 = NM * 3 / 4;
+            fill();
+            EACH(q, 0, NM,
+                multiply_one(now, q);
+                EACH(u, q * NR / H0, (q + 1) * NR / H0 < NR ? (q + 1) * NR / H0 : NR, read_one(t + 1, s1, next, u););
+                EACH(u, q * C::LOADS / NM, (q + 1) * C::LOADS / NM, issue_one(t + R, slot, u););
+                __builtin_amdgcn_sched_barrier(0););
+        }
+        scales_of(t + 1, next);
+        slot = s1;
+    };
+    int t = 0;
+    if constexpr (C::HALVES) {
+        for (; t < nst; ++t) {
+            Frags next;
+            step(t, f0, next);
+            f0 = next;
         }
     } else {
-        // stage t is multiplied from registers while stage t + 1 is read from
-        // LDS into the other set
-#pragma unroll
-        for (int s = 0; s < R; ++s)
-            if (s < nst) issue(s, s);
-        Frags f0, f1;
-        wait_stages<C::LOADS, R - 1>(nst - 1);
-        asm volatile("s_barrier" ::: "memory");
-        read(0, 0, f0);
-        int slot = 0;                                          // of stage t
-        auto step = [&](int t, const Frags &now, Frags &next) {
-            // every wave has stage t in registers, whose slot is refilled, and
-            // every wave's loads of stage t + 1 have landed
-            const int s1 = slot + 1 == R ? 0 : slot + 1;
-            wait_stages<C::LOADS, R - 2>(nst - 2 - t);
-            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            read(t + 1, s1, next);
-            if (t + R < nst) issue(t + R, slot);
-            multiply(now);
-            slot = s1;
-        };
-        int t = 0;
-        for (; t + 2 < nst; t += 2) {
+        Frags f1;
+        for (; t + 1 < nst; t += 2) {
             step(t, f0, f1);
             step(t + 1, f1, f0);
         }
-        if (t + 1 < nst) {
-            step(t, f0, f1);
-            multiply(f1);
-        } else {
-            multiply(f0);
-        }
+        if (t < nst) step(t, f0, f1);
     }
+    wait_vm<0>();
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
@@ -549,33 +553,33 @@ hipError_t launch_tile(const MxGemm &p, hipStream_t s) {
     launch_kernel(mx_gemm_tile_kernel<C>, dim3((unsigned) ((T + 7) / 8 * 8)), dim3(C::NW * 64), C::LDS, s, p, tiles_m, tiles_n);
     return hipGetLastError();
 }
-template <int XT, int WM, int WN, int TM, int TN, int SK, int R, bool PIPE = false>
+template <int XT, int WM, int WN, int TM, int TN, int SK, int R, bool HALVES>
 hipError_t launch_tile_k(const MxGemm &p, hipStream_t s) {
-    if (p.K % 128 == 0) return launch_tile<Cfg<XT, WM, WN, TM, TN, SK, R, 16, PIPE>>(p, s);
-    if (p.K % 64 == 0) return launch_tile<Cfg<XT, WM, WN, TM, TN, SK, R, 2, PIPE>>(p, s);
-    return launch_tile<Cfg<XT, WM, WN, TM, TN, SK, R - (R > 2), 1, PIPE>>(p, s);
+    if (p.K % 128 == 0) return launch_tile<Cfg<XT, WM, WN, TM, TN, SK, R, 16, HALVES>>(p, s);
+    if (p.K % 64 == 0) return launch_tile<Cfg<XT, WM, WN, TM, TN, SK, R, 2, HALVES>>(p, s);
+    return launch_tile<Cfg<XT, WM, WN, TM, TN, SK, R - (R > 2), 1, HALVES>>(p, s);
 }
 
 // Shapes, by number (TSK_MX_CFG), and the us of a round of their tiles at K = 5120:
 //        both operands MXFP4             bf16 activations
-//   1    256 x 256, 8 waves     45       -
-//   2    128 x 256, 8 waves     29       256 x 128, 8 waves    64
-//   3    128 x 128, 8 waves     22       the same              45
-//   4    64 x 128, 4 waves      15       the same              33
-//   5    64 x 32, 4 waves       10       the same              20
-//   6    192 x 128, 8 waves     25       the same              55
-//   7    128 x 192, 8 waves     26       the same              55
+//   1    256 x 256, 8 waves     50       -
+//   2    128 x 256, 8 waves     33       256 x 128, 8 waves    73
+//   3    128 x 128, 8 waves     21       the same              42
+//   4    64 x 128, 8 waves      14       the same              31
+//   5    64 x 32, 4 waves       10       the same              19
+//   6    192 x 128, 8 waves     22       the same              51
+//   7    128 x 192, 8 waves     22       the same              50
 //   8    192 x 256, 8 waves     35       -
 //   11   rows kernel, 16 x 16 outputs (f32 activations too, as 12 to 15)
 //   12   32 x 16,  13  32 x 32,  14  64 x 32,  15  64 x 16
 //
 // Tiles run in rounds of the 256 CUs (64 x 32: two a CU), so the choice is the
 // shape of the least rounds times the time of one. Some pairs (us, taken /
-// next; outputs as rows x M): MXFP4, 512 x 5120, K = 2048 128 x 128 11.2 / 15.6;
-// 388 x 4096, K = 1024 64 x 128 6.2 / 7.6; 1292 x 4096, K = 1024 192 x 128 10.2 /
-// 128 x 256 11.2; 2047 x 2050, K = 5120 192 x 128 (176 tiles) 25.4 / 128 x 256 (144)
-// 28.7 / 128 x 128 (272) 40.7, with bf16 activations 54.9 / 63.7 / 87.4; 4096 x 4096,
-// K = 5120 256 x 256 56 / 192 x 128 75.
+// next; outputs as rows x M): MXFP4, 4096 x 4096, K = 5120 256 x 256 51 / 128 x 192
+// 66; 2047 x 2050, K = 5120 192 x 128 (176 tiles) 21.4 / 128 x 256 (144) 27.6 / 128 x
+// 128 (272) 35.8, with bf16 activations 47.6 / 59.6 / 74.3; 1292 x 4096, K = 1024
+// 192 x 128 10.4 / 128 x 256 11.4; 1292 x 1024, K = 4096 64 x 128 12.4 / 64 x 32 14.4;
+// 388 x 4096, K = 1024 64 x 128 6.4 / 128 x 128 7.8, with bf16 9.7 / 11.4.
 // At most 32 rows, or too few tiles of the smallest shape: the rows kernel
 // (MXFP4, K = 2048, 96 x 3000, 141 tiles 5.2 / rows 6.9; K = 4096, 33 x 4096, 128
 // tiles 7.5 / 7.8, with bf16 activations 14.3 / 12.7), in the largest of its
@@ -589,9 +593,9 @@ int shape_for(const MxGemm &p) {
     if constexpr (XT != X_F32) {
         constexpr bool MX = XT == X_MX;
         struct Shape { int bm, bn, a_round, us; };
-        constexpr Shape shapes[8] = {{256, 256, 256, 45}, {MX ? 128 : 256, MX ? 256 : 128, 256, MX ? 29 : 64},
-                                     {128, 128, 256, MX ? 22 : 45}, {64, 128, 256, MX ? 15 : 33}, {64, 32, 512, MX ? 10 : 20},
-                                     {192, 128, 256, MX ? 25 : 55}, {128, 192, 256, MX ? 26 : 55}, {192, 256, 256, 35}};
+        constexpr Shape shapes[8] = {{256, 256, 256, 50}, {MX ? 128 : 256, MX ? 256 : 128, 256, MX ? 33 : 73},
+                                     {128, 128, 256, MX ? 21 : 42}, {64, 128, 256, MX ? 14 : 31}, {64, 32, 512, MX ? 10 : 19},
+                                     {192, 128, 256, MX ? 22 : 51}, {128, 192, 256, MX ? 22 : 50}, {192, 256, 256, 35}};
         if (p.N > 32 && tiles(64, 32) >= 130) {
             int best = 0;
             int64_t least = 0;
@@ -619,18 +623,18 @@ hipError_t launch_kind(const MxGemm &p, hipStream_t s) {
         const int64_t xrow = MX ? p.K / 2 : p.ld_x * 2, most = (int64_t) 1 << 31;
         if (256 * (int64_t) (p.K / 2) >= most || 256 * xrow + (int64_t) p.K * 2 >= most) shape = std::max(shape, 11);
         switch (shape) {
-            case 1: if constexpr (MX) return launch_tile_k<XT, 2, 4, 8, 4, 8, 2>(p, s);
+            case 1: if constexpr (MX) return launch_tile_k<XT, 2, 4, 8, 4, 8, 2, true>(p, s);
             [[fallthrough]];
-            case 2: if constexpr (MX) return launch_tile_k<XT, 2, 4, 4, 4, 8, 2>(p, s);
-                    else return launch_tile_k<XT, 4, 2, 4, 4, 4, 2>(p, s);
-            case 3: if constexpr (MX) return launch_tile_k<XT, 2, 4, 4, 2, 8, 4>(p, s);
-                    else return launch_tile_k<XT, 4, 2, 2, 4, 4, 3>(p, s);
-            case 4: return launch_tile_k<XT, 2, 2, 2, 4, MX ? 8 : 4, MX ? 5 : 4>(p, s);
-            case 5: return launch_tile_k<XT, 4, 1, 1, 2, MX ? 8 : 4, 5, true>(p, s);
-            case 6: return launch_tile_k<XT, 4, 2, 3, 4, MX ? 8 : 4, MX ? 3 : 2>(p, s);
-            case 7: if constexpr (MX) return launch_tile_k<XT, 2, 4, 4, 3, 8, 3>(p, s);
-                    else return launch_tile_k<XT, 4, 2, 2, 6, 4, 2>(p, s);
-            case 8: if constexpr (MX) return launch_tile_k<XT, 2, 4, 6, 4, 8, 2>(p, s);
+            case 2: if constexpr (MX) return launch_tile_k<XT, 2, 4, 4, 4, 8, 2, true>(p, s);
+                    else return launch_tile_k<XT, 4, 2, 4, 4, 4, 2, true>(p, s);
+            case 3: if constexpr (MX) return launch_tile_k<XT, 2, 4, 4, 2, 8, 4, true>(p, s);
+                    else return launch_tile_k<XT, 4, 2, 2, 4, 4, 3, true>(p, s);
+            case 4: return launch_tile_k<XT, 2, 4, 2, 2, MX ? 8 : 4, MX ? 5 : 4, true>(p, s);
+            case 5: return launch_tile_k<XT, 4, 1, 1, 2, MX ? 8 : 4, 5, false>(p, s);
+            case 6: return launch_tile_k<XT, 4, 2, 3, 4, MX ? 8 : 4, MX ? 3 : 2, true>(p, s);
+            case 7: if constexpr (MX) return launch_tile_k<XT, 2, 4, 4, 3, 8, 3, true>(p, s);
+                    else return launch_tile_k<XT, 4, 2, 2, 6, 4, 2, true>(p, s);
+            case 8: if constexpr (MX) return launch_tile_k<XT, 2, 4, 6, 4, 8, 2, true>(p, s);
         }
     }
     switch (shape) {
