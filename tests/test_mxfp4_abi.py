@@ -191,6 +191,51 @@ def test_block_norm_refusals(uninit):  # noqa: F811
     assert bn(wide[0], y, params(T), wide[1], dst) == ARG
 
 
+def test_outputs_whose_rows_share_bytes(uninit):  # noqa: F811
+    """rows of an output that overlap, strides of extents of 1 aside; broadcast inputs are taken"""
+    T = uninit
+
+    def strided(shape, nb, typ=None, data=0x100000):
+        d = fake(T, T.F32 if typ is None else typ, shape, 2 if typ == T.BF16 else 4)
+        d.nb[1], d.nb[2], d.nb[3] = nb
+        d.data = data
+        return d
+
+    S, B = (2, 7, 64), 256                                      # rows of 256 bytes
+    q = mx(T, 14, 64, data=0x800000)
+    q.ne[1], q.ne[2] = 7, 2
+    good, bad = [(B, 7 * B, 0), (2 * B, B, 0), (B + 4, 8 * B, 1)], [(0, 7 * B, 0), (B, 0, 0), (B, 6 * B, 0), (B - 4, 7 * B, 0)]
+    for nb in good:                                             # the second: two interleaved sets of rows
+        assert call(T, "tsk_mxfp4_dequantize", q, strided(S, nb)) == NOT_INIT
+    w, x = mx(T, 64, 64), strided(S, (0, 0, 0), data=0x300000)
+    for nb in bad:
+        assert call(T, "tsk_mxfp4_dequantize", q, strided(S, nb)) == STRIDE
+        y, other = strided(S, nb, data=0x100000), strided(S, (B, 7 * B, 0), data=0x200000)
+        p = params(T)
+        for res, dst in ((y, other), (other, y)):
+            assert call(T, "tsk_block_norm", x, None, p, res, dst) == STRIDE
+        if nb[0] % 16 == 0:
+            assert call(T, "tsk_mul_mat", w, x, None, y) == STRIDE
+    in_place = strided(S, (0, 7 * B, 0))
+    assert call(T, "tsk_block_norm", in_place, None, params(T, pre_norm=0), in_place, None) == STRIDE
+    assert call(T, "tsk_block_norm", x, None, params(T), None, strided(S, (B, 7 * B, 0))) == NOT_INIT
+    assert call(T, "tsk_mul_mat", w, x, None, strided(S, (B, 7 * B, 0))) == NOT_INIT
+    # blocks: rows along the third extent alone
+    x = strided((3, 1, 1, 64), (4, 4, B), data=0x300000)
+    for nb, rc in (((3, 5, 34), NOT_INIT), ((34, 34, 33), STRIDE), ((34, 34, 0), STRIDE)):
+        d = mx(T, 1, 64, split=False, data=0x800000)
+        d.ne[3] = 3
+        d.nb[1], d.nb[2], d.nb[3] = nb
+        assert call(T, "tsk_mxfp4_quantize", x, d) == rc
+        assert call(T, "tsk_mxfp4_dequantize", d, strided((3, 1, 1, 64), (4, 4, B))) == rc
+
+
+def test_planes_of_too_few_bytes(tsk):  # noqa: F811
+    tsk.SplitMXFP4(np.zeros(4 * 34, np.uint8), 64, 4)
+    with pytest.raises(ValueError):
+        tsk.SplitMXFP4(np.zeros(4 * 34 - 1, np.uint8), 64, 4)
+
+
 def test_reference_rounding():
     """the 64-bit restatement itself: the numbers, the ties and the ends of the scale"""
     top = 7.9

@@ -275,13 +275,45 @@ bool rows_fit(const tsk_tensor *t) {
     }
     return true;
 }
-int64_t row_count(const tsk_tensor *t) { return t->ne[1] * t->ne[2] * t->ne[3]; }
 
+int64_t row_count(const tsk_tensor *t) { return t->ne[1] * t->ne[2] * t->ne[3]; }
+// bytes of a row
+size_t row_bytes(const tsk_tensor *t) {
+    const size_t n = (size_t) t->ne[0];
+    return t->type == TSK_TYPE_MXFP4 ? n / 32 * 17 : n * (size_t) elt_size(t->type);
+}
+// bytes from each row to the next where that is the same throughout, or 0; the
+// strides of extents of 1 do not count
+size_t row_stride(const tsk_tensor *t) {
+    size_t ld = 0, next = 0;
+    for (int i = 1; i < 4; ++i) {
+        if (t->ne[i] == 1) continue;
+        if (ld && t->nb[i] != next) return 0;
+        if (!ld) ld = t->nb[i];
+        next = t->nb[i] * (size_t) t->ne[i];
+    }
+    return ld || row_count(t) > 1 ? ld : row_bytes(t);
+}
+// an output: no two rows share bytes
+int check_rows_apart(const tsk_tensor *t, const char *name) {
+    size_t span = row_bytes(t);
+    bool done[4] = {true, false, false, false};
+    for (int k = 1; k < 4; ++k) {
+        int m = 0;                                           // the smallest stride left
+        for (int i = 1; i < 4; ++i)
+            if (!done[i] && t->ne[i] > 1 && (!m || t->nb[i] < t->nb[m])) m = i;
+        if (!m) break;
+        done[m] = true;
+        if (t->nb[m] < span) return fail(TSK_ERR_STRIDE, "%s: rows overlap", name);
+        span += t->nb[m] * (size_t) (t->ne[m] - 1);
+    }
+    return TSK_OK;
+}
 // MXFP4 blocks: 17 bytes each, whole rows that do not overlap
 int check_mx_blocks(const tsk_tensor *t, const char *name) {
     if (t->nb[0] != 17) return fail(TSK_ERR_STRIDE, "%s: MXFP4 nb[0] must be 17 (block size)", name);
-    if (t->ne[1] > 1 && t->nb[1] < (size_t) (t->ne[0] / 32) * 17) return fail(TSK_ERR_STRIDE, "%s: MXFP4 rows overlap", name);
-    if (!rows_uniform(t)) return fail(TSK_ERR_STRIDE, "%s: MXFP4 rows must be uniformly strided", name);
+    if (!row_stride(t)) return fail(TSK_ERR_STRIDE, "%s: MXFP4 rows must be uniformly strided", name);
+    if (row_stride(t) < row_bytes(t)) return fail(TSK_ERR_STRIDE, "%s: MXFP4 rows overlap", name);
     return TSK_OK;
 }
 // either MXFP4 layout, of rows of ne0 % 32 == 0
@@ -297,11 +329,7 @@ int check_mx(const tsk_tensor *t, const char *name) {
 uint8_t *mx_codes(const tsk_tensor *t) { return (uint8_t *) t->data; }
 uint8_t *mx_scales(const tsk_tensor *t) { return (uint8_t *) t->data + (size_t) row_count(t) * (size_t) (t->ne[0] / 2); }
 
-// bytes of a row, and from the first byte of a tensor to past its last
-size_t row_bytes(const tsk_tensor *t) {
-    const size_t n = (size_t) t->ne[0];
-    return t->type == TSK_TYPE_MXFP4 ? n / 32 * 17 : n * (size_t) elt_size(t->type);
-}
+// bytes from the first of a tensor to past its last
 size_t span_bytes(const tsk_tensor *t) {
     if (t->type == TSK_TYPE_MXFP4_SPLIT) return (size_t) row_count(t) * (size_t) (t->ne[0] / 32 * 17);
     size_t n = row_bytes(t);
@@ -466,6 +494,7 @@ int validate_mul_mat(const tsk_tensor *a, const tsk_tensor *b, const tsk_tensor 
             if (K % 32) return fail(TSK_ERR_SHAPE, "K=%lld must be a multiple of 32 for MXFP4", (long long) K);
             if (K > MX_MAX_WEIGHT || M > MX_MAX_WEIGHT) return fail(TSK_ERR_SHAPE, "MXFP4 weights of [%lld, %lld]", (long long) K, (long long) M);
             if (!rows_fit(b)) return fail(TSK_ERR_SHAPE, "b has too many rows");
+            if ((rc = check_rows_apart(dst, "dst"))) return rc;
             if (a->type == TSK_TYPE_MXFP4) return check_mx_blocks(a, "a");
             if (!aligned(a->data, 16)) return fail(TSK_ERR_ALIGN, "MXFP4_SPLIT data must be 16-byte aligned");
             break;
@@ -580,10 +609,11 @@ MulMatPlan plan_mul_mat(const tsk_tensor *a, const tsk_tensor *b, const tsk_tens
     memset(&pl, 0, sizeof(pl));
     const int64_t K = a->ne[0], M = a->ne[1];
     // slices of uniformly strided rows: one launch per (i2, i3) unless rows are uniform
-    pl.uni = (b->type == TSK_TYPE_MXFP4_SPLIT || rows_uniform(b)) && rows_uniform(dst);
+    const bool mx = a->type == TSK_TYPE_MXFP4 || a->type == TSK_TYPE_MXFP4_SPLIT;
+    pl.uni = mx ? (b->type == TSK_TYPE_MXFP4_SPLIT || row_stride(b)) && row_stride(dst) : rows_uniform(b) && rows_uniform(dst);
     pl.nslices = pl.uni ? 1 : b->ne[2] * b->ne[3];
     pl.Nslice = pl.uni ? b->ne[1] * b->ne[2] * b->ne[3] : b->ne[1];
-    if (a->type == TSK_TYPE_MXFP4 || a->type == TSK_TYPE_MXFP4_SPLIT) {
+    if (mx) {
         // f32 activations: read and rounded by the rows kernel in every one of its
         // workgroups, or once by a launch before the product (us, M = K = 4096: 16
         // rows 10.6 / 9.6, 32 rows 12.9 / 11.3; K = 1024, M = 4096, 64 rows 6.6 /
@@ -627,7 +657,7 @@ int mul_mat_mx(const tsk_tensor *a, const tsk_tensor *b, const tsk_tensor *bias,
     int rc;
     if (pl.bytes && (rc = scr.get(pl.bytes, &ws))) return rc;
     if (a->type == TSK_TYPE_MXFP4) {
-        e = launch_mx_repack((const uint8_t *) a->data, (int64_t) a->nb[1], M, K, (uint8_t *) ws,
+        e = launch_mx_repack((const uint8_t *) a->data, (int64_t) row_stride(a), M, K, (uint8_t *) ws,
                              (uint8_t *) ws + (size_t) M * (size_t) (K / 2), scr.s);
         if (e != hipSuccess) return hip_fail(e, "mxfp4 repack");
         p.wq = (const uint8_t *) ws;
@@ -639,8 +669,11 @@ int mul_mat_mx(const tsk_tensor *a, const tsk_tensor *b, const tsk_tensor *bias,
     p.M = (int) M; p.N = (int) pl.Nslice; p.K = (int) K;
     const bool mx_b = b->type == TSK_TYPE_MXFP4_SPLIT;
     // (a single row's stride may be anything)
-    p.ld_x = mx_b ? 0 : p.N == 1 ? K : (int64_t) b->nb[1] / elt_size(b->type);
-    p.ld_y = p.N == 1 ? M : (int64_t) dst->nb[1] / elt_size(dst->type);
+    auto ld = [&](const tsk_tensor *t, int64_t n) {
+        return p.N == 1 ? n : (int64_t) (pl.uni ? row_stride(t) : t->nb[1]) / elt_size(t->type);
+    };
+    p.ld_x = mx_b ? 0 : ld(b, K);
+    p.ld_y = ld(dst, M);
     for (int64_t sl = 0; sl < pl.nslices; ++sl) {
         const int64_t i2 = sl % b->ne[2], i3 = sl / b->ne[2];
         p.y = (char *) dst->data + i2 * dst->nb[2] + i3 * dst->nb[3];
@@ -651,7 +684,7 @@ int mul_mat_mx(const tsk_tensor *a, const tsk_tensor *b, const tsk_tensor *bias,
             p.x = (const char *) b->data + i2 * b->nb[2] + i3 * b->nb[3];
             if (pl.cast_bytes) {
                 uint16_t *xb = (uint16_t *) ((char *) ws + pl.wbytes);
-                e = launch_cast_rows_bf16((const float *) p.x, pl.Nslice == 1 ? K : (int64_t) b->nb[1] / 4, 0, (int) std::min<int64_t>(pl.Nslice, 1 << 30),
+                e = launch_cast_rows_bf16((const float *) p.x, ld(b, K), 0, (int) std::min<int64_t>(pl.Nslice, 1 << 30),
                                           pl.Nslice, (int) K, xb, scr.s);
                 if (e != hipSuccess) return hip_fail(e, "mul_mat input cast");
                 p.x = xb;
@@ -1210,7 +1243,7 @@ extern "C" int tsk_mxfp4_quantize(const tsk_tensor *x, tsk_tensor *dst, tsk_stre
     if ((rc = require_init())) return rc;
     const bool split = dst->type == TSK_TYPE_MXFP4_SPLIT;
     hipError_t e = launch_mx_quantize(view(x), split ? mx_codes(dst) : nullptr, split ? mx_scales(dst) : nullptr,
-                                      split ? nullptr : (uint8_t *) dst->data, (int64_t) dst->nb[1], (hipStream_t) stream);
+                                      split ? nullptr : (uint8_t *) dst->data, split ? 0 : (int64_t) row_stride(dst), (hipStream_t) stream);
     return e == hipSuccess ? TSK_OK : hip_fail(e, "mxfp4 quantize launch");
 }
 
@@ -1220,12 +1253,12 @@ extern "C" int tsk_mxfp4_dequantize(const tsk_tensor *x, tsk_tensor *dst, tsk_st
     if ((rc = check_mx(x, "x"))) return rc;
     if (dst->type != TSK_TYPE_F32 && dst->type != TSK_TYPE_BF16) return fail(TSK_ERR_TYPE, "dst must be F32 or BF16");
     if (!same_shape(x, dst)) return fail(TSK_ERR_SHAPE, "shapes differ");
-    if ((rc = check_rows(dst, "dst", elt_size(dst->type)))) return rc;
+    if ((rc = check_rows(dst, "dst", elt_size(dst->type))) || (rc = check_rows_apart(dst, "dst"))) return rc;
     if (may_overlap(x, dst)) return fail(TSK_ERR_INVALID_ARG, "x and dst overlap");
     if ((rc = require_init())) return rc;
     const bool split = x->type == TSK_TYPE_MXFP4_SPLIT;
     hipError_t e = launch_mx_dequantize(split ? mx_codes(x) : nullptr, split ? mx_scales(x) : nullptr,
-                                        split ? nullptr : (const uint8_t *) x->data, (int64_t) x->nb[1], view(dst),
+                                        split ? nullptr : (const uint8_t *) x->data, split ? 0 : (int64_t) row_stride(x), view(dst),
                                         (hipStream_t) stream);
     return e == hipSuccess ? TSK_OK : hip_fail(e, "mxfp4 dequantize launch");
 }
@@ -1238,7 +1271,7 @@ extern "C" int tsk_mxfp4_repack(const tsk_tensor *src, tsk_tensor *dst, tsk_stre
     if ((rc = check_mx(src, "src")) || (rc = check_mx(dst, "dst"))) return rc;
     if (may_overlap(src, dst)) return fail(TSK_ERR_INVALID_ARG, "src and dst overlap");
     if ((rc = require_init())) return rc;
-    hipError_t e = launch_mx_repack((const uint8_t *) src->data, (int64_t) src->nb[1], src->ne[1], src->ne[0], mx_codes(dst),
+    hipError_t e = launch_mx_repack((const uint8_t *) src->data, (int64_t) row_stride(src), src->ne[1], src->ne[0], mx_codes(dst),
                                     mx_scales(dst), (hipStream_t) stream);
     return e == hipSuccess ? TSK_OK : hip_fail(e, "mxfp4 repack launch");
 }
@@ -1289,14 +1322,14 @@ int validate_block_norm(const tsk_tensor *x, const tsk_tensor *y, const tsk_bloc
         (rc = check_bn_factor(p->shift, "shift", x)))
         return rc;
     if (res) {
-        if ((rc = check_bn_rows(res, "res", x))) return rc;
+        if ((rc = check_bn_rows(res, "res", x)) || (rc = check_rows_apart(res, "res"))) return rc;
         if (res->type != x->type) return fail(TSK_ERR_TYPE, "res must have x's type");
     }
     if (dst) {
         if (dst->type == TSK_TYPE_MXFP4_SPLIT) {
             if ((rc = check_tensor(dst, "dst")) || (rc = check_mx(dst, "dst"))) return rc;
             if (!same_shape(dst, x)) return fail(TSK_ERR_SHAPE, "dst must have x's shape");
-        } else if ((rc = check_bn_rows(dst, "dst", x))) {
+        } else if ((rc = check_bn_rows(dst, "dst", x)) || (rc = check_rows_apart(dst, "dst"))) {
             return rc;
         }
     }

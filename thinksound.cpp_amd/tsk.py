@@ -647,10 +647,22 @@ class SplitMXFP4:
     ttype = MXFP4_SPLIT
 
     def __init__(self, buf, K, rows):
+        if buf.nbytes < rows * K // 32 * 17:
+            raise ValueError("%d bytes for MXFP4 planes of (%d, %d)" % (buf.nbytes, rows, K))
         self.buf, self.logical_shape = buf, (K, rows)
 
     def data_ptr(self):
         return self.buf.data_ptr()
+
+
+def _desc_planes(out, x):
+    """an output SplitMXFP4's descriptor with the extents of x's rows"""
+    if out.logical_shape != (x.shape[-1], int(np.prod(x.shape[:-1]))):
+        raise ValueError("MXFP4 planes of (K, rows) = %s for x of %s" % (out.logical_shape, tuple(x.shape)))
+    dd, dx = desc(out, MXFP4_SPLIT), desc(x)
+    for k in range(1, 4):
+        dd.ne[k] = dx.ne[k]
+    return dd
 
 
 def _split_mxfp4(K, rows):
@@ -663,12 +675,9 @@ def mxfp4_quantize(x, split=True, out=None, stream=None):
     K, rows = x.shape[-1], int(np.prod(x.shape[:-1]))
     if out is None:
         out = _split_mxfp4(K, rows) if split else DeviceArray((rows, K // 32, 17), "u8")
-    dx, dd = desc(x), desc(out, MXFP4_SPLIT if isinstance(out, SplitMXFP4) else MXFP4)
-    if isinstance(out, SplitMXFP4):                        # planes take x's extents
-        for k in range(1, 4):
-            dd.ne[k] = dx.ne[k]
-    elif len(x.shape) > 2:
+    if not isinstance(out, SplitMXFP4) and len(x.shape) > 2:
         raise ValueError("blocks are 2-D here")
+    dx, dd = desc(x), _desc_planes(out, x) if isinstance(out, SplitMXFP4) else desc(out, MXFP4)
     check(load().tsk_mxfp4_quantize(ctypes.byref(dx), ctypes.byref(dd), _stream(stream)))
     return out
 
@@ -706,11 +715,7 @@ def block_norm(x, y=None, gate=None, post=NORM_NONE, post_w=None, post_eps=1e-5,
     dx = desc(x)
     dd = None
     if dst is not None:
-        split = isinstance(dst, SplitMXFP4)
-        dd = desc(dst, MXFP4_SPLIT if split else None)
-        if split:
-            for k in range(1, 4):
-                dd.ne[k] = dx.ne[k]
+        dd = _desc_planes(dst, x) if isinstance(dst, SplitMXFP4) else desc(dst)
     dy, dr = (desc(t) if t is not None else None for t in (y, res))
     check(load().tsk_block_norm(ctypes.byref(dx), _ref(dy), ctypes.byref(p), _ref(dr), _ref(dd), _stream(stream)))
     return res, dst
