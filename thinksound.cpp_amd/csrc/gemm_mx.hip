@@ -10,8 +10,8 @@
 //
 // Bound: few rows by the weights' bytes (8 x 8192, K = 8192 12.6 us, 2.8 TB/s);
 // many rows by the matrix units, LDS and power together: 8192 x 8192, K = 8192
-// 300 us with MXFP4 X (3.7 PFLOP/s; products alone, without their loads, take
-// 200), 850 us with bf16 X (1.30 PFLOP/s).
+// 275 us with MXFP4 X (4.0 PFLOP/s; products alone, without their loads, take
+// 200), 850-930 us with bf16 X (1.2-1.3 PFLOP/s).
 #include <algorithm>
 #include <utility>
 
@@ -280,7 +280,7 @@ __device__ __forceinline__ void load_scales(__amdgpu_buffer_rsrc_t rsrc, uint8_t
 // few products a half to hide a read) a whole stage is read while the one before
 // is multiplied. Measured (us): all reads before the products, loads before the
 // reads 8192^3 320-333, 4096 x 4096, K = 5120 56; whole stages in order, 128 x 256
-// tiles 8192^3 397, halves 322; halves, 256 x 256 tiles 302 and 51; 64 x 32 tiles,
+// tiles 8192^3 397, halves 322; halves, 256 x 256 tiles 275-302 and 49-51; 64 x 32 tiles,
 // 1292 x 1024, K = 4096 halves 16.2, whole 14.4.
 template <int XT_, int WM_, int WN_, int TM_, int TN_, int SK_, int R_, int SCB_, bool HALVES_>
 struct Cfg {
@@ -345,19 +345,30 @@ __device__ __forceinline__ void mx_gemm_tile(const MxGemm &p, int tiles_m, int t
     const __amdgpu_buffer_rsrc_t rsb = MX ? rsrc_of(p.xs + (int64_t) n0 * KB, (int64_t) rn * KB) : rsa;
     constexpr int FAR = (int) 0x80000000u;
     // A lane's part of a load: rows of SK 16-byte chunks of codes, 64 / SK rows
-    // a load, chunk c of row t at slot c ^ key(t). An MFMA read takes one chunk
-    // of 16 rows at a time, which the keys spread over all 256 bytes of banks.
+    // a load, chunk c of row t at slot c ^ key(t). A 16-byte LDS read of a wave
+    // takes four turns, of lanes 0-3, 12-15, 20-27 and 4-11, 16-19, 28-31, and the
+    // same 32 further: 8 rows of one lane group's chunk and the other 8 of its
+    // neighbour's. The keys spread these over all 256 bytes of banks (a quarter of
+    // the 16 rows takes its own part of the chunks, in the order 0, 2, 3, 1; in the
+    // order 0 to 3 every read met itself twice: 8192^3 45 million cycles of
+    // conflicts and 285 us, so 6.5 million and 275).
     constexpr int AR = 64 / SK;
-    auto key = [](int row) { return SK == 8 ? row >> 1 & 7 : row >> 2 & 3; };
+    auto quarter = [](int row) {
+        const int t = row >> 2 & 3;
+        return ((t ^ t >> 1) & 1) << 1 | t >> 1;
+    };
+    auto key = [&](int row) { return SK == 8 ? quarter(row) << 1 | (row >> 1 & 1) : quarter(row); };
+    auto bf16_key = [&](int row) { return quarter(row) << 2 | (row & 3); };
     const int a_chk = (lane % SK) ^ key(wave * AR + lane / SK);                // (a wave's loads are NW, a multiple of 4, apart)
-    // bf16 rows: 16 chunks, 4 rows a load, chunk c of row t at slot c ^ (t % 16)
+    // bf16 rows: 16 chunks, 4 rows a load, chunk c of row t at slot c ^ bf16_key(t)
     static_assert(MX || SK == 4, "bf16 rows of 256 bytes");
     constexpr int BC = MX ? SK : 4 * SK, BR = 64 / BC;
     const int b_row = wave * BR + lane / BC;
-    const int b_chk = (lane % BC) ^ (MX ? key(b_row) : b_row & 15), b_blk = MX ? b_chk : b_chk / 4;
-    // scales with their stage: SCB bytes a lane, zero-extended to a dword; chunks: 16 bytes of a row's 32
+    const int b_chk = (lane % BC) ^ (MX ? key(b_row) : bf16_key(b_row)), b_blk = MX ? b_chk : b_chk / 4;
+    // scales with their stage: SCB bytes a lane, zero-extended to a dword; chunks: 16
+    // bytes of a row's 32, the halves of rows 8 to 15 of 16 swapped (banks again)
     constexpr int SL = CHUNK ? 2 : SK / SCB, SR = 64 / SL;
-    const int s_row = lane / SL, s_blk = lane % SL * SCB, s_off = s_row * KB + s_blk;
+    const int s_row = lane / SL, s_blk = (CHUNK ? lane % SL ^ (s_row >> 3 & 1) : lane % SL) * SCB, s_off = s_row * KB + s_blk;
     uint8_t *chunks = lds + R * C::STAGE;
 
     // scale load f (of SR rows: the weights' first, then the activations') from block blk on
@@ -427,7 +438,7 @@ __device__ __forceinline__ void mx_gemm_tile(const MxGemm &p, int tiles_m, int t
     auto read_one = [&](int t, int slot, Frags &f, int q) __attribute__((always_inline)) {
         const uint8_t *st = lds + slot * C::STAGE, *sb = st + C::A_BYTES;
         if (q < NSC) {
-            const uint8_t *ss = CHUNK ? chunks + t / C::CS % C::CHUNKS * C::CHUNK_BYTES + t % C::CS * SK : sb + C::B_BYTES;
+            const uint8_t *ss = CHUNK ? chunks + t / C::CS % C::CHUNKS * C::CHUNK_BYTES + (t % C::CS * SK ^ (r >> 3) * 16) : sb + C::B_BYTES;
             const bool x = q >= TM;
             if (x) f.sx[MX ? q - TM : 0] = scale_at(ss, C::BM / 16 + wn * TN + q - TM);
             else f.sa[q] = scale_at(ss, wm * TM + q);
@@ -441,7 +452,7 @@ __device__ __forceinline__ void mx_gemm_tile(const MxGemm &p, int tiles_m, int t
         } else {
             const int u = q - NSC, a = u - 2 * TN, h = u < 2 * TN ? u : u - TM;
             if (a >= 0 && a < TM) f.a[0][a] = *(const u32x4 *) (st + (wm * TM + a) * (16 * SK * 16) + a_at);
-            else f.b[0][h] = *(const u32x4 *) (sb + ((wn * TN + h % TN) * 16 + r) * C::XROW + ((4 * g + h / TN) ^ r) * 16);
+            else f.b[0][h] = *(const u32x4 *) (sb + ((wn * TN + h % TN) * 16 + r) * C::XROW + ((4 * g + h / TN) ^ bf16_key(r)) * 16);
         }
     };
     constexpr int NR0 = MX ? NSC + NKS : NSC + 2 * TN + TM;               // reads of the first half
