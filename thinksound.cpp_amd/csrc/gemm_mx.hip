@@ -219,7 +219,7 @@ __global__ __launch_bounds__(NW * 64) void mx_gemm_rows_kernel(const MxGemm p, i
 // their rows (16 rows at least, of M < 2^26 outputs each: 2^30 threads).
 constexpr int64_t MAX_THREADS = (int64_t) 1 << 31;
 template <class F>
-hipError_t halves(const MxGemm &p, F launch) {
+hipError_t in_two(const MxGemm &p, F launch) {
     MxGemm a = p, b = p;
     a.N = (p.N / 2 + 15) / 16 * 16;
     b.N = p.N - a.N;
@@ -239,7 +239,7 @@ template <int XT, int MT, int NT, int NW>
 hipError_t launch_rows(const MxGemm &p, hipStream_t s) {
     const int tiles_m = (p.M + 16 * MT - 1) / (16 * MT), tiles_n = (p.N + 16 * NT - 1) / (16 * NT);
     const int64_t T = (int64_t) tiles_m * tiles_n;
-    if (T * NW * 64 >= MAX_THREADS) return halves(p, [&](const MxGemm &q) { return launch_rows<XT, MT, NT, NW>(q, s); });
+    if (T * NW * 64 >= MAX_THREADS) return in_two(p, [&](const MxGemm &q) { return launch_rows<XT, MT, NT, NW>(q, s); });
     launch_kernel(mx_gemm_rows_kernel<XT, MT, NT, NW>, dim3((unsigned) T), dim3(NW * 64), 0, s, p, tiles_m);
     return hipGetLastError();
 }
@@ -559,7 +559,7 @@ template <class C>
 hipError_t launch_tile(const MxGemm &p, hipStream_t s) {
     const int tiles_m = (p.M + C::BM - 1) / C::BM, tiles_n = (p.N + C::BN - 1) / C::BN;
     const int64_t T = (int64_t) tiles_m * tiles_n;
-    if ((T + 7) * C::NW * 64 >= MAX_THREADS) return halves(p, [&](const MxGemm &q) { return launch_tile<C>(q, s); });
+    if ((T + 7) * C::NW * 64 >= MAX_THREADS) return in_two(p, [&](const MxGemm &q) { return launch_tile<C>(q, s); });
     lds_opt_in((const void *) mx_gemm_tile_kernel<C>, C::LDS);
     launch_kernel(mx_gemm_tile_kernel<C>, dim3((unsigned) ((T + 7) / 8 * 8)), dim3(C::NW * 64), C::LDS, s, p, tiles_m, tiles_n);
     return hipGetLastError();
