@@ -180,7 +180,7 @@ def shape(T, monkeypatch):
     T.init(0, reread=True)
 
 
-@pytest.mark.parametrize("cfg", [1, 2, 3, 4, 5, 6, 7, 8, 11, 12, 13, 14, 15])
+@pytest.mark.parametrize("cfg", [1, 2, 3, 4, 5, 6, 7, 8, 9, 11, 12, 13, 14, 15])
 @pytest.mark.parametrize("act", ["mxfp4", "bf16", "f32"])
 def test_every_launch_shape(T, shape, cfg, act):
     """ragged in rows, outputs and K (blocks of scales whole, by twos and odd; K shorter than a stage and longer than a

@@ -13,6 +13,7 @@
 // 275 us with MXFP4 X (4.0 PFLOP/s; products alone, without their loads, take
 // 200), 850-930 us with bf16 X (1.2-1.3 PFLOP/s).
 #include <algorithm>
+#include <cmath>
 #include <utility>
 
 #include "mxfp4.h"
@@ -278,10 +279,12 @@ __device__ __forceinline__ void load_scales(__amdgpu_buffer_rsrc_t rsrc, uint8_t
 // the second half's operands, the second half the next stage's first, with the
 // one barrier of a stage inside it. Otherwise (one row of sub-tiles a wave: too
 // few products a half to hide a read) a whole stage is read while the one before
-// is multiplied. Measured (us): all reads before the products, loads before the
-// reads 8192^3 320-333, 4096 x 4096, K = 5120 56; whole stages in order, 128 x 256
-// tiles 8192^3 397, halves 322; halves, 256 x 256 tiles 275-302 and 49-51; 64 x 32 tiles,
-// 1292 x 1024, K = 4096 halves 16.2, whole 14.4.
+// is multiplied. Three stages where they leave a CU two tiles or more: longer rings
+// only delay the first products (64 x 128, 1292 x 1024, K = 4096, five stages 11.9,
+// three 11.1; 64 x 32, 14.1 and 11.4). Measured (us): all reads before the products,
+// loads before the reads 8192^3 320-333, 4096 x 4096, K = 5120 56; whole stages in
+// order, 128 x 256 tiles 8192^3 397, halves 322; halves, 256 x 256 tiles 275-302 and
+// 49-51; 64 x 32 tiles of five stages, 1292 x 1024, K = 4096 halves 16.2, whole 14.4.
 template <int XT_, int WM_, int WN_, int TM_, int TN_, int SK_, int R_, int SCB_, bool HALVES_>
 struct Cfg {
     static constexpr int XT = XT_, WM = WM_, WN = WN_, TM = TM_, TN = TN_, SK = SK_, R = R_, SCB = SCB_;
@@ -571,48 +574,62 @@ hipError_t launch_tile_k(const MxGemm &p, hipStream_t s) {
     return launch_tile<Cfg<XT, WM, WN, TM, TN, SK, R - (R > 2), 1, HALVES>>(p, s);
 }
 
-// Shapes, by number (TSK_MX_CFG), and the us of a round of their tiles at K = 5120:
-//        both operands MXFP4             bf16 activations
-//   1    256 x 256, 8 waves     50       -
-//   2    128 x 256, 8 waves     33       256 x 128, 8 waves    73
-//   3    128 x 128, 8 waves     21       the same              42
-//   4    64 x 128, 8 waves      14       the same              31
-//   5    64 x 32, 4 waves       10       the same              19
-//   6    192 x 128, 8 waves     22       the same              51
-//   7    128 x 192, 8 waves     22       the same              50
-//   8    192 x 256, 8 waves     35       -
+// Shapes, by number (TSK_MX_CFG), and the us of one tile a CU at K = 5120 without
+// the launch (64 x 32 and 64 x 64: alone on a CU / among two or three):
+//        both operands MXFP4                  bf16 activations
+//   1    256 x 256, 8 waves     44            -
+//   2    128 x 256, 8 waves     26            256 x 128, 8 waves    72
+//   3    128 x 128, 8 waves     16            the same              42
+//   4    64 x 128, 8 waves      9             the same              26
+//   5    64 x 32, 4 waves       3.4 / 3.4     the same              12.6 / 8.3
+//   6    192 x 128, 8 waves     17.5          the same              49
+//   7    128 x 192, 8 waves     17            the same              49
+//   8    192 x 256, 8 waves     31            -
+//   9    64 x 64, 4 waves       5.5 / 5       the same              19 / 13.9
 //   11   rows kernel, 16 x 16 outputs (f32 activations too, as 12 to 15)
 //   12   32 x 16,  13  32 x 32,  14  64 x 32,  15  64 x 16
 //
-// Tiles run in rounds of the 256 CUs (64 x 32: two a CU), so the choice is the
-// shape of the least rounds times the time of one. Some pairs (us, taken /
-// next; outputs as rows x M): MXFP4, 4096 x 4096, K = 5120 256 x 256 51 / 128 x 192
-// 66; 2047 x 2050, K = 5120 192 x 128 (176 tiles) 21.4 / 128 x 256 (144) 27.6 / 128 x
-// 128 (272) 35.8, with bf16 activations 47.6 / 59.6 / 74.3; 1292 x 4096, K = 1024
-// 192 x 128 10.4 / 128 x 256 11.4; 1292 x 1024, K = 4096 64 x 128 12.4 / 64 x 32 14.4;
-// 388 x 4096, K = 1024 64 x 128 6.4 / 128 x 128 7.8, with bf16 9.7 / 11.4.
-// At most 32 rows, or too few tiles of the smallest shape: the rows kernel
-// (MXFP4, K = 2048, 96 x 3000, 141 tiles 5.2 / rows 6.9; K = 4096, 33 x 4096, 128
-// tiles 7.5 / 7.8, with bf16 activations 14.3 / 12.7), in the largest of its
-// shapes of which there are 200 (16 rows, M = K = 4096, 128 of 32 x 16 6.3 / 4.7;
-// 1 row, M = K = 8192, 256 of them 9.6 / 11.0; bf16, 16 rows, K = 4096, M = 16384
-// 64 x 16 12.1 / 15.1).
+// The choice is the shape of the least time: its tiles on the fullest of 256 CUs
+// times that of one, by K, and 0.8 for every time that a CU starts over (first
+// loads, stores). Some pairs (us, taken / next; outputs as rows x M): MXFP4,
+// 4096 x 4096, K = 5120 256 x 256 49 / 128 x 256 65; 2047 x 2050, K = 5120 128 x 192
+// 22.0 / 128 x 256 (144 tiles) 27.0 / 128 x 128 (272) 34.8, with bf16 activations
+// 48.1 / 61.0 / 73.9; 1292 x 1024, K = 4096 64 x 128 11.2 / 64 x 64 11.0 / 128 x 128
+// 14.8; 388 x 4096, K = 1024 64 x 128 5.7 / 128 x 128 7.4, with bf16 9.2 / 11.2;
+// 1024 x 1024, K = 1024 64 x 64 4.8 / 64 x 128 5.6; 388 x 1024, K = 4096 64 x 32 6.9 /
+// 64 x 64 8.4, with bf16 14.1 / 19.5.
+// Few rows, or too few tiles of the smallest shape: the rows kernel (us, 64 x 32
+// tiles / rows: MXFP4, 17 x 8192, K = 8192 11.4 / 12.9; 64 x 4096, K = 4096, 128
+// tiles 6.8 / 7.8, with bf16 activations 14.0 / 12.6; 32 x 4096, 64 tiles 6.7 / 6.5;
+// bf16, 64 x 8192, K = 8192, 256 tiles 25.1 / 28.7), in the largest of its shapes
+// that more than half of the CUs get, since of the next there would be two each
+// (bf16, 96 x 1500, K = 2048, 141 of 32 x 32 7.3 / 282 of 32 x 16 8.4; 16 rows, M = K =
+// 4096, 256 of 16 x 16 7.1 / 128 of 32 x 16 8.7; 8 rows, M = K = 8192, 256 of 32 x 16
+// 12.6 / 128 of 64 x 16 18).
 template <int XT>
 int shape_for(const MxGemm &p) {
     if (tuning().mx_cfg) return tuning().mx_cfg;
     auto tiles = [&](int bm, int bn) { return (int64_t) ((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
     if constexpr (XT != X_F32) {
         constexpr bool MX = XT == X_MX;
-        struct Shape { int bm, bn, a_round, us; };
-        constexpr Shape shapes[8] = {{256, 256, 256, 50}, {MX ? 128 : 256, MX ? 256 : 128, 256, MX ? 33 : 73},
-                                     {128, 128, 256, MX ? 21 : 42}, {64, 128, 256, MX ? 14 : 31}, {64, 32, 512, MX ? 10 : 19},
-                                     {192, 128, 256, MX ? 22 : 51}, {128, 192, 256, MX ? 22 : 50}, {192, 256, 256, 35}};
-        if (p.N > 32 && tiles(64, 32) >= 130) {
+        struct Shape { int bm, bn, on_a_cu; double alone, us; };
+        constexpr Shape shapes[9] = {{256, 256, 1, 0, 44},
+                                     {MX ? 128 : 256, MX ? 256 : 128, 1, 0, MX ? 26 : 72},
+                                     {128, 128, 1, 0, MX ? 16 : 42},
+                                     {64, 128, 1, 0, MX ? 9 : 26},
+                                     {64, 32, 3, MX ? 3.4 : 12.6, MX ? 3.4 : 8.3},
+                                     {192, 128, 1, 0, MX ? 17.5 : 49},
+                                     {128, 192, 1, 0, MX ? 17 : 49},
+                                     {192, 256, 1, 0, 31},
+                                     {64, 64, 2, MX ? 5.5 : 19, MX ? 5 : 13.9}};
+        if (p.N > (MX ? 16 : 32) && tiles(64, 32) >= (MX ? 100 : 130)) {
             int best = 0;
-            int64_t least = 0;
-            for (int i = MX ? 0 : 1; i < (MX ? 8 : 7); ++i) {
+            double least = 0;
+            for (int i = 0; i < 9; ++i) {
                 const Shape &c = shapes[i];
-                const int64_t cost = (tiles(c.bm, c.bn) + c.a_round - 1) / c.a_round * c.us;
+                if (!MX && (i == 0 || i == 7)) continue;
+                const double each = (double) ((tiles(c.bm, c.bn) + 255) / 256);      // tiles of a CU
+                const double cost = std::max(c.alone, each * c.us) * p.K / 5120 + std::ceil(each / c.on_a_cu) * 0.8;
                 if (!best || cost < least) {
                     best = i + 1;
                     least = cost;
@@ -621,8 +638,8 @@ int shape_for(const MxGemm &p) {
             return best;
         }
     }
-    if (p.N <= 16) return tiles(64, 16) >= 200 ? 15 : tiles(32, 16) >= 200 ? 12 : 11;
-    return tiles(64, 32) >= 200 ? 14 : tiles(32, 32) >= 200 ? 13 : tiles(32, 16) >= 200 ? 12 : 11;
+    if (p.N <= 16) return tiles(64, 16) > 128 ? 15 : tiles(32, 16) > 128 ? 12 : 11;
+    return tiles(64, 32) > 128 ? 14 : tiles(32, 32) > 128 ? 13 : tiles(32, 16) > 128 ? 12 : 11;
 }
 
 template <int XT>
@@ -638,14 +655,16 @@ hipError_t launch_kind(const MxGemm &p, hipStream_t s) {
             [[fallthrough]];
             case 2: if constexpr (MX) return launch_tile_k<XT, 2, 4, 4, 4, 8, 2, true>(p, s);
                     else return launch_tile_k<XT, 4, 2, 4, 4, 4, 2, true>(p, s);
-            case 3: if constexpr (MX) return launch_tile_k<XT, 2, 4, 4, 2, 8, 4, true>(p, s);
+            case 3: if constexpr (MX) return launch_tile_k<XT, 2, 4, 4, 2, 8, 3, true>(p, s);
                     else return launch_tile_k<XT, 4, 2, 2, 4, 4, 3, true>(p, s);
-            case 4: return launch_tile_k<XT, 2, 4, 2, 2, MX ? 8 : 4, MX ? 5 : 4, true>(p, s);
-            case 5: return launch_tile_k<XT, 4, 1, 1, 2, MX ? 8 : 4, 5, false>(p, s);
+            case 4: return launch_tile_k<XT, 2, 4, 2, 2, MX ? 8 : 4, 3, true>(p, s);
+            case 5: return launch_tile_k<XT, 4, 1, 1, 2, MX ? 8 : 4, 3, false>(p, s);
             case 6: return launch_tile_k<XT, 4, 2, 3, 4, MX ? 8 : 4, MX ? 3 : 2, true>(p, s);
             case 7: if constexpr (MX) return launch_tile_k<XT, 2, 4, 4, 3, 8, 3, true>(p, s);
                     else return launch_tile_k<XT, 4, 2, 2, 6, 4, 2, true>(p, s);
             case 8: if constexpr (MX) return launch_tile_k<XT, 2, 4, 6, 4, 8, 2, true>(p, s);
+                    break;
+            case 9: return launch_tile_k<XT, 2, 2, 2, 2, MX ? 8 : 4, 3, false>(p, s);
         }
     }
     switch (shape) {
