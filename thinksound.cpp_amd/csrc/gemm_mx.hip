@@ -277,14 +277,15 @@ __device__ __forceinline__ void load_scales(__amdgpu_buffer_rsrc_t rsrc, uint8_t
 // read of what the next ones take and a load of a later stage, in the program's
 // order (sched_barrier). HALVES: the first half of a stage's products reads
 // the second half's operands, the second half the next stage's first, with the
-// one barrier of a stage inside it. Otherwise (one row of sub-tiles a wave: too
-// few products a half to hide a read) a whole stage is read while the one before
-// is multiplied. Three stages where they leave a CU two tiles or more: longer rings
+// one barrier of a stage inside it. Otherwise (the tiles of four waves, whose CU has
+// other tiles to fill the waits) a whole stage is read while the one before is
+// multiplied. Three stages where they leave a CU two tiles or more: longer rings
 // only delay the first products (64 x 128, 1292 x 1024, K = 4096, five stages 11.9,
 // three 11.1; 64 x 32, 14.1 and 11.4). Measured (us): all reads before the products,
 // loads before the reads 8192^3 320-333, 4096 x 4096, K = 5120 56; whole stages in
 // order, 128 x 256 tiles 8192^3 397, halves 322; halves, 256 x 256 tiles 275-302 and
-// 49-51; 64 x 32 tiles of five stages, 1292 x 1024, K = 4096 halves 16.2, whole 14.4.
+// 49-51; 1292 x 1024, K = 4096, 64 x 32 tiles of five stages halves 16.2, whole
+// 14.4, 64 x 64 tiles halves 11.9, whole 11.1.
 template <int XT_, int WM_, int WN_, int TM_, int TN_, int SK_, int R_, int SCB_, bool HALVES_>
 struct Cfg {
     static constexpr int XT = XT_, WM = WM_, WN = WN_, TM = TM_, TN = TN_, SK = SK_, R = R_, SCB = SCB_;
@@ -423,8 +424,8 @@ __device__ __forceinline__ void mx_gemm_tile(const MxGemm &p, int tiles_m, int t
 #pragma unroll
         for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
 
-    // step ks of a stage: lane group g takes block SK / 4 * g + ks of every row
-    // the scale bytes of this lane's blocks of a stage, byte ks for step ks: base at its row 16 u
+    // Step ks of a stage: lane group g takes block SK / 4 * g + ks of every row.
+    // The scale bytes of this lane's blocks of a stage, byte ks for step ks: base at its row 16 u
     auto scale_at = [&](const uint8_t *base, int u) __attribute__((always_inline)) -> int {
         const uint8_t *q = base + u * (CHUNK ? 512 : 16 * C::SROW) + s_at;
         if constexpr (CHUNK) return SK == 8 ? *(const uint16_t *) q : *q;
@@ -495,8 +496,8 @@ __device__ __forceinline__ void mx_gemm_tile(const MxGemm &p, int tiles_m, int t
     EACH(q, 0, (C::HALVES ? NR0 : NR), read_one(0, 0, f0, q););
     scales_of(0, f0);
     int slot = 0;                                                              // of stage t
-    // `fill` after it every wave has stage t in registers, whose slot is
-    // refilled, and every wave's loads of stage t + 1 have landed
+    // past it every wave has stage t in registers, whose slot is refilled, and
+    // every wave's loads of stage t + 1 have landed
     auto fill = [&]() __attribute__((always_inline)) {
         wait_vm<(R - 2) * C::LOADS>();
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -582,7 +583,7 @@ hipError_t launch_tile_k(const MxGemm &p, hipStream_t s) {
 //   3    128 x 128, 8 waves     16            the same              42
 //   4    64 x 128, 8 waves      9             the same              26
 //   5    64 x 32, 4 waves       3.4 / 3.4     the same              12.6 / 8.3
-//   6    192 x 128, 8 waves     17.5          the same              49
+//   6    192 x 128, 8 waves     17.5          the same              50
 //   7    128 x 192, 8 waves     17            the same              49
 //   8    192 x 256, 8 waves     31            -
 //   9    64 x 64, 4 waves       5.5 / 5       the same              19 / 13.9
@@ -618,7 +619,7 @@ int shape_for(const MxGemm &p) {
                                      {128, 128, 1, 0, MX ? 16 : 42},
                                      {64, 128, 1, 0, MX ? 9 : 26},
                                      {64, 32, 3, MX ? 3.4 : 12.6, MX ? 3.4 : 8.3},
-                                     {192, 128, 1, 0, MX ? 17.5 : 49},
+                                     {192, 128, 1, 0, MX ? 17.5 : 50},
                                      {128, 192, 1, 0, MX ? 17 : 49},
                                      {192, 256, 1, 0, 31},
                                      {64, 64, 2, MX ? 5.5 : 19, MX ? 5 : 13.9}};
