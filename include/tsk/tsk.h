@@ -165,7 +165,7 @@ const char *tsk_version(void);
  * K must be a multiple of 32 for Q8_0 and MXFP4 (their block) and of 8 otherwise.
  * MXFP4: products are exact and summed in fp32 (sums below fp32's normal range
  * may be flushed to zero); a scale byte of 255 makes its block 32 NaNs; M and K up
- * to 2^26. Scratch: MXFP4 blocks are repacked on every call (MXFP4_SPLIT weights are
+ * to 2^26; dst overlaps no operand and no row of its own. Scratch: MXFP4 blocks are repacked on every call (MXFP4_SPLIT weights are
  * read in place), and f32 b of larger products is rounded to bf16 rows first.
  */
 int tsk_mul_mat(const tsk_tensor *a, const tsk_tensor *b, const tsk_tensor *bias,
