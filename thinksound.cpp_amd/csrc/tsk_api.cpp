@@ -282,17 +282,19 @@ size_t row_bytes(const tsk_tensor *t) {
     const size_t n = (size_t) t->ne[0];
     return t->type == TSK_TYPE_MXFP4 ? n / 32 * 17 : n * (size_t) elt_size(t->type);
 }
-// bytes from each row to the next where that is the same throughout, or 0; the
-// strides of extents of 1 do not count
+// bytes from each row to the next where that is the same throughout and not 0, or
+// 0; the strides of extents of 1 do not count, a stride of 0 (a broadcast) does
 size_t row_stride(const tsk_tensor *t) {
-    size_t ld = 0, next = 0;
+    size_t ld = row_bytes(t), next = 0;
+    bool found = false;
     for (int i = 1; i < 4; ++i) {
         if (t->ne[i] == 1) continue;
-        if (ld && t->nb[i] != next) return 0;
-        if (!ld) ld = t->nb[i];
+        if (found && t->nb[i] != next) return 0;
+        if (!found) ld = t->nb[i];
+        found = true;
         next = t->nb[i] * (size_t) t->ne[i];
     }
-    return ld || row_count(t) > 1 ? ld : row_bytes(t);
+    return ld;
 }
 // an output: no two rows share bytes
 int check_rows_apart(const tsk_tensor *t, const char *name) {
