@@ -695,10 +695,11 @@ __global__ void im2col_1d_kernel(const float *x, int64_t sp, int64_t sc, int64_t
 }
 
 // f32 rows -> bf16 (RNE), 4 elements per thread: row r = b * rows_per_b + i of
-// x at b * ld_b + i * ld_x, y contiguous rows of `cols`
-__global__ void cast_rows_bf16_kernel(const float *x, int64_t ld_x, int64_t ld_b, int rows_per_b, int64_t rows,
-                                      int cols, uint16_t *y) {
-    const int64_t q = (int64_t) blockIdx.x * blockDim.x + threadIdx.x;
+// x at b * ld_b + i * ld_x, y contiguous rows of `cols`. `done`: threads of the
+// launches before this one
+__global__ void cast_rows_bf16_kernel(const float *x, int64_t ld_x, int64_t ld_b, int64_t rows_per_b, int64_t rows,
+                                      int cols, uint16_t *y, int64_t done) {
+    const int64_t q = done + (int64_t) blockIdx.x * blockDim.x + threadIdx.x;
     const int cq = cols / 4;
     if (q >= rows * cq) return;
     const int64_t r = q / cq;
@@ -1273,12 +1274,18 @@ hipError_t launch_im2col_1d(const float *x, int64_t sp, int64_t sc, int64_t sn, 
     return hipGetLastError();
 }
 
-hipError_t launch_cast_rows_bf16(const float *x, int64_t ld_x, int64_t ld_b, int rows_per_b, int64_t rows, int cols,
+hipError_t launch_cast_rows_bf16(const float *x, int64_t ld_x, int64_t ld_b, int64_t rows_per_b, int64_t rows, int cols,
                                  uint16_t *y, hipStream_t s) {
     if (rows < 1 || cols < 4 || cols % 4 || rows_per_b < 1 || ld_x % 4 || ld_b % 4) return hipErrorInvalidValue;
-    const int64_t n = rows * (cols / 4);
-    launch_kernel(cast_rows_bf16_kernel, dim3(blocks_for(n, 256)), dim3(256), 0, s, x, ld_x, ld_b, rows_per_b, rows, cols, y);
-    return hipGetLastError();
+    // (a launch holds fewer than 2^32 threads)
+    const int64_t n = rows * (cols / 4), most = (int64_t) 1 << 31;
+    for (int64_t done = 0; done < n; done += most) {
+        launch_kernel(cast_rows_bf16_kernel, dim3(blocks_for(std::min(n - done, most), 256)), dim3(256), 0, s, x, ld_x, ld_b,
+                      rows_per_b, rows, cols, y, done);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 hipError_t launch_conv_pack(const void *w, int es, int64_t s0, int64_t s1, int64_t s2, int KW, int IC, int OC, void *dst,

@@ -686,8 +686,7 @@ int mul_mat_mx(const tsk_tensor *a, const tsk_tensor *b, const tsk_tensor *bias,
             p.x = (const char *) b->data + i2 * b->nb[2] + i3 * b->nb[3];
             if (pl.cast_bytes) {
                 uint16_t *xb = (uint16_t *) ((char *) ws + pl.wbytes);
-                e = launch_cast_rows_bf16((const float *) p.x, ld(b, K), 0, (int) std::min<int64_t>(pl.Nslice, 1 << 30),
-                                          pl.Nslice, (int) K, xb, scr.s);
+                e = launch_cast_rows_bf16((const float *) p.x, ld(b, K), 0, pl.Nslice, pl.Nslice, (int) K, xb, scr.s);
                 if (e != hipSuccess) return hip_fail(e, "mul_mat input cast");
                 p.x = xb;
                 p.x_f32 = 0;
@@ -746,8 +745,7 @@ int mul_mat_impl(const tsk_tensor *a, const tsk_tensor *b, const tsk_tensor *bia
                           coop_xf32(M, N, K, 0, (int64_t) (a->nb[1] / 2), sliced ? pl.splits : 1);
         if (b->type == TSK_TYPE_F32 && !xf32) {
             xb = (uint16_t *) ws;
-            hipError_t e = launch_cast_rows_bf16((const float *) b->data, ld_b, 0, (int) std::min<int64_t>(N, 1 << 30), N,
-                                                 (int) K, xb, s);
+            hipError_t e = launch_cast_rows_bf16((const float *) b->data, ld_b, 0, N, N, (int) K, xb, s);
             if (e != hipSuccess) return hip_fail(e, "mul_mat input cast");
         }
         GemmGroup g;

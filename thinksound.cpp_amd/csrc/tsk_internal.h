@@ -463,7 +463,7 @@ hipError_t launch_im2col_1d(const float *x, int64_t sp, int64_t sc, int64_t sn, 
                            int s0, int p0, int d0, void *dst, int dst_type, int64_t ld, hipStream_t s);
 // f32 rows -> contiguous bf16 rows (RNE): row b * rows_per_b + i read at
 // x + b * ld_b + i * ld_x (element strides, multiples of 4; cols % 4 == 0)
-hipError_t launch_cast_rows_bf16(const float *x, int64_t ld_x, int64_t ld_b, int rows_per_b, int64_t rows, int cols,
+hipError_t launch_cast_rows_bf16(const float *x, int64_t ld_x, int64_t ld_b, int64_t rows_per_b, int64_t rows, int cols,
                                  uint16_t *y, hipStream_t s);
 // conv kernel [KW, IC, OC] of es-byte elements (element strides s0..s2) ->
 // kw-major rows dst[oc][kw * IC + ic]
