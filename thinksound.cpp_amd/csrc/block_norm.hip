@@ -15,6 +15,11 @@
 #include "mxfp4.h"
 #include "tsk_internal.h"
 
+// Products and sums are rounded one at a time in this file, but where it writes
+// __builtin_fmaf: an element goes through the same operations in every kernel, and
+// the second norm reads the residual that is stored.
+#pragma clang fp contract(off)
+
 namespace tsk {
 
 namespace {
@@ -73,7 +78,7 @@ __device__ __forceinline__ void store_bf16(uint16_t *p, const float *v) {
     }
 }
 
-// ---- the arithmetic, one operation at a time (no contraction that differs from kernel to kernel)
+// ---- the arithmetic
 __device__ __forceinline__ float branch(float y, int norm, float mean, float inv, bool has_w, float w) {
     const float b = norm ? (y - mean) * inv : y;
     return has_w ? b * w : b;
