@@ -5,7 +5,7 @@ import ctypes
 import pytest
 
 from test_abi import fake, tsk, uninit  # noqa: F401  (fixtures)
-from test_mxfp4_abi import NOT_INIT, STRIDE, call, mx
+from test_mxfp4_abi import ARG, NOT_INIT, STRIDE, call, mx
 
 
 def strided(T, shape, nb, typ=None, data=0x100000):
@@ -78,3 +78,16 @@ def test_evenly_spaced_blocks(uninit, ne, nb):  # noqa: F811
     rows = fake(T, T.F32, ne[::-1], 4)
     assert call(T, "tsk_mxfp4_quantize", rows, blocks(T, ne, nb)) == NOT_INIT
     assert call(T, "tsk_mxfp4_dequantize", blocks(T, ne, nb), rows) == NOT_INIT
+
+
+def test_columns_beside_broadcast_rows(uninit):  # noqa: F811
+    """columns of one array are apart where the rows of an input are broadcast along any extent, and meet where they do"""
+    T = uninit
+    ld, base = 1024, 0x200000
+    y = strided(T, (2, 3, 5, 64), (ld, 5 * ld, 15 * ld), data=base)
+    p = T.BlockNormParams(0, 1e-5, None, None, 1.0, T.NORM_LAYER, 1e-5, None, None, None)
+    for nb in ((0, 5 * ld, 15 * ld), (ld, 0, 15 * ld), (ld, 5 * ld, 0), (0, 0, 15 * ld), (ld, 0, 0), (0, 5 * ld, 0)):
+        for at in (256, 768, -256):
+            assert call(T, "tsk_block_norm", strided(T, (2, 3, 5, 64), nb, data=base + at), None, p, None, y) == NOT_INIT
+        for at in (252, 0, -252, 772):
+            assert call(T, "tsk_block_norm", strided(T, (2, 3, 5, 64), nb, data=base + at), None, p, None, y) == ARG

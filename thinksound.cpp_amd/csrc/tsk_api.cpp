@@ -338,8 +338,8 @@ size_t span_bytes(const tsk_tensor *t) {
     for (int i = 1; i < 4; ++i) n += (size_t) (t->ne[i] - 1) * t->nb[i];
     return n;
 }
-// whether two tensors may share bytes: their spans meet, and they are not
-// columns of one array of rows (every stride a multiple of one row's) side by side
+// whether two tensors may share bytes: their spans meet, and they are not columns
+// of one array of rows (every stride a multiple of one row's, 0 among them) side by side
 bool may_overlap(const tsk_tensor *a, const tsk_tensor *b) {
     const uintptr_t pa = (uintptr_t) a->data, pb = (uintptr_t) b->data;
     if (pa + span_bytes(a) <= pb || pb + span_bytes(b) <= pa) return false;
@@ -347,7 +347,7 @@ bool may_overlap(const tsk_tensor *a, const tsk_tensor *b) {
     size_t ld = 0;
     for (const tsk_tensor *t : {a, b})
         for (int i = 1; i < 4; ++i)
-            if (t->ne[i] > 1 && (!ld || t->nb[i] < ld)) ld = t->nb[i];
+            if (t->ne[i] > 1 && t->nb[i] && (!ld || t->nb[i] < ld)) ld = t->nb[i];
     if (!ld) return true;
     for (const tsk_tensor *t : {a, b})
         for (int i = 1; i < 4; ++i)
