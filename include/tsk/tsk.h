@@ -156,17 +156,23 @@ const char *tsk_version(void);
  *          round b to bf16 (RNE); Q8_0 weights quantize b per 32-block to Q8_0
  *          (amax/127 scale, round-to-nearest-even); F16 weights round to fp16.
  *          MXFP4 weights multiply F32 / BF16 b as BF16 weights do (b rounded to
- *          bf16, the weights' values exact in bf16; ggml's own MXFP4 product
- *          would round b to Q8_0, which is coarser), or b of type MXFP4_SPLIT
- *          (ne = [K, N, n2, n3], tsk_mxfp4_quantize): both operands in 4 bits on
- *          the block-scaled matrix instructions.
+ *          bf16, the weights' values exact in bf16, but for those of 2^128 and
+ *          more, infinite there as tsk_mxfp4_dequantize has them, and NaN times 0;
+ *          ggml's own MXFP4 product would round b to Q8_0, which is coarser), or
+ *          b of type MXFP4_SPLIT (ne = [K, N, n2, n3], tsk_mxfp4_quantize): both
+ *          operands in 4 bits on the block-scaled matrix instructions, whatever
+ *          their scales.
  *   bias : nullable, F32 ne = [M]; fused ggml_add broadcast over N.
  *   dst  : F32 (or BF16), ne = [M, N, n2, n3]; rows contiguous.
  * K must be a multiple of 32 for Q8_0 and MXFP4 (their block) and of 8 otherwise.
  * MXFP4: products are exact and summed in fp32 (sums below fp32's normal range
  * may be flushed to zero); a scale byte of 255 makes its block 32 NaNs; M and K up
- * to 2^26; dst overlaps no operand and no row of its own. Scratch: MXFP4 blocks are repacked on every call (MXFP4_SPLIT weights are
- * read in place), and f32 b of larger products is rounded to bf16 rows first.
+ * to 2^26. Rows of dst that share bytes are refused (TSK_ERR_STRIDE); that dst
+ * shares none with a, b or bias is the caller's to see to, as for every weight type.
+ * Rows of b may be broadcast (strides of 0); rows that are not evenly spaced over
+ * ne1, ne2 and ne3 take a launch for every (i2, i3).
+ * Scratch: MXFP4 blocks are repacked on every call (MXFP4_SPLIT weights are read
+ * in place), and f32 b of larger products is rounded to bf16 rows first.
  */
 int tsk_mul_mat(const tsk_tensor *a, const tsk_tensor *b, const tsk_tensor *bias,
                 tsk_tensor *dst, tsk_stream stream);

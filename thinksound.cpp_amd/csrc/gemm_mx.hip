@@ -4,8 +4,8 @@
 //
 // with X in bf16 (or f32, rounded to bf16 as it is read), or X in MXFP4 too.
 // Sums are f32. With bf16 X a code times its scale is a bf16 number exactly
-// (the conversion instruction takes the scale), so v_mfma_f32_16x16x32_bf16
-// adds exact products; with MXFP4 X v_mfma_scale_f32_16x16x128_f8f6f4 takes
+// (the conversion instruction takes the scale; 2^128 and up become infinite), so
+// v_mfma_f32_16x16x32_bf16 adds exact products; with MXFP4 X v_mfma_scale_f32_16x16x128_f8f6f4 takes
 // codes and scale bytes as they lie in memory.
 //
 // Bound: few rows by the weights' bytes (8 x 8192, K = 8192 12.6 us, 2.8 TB/s);
