@@ -256,10 +256,11 @@ bool same_shape(const tsk_tensor *a, const tsk_tensor *b) {
     return true;
 }
 
-// b rows are uniformly strided over (ne1, ne2, ne3) -> one GEMM with N = ne1*ne2*ne3
+// rows nb[1] apart over all of (ne1, ne2, ne3) -> one GEMM with N = ne1*ne2*ne3;
+// the strides of outer extents of 1 do not count
 bool rows_uniform(const tsk_tensor *t) {
-    return (t->ne[2] == 1 || t->nb[2] == t->nb[1] * (size_t) t->ne[1]) &&
-           (t->ne[3] == 1 || t->nb[3] == t->nb[2] * (size_t) t->ne[2]);
+    const size_t plane = t->nb[1] * (size_t) t->ne[1];
+    return (t->ne[2] == 1 || t->nb[2] == plane) && (t->ne[3] == 1 || t->nb[3] == plane * (size_t) t->ne[2]);
 }
 
 // ---- MXFP4 tensors
