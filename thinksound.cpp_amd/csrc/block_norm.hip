@@ -5,8 +5,8 @@
 //   dst = pre(res) * pre_w * (1 + scale) + shift    (f32, bf16 or MXFP4)
 //
 // Bound by memory: x and y are read once, res and dst written once (16384 bf16 rows
-// of 4096 with both norms 129 us, 4.2 TB/s; 16384 f32 rows of 2048 with gate, scale
-// and shift 111 us, 4.9 TB/s; 388 f32 rows of 1024 4.5 us, the launch). A row's
+// of 4096 with both norms 123 us, 4.4 TB/s; 16384 f32 rows of 2048 with gate, scale
+// and shift 111 us, 4.9 TB/s; 388 f32 rows of 1024 5.1 us, the launch). A row's
 // values stay in the registers of one wave or workgroup between its passes:
 // the branch's statistics (mean, then the squared deviations from it), the
 // sum, the sum's statistics, the output.
@@ -241,10 +241,12 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void block_norm_kernel(const B
     }
 }
 
-// Rows of any length, read from memory in every pass: longer ones than the
-// registers of a workgroup hold (2000 bf16 rows of 16384, the longest that they
-// hold, 80 us, 3.3 TB/s), and MXFP4 outputs of rows that are not aligned to 16 bytes
-// (a thread holds whole blocks there, a lane of the register kernel one value).
+// Rows of any length, read from memory again in every pass, one value a load:
+// longer ones than the registers of a workgroup hold (2000 bf16 rows of 16384, the
+// longest that they hold, 71 us, 3.7 TB/s; of 16416, here, 456), and MXFP4 outputs
+// of rows that are not aligned to 16 bytes (a thread holds whole blocks there, a
+// lane of the register kernel one value: 16384 bf16 rows of 4096 1043 us, on 16-byte
+// starts 124; f32 rows of 1024 325 and 36).
 __device__ __forceinline__ float load_elt(const void *row, int bf16, int i) {
     return bf16 ? bf16_bits_to_f32(((const uint16_t *) row)[i]) : ((const float *) row)[i];
 }
@@ -341,11 +343,11 @@ hipError_t launch_nt(const BlockNorm &p, int64_t rows, hipStream_t s) {
 }
 
 // Threads a row: as few as hold it in 16 values each (8 where they come
-// alone); more cost occupancy, fewer a longer chain of sums (us, bf16 rows,
-// compared when 16384 of 4096 took 138, now 129: 256 threads 138, 128 of 32
-// values 190, 512 145; 16384 of 1024, 64 threads 32.6, now 29.4, 256 51; f32, 8192
-// of 256, 16 threads 9.7, now 9.1, 64 11.3). Where the rows leave CUs idle, twice
-// as many each time (388 f32 rows of 1024: 64 threads 5.3, 128 4.7, 256 5.2).
+// alone); more cost occupancy, fewer a longer chain of sums (us, each pair on one
+// build: 16384 bf16 rows of 4096, 256 threads 138, 128 of 32 values 190, 512 145;
+// 16384 of 1024, 64 threads 32.6, 256 51; 8192 f32 rows of 256, 16 threads 9.7, 64
+// 11.3). Where the rows leave CUs idle, twice as many each time (388 f32 rows of
+// 1024: 64 threads 5.3, 128 4.7, 256 5.2).
 template <int V>
 hipError_t launch_v(const BlockNorm &p, int64_t rows, hipStream_t s) {
     constexpr int MOST = V == 8 ? 16 : 8;

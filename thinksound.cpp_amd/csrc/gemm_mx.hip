@@ -353,9 +353,9 @@ __device__ __forceinline__ void mx_gemm_tile(const MxGemm &p, int tiles_m, int t
     // takes four turns, of lanes 0-3, 12-15, 20-27 and 4-11, 16-19, 28-31, and the
     // same 32 further: 8 rows of one lane group's chunk and the other 8 of its
     // neighbour's. The keys spread these over all 256 bytes of banks (a quarter of
-    // the 16 rows takes its own part of the chunks, in the order 0, 2, 3, 1; in the
-    // order 0 to 3 every read met itself twice: 8192^3 45 million cycles of
-    // conflicts and 285 us, so 6.5 million and 275).
+    // the 16 rows takes its own part of the chunks, in the order 0, 2, 3, 1: 8192^3
+    // 6.5 million cycles of conflicts and 275 us; in the order 0 to 3 every read
+    // meets itself twice, 45 million and 285).
     constexpr int AR = 64 / SK;
     auto quarter = [](int row) {
         const int t = row >> 2 & 3;
@@ -576,7 +576,11 @@ hipError_t launch_tile_k(const MxGemm &p, hipStream_t s) {
 }
 
 // Shapes, by number (TSK_MX_CFG), and the us of one tile a CU at K = 5120 without
-// the launch (64 x 32 and 64 x 64: alone on a CU / among two or three):
+// the launch (64 x 32 and 64 x 64: alone on a CU / among two or three). All were
+// measured with scales in chunks; where K % 128 != 0 they come with their stage and
+// the same table serves, though tiles then take longer (K = 5120 / 5056 / 5088:
+// 4096 x 4096, MXFP4 49 / 58 / 65, 2047 x 2050, bf16 54 / 55 / 57; K = 4096 / 4032 /
+// 4064: 1292 x 1024, MXFP4 11.8 / 13.0 / 15.2):
 //        both operands MXFP4                  bf16 activations
 //   1    256 x 256, 8 waves     44            -
 //   2    128 x 256, 8 waves     26            256 x 128, 8 waves    72

@@ -30,7 +30,8 @@ __device__ __forceinline__ int64_t byte_at(const Rows &t, int64_t i, int P, int 
 
 // Rows on 16-byte starts into planes: a thread takes 8 values, four neighbours a
 // block, so that a wave's loads and stores are runs of whole lines. 8192 x 8192
-// values from f32 52 us (5.8 TB/s read and written), from bf16 33 us (5.1 TB/s).
+// values from f32 53 us (5.8 TB/s read and written; 70 in turns with as large a
+// dequantization), from bf16 33 us (5.1 TB/s).
 template <bool BF16>
 __global__ void mx_quantize_kernel(const void *x, const Rows t, int64_t n8, int K8, uint8_t *codes, uint8_t *scales) {
     for (int64_t i = (int64_t) blockIdx.x * blockDim.x + threadIdx.x; i < n8; i += (int64_t) gridDim.x * blockDim.x) {

@@ -618,9 +618,11 @@ MulMatPlan plan_mul_mat(const tsk_tensor *a, const tsk_tensor *b, const tsk_tens
     pl.Nslice = pl.uni ? b->ne[1] * b->ne[2] * b->ne[3] : b->ne[1];
     if (mx) {
         // f32 activations: read and rounded by the rows kernel in every one of its
-        // workgroups, or once by a launch before the product (us, M = K = 4096: 16
-        // rows 10.6 / 9.6, 32 rows 12.9 / 11.3; K = 1024, M = 4096, 64 rows 6.6 /
-        // 7.2; K = M = 1024, 77 rows 4.5 / 6.2; K = M = 8192, 8 rows 17.4 / 15.1)
+        // workgroups, or once by a launch before the product (us: K = M = 1024, 77
+        // rows 4.5 / 6.2; K = 1024, M = 4096, 64 rows 6.6 / 7.2; M = K = 4096, 16
+        // rows 10.6 / 9.6, 32 rows 12.9 / 11.3; K = M = 8192, 8 rows 17.4 / 15.1).
+        // The product of the sizes alone does not separate the two: at 2^28, which
+        // goes to the rows kernel, 64 rows gain 0.6 by that and 16 lose 1.0
         pl.mx = true;
         pl.wbytes = a->type == TSK_TYPE_MXFP4 ? align256(tsk_mxfp4_split_nbytes(K, M)) : 0;
         if (b->type == TSK_TYPE_F32 && (double) pl.Nslice * (double) K * (double) M > (double) (1 << 28))
