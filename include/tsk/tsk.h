@@ -30,7 +30,10 @@
  *   tsk_block_norm      <- the adaLN glue of a block: x + gate * y, ggml_norm,
  *                          x * (1 + scale) + shift             src/mmdit.cpp:55-59, :231-234
  *   tsk_mxfp4_*         4-bit block-scaled (MXFP4) tensors, no counterpart in
- *                       the reference's files
+ *                       the reference's files; nor have these:
+ *   tsk_i8_*            8-bit rows with one scale each
+ *   tsk_rope_axes       rotary positions over several axes
+ *   tsk_cross_attention attention to an encoder's states of another length
  *
  * Conventions (all follow ggml):
  *   - tensors are non-owning views: ne[] = extents with ne[0] fastest,
@@ -78,7 +81,13 @@ enum tsk_type {
      * r = (i3 * ne2 + i2) * ne1 + i1: codes uint8 [rows][ne0 / 2] (value 2 i in
      * byte i's low nibble, 2 i + 1 in the high one) followed by scale bytes
      * uint8 [rows][ne0 / 32]; nb[] are ignored. data is 16-byte aligned. */
-    TSK_TYPE_MXFP4_SPLIT = 0x1027
+    TSK_TYPE_MXFP4_SPLIT = 0x1027,
+    /* Extension: rows of 8-bit integers with one scale each (a scale a token of
+     * activations, a scale a channel of weights), two planes over the rows r as
+     * above: int8 q[rows][ld], ld = ne0 rounded up to a multiple of 16, the bytes
+     * past ne0 zero, followed by f32 d[rows]; nb[] are ignored. Value i of row r is
+     * d[r] * q[r][i]. data is 16-byte aligned. */
+    TSK_TYPE_I8_SPLIT = 0x1018
 };
 
 /* ggml_prec values (ggml_flash_attn_ext_set_prec). */
@@ -149,8 +158,8 @@ const char *tsk_version(void);
 
 /*
  * dst = a x b (+ bias), ggml_mul_mat semantics.
- *   a    : weight, ne = [K, M, 1, 1]; F32, F16, BF16, Q8_0, Q8_0_SPLIT, MXFP4
- *          or MXFP4_SPLIT. Rows must be contiguous (nb[0] = element/block size).
+ *   a    : weight, ne = [K, M, 1, 1]; F32, F16, BF16, Q8_0, Q8_0_SPLIT, MXFP4,
+ *          MXFP4_SPLIT or I8_SPLIT. Rows must be contiguous (nb[0] = element/block size).
  *   b    : activations, ne = [K, N, n2, n3]; F32 (or BF16), rows contiguous.
  *          As in ggml, b is first converted to a's vec_dot type: BF16 weights
  *          round b to bf16 (RNE); Q8_0 weights quantize b per 32-block to Q8_0
@@ -161,10 +170,14 @@ const char *tsk_version(void);
  *          ggml's own MXFP4 product would round b to Q8_0, which is coarser), or
  *          b of type MXFP4_SPLIT (ne = [K, N, n2, n3], tsk_mxfp4_quantize): both
  *          operands in 4 bits on the block-scaled matrix instructions, whatever
- *          their scales.
+ *          their scales. I8_SPLIT weights multiply F32 / BF16 b as tsk_i8_quantize
+ *          rounds its rows (a scale a token), or b of type I8_SPLIT (ne = [K, N, n2, n3]).
  *   bias : nullable, F32 ne = [M]; fused ggml_add broadcast over N.
  *   dst  : F32 (or BF16), ne = [M, N, n2, n3]; rows contiguous.
- * K must be a multiple of 32 for Q8_0 and MXFP4 (their block) and of 8 otherwise.
+ * K must be a multiple of 32 for Q8_0 and MXFP4 (their block), any for I8_SPLIT and a
+ * multiple of 8 otherwise.
+ * I8_SPLIT: sums are exact (int32; K below 2^17), rounded once to fp32, then times the
+ * token's scale, times the channel's, plus bias; M up to 2^26, dst as for MXFP4.
  * MXFP4: products are exact and summed in fp32 (sums below fp32's normal range
  * may be flushed to zero); a scale byte of 255 makes its block 32 NaNs; M and K up
  * to 2^26. Rows of dst that share bytes are refused (TSK_ERR_STRIDE); that dst
@@ -172,7 +185,8 @@ const char *tsk_version(void);
  * Rows of b may be broadcast (strides of 0); rows that are not evenly spaced over
  * ne1, ne2 and ne3 take a launch for every (i2, i3).
  * Scratch: MXFP4 blocks are repacked on every call (MXFP4_SPLIT weights are read
- * in place), and f32 b of larger products is rounded to bf16 rows first.
+ * in place), and f32 b of larger products is rounded to bf16 rows first; I8_SPLIT
+ * weights: the planes of F32 / BF16 b.
  */
 int tsk_mul_mat(const tsk_tensor *a, const tsk_tensor *b, const tsk_tensor *bias,
                 tsk_tensor *dst, tsk_stream stream);
@@ -306,6 +320,80 @@ int tsk_mxfp4_repack(const tsk_tensor *src, tsk_tensor *dst, tsk_stream stream);
 /* Bytes an MXFP4_SPLIT tensor of ne = [K, M] occupies (0 unless K % 32 == 0). */
 size_t tsk_mxfp4_split_nbytes(int64_t K, int64_t M);
 
+/* ---- 8-bit rows: symmetric integers, one scale a row ------------------------ */
+
+/*
+ * Quantize rows to I8_SPLIT: x F32 or BF16, rows contiguous and aligned to their
+ * element, any ne0; dst I8_SPLIT of the same shape. Per row: amax = max |x|, d =
+ * max(amax, 2^-100) / 127 in fp32, q = the integer nearest to x / d (ties to even),
+ * within [-127, 127]. A row that holds an infinity or a NaN gets d = NaN and q = 0.
+ * x and dst must not overlap.
+ */
+int tsk_i8_quantize(const tsk_tensor *x, tsk_tensor *dst, tsk_stream stream);
+/* d * q of an I8_SPLIT tensor, an fp32 product, as F32 rows or rounded to BF16 rows. */
+int tsk_i8_dequantize(const tsk_tensor *x, tsk_tensor *dst, tsk_stream stream);
+/* Bytes an I8_SPLIT tensor of `rows` rows of K values occupies. */
+size_t tsk_i8_split_nbytes(int64_t K, int64_t rows);
+
+/* ---- rotary positions over several axes ------------------------------------- */
+
+enum tsk_rope_pairs {
+    TSK_ROPE_PAIRS_ADJACENT = 0,   /* pair i: values 2 i and 2 i + 1                    */
+    TSK_ROPE_PAIRS_HALVES   = 1    /* pair i: values i and n / 2 + i, n = sum of dims   */
+};
+typedef struct tsk_rope_axes_params {
+    int   n_axes;                /* 1 .. 4                                               */
+    int   dims[4];               /* values of a head that turn with each axis, even; 0: none */
+    int   pairs;                 /* enum tsk_rope_pairs                                  */
+    int   shared_freqs;          /* 0: pair j of axis a has freq_base^(-2 j / dims[a]),
+                                  * else pair i of all has freq_base^(-2 i / n)          */
+    float freq_base, freq_scale; /* angle = freq_scale * position * frequency            */
+    const tsk_tensor *w;         /* nullable, F32 [D]: RMS norm of every head times w first */
+    float eps;                   /* of that norm                                         */
+} tsk_rope_axes_params;
+/*
+ * Rotary positions of tokens that have several (time, height and width of a video's
+ * patches, say): the pairs of a head are dealt to the axes in order, dims[a] / 2 each,
+ * and pair (x, y) on axis a becomes (x cos t - y sin t, x sin t + y cos t), t =
+ * freq_scale * pos[a] * its frequency. Values past the pairs are copied (after the norm).
+ *   x   : F32 or BF16, ne = [D, n_head, S, B], D <= 384, rows contiguous
+ *   pos : I32 or F32, ne = [S, n_axes, B or 1], rows contiguous; fractions are taken
+ *   dst : F32 or BF16 of x's shape; may be x itself, no other overlap
+ * Angles are formed in 64 bits (tsk_rope_ext: as ggml's running fp32 product), sines and
+ * cosines are within 2^-22; a position that is infinite or NaN gives NaN.
+ */
+int tsk_rope_axes(const tsk_tensor *x, const tsk_tensor *pos, const tsk_rope_axes_params *p, tsk_tensor *dst,
+                  tsk_stream stream);
+
+/* ---- attention to an encoder's states ---------------------------------------- */
+
+typedef struct tsk_cross_attn_params {
+    float scale;                 /* factor of q . k, > 0                                 */
+    const tsk_tensor *kv_len;    /* nullable, I32 [B]: states of each sequence, those from
+                                  * there on do not count (clamped to 0 .. Nkv)          */
+    const tsk_tensor *q_len;     /* nullable, I32 [B]: tokens of each sequence (clamped)  */
+    const uint8_t *kv_valid;     /* nullable, DEVICE [B][Nkv]: 0 marks a state that does not count */
+    int64_t kv_valid_nb;         /* bytes between two sequences' flags; 0 shares one       */
+} tsk_cross_attn_params;
+/*
+ * Attention of tokens to states of another number (a text's or a video's), softmax over
+ * the states that count:
+ *   q    : ne = [D, Nq, H, B]    F32, F16 or BF16, converted to k's type
+ *   k, v : ne = [D, Nkv, Hkv, B] F16 or BF16, H % Hkv == 0 (head h reads h / (H / Hkv))
+ *   dst  : ne = [D, H, Nq, B]    F32, F16 or BF16 (ggml's permuted result)
+ * D is a multiple of 8, at most 128; rows are contiguous on 16-byte starts, and their
+ * strides any (k and v: at most 2^24 bytes from a state to the next). A token that no
+ * state counts for gets 0; what the states that do not count hold, infinities and NaNs
+ * too, has no effect. Tokens from q_len on are not written.
+ * Products are exact and logits, softmax and sums fp32; the weights are rounded to k's
+ * type before they multiply v (bf16: within 2^-8, f16: 2^-11) and are divided by
+ * the sum of what they were rounded to. dst must not overlap an input. Scratch: long
+ * states of few tokens are dealt to several workgroups, whose sums meet in the stream's
+ * workspace (tsk_workspace_size, TSK_OP_CROSS_ATTENTION).
+ */
+int tsk_cross_attention(const tsk_tensor *q, const tsk_tensor *k, const tsk_tensor *v,
+                        const tsk_cross_attn_params *p, tsk_tensor *dst, tsk_stream stream);
+
 /* ---- norms before and after a block, its gate and residual ---------------- */
 
 enum tsk_norm_kind {
@@ -338,8 +426,9 @@ typedef struct tsk_block_norm_params {
  *   gate, scale, shift: F32, ne[0] = C, every other extent x's or 1; rows contiguous
  *   res : nullable; x's type and shape. May be x itself (the same data and strides)
  *   dst : nullable (the residual alone: pre_norm NONE, no pre_w / scale / shift);
- *         F32, BF16, or MXFP4_SPLIT (C % 32 == 0: tsk_mxfp4_quantize's rounding of
- *         the row, the operand of an MXFP4 product). At least one of res and dst.
+ *         F32, BF16, MXFP4_SPLIT (C % 32 == 0: tsk_mxfp4_quantize's rounding of
+ *         the row, the operand of an MXFP4 product) or I8_SPLIT (tsk_i8_quantize's,
+ *         that of an 8-bit product). At least one of res and dst.
  * Outputs must not overlap each other or any input, but for res in place of x.
  */
 int tsk_block_norm(const tsk_tensor *x, const tsk_tensor *y, const tsk_block_norm_params *p,
@@ -428,7 +517,8 @@ enum tsk_op {
     TSK_OP_CONV1D         = 7,   /* srcs: w, x, bias; tsk_supports_op: s0 = 1, p0 = 1, d0 = 1 */
     TSK_OP_CONV_MLP_SWIGLU = 8,  /* srcs: w1, w3, w2, x */
     TSK_OP_MLP_SWIGLU     = 9,   /* srcs: w1, w3, w2, x */
-    TSK_OP_RMS_NORM_Q8_0  = 10   /* srcs: x, w */
+    TSK_OP_RMS_NORM_Q8_0  = 10,  /* srcs: x, w */
+    TSK_OP_CROSS_ATTENTION = 11  /* srcs: q, k, v */
 };
 /* Mirror of a ggml backend's supports_op: 1 if tsk would run the node with
  * these operand descriptors (data pointers are not inspected), else 0.

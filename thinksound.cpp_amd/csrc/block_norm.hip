@@ -2,7 +2,7 @@
 // (x + gate * y, ggml_norm and modulate of src/mmdit.cpp:55-59, :231-234):
 //
 //   r   = res_scale * x + gate * post(y),  res = r in x's type
-//   dst = pre(res) * pre_w * (1 + scale) + shift    (f32, bf16 or MXFP4)
+//   dst = pre(res) * pre_w * (1 + scale) + shift    (f32, bf16, MXFP4 or 8-bit rows)
 //
 // Bound by memory: x and y are read once, res and dst written once (16384 bf16 rows
 // of 4096 with both norms 123 us, 4.4 TB/s; 16384 f32 rows of 2048 with gate, scale
@@ -12,6 +12,7 @@
 // sum, the sum's statistics, the output.
 #include <algorithm>
 
+#include "i8.h"
 #include "mxfp4.h"
 #include "tsk_internal.h"
 
@@ -114,6 +115,21 @@ __device__ __forceinline__ float row_sum(float v, float *red, int &turn) {
     return v;
 }
 
+// the largest of magnitudes' bits over the NT threads of a row, as row_sum sums
+template <int NT>
+__device__ __forceinline__ uint32_t row_top(uint32_t v, float *red, int &turn) {
+    for (int m = 1; m < (NT < 64 ? NT : 64); m *= 2) v = max(v, (uint32_t) __shfl_xor((int) v, m));
+    if constexpr (NT > 64) {
+        uint32_t *half = (uint32_t *) red + (turn ^= 1) * (NT / 64);
+        if ((threadIdx.x & 63) == 0) half[threadIdx.x % NT >> 6] = v;
+        __syncthreads();
+        v = 0;
+#pragma unroll
+        for (int i = 0; i < NT / 64; ++i) v = max(v, half[i]);
+    }
+    return v;
+}
+
 // One row: thread t holds the V-vectors t, t + NT, ..., VN of them at most.
 // mean and 1 / sqrt(var + eps) of the C values (LAYER), or 0 and 1 / sqrt(mean of squares + eps) (RMS)
 template <int V, int VN, int NT>
@@ -187,7 +203,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void block_norm_kernel(const B
         const int i1 = (int) (r % p.n1), i2 = (int) (r / p.n1 % p.n2), i3 = (int) (r / p.n1 / p.n2);
         const bool has_y = p.y.data, has_gate = MOD && p.gate.data, has_scale = MOD && p.scale.data, has_shift = MOD && p.shift.data;
         const bool has_post_w = WTS && p.post_w, has_pre_w = WTS && p.pre_w;
-        const bool has_out = p.dst.data || p.scales;
+        const bool has_out = p.dst.data || p.scales || p.i8;
         float x[VN][V], y[VN][V], w[VN][V] = {}, f[VN][V] = {}, h[VN][V] = {}, mean, inv;
         load_row<V, VN, NT>(row_of(p.x, i1, i2, i3), p.x_bf16, C, t, x);
         if (has_y) {
@@ -223,6 +239,26 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void block_norm_kernel(const B
                 x[j][e] = modulated(x[j][e], p.pre_norm, mean, inv, has_pre_w, w[j][e], has_scale, f[j][e], has_shift, h[j][e]);
         if (p.dst.data) {
             if (mine) store_row<V, VN, NT>(row_of(p.dst, i1, i2, i3), p.dst_bf16, C, t, x);
+        } else if (p.i8) {
+            const int ld = (int) i8_ld(C);
+            uint32_t top = 0;
+#pragma unroll
+            for (int j = 0; j < VN; ++j)
+                if ((t + NT * j) * V < C)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) top = max(top, i8_abs_bits(x[j][e]));
+            const I8Scale s = i8_scale(row_top<NT>(top, my_red, turn));
+            if (!mine) continue;
+            int8_t *q = p.i8 + r * ld;
+#pragma unroll
+            for (int j = 0; j < VN; ++j) {
+                const int c = (t + NT * j) * V;
+                if (c >= C) continue;
+                if constexpr (V == 8) *(u32x2 *) (q + c) = u32x2{i8_pack4(x[j], s), i8_pack4(x[j] + 4, s)};
+                else q[c] = s.inv == 0.0f ? (int8_t) 0 : (int8_t) i8_code(x[j][0], s);
+            }
+            if (t < ld - C) q[C + t] = 0;                        // (at most 15: a row has 16 threads at least)
+            if (t == 0) p.i8_d[r] = s.d;
         } else if constexpr (V == 8) {
             // a block of 32 is four threads' vectors (C % 32 == 0: all four hold one, or none)
 #pragma unroll
@@ -286,13 +322,22 @@ __global__ __launch_bounds__(256) void block_norm_long_kernel(const BlockNorm p)
             const float b = branch(load_elt(y, p.y_bf16, i), p.post_norm, ymean, yinv, p.post_w, p.post_w ? p.post_w[i] : 0.0f);
             return as_type(residual(xv, p.res_scale, b, gate, gate ? gate[i] : 0.0f), p.x_bf16);
         };
-        if (p.dst.data || p.scales) {
+        if (p.dst.data || p.scales || p.i8) {
             long_stats(p.pre_norm, C, p.pre_eps, red, turn, sum, mean, inv);
             auto out = [&](int i) {
                 return modulated(sum(i), p.pre_norm, mean, inv, p.pre_w, p.pre_w ? p.pre_w[i] : 0.0f, scale,
                                  scale ? scale[i] : 0.0f, shift, shift ? shift[i] : 0.0f);
             };
-            if (p.scales) {
+            if (p.i8) {
+                const int64_t ld = i8_ld(C);
+                uint32_t top = 0;
+                for (int i = threadIdx.x; i < C; i += 256) top = max(top, i8_abs_bits(out(i)));
+                const I8Scale s = i8_scale(row_top<256>(top, red, turn));
+                int8_t *q = p.i8 + r * ld;
+                for (int64_t i = threadIdx.x; i < ld; i += 256)
+                    q[i] = i < C && s.inv != 0.0f ? (int8_t) i8_code(out((int) i), s) : (int8_t) 0;
+                if (threadIdx.x == 0) p.i8_d[r] = s.d;
+            } else if (p.scales) {
                 for (int kb = threadIdx.x; kb < C / 32; kb += 256) {
                     float v[32];
                     uint32_t top = 0;

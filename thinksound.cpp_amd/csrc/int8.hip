@@ -1,0 +1,196 @@
+// int8.hip — rows to 8-bit integers with one scale each, and back.
+//
+// d = max(amax, 2^-100) / 127, q = the integer nearest to x / d (i8.h). Bound by memory:
+// a row is read once into the registers of the threads that share it, whose largest
+// magnitude is found between the load and the store.
+#include <algorithm>
+
+#include "i8.h"
+#include "tsk_internal.h"
+
+namespace tsk {
+
+namespace {
+
+struct Rows {
+    int64_t nb1, nb2, nb3;
+    int ne1, ne2;
+};
+__device__ __forceinline__ int64_t row_at(const Rows &t, int64_t r) {
+    const int64_t i1 = r % t.ne1, q = r / t.ne1;
+    return i1 * t.nb1 + q % t.ne2 * t.nb2 + q / t.ne2 * t.nb3;
+}
+
+// 8 values from column c on, those past K zeros
+template <bool BF16, bool WIDE>
+__device__ __forceinline__ void load8(const char *row, int c, int K, float *v) {
+    if (WIDE && c + 8 <= K) {
+        if constexpr (BF16) {
+            const u32x4 w = *(const u32x4 *) (row + (int64_t) c * 2);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                v[2 * q] = __uint_as_float(w[q] << 16);
+                v[2 * q + 1] = __uint_as_float(w[q] & 0xffff0000u);
+            }
+        } else {
+            const f32x4 a = ((const f32x4 *) (row + (int64_t) c * 4))[0], b = ((const f32x4 *) (row + (int64_t) c * 4))[1];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[e] = a[e];
+                v[4 + e] = b[e];
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = c + e < K ? load_as_f32<BF16 ? Elt::BF16 : Elt::F32>(row, c + e) : 0.0f;
+}
+
+// the largest of the NT threads of a row: 8 to 64 lanes of a wave, or NT / 64 waves
+template <int NT>
+__device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t *red) {
+    // (magnitudes' bits order like unsigned integers, NaNs on top)
+    for (int m = 1; m < (NT < 64 ? NT : 64); m *= 2) v = max(v, (uint32_t) __shfl_xor((int) v, m));
+    if constexpr (NT > 64) {
+        uint32_t *own = red + threadIdx.x / NT * (NT / 64);
+        __syncthreads();                                     // (the row before may still be read)
+        if ((threadIdx.x & 63) == 0) own[threadIdx.x % NT >> 6] = v;
+        __syncthreads();
+        v = 0;
+#pragma unroll
+        for (int i = 0; i < NT / 64; ++i) v = max(v, own[i]);
+    }
+    return v;
+}
+
+// NT threads a row, VN vectors of 8 values each in registers; rows longer than that
+// (LONG) are read a second time.
+template <bool BF16, bool WIDE, int VN, int NT, bool LONG>
+__global__ __launch_bounds__(NT < 256 ? 256 : NT) void i8_quantize_kernel(const void *x, const Rows t, int64_t rows, int K, int64_t ld,
+                                                                          int8_t *q, float *d) {
+    __shared__ uint32_t red[NT > 64 ? (NT < 256 ? 256 : NT) / 64 : 1];
+    constexpr int RW = NT < 256 ? 256 / NT : 1;
+    const int th = threadIdx.x % NT;
+    for (int64_t r0 = (int64_t) blockIdx.x * RW; r0 < rows; r0 += (int64_t) gridDim.x * RW) {
+        const bool mine = r0 + threadIdx.x / NT < rows;
+        const int64_t r = mine ? r0 + threadIdx.x / NT : rows - 1;
+        const char *row = (const char *) x + row_at(t, r);
+        float v[VN][8];
+        uint32_t top = 0;
+        if constexpr (LONG) {
+            for (int c = th * 8; c < K; c += NT * 8) {
+                load8<BF16, WIDE>(row, c, K, v[0]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = max(top, i8_abs_bits(v[0][e]));
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < VN; ++j) load8<BF16, WIDE>(row, (th + NT * j) * 8, K, v[j]);
+#pragma unroll
+            for (int j = 0; j < VN; ++j)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = max(top, i8_abs_bits(v[j][e]));
+        }
+        top = row_max<NT>(top, red);
+        const I8Scale s = i8_scale(top);
+        if (!mine) continue;
+        auto store = [&](int c, const float *w) {
+            if (c < ld) *(u32x2 *) (q + r * ld + c) = u32x2{i8_pack4(w, s), i8_pack4(w + 4, s)};
+        };
+        if constexpr (LONG) {
+            for (int c = th * 8; c < ld; c += NT * 8) {
+                load8<BF16, WIDE>(row, c, K, v[0]);
+                store(c, v[0]);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < VN; ++j) store((th + NT * j) * 8, v[j]);
+        }
+        if (th == 0) d[r] = s.d;
+    }
+}
+
+template <bool BF16, bool WIDE>
+hipError_t launch_quantize(const void *x, const Rows &t, int64_t rows, int K, int64_t ld, int8_t *q, float *d, hipStream_t s) {
+    auto go = [&](auto kern, int nt) {
+        const int rw = nt < 256 ? 256 / nt : 1;
+        launch_kernel(kern, dim3((unsigned) std::min<int64_t>((rows + rw - 1) / rw, 1 << 20)), dim3(nt < 256 ? 256 : nt), 0, s, x, t,
+                      rows, K, ld, q, d);
+        return hipGetLastError();
+    };
+    if (ld <= 16 * 8) return go(i8_quantize_kernel<BF16, WIDE, 1, 16, false>, 16);
+    if (ld <= 64 * 8) return go(i8_quantize_kernel<BF16, WIDE, 1, 64, false>, 64);
+    if (ld <= 128 * 8) return go(i8_quantize_kernel<BF16, WIDE, 1, 128, false>, 128);
+    if (ld <= 256 * 16) return go(i8_quantize_kernel<BF16, WIDE, 2, 256, false>, 256);
+    if (ld <= 512 * 16) return go(i8_quantize_kernel<BF16, WIDE, 2, 512, false>, 512);
+    if (ld <= 1024 * 16) return go(i8_quantize_kernel<BF16, WIDE, 2, 1024, false>, 1024);
+    return go(i8_quantize_kernel<BF16, WIDE, 1, 1024, true>, 1024);
+}
+
+// One thread per 8 values
+template <bool BF16, bool WIDE>
+__global__ void i8_dequantize_kernel(const int8_t *q, const float *d, int64_t rows, int K, int P, void *y, const Rows t) {
+    const int64_t n = rows * P, ld = i8_ld(K);
+    for (int64_t i = (int64_t) blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t) gridDim.x * blockDim.x) {
+        const int64_t r = i / P;
+        const int c = (int) (i - r * P) * 8;
+        const u32x2 w = *(const u32x2 *) (q + r * ld + c);
+        const float s = d[r];
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = s * (float) (int8_t) (w[e >> 2] >> 8 * (e & 3));
+        char *row = (char *) y + row_at(t, r);
+        if (WIDE && c + 8 <= K) {
+            if constexpr (BF16) {
+                u32x4 h;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) h[e] = f32_to_bf16_bits(v[2 * e]) | (uint32_t) f32_to_bf16_bits(v[2 * e + 1]) << 16;
+                *(u32x4 *) (row + (int64_t) c * 2) = h;
+            } else {
+                ((f32x4 *) (row + (int64_t) c * 4))[0] = f32x4{v[0], v[1], v[2], v[3]};
+                ((f32x4 *) (row + (int64_t) c * 4))[1] = f32x4{v[4], v[5], v[6], v[7]};
+            }
+            continue;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (c + e < K) store_from_f32<BF16 ? Elt::BF16 : Elt::F32>(row, c + e, v[e]);
+    }
+}
+
+Rows rows_of(const View4 &t) {
+    Rows r;
+    r.nb1 = t.nb[1]; r.nb2 = t.nb[2]; r.nb3 = t.nb[3];
+    r.ne1 = (int) t.ne[1]; r.ne2 = (int) t.ne[2];
+    return r;
+}
+bool on_16(const View4 &t) {
+    bool ok = (uintptr_t) t.data % 16 == 0;
+    for (int i = 1; i < 4; ++i) ok = ok && (t.ne[i] == 1 || t.nb[i] % 16 == 0);
+    return ok;
+}
+
+}  // namespace
+
+hipError_t launch_i8_quantize(const View4 &x, int8_t *q, float *d, hipStream_t s) {
+    const int64_t rows = x.ne[1] * x.ne[2] * x.ne[3], ld = i8_ld(x.ne[0]);
+    const int K = (int) x.ne[0];
+    const Rows t = rows_of(x);
+    const bool wide = on_16(x);
+    if (x.type == TSK_TYPE_BF16)
+        return wide ? launch_quantize<true, true>(x.data, t, rows, K, ld, q, d, s) : launch_quantize<true, false>(x.data, t, rows, K, ld, q, d, s);
+    return wide ? launch_quantize<false, true>(x.data, t, rows, K, ld, q, d, s) : launch_quantize<false, false>(x.data, t, rows, K, ld, q, d, s);
+}
+
+hipError_t launch_i8_dequantize(const int8_t *q, const float *d, const View4 &y, hipStream_t s) {
+    const int64_t rows = y.ne[1] * y.ne[2] * y.ne[3];
+    const int K = (int) y.ne[0], P = (K + 7) / 8;
+    const bool bf16 = y.type == TSK_TYPE_BF16, wide = on_16(y);
+    launch_kernel(bf16 ? wide ? i8_dequantize_kernel<true, true> : i8_dequantize_kernel<true, false>
+                       : wide ? i8_dequantize_kernel<false, true> : i8_dequantize_kernel<false, false>,
+                  dim3((unsigned) std::min<int64_t>((rows * P + 255) / 256, 1 << 20)), dim3(256), 0, s, q, d, rows, K, P, (void *) y.data,
+                  rows_of(y));
+    return hipGetLastError();
+}
+
+}  // namespace tsk

@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -13,6 +14,7 @@
 #include <utility>
 
 #include "../../include/tsk/tsk.h"
+#include "i8.h"
 #include "tsk_internal.h"
 #include "tsk_runtime.h"
 
@@ -266,6 +268,7 @@ bool rows_uniform(const tsk_tensor *t) {
 // ---- MXFP4 tensors
 constexpr int64_t MX_MAX_EXTENT = 0x7fffffff - 255;     // (tiles past the end stay in int)
 constexpr int64_t MX_MAX_WEIGHT = 1 << 26;              // K and M of a product's weights
+constexpr int64_t I8_MAX_K = (1 << 17) - 1;             // 8-bit products: 2^14 K, the largest sum, stays below 2^31
 
 // rows of ne1 x ne2 x ne3 within MX_MAX_EXTENT (the extents are >= 1)
 bool rows_fit(const tsk_tensor *t) {
@@ -329,12 +332,24 @@ int check_mx(const tsk_tensor *t, const char *name) {
     if (!aligned(t->data, 16)) return fail(TSK_ERR_ALIGN, "%s: MXFP4_SPLIT data must be 16-byte aligned", name);
     return TSK_OK;
 }
+// 8-bit rows with a scale each
+int check_i8(const tsk_tensor *t, const char *name) {
+    if (t->type != TSK_TYPE_I8_SPLIT) return fail(TSK_ERR_TYPE, "%s must be I8_SPLIT", name);
+    if (t->ne[0] > MX_MAX_EXTENT || !rows_fit(t)) return fail(TSK_ERR_SHAPE, "%s is too large", name);
+    if (!aligned(t->data, 16)) return fail(TSK_ERR_ALIGN, "%s: I8_SPLIT data must be 16-byte aligned", name);
+    return TSK_OK;
+}
+int8_t *i8_codes(const tsk_tensor *t) { return (int8_t *) t->data; }
+float *i8_scales(const tsk_tensor *t) { return (float *) ((char *) t->data + (size_t) row_count(t) * (size_t) i8_ld(t->ne[0])); }
+size_t i8_bytes(int64_t K, int64_t rows) { return (size_t) rows * ((size_t) i8_ld(K) + 4); }
+
 uint8_t *mx_codes(const tsk_tensor *t) { return (uint8_t *) t->data; }
 uint8_t *mx_scales(const tsk_tensor *t) { return (uint8_t *) t->data + (size_t) row_count(t) * (size_t) (t->ne[0] / 2); }
 
 // bytes from the first of a tensor to past its last
 size_t span_bytes(const tsk_tensor *t) {
     if (t->type == TSK_TYPE_MXFP4_SPLIT) return (size_t) row_count(t) * (size_t) (t->ne[0] / 32 * 17);
+    if (t->type == TSK_TYPE_I8_SPLIT) return i8_bytes(t->ne[0], row_count(t));
     size_t n = row_bytes(t);
     for (int i = 1; i < 4; ++i) n += (size_t) (t->ne[i] - 1) * t->nb[i];
     return n;
@@ -344,7 +359,8 @@ size_t span_bytes(const tsk_tensor *t) {
 bool may_overlap(const tsk_tensor *a, const tsk_tensor *b) {
     const uintptr_t pa = (uintptr_t) a->data, pb = (uintptr_t) b->data;
     if (pa + span_bytes(a) <= pb || pb + span_bytes(b) <= pa) return false;
-    if (a->type == TSK_TYPE_MXFP4_SPLIT || b->type == TSK_TYPE_MXFP4_SPLIT) return true;
+    for (const tsk_tensor *t : {a, b})
+        if (t->type == TSK_TYPE_MXFP4_SPLIT || t->type == TSK_TYPE_I8_SPLIT) return true;
     size_t ld = 0;
     for (const tsk_tensor *t : {a, b})
         for (int i = 1; i < 4; ++i)
@@ -467,11 +483,12 @@ int validate_mul_mat(const tsk_tensor *a, const tsk_tensor *b, const tsk_tensor 
     if (dst->ne[0] != M || dst->ne[1] != b->ne[1] || dst->ne[2] != b->ne[2] || dst->ne[3] != b->ne[3])
         return fail(TSK_ERR_SHAPE, "dst must be [M=%lld, %lld, %lld, %lld]", (long long) M, (long long) b->ne[1], (long long) b->ne[2], (long long) b->ne[3]);
     const bool mx = a->type == TSK_TYPE_MXFP4 || a->type == TSK_TYPE_MXFP4_SPLIT, mx_b = mx && b->type == TSK_TYPE_MXFP4_SPLIT;
-    if (b->type != TSK_TYPE_F32 && b->type != TSK_TYPE_BF16 && !mx_b)
-        return fail(TSK_ERR_TYPE, mx ? "b must be F32, BF16 or MXFP4_SPLIT" : "b must be F32 or BF16");
+    const bool i8 = a->type == TSK_TYPE_I8_SPLIT, i8_b = i8 && b->type == TSK_TYPE_I8_SPLIT, planes_b = mx_b || i8_b;
+    if (b->type != TSK_TYPE_F32 && b->type != TSK_TYPE_BF16 && !planes_b)
+        return fail(TSK_ERR_TYPE, mx ? "b must be F32, BF16 or MXFP4_SPLIT" : i8 ? "b must be F32, BF16 or I8_SPLIT" : "b must be F32 or BF16");
     if (dst->type != TSK_TYPE_F32 && dst->type != TSK_TYPE_BF16) return fail(TSK_ERR_TYPE, "dst must be F32 or BF16");
-    if (mx_b && !aligned(b->data, 16)) return fail(TSK_ERR_ALIGN, "MXFP4_SPLIT b must be 16-byte aligned");
-    if ((!mx_b && (rc = check_rows(b, "b", 16))) || (rc = check_rows(dst, "dst", 16))) return rc;
+    if (planes_b && !aligned(b->data, 16)) return fail(TSK_ERR_ALIGN, "%s b must be 16-byte aligned", mx_b ? "MXFP4_SPLIT" : "I8_SPLIT");
+    if ((!planes_b && (rc = check_rows(b, "b", 16))) || (rc = check_rows(dst, "dst", 16))) return rc;
     if (bias) {
         if (bias->type != TSK_TYPE_F32 || bias->ne[0] != M || bias->ne[1] * bias->ne[2] * bias->ne[3] != 1)
             return fail(TSK_ERR_SHAPE, "bias must be F32 [M]");
@@ -500,6 +517,12 @@ int validate_mul_mat(const tsk_tensor *a, const tsk_tensor *b, const tsk_tensor 
             if ((rc = check_rows_apart(dst, "dst"))) return rc;
             if (a->type == TSK_TYPE_MXFP4) return check_mx_blocks(a, "a");
             if (!aligned(a->data, 16)) return fail(TSK_ERR_ALIGN, "MXFP4_SPLIT data must be 16-byte aligned");
+            break;
+        case TSK_TYPE_I8_SPLIT:
+            if (K > I8_MAX_K || M > MX_MAX_WEIGHT) return fail(TSK_ERR_SHAPE, "I8_SPLIT weights of [%lld, %lld]", (long long) K, (long long) M);
+            if (!rows_fit(b)) return fail(TSK_ERR_SHAPE, "b has too many rows");
+            if ((rc = check_rows_apart(dst, "dst"))) return rc;
+            if (!aligned(a->data, 16)) return fail(TSK_ERR_ALIGN, "I8_SPLIT data must be 16-byte aligned");
             break;
         case TSK_TYPE_F32:
             // vec_dot type F32: the activations stay fp32
@@ -604,6 +627,7 @@ struct MulMatPlan {
     size_t wbytes;       // Q8_0: the weights repacked into planes
     size_t act_bytes;    // Q8_0 / Q8_0_SPLIT: the quantized activation planes
     bool mx;             // MXFP4 weights
+    bool i8;             // I8_SPLIT weights; act_bytes: the planes of f32 / bf16 activations
     size_t bytes;        // scratch the call needs
 };
 
@@ -611,6 +635,15 @@ MulMatPlan plan_mul_mat(const tsk_tensor *a, const tsk_tensor *b, const tsk_tens
     MulMatPlan pl;
     memset(&pl, 0, sizeof(pl));
     const int64_t K = a->ne[0], M = a->ne[1];
+    if (a->type == TSK_TYPE_I8_SPLIT) {
+        pl.i8 = true;
+        pl.uni = row_stride(dst) != 0;
+        pl.nslices = pl.uni ? 1 : b->ne[2] * b->ne[3];
+        pl.Nslice = pl.uni ? row_count(b) : b->ne[1];
+        if (b->type != TSK_TYPE_I8_SPLIT) pl.act_bytes = align256(i8_bytes(K, row_count(b)));
+        pl.bytes = pl.act_bytes;
+        return pl;
+    }
     // slices of uniformly strided rows: one launch per (i2, i3) unless rows are uniform
     const bool mx = a->type == TSK_TYPE_MXFP4 || a->type == TSK_TYPE_MXFP4_SPLIT;
     pl.uni = mx ? (b->type == TSK_TYPE_MXFP4_SPLIT || row_stride(b)) && row_stride(dst) : rows_uniform(b) && rows_uniform(dst);
@@ -701,12 +734,47 @@ int mul_mat_mx(const tsk_tensor *a, const tsk_tensor *b, const tsk_tensor *bias,
     return TSK_OK;
 }
 
+// I8_SPLIT weights (gemm_i8.hip); f32 / bf16 activations become planes in the scratch first
+int mul_mat_i8(const tsk_tensor *a, const tsk_tensor *b, const tsk_tensor *bias, tsk_tensor *dst, const MulMatPlan &pl,
+               const Scratch &scr) {
+    const int64_t K = a->ne[0], M = a->ne[1], ld = i8_ld(K);
+    I8Gemm p;
+    memset(&p, 0, sizeof(p));
+    p.wq = i8_codes(a);
+    p.wd = i8_scales(a);
+    p.bias = bias ? (const float *) bias->data : nullptr;
+    p.y_bf16 = dst->type == TSK_TYPE_BF16;
+    p.M = (int) M; p.N = (int) pl.Nslice; p.K = (int) K;
+    // (a single row's stride may be anything)
+    p.ld_y = p.N == 1 ? M : (int64_t) (pl.uni ? row_stride(dst) : dst->nb[1]) / elt_size(dst->type);
+    const int8_t *xq = i8_codes(b);
+    const float *xd = i8_scales(b);
+    hipError_t e;
+    if (pl.act_bytes) {
+        void *ws = nullptr;
+        int rc;
+        if ((rc = scr.get(pl.bytes, &ws))) return rc;
+        float *d = (float *) ((char *) ws + (size_t) row_count(b) * (size_t) ld);
+        if ((e = launch_i8_quantize(view(b), (int8_t *) ws, d, scr.s)) != hipSuccess) return hip_fail(e, "mul_mat input quantize");
+        xq = (const int8_t *) ws;
+        xd = d;
+    }
+    for (int64_t sl = 0; sl < pl.nslices; ++sl) {
+        p.y = (char *) dst->data + sl % b->ne[2] * dst->nb[2] + sl / b->ne[2] * dst->nb[3];
+        p.xq = xq + sl * pl.Nslice * ld;
+        p.xd = xd + sl * pl.Nslice;
+        if ((e = launch_gemm_i8(p, scr.s)) != hipSuccess) return hip_fail(e, "mul_mat launch");
+    }
+    return TSK_OK;
+}
+
 int mul_mat_impl(const tsk_tensor *a, const tsk_tensor *b, const tsk_tensor *bias, tsk_tensor *dst,
                  const Scratch &scr) {
     hipStream_t s = scr.s;
     const int64_t K = a->ne[0], M = a->ne[1];
     const MulMatPlan pl = plan_mul_mat(a, b, dst);
     if (pl.mx) return mul_mat_mx(a, b, bias, dst, pl, scr);
+    if (pl.i8) return mul_mat_i8(a, b, bias, dst, pl, scr);
     const int es_b = elt_size(b->type), es_d = elt_size(dst->type);
     int rc;
     char *ws = nullptr;
@@ -1279,6 +1347,188 @@ extern "C" int tsk_mxfp4_repack(const tsk_tensor *src, tsk_tensor *dst, tsk_stre
     return e == hipSuccess ? TSK_OK : hip_fail(e, "mxfp4 repack launch");
 }
 
+// ------------------------------------------------------------------ 8-bit rows
+extern "C" size_t tsk_i8_split_nbytes(int64_t K, int64_t rows) {
+    if (K <= 0 || rows <= 0) return 0;
+    return i8_bytes(K, rows);
+}
+
+extern "C" int tsk_i8_quantize(const tsk_tensor *x, tsk_tensor *dst, tsk_stream stream) {
+    int rc;
+    if ((rc = check_tensor(x, "x")) || (rc = check_tensor(dst, "dst"))) return rc;
+    if (x->type != TSK_TYPE_F32 && x->type != TSK_TYPE_BF16) return fail(TSK_ERR_TYPE, "x must be F32 or BF16");
+    if ((rc = check_i8(dst, "dst"))) return rc;
+    if (!same_shape(x, dst)) return fail(TSK_ERR_SHAPE, "shapes differ");
+    if ((rc = check_rows(x, "x", elt_size(x->type)))) return rc;
+    if (may_overlap(x, dst)) return fail(TSK_ERR_INVALID_ARG, "x and dst overlap");
+    if ((rc = require_init())) return rc;
+    const hipError_t e = launch_i8_quantize(view(x), i8_codes(dst), i8_scales(dst), (hipStream_t) stream);
+    return e == hipSuccess ? TSK_OK : hip_fail(e, "i8 quantize launch");
+}
+
+extern "C" int tsk_i8_dequantize(const tsk_tensor *x, tsk_tensor *dst, tsk_stream stream) {
+    int rc;
+    if ((rc = check_tensor(x, "x")) || (rc = check_tensor(dst, "dst"))) return rc;
+    if ((rc = check_i8(x, "x"))) return rc;
+    if (dst->type != TSK_TYPE_F32 && dst->type != TSK_TYPE_BF16) return fail(TSK_ERR_TYPE, "dst must be F32 or BF16");
+    if (!same_shape(x, dst)) return fail(TSK_ERR_SHAPE, "shapes differ");
+    if ((rc = check_rows(dst, "dst", elt_size(dst->type))) || (rc = check_rows_apart(dst, "dst"))) return rc;
+    if (may_overlap(x, dst)) return fail(TSK_ERR_INVALID_ARG, "x and dst overlap");
+    if ((rc = require_init())) return rc;
+    const hipError_t e = launch_i8_dequantize(i8_codes(x), i8_scales(x), view(dst), (hipStream_t) stream);
+    return e == hipSuccess ? TSK_OK : hip_fail(e, "i8 dequantize launch");
+}
+
+// ------------------------------------------------------------------ rotary positions over several axes
+namespace {
+
+// t in place of x: the same bytes in the same order
+bool same_place(const tsk_tensor *x, const tsk_tensor *t) {
+    bool same = t->data == x->data && t->type == x->type;
+    for (int i = 1; same && i < 4; ++i) same = x->ne[i] == 1 || t->nb[i] == x->nb[i];
+    return same;
+}
+
+int validate_rope_axes(const tsk_tensor *x, const tsk_tensor *pos, const tsk_rope_axes_params *p, const tsk_tensor *dst) {
+    int rc;
+    if (!p) return fail(TSK_ERR_INVALID_ARG, "params is NULL");
+    if ((rc = check_unary(x, dst)) || (rc = check_tensor(pos, "pos")) || (rc = check_rows_apart(dst, "dst"))) return rc;
+    if (x->ne[0] > 2 * ROPE_AXES_PAIRS) return fail(TSK_ERR_UNSUPPORTED, "heads of %lld values (at most %d)", (long long) x->ne[0], 2 * ROPE_AXES_PAIRS);
+    if (!rows_fit(x)) return fail(TSK_ERR_SHAPE, "x is too large");
+    if (p->n_axes < 1 || p->n_axes > 4) return fail(TSK_ERR_INVALID_ARG, "n_axes %d", p->n_axes);
+    int64_t n = 0;
+    for (int a = 0; a < p->n_axes; ++a) {
+        if (p->dims[a] < 0 || (p->dims[a] & 1) || p->dims[a] > x->ne[0]) return fail(TSK_ERR_INVALID_ARG, "dims[%d] = %d", a, p->dims[a]);
+        n += p->dims[a];
+    }
+    if (n < 2 || n > x->ne[0]) return fail(TSK_ERR_INVALID_ARG, "axes of %lld values in heads of %lld", (long long) n, (long long) x->ne[0]);
+    if (p->pairs != TSK_ROPE_PAIRS_ADJACENT && p->pairs != TSK_ROPE_PAIRS_HALVES) return fail(TSK_ERR_INVALID_ARG, "pairs %d", p->pairs);
+    if (!(p->freq_base > 0.0f) || !std::isfinite(p->freq_base) || !std::isfinite(p->freq_scale)) return fail(TSK_ERR_INVALID_ARG, "freq_base / freq_scale");
+    if (pos->type != TSK_TYPE_I32 && pos->type != TSK_TYPE_F32) return fail(TSK_ERR_TYPE, "pos must be I32 or F32");
+    if (pos->ne[0] != x->ne[2] || pos->ne[1] != p->n_axes || (pos->ne[2] != 1 && pos->ne[2] != x->ne[3]) || pos->ne[3] != 1)
+        return fail(TSK_ERR_SHAPE, "pos must be [S = %lld, n_axes = %d, B = %lld or 1]", (long long) x->ne[2], p->n_axes, (long long) x->ne[3]);
+    if ((rc = check_rows(pos, "pos", 4))) return rc;
+    if (p->w) {
+        if ((rc = check_w(p->w, x->ne[0])) || (rc = check_rows(p->w, "w", 4))) return rc;
+        if (!(p->eps >= 0.0f)) return fail(TSK_ERR_INVALID_ARG, "eps");
+    }
+    if (!same_place(x, dst) && may_overlap(x, dst)) return fail(TSK_ERR_INVALID_ARG, "dst overlaps x");
+    if (may_overlap(pos, dst) || (p->w && may_overlap(p->w, dst))) return fail(TSK_ERR_INVALID_ARG, "dst overlaps an input");
+    return TSK_OK;
+}
+
+}  // namespace
+
+extern "C" int tsk_rope_axes(const tsk_tensor *x, const tsk_tensor *pos, const tsk_rope_axes_params *p, tsk_tensor *dst,
+                             tsk_stream stream) {
+    int rc;
+    if ((rc = validate_rope_axes(x, pos, p, dst)) || (rc = require_init())) return rc;
+    RopeAxes r;
+    memset(&r, 0, sizeof(r));
+    r.x = view(x); r.y = view(dst);
+    r.pos = pos->data; r.pos_f32 = pos->type == TSK_TYPE_F32;
+    r.pos_nb1 = p->n_axes > 1 ? (int64_t) pos->nb[1] : 0;
+    r.pos_nb2 = pos->ne[2] > 1 ? (int64_t) pos->nb[2] : 0;
+    r.w = p->w ? (const float *) p->w->data : nullptr;
+    r.eps = p->eps;
+    r.halves = p->pairs == TSK_ROPE_PAIRS_HALVES;
+    r.n_axes = p->n_axes;
+    int total = 0;
+    for (int a = 0; a < p->n_axes; ++a) total += p->dims[a] / 2;
+    r.n = 2 * total;
+    int i = 0;
+    for (int a = 0; a < 4; ++a) {
+        r.first[a] = i;
+        for (int j = 0; a < p->n_axes && j < p->dims[a] / 2; ++j, ++i)
+            r.quarters[i] = (double) p->freq_scale * 0.63661977236758134 *
+                            pow((double) p->freq_base, p->shared_freqs ? -(double) i / total : -2.0 * j / p->dims[a]);
+    }
+    r.first[4] = i;
+    const hipError_t e = launch_rope_axes(r, (hipStream_t) stream);
+    return e == hipSuccess ? TSK_OK : hip_fail(e, "rope_axes launch");
+}
+
+// ------------------------------------------------------------------ cross attention
+namespace {
+
+// the lengths of B sequences, nullable
+int check_lengths(const tsk_tensor *t, const char *name, int64_t B) {
+    int rc;
+    if (!t) return TSK_OK;
+    if ((rc = check_tensor(t, name))) return rc;
+    if (t->type != TSK_TYPE_I32) return fail(TSK_ERR_TYPE, "%s must be I32", name);
+    if (t->ne[0] != B || row_count(t) != 1) return fail(TSK_ERR_SHAPE, "%s must be [B = %lld]", name, (long long) B);
+    return check_rows(t, name, 4);
+}
+
+int validate_cross_shapes(const tsk_tensor *q, const tsk_tensor *k, const tsk_tensor *v, const tsk_tensor *dst) {
+    int rc;
+    if ((rc = check_tensor(q, "q")) || (rc = check_tensor(k, "k")) || (rc = check_tensor(v, "v")) || (rc = check_tensor(dst, "dst"))) return rc;
+    const int64_t D = q->ne[0], Nq = q->ne[1], H = q->ne[2], B = q->ne[3];
+    if (q->type != TSK_TYPE_F32 && q->type != TSK_TYPE_F16 && q->type != TSK_TYPE_BF16) return fail(TSK_ERR_TYPE, "q must be F32, F16 or BF16");
+    if (k->type != TSK_TYPE_F16 && k->type != TSK_TYPE_BF16) return fail(TSK_ERR_TYPE, "k and v must be F16 or BF16");
+    if (v->type != k->type) return fail(TSK_ERR_TYPE, "k and v must have the same type");
+    if (dst->type != TSK_TYPE_F32 && dst->type != TSK_TYPE_F16 && dst->type != TSK_TYPE_BF16) return fail(TSK_ERR_TYPE, "dst must be F32, F16 or BF16");
+    if (D % 8 || D > 128) return fail(TSK_ERR_UNSUPPORTED, "head size %lld (a multiple of 8, at most 128)", (long long) D);
+    if (!same_shape(k, v)) return fail(TSK_ERR_SHAPE, "k and v shapes differ");
+    if (k->ne[0] != D || k->ne[3] != B || H % k->ne[2]) return fail(TSK_ERR_SHAPE, "k must be [D = %lld, Nkv, a divisor of H = %lld, B = %lld]", (long long) D, (long long) H, (long long) B);
+    if (dst->ne[0] != D || dst->ne[1] != H || dst->ne[2] != Nq || dst->ne[3] != B)
+        return fail(TSK_ERR_SHAPE, "dst must be [D, H, Nq, B]");
+    if (!rows_fit(q) || !rows_fit(k)) return fail(TSK_ERR_SHAPE, "q or k is too large");
+    // (a workgroup for every 32 rows at most, and a launch of fewer than 2^32 threads)
+    if (((H / k->ne[2] * Nq + 31) / 32) * k->ne[2] * B > (1 << 22)) return fail(TSK_ERR_SHAPE, "q has too many rows");
+    if ((rc = check_rows(q, "q", 16)) || (rc = check_rows(k, "k", 16)) || (rc = check_rows(v, "v", 16)) || (rc = check_rows(dst, "dst", 16)) ||
+        (rc = check_rows_apart(dst, "dst")))
+        return rc;
+    for (const tsk_tensor *t : {k, v})
+        if (t->ne[1] > 1 && (t->nb[1] < row_bytes(t) || t->nb[1] > (1 << 24))) return fail(TSK_ERR_STRIDE, "k, v: rows overlap or are too far apart");
+    return TSK_OK;
+}
+
+int validate_cross(const tsk_tensor *q, const tsk_tensor *k, const tsk_tensor *v, const tsk_cross_attn_params *p, const tsk_tensor *dst) {
+    int rc;
+    if (!p) return fail(TSK_ERR_INVALID_ARG, "params is NULL");
+    if ((rc = validate_cross_shapes(q, k, v, dst))) return rc;
+    const int64_t B = q->ne[3];
+    if (!(p->scale > 0.0f) || !std::isfinite(p->scale)) return fail(TSK_ERR_INVALID_ARG, "scale");
+    if ((rc = check_lengths(p->kv_len, "kv_len", B)) || (rc = check_lengths(p->q_len, "q_len", B))) return rc;
+    if (p->kv_valid && p->kv_valid_nb < 0) return fail(TSK_ERR_INVALID_ARG, "kv_valid_nb");
+    for (const tsk_tensor *t : {q, k, v, p->kv_len, p->q_len})
+        if (t && may_overlap(t, dst)) return fail(TSK_ERR_INVALID_ARG, "dst overlaps an input");
+    return TSK_OK;
+}
+
+}  // namespace
+
+extern "C" int tsk_cross_attention(const tsk_tensor *q, const tsk_tensor *k, const tsk_tensor *v, const tsk_cross_attn_params *p,
+                                   tsk_tensor *dst, tsk_stream stream) {
+    int rc;
+    if ((rc = validate_cross(q, k, v, p, dst)) || (rc = require_init())) return rc;
+    CrossAttn a;
+    memset(&a, 0, sizeof(a));
+    a.q = q->data; a.k = k->data; a.v = v->data; a.o = dst->data;
+    a.q_type = q->type; a.kv_bf16 = k->type == TSK_TYPE_BF16; a.o_type = dst->type;
+    a.D = (int) q->ne[0]; a.Nq = (int) q->ne[1]; a.H = (int) q->ne[2]; a.B = (int) q->ne[3];
+    a.Nkv = (int) k->ne[1]; a.Hkv = (int) k->ne[2];
+    // (the strides of extents of 1 may be anything)
+    auto nb = [](const tsk_tensor *t, int i) { return t->ne[i] > 1 ? (int64_t) t->nb[i] : (int64_t) row_bytes(t); };
+    a.q_nb1 = nb(q, 1); a.q_nb2 = nb(q, 2); a.q_nb3 = nb(q, 3);
+    a.k_nb1 = nb(k, 1); a.k_nb2 = nb(k, 2); a.k_nb3 = nb(k, 3);
+    a.v_nb1 = nb(v, 1); a.v_nb2 = nb(v, 2); a.v_nb3 = nb(v, 3);
+    a.o_nb1 = nb(dst, 1); a.o_nb2 = nb(dst, 2); a.o_nb3 = nb(dst, 3);
+    a.kv_len = p->kv_len ? (const int32_t *) p->kv_len->data : nullptr;
+    a.q_len = p->q_len ? (const int32_t *) p->q_len->data : nullptr;
+    a.kv_valid = p->kv_valid; a.kv_valid_nb = p->kv_valid_nb;
+    a.c = p->scale * 1.4426950408889634f;
+    size_t bytes = 0;
+    void *ws = nullptr;
+    a.splits = cross_attn_splits(a.D, a.Nq, a.Nkv, a.H, a.Hkv, a.B, &bytes);
+    if (bytes && (rc = workspace((hipStream_t) stream, bytes, &ws))) return rc;
+    a.part = (float *) ws;
+    const hipError_t e = launch_cross_attn(a, (hipStream_t) stream);
+    return e == hipSuccess ? TSK_OK : hip_fail(e, "cross_attention launch");
+}
+
 // ------------------------------------------------------------------ block norm
 namespace {
 
@@ -1332,6 +1582,9 @@ int validate_block_norm(const tsk_tensor *x, const tsk_tensor *y, const tsk_bloc
         if (dst->type == TSK_TYPE_MXFP4_SPLIT) {
             if ((rc = check_tensor(dst, "dst")) || (rc = check_mx(dst, "dst"))) return rc;
             if (!same_shape(dst, x)) return fail(TSK_ERR_SHAPE, "dst must have x's shape");
+        } else if (dst->type == TSK_TYPE_I8_SPLIT) {
+            if ((rc = check_tensor(dst, "dst")) || (rc = check_i8(dst, "dst"))) return rc;
+            if (!same_shape(dst, x)) return fail(TSK_ERR_SHAPE, "dst must have x's shape");
         } else if ((rc = check_bn_rows(dst, "dst", x)) || (rc = check_rows_apart(dst, "dst"))) {
             return rc;
         }
@@ -1379,6 +1632,9 @@ extern "C" int tsk_block_norm(const tsk_tensor *x, const tsk_tensor *y, const ts
     if (dst && dst->type == TSK_TYPE_MXFP4_SPLIT) {
         b.codes = mx_codes(dst);
         b.scales = mx_scales(dst);
+    } else if (dst && dst->type == TSK_TYPE_I8_SPLIT) {
+        b.i8 = i8_codes(dst);
+        b.i8_d = i8_scales(dst);
     } else {
         b.dst = bn_view(dst);
     }
@@ -1870,6 +2126,9 @@ extern "C" int tsk_supports_op(int op, const tsk_tensor *const *srcs, int n_srcs
             rc = n_srcs >= 3 ? validate_fa(&t[0], &t[1], &t[2], opt(3), 0.125f, 0.0f, 0.0f, TSK_PREC_F32, &d)
                              : TSK_ERR_INVALID_ARG;
             break;
+        case TSK_OP_CROSS_ATTENTION:
+            rc = n_srcs >= 3 ? validate_cross_shapes(&t[0], &t[1], &t[2], &d) : TSK_ERR_INVALID_ARG;
+            break;
         case TSK_OP_RMS_NORM_MUL:
             rc = check_unary(&t[0], &d);
             if (!rc && opt(1)) rc = check_w(&t[1], t[0].ne[0]);
@@ -1953,6 +2212,10 @@ extern "C" int tsk_workspace_size(int op, const tsk_tensor *const *srcs, int n_s
         case TSK_OP_RMS_NORM_Q8_0:
             if ((rc = need(2)) || (rc = validate_rms_norm_q8(&t[0], &t[1], &d))) return rc;
             *bytes = rms_norm_q8_ws_bytes(&t[0]);
+            return TSK_OK;
+        case TSK_OP_CROSS_ATTENTION:
+            if ((rc = need(3)) || (rc = validate_cross_shapes(&t[0], &t[1], &t[2], &d))) return rc;
+            cross_attn_splits((int) t[0].ne[0], t[0].ne[1], t[1].ne[1], t[0].ne[2], t[1].ne[2], t[0].ne[3], bytes);
             return TSK_OK;
         case TSK_OP_RMS_NORM_MUL: case TSK_OP_ROPE_EXT: case TSK_OP_NORM: case TSK_OP_IM2COL:
             return TSK_OK;   // no scratch

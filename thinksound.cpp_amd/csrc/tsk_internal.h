@@ -375,6 +375,62 @@ struct MxGemm {
 };
 hipError_t launch_gemm_mx(const MxGemm &p, hipStream_t s);
 
+// ---------------------------------------------------------------- 8-bit rows with a scale each
+// rows of x (f32 / bf16) -> q [rows][i8_ld(K)] (zeros past K), d [rows]
+hipError_t launch_i8_quantize(const View4 &x, int8_t *q, float *d, hipStream_t s);
+// and back into rows of y (f32 / bf16)
+hipError_t launch_i8_dequantize(const int8_t *q, const float *d, const View4 &y, hipStream_t s);
+// Y[n, m] = (sum_k XQ[n, k] WQ[m, k]) XD[n] WD[m] + bias[m] (gemm_i8.hip): 16-byte
+// aligned planes, K < 2^17; Y rows 16-byte aligned
+struct I8Gemm {
+    const int8_t *wq;              // [M][i8_ld(K)]
+    const float *wd;               // [M]
+    const int8_t *xq;              // [N][i8_ld(K)]
+    const float *xd;               // [N]
+    const float *bias;             // [M], nullable, 16-byte aligned
+    void *y;
+    int y_bf16;
+    int64_t ld_y;
+    int M, N, K;
+};
+hipError_t launch_gemm_i8(const I8Gemm &p, hipStream_t s);
+
+// ---------------------------------------------------------------- rotary positions over several axes
+// tsk_rope_axes' operands (rope_axes.hip): x and y [D, heads, S, B]
+constexpr int ROPE_AXES_PAIRS = 192;      // pairs of a head at most (D <= 384)
+struct RopeAxes {
+    View4 x, y;
+    const void *pos;               // [S, n_axes, B or 1]
+    int pos_f32;
+    int64_t pos_nb1, pos_nb2;      // bytes between axes and between batch items (0: shared)
+    const float *w;                // [D], nullable: RMS norm of every head first
+    float eps;
+    int halves, n;                 // pairs (i, i + n / 2) instead of (2 i, 2 i + 1); values turned
+    int n_axes, first[5];          // pairs first[a] .. first[a + 1] - 1 belong to axis a
+    double quarters[ROPE_AXES_PAIRS];   // quarter turns of a pair per position
+};
+hipError_t launch_rope_axes(const RopeAxes &p, hipStream_t s);
+
+// ---------------------------------------------------------------- cross attention
+// tsk_cross_attention's operands (attn_cross.hip): byte strides, 16-byte aligned rows
+struct CrossAttn {
+    const void *q, *k, *v;
+    void *o;
+    int q_type, kv_bf16, o_type;   // kv: F16 or BF16
+    int D, Nq, Nkv, H, Hkv, B;
+    int64_t q_nb1, q_nb2, q_nb3, k_nb1, k_nb2, k_nb3, v_nb1, v_nb2, v_nb3;
+    int64_t o_nb1, o_nb2, o_nb3;   // dst [D, H, Nq, B]
+    const int32_t *kv_len, *q_len; // [B], nullable
+    const uint8_t *kv_valid;       // [B][kv_valid_nb], nullable
+    int64_t kv_valid_nb;
+    float c;                       // scale * log2(e)
+    int splits;                    // key ranges, each a workgroup; > 1: part holds their sums
+    float *part;
+};
+// key ranges for the node, and the scratch bytes they take
+int cross_attn_splits(int D, int64_t Nq, int64_t Nkv, int64_t H, int64_t Hkv, int64_t B, size_t *bytes);
+hipError_t launch_cross_attn(const CrossAttn &p, hipStream_t s);
+
 // ---------------------------------------------------------------- block norm
 // tsk_block_norm's operands; a stride of 0 broadcasts, data null: absent
 struct BnView {
@@ -386,6 +442,8 @@ struct BlockNorm {
     int x_bf16, y_bf16, dst_bf16;
     const float *post_w, *pre_w;
     uint8_t *codes, *scales;       // dst as MXFP4 planes (dst.data null)
+    int8_t *i8;                    // dst as 8-bit rows and their scales (dst.data null)
+    float *i8_d;
     int post_norm, pre_norm;       // tsk_norm_kind
     float post_eps, pre_eps, res_scale;
     int C, n1, n2, n3;

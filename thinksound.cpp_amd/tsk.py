@@ -17,12 +17,13 @@ import numpy as np
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "lib", "libtsk.so")
 
-F32, F16, Q8_0, I32, BF16, MXFP4, Q8_0_SPLIT, MXFP4_SPLIT = 0, 1, 8, 26, 30, 39, 0x1008, 0x1027
+F32, F16, Q8_0, I32, BF16, MXFP4, Q8_0_SPLIT, MXFP4_SPLIT, I8_SPLIT = 0, 1, 8, 26, 30, 39, 0x1008, 0x1027, 0x1018
 NORM_NONE, NORM_LAYER, NORM_RMS = 0, 1, 2
 PREC_DEFAULT, PREC_F32 = 0, 10
 ROPE_NORMAL = 0
+ROPE_ADJACENT, ROPE_HALVES = 0, 1
 OP_MUL_MAT, OP_FLASH_ATTN_EXT, OP_RMS_NORM_MUL, OP_ROPE_EXT, OP_NORM, OP_IM2COL, OP_CONV1D = 1, 2, 3, 4, 5, 6, 7
-OP_CONV_MLP_SWIGLU, OP_MLP_SWIGLU, OP_RMS_NORM_Q8_0 = 8, 9, 10
+OP_CONV_MLP_SWIGLU, OP_MLP_SWIGLU, OP_RMS_NORM_Q8_0, OP_CROSS_ATTENTION = 8, 9, 10, 11
 STATUS = {0: "TSK_OK", -1: "TSK_ERR_INVALID_ARG", -2: "TSK_ERR_TYPE", -3: "TSK_ERR_SHAPE",
           -4: "TSK_ERR_STRIDE", -5: "TSK_ERR_ALIGN", -6: "TSK_ERR_UNSUPPORTED",
           -7: "TSK_ERR_NOT_INIT", -8: "TSK_ERR_HIP", -9: "TSK_ERR_NOMEM"}
@@ -44,6 +45,17 @@ class BlockNormParams(ctypes.Structure):
                 ("gate", ctypes.POINTER(TskTensor)), ("res_scale", ctypes.c_float), ("pre_norm", ctypes.c_int),
                 ("pre_eps", ctypes.c_float), ("pre_w", ctypes.POINTER(TskTensor)),
                 ("scale", ctypes.POINTER(TskTensor)), ("shift", ctypes.POINTER(TskTensor))]
+
+
+class RopeAxesParams(ctypes.Structure):
+    _fields_ = [("n_axes", ctypes.c_int), ("dims", ctypes.c_int * 4), ("pairs", ctypes.c_int), ("shared_freqs", ctypes.c_int),
+                ("freq_base", ctypes.c_float), ("freq_scale", ctypes.c_float), ("w", ctypes.POINTER(TskTensor)),
+                ("eps", ctypes.c_float)]
+
+
+class CrossAttnParams(ctypes.Structure):
+    _fields_ = [("scale", ctypes.c_float), ("kv_len", ctypes.POINTER(TskTensor)), ("q_len", ctypes.POINTER(TskTensor)),
+                ("kv_valid", ctypes.c_void_p), ("kv_valid_nb", ctypes.c_int64)]
 
 
 class T5Config(ctypes.Structure):
@@ -103,6 +115,10 @@ def load():
         "tsk_mxfp4_quantize": ([P, P, vp], i), "tsk_mxfp4_dequantize": ([P, P, vp], i),
         "tsk_mxfp4_repack": ([P, P, vp], i),
         "tsk_mxfp4_split_nbytes": ([ctypes.c_int64, ctypes.c_int64], ctypes.c_size_t),
+        "tsk_i8_quantize": ([P, P, vp], i), "tsk_i8_dequantize": ([P, P, vp], i),
+        "tsk_i8_split_nbytes": ([ctypes.c_int64, ctypes.c_int64], ctypes.c_size_t),
+        "tsk_rope_axes": ([P, P, ctypes.POINTER(RopeAxesParams), P, vp], i),
+        "tsk_cross_attention": ([P, P, P, ctypes.POINTER(CrossAttnParams), P, vp], i),
         "tsk_block_norm": ([P, P, ctypes.POINTER(BlockNormParams), P, P, vp], i),
         "tsk_supports_op": ([i, ctypes.POINTER(P), i, P], i),
         "tsk_workspace_size": ([i, ctypes.POINTER(P), i, P, ctypes.POINTER(ctypes.c_size_t)], i),
@@ -390,7 +406,7 @@ def desc(t, ttype=None):
         rows, nblk = t.shape[0], t.shape[1]
         ne = [nblk * 32, rows]
         nb = [34 if ttype == Q8_0 else 17, t.stride(0)]
-    elif ttype in (Q8_0_SPLIT, MXFP4_SPLIT):
+    elif ttype in (Q8_0_SPLIT, MXFP4_SPLIT, I8_SPLIT):
         ne = list(t.logical_shape)
         nb = [1, ne[0]]
     else:
@@ -468,8 +484,8 @@ def _ref(x):
 def _mul_mat(fn, a, b, bias, out, a_type, out_dtype, stream):
     init()
     at = a_type if a_type is not None else a.ttype
-    M = a.logical_shape[1] if at in (Q8_0_SPLIT, MXFP4_SPLIT) else a.shape[0]
-    bt = MXFP4_SPLIT if isinstance(b, SplitMXFP4) else None
+    M = a.logical_shape[1] if at in (Q8_0_SPLIT, MXFP4_SPLIT, I8_SPLIT) else a.shape[0]
+    bt = b.ttype if isinstance(b, (SplitMXFP4, SplitI8)) else None
     if out is None:
         rows = (b.logical_shape[1],) if bt else tuple(b.shape[:-1])
         out = DeviceArray(rows + (M,), out_dtype)
@@ -481,7 +497,8 @@ def _mul_mat(fn, a, b, bias, out, a_type, out_dtype, stream):
 
 def mul_mat(a, b, bias=None, out=None, a_type=None, out_dtype="f32", stream=None):
     """ggml_mul_mat(a, b) (+bias): a (M, K) weights, b (..., N, K) -> (..., N, M).
-    MXFP4 weights: a u8 blocks with a_type=MXFP4 or a SplitMXFP4; b then also a SplitMXFP4 of N rows."""
+    MXFP4 weights: a u8 blocks with a_type=MXFP4 or a SplitMXFP4; b then also a SplitMXFP4 of N rows.
+    8-bit weights: a SplitI8; b then also a SplitI8 of N rows."""
     return _mul_mat("tsk_mul_mat", a, b, bias, out, a_type, out_dtype, stream)
 
 
@@ -656,10 +673,10 @@ class SplitMXFP4:
 
 
 def _desc_planes(out, x):
-    """an output SplitMXFP4's descriptor with the extents of x's rows"""
+    """an output SplitMXFP4's or SplitI8's descriptor with the extents of x's rows"""
     if out.logical_shape != (x.shape[-1], int(np.prod(x.shape[:-1]))):
-        raise ValueError("MXFP4 planes of (K, rows) = %s for x of %s" % (out.logical_shape, tuple(x.shape)))
-    dd, dx = desc(out, MXFP4_SPLIT), desc(x)
+        raise ValueError("planes of (K, rows) = %s for x of %s" % (out.logical_shape, tuple(x.shape)))
+    dd, dx = desc(out, out.ttype), desc(x)
     for k in range(1, 4):
         dd.ne[k] = dx.ne[k]
     return dd
@@ -702,12 +719,85 @@ def mxfp4_repack(blocks, stream=None):
     return sp
 
 
+# ---------------------------------------------------------------- 8-bit rows
+class SplitI8:
+    """A (rows, K) matrix in 8-bit planes (TSK_TYPE_I8_SPLIT): rows of K int8 padded to 16, then an f32 scale a row."""
+    ttype = I8_SPLIT
+
+    def __init__(self, buf, K, rows):
+        if buf.nbytes < rows * ((K + 15) // 16 * 16 + 4):
+            raise ValueError("%d bytes for 8-bit planes of (%d, %d)" % (buf.nbytes, rows, K))
+        self.buf, self.logical_shape = buf, (K, rows)
+
+    def data_ptr(self):
+        return self.buf.data_ptr()
+
+
+def i8_quantize(x, out=None, stream=None):
+    """(..., K) f32 / bf16 rows -> SplitI8 of all rows, an integer plane and a scale a row."""
+    init()
+    K, rows = x.shape[-1], int(np.prod(x.shape[:-1]))
+    if out is None:
+        out = SplitI8(DeviceArray((load().tsk_i8_split_nbytes(K, rows),), "u8"), K, rows)
+    dx, dd = desc(x), _desc_planes(out, x)
+    check(load().tsk_i8_quantize(ctypes.byref(dx), ctypes.byref(dd), _stream(stream)))
+    return out
+
+
+def i8_dequantize(x, dtype="f32", out=None, stream=None):
+    """SplitI8 -> (rows, K) f32 / bf16."""
+    init()
+    out = DeviceArray(x.logical_shape[::-1], dtype) if out is None else out
+    dx, dd = _desc_planes(x, out), desc(out)
+    check(load().tsk_i8_dequantize(ctypes.byref(dx), ctypes.byref(dd), _stream(stream)))
+    return out
+
+
+# ---------------------------------------------------------------- positions and attention of tokens and states
+def rope_axes(x, pos, dims, pairs=ROPE_ADJACENT, shared_freqs=False, freq_base=10000.0, freq_scale=1.0, w=None, eps=1e-6,
+              out=None, stream=None):
+    """Rotary positions over len(dims) axes (tsk_rope_axes): x (B, S, H, D) f32 / bf16, pos (axes, S) or (B, axes, S) i32 / f32,
+    w (D,) f32: RMS norm of every head first. out may be x."""
+    init()
+    out = DeviceArray(x.shape, x.dtype) if out is None else out
+    p = RopeAxesParams()
+    p.n_axes, p.pairs, p.shared_freqs, p.freq_base, p.freq_scale, p.eps = len(dims), pairs, int(shared_freqs), freq_base, freq_scale, eps
+    for a, n in enumerate(dims[:4]):
+        p.dims[a] = n
+    if w is not None:
+        p.w = ctypes.pointer(desc(w))
+    dx, dp, dd = desc(x), desc(pos), desc(out)
+    check(load().tsk_rope_axes(ctypes.byref(dx), ctypes.byref(dp), ctypes.byref(p), ctypes.byref(dd), _stream(stream)))
+    return out
+
+
+def cross_attention(q, k, v, scale=None, kv_len=None, q_len=None, kv_valid=None, out=None, out_dtype="f32", stream=None):
+    """Attention to states of another number (tsk_cross_attention): q (B, H, Nq, D), k / v (B, Hkv, Nkv, D) f16 / bf16 ->
+    (B, Nq, H, D). kv_len, q_len (B,) i32; kv_valid u8 (B, Nkv), or (Nkv,) for all; scale None: D ** -0.5."""
+    init()
+    B, H, Nq, D = q.shape
+    out = DeviceArray((B, Nq, H, D), out_dtype) if out is None else out
+    p = CrossAttnParams()
+    p.scale = D ** -0.5 if scale is None else scale
+    for name, t in (("kv_len", kv_len), ("q_len", q_len)):
+        if t is not None:
+            setattr(p, name, ctypes.pointer(desc(t)))
+    if kv_valid is not None:
+        if tuple(kv_valid.shape) not in ((B, k.shape[2]), (k.shape[2],)) or kv_valid.stride(-1) != 1:
+            raise ValueError("kv_valid of %s for k of %s" % (tuple(kv_valid.shape), tuple(k.shape)))
+        p.kv_valid, p.kv_valid_nb = kv_valid.data_ptr(), kv_valid.stride(0) if len(kv_valid.shape) == 2 else 0
+    dq, dk, dv, dd = desc(q), desc(k), desc(v), desc(out)
+    check(load().tsk_cross_attention(ctypes.byref(dq), ctypes.byref(dk), ctypes.byref(dv), ctypes.byref(p), ctypes.byref(dd),
+                                     _stream(stream)))
+    return out
+
+
 # ---------------------------------------------------------------- norms around a block
 def block_norm(x, y=None, gate=None, post=NORM_NONE, post_w=None, post_eps=1e-5, res_scale=1.0, pre=NORM_LAYER,
                pre_w=None, pre_eps=1e-5, scale=None, shift=None, res=None, dst=None, stream=None):
     """res = res_scale x + gate post(y), dst = pre(res) pre_w (1 + scale) + shift (tsk_block_norm):
     x / y (..., C), gate / scale / shift (..., C) broadcast over x's rows; res None: not kept,
-    dst a DeviceArray or SplitMXFP4, None: the residual alone (pre=NORM_NONE). Returns (res, dst)."""
+    dst a DeviceArray, SplitMXFP4 or SplitI8, None: the residual alone (pre=NORM_NONE). Returns (res, dst)."""
     init()
     ptr = lambda t: None if t is None else ctypes.pointer(desc(t))
     p = BlockNormParams(post, post_eps, ptr(post_w), ptr(gate), res_scale, pre, pre_eps, ptr(pre_w), ptr(scale),
@@ -715,7 +805,7 @@ def block_norm(x, y=None, gate=None, post=NORM_NONE, post_w=None, post_eps=1e-5,
     dx = desc(x)
     dd = None
     if dst is not None:
-        dd = _desc_planes(dst, x) if isinstance(dst, SplitMXFP4) else desc(dst)
+        dd = _desc_planes(dst, x) if isinstance(dst, (SplitMXFP4, SplitI8)) else desc(dst)
     dy, dr = (desc(t) if t is not None else None for t in (y, res))
     check(load().tsk_block_norm(ctypes.byref(dx), _ref(dy), ctypes.byref(p), _ref(dr), _ref(dd), _stream(stream)))
     return res, dst
