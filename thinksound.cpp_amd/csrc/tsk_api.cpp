@@ -66,6 +66,7 @@ void read_tuning() {
     t.q8_pair = env_int("TSK_Q8_PAIR", 1) != 0;
     t.coop_cfg = env_int("TSK_COOP_CFG", 0);
     t.mx_cfg = env_int("TSK_MX_CFG", 0);
+    t.i8_cfg = env_int("TSK_I8_CFG", 0);
     t.attn_cfg = env_int("TSK_ATTN_CFG", 0);
     t.dit_sched = env_int("TSK_DIT_SCHED", 1) != 0;
     t.ln_block = env_int("TSK_LN_BLOCK", 0) != 0;
