@@ -63,62 +63,130 @@ __device__ __forceinline__ void store4(const I8Gemm &p, int n, int m, f32x4 v) {
 
 // ---------------------------------------------------------------- few rows
 // Operands straight into registers. NW waves share 16 MT x 16 NT outputs and
-// deal the K range among them in turns of 128 k; their sums meet in LDS.
+// deal the K range among them in turns of 64 KS k; their sums meet in LDS.
 // Lane l holds row l % 16 of either operand and of each 64 k the 16 bytes l / 16.
+//
+// Bound by the weights' bytes (8 x 8192, K = 8192 15.4 us, 4.4 TB/s) and, where they are
+// few, by the launch; turns of 256 or 512 k and 8 waves are no faster (16.4 to 18.3).
+//
+// XT: f32 or bf16 activations, quantized by every workgroup into LDS while its first
+// weights are on their way (gemm_i8_fused).
+enum : int { X_I8 = 0, X_BF16 = 1, X_F32 = 2 };
+
+constexpr int NW = 4, KS = 2;
+
 template <int MT, int NT>
 struct RowFrags {
-    i32x4 a[MT][2], b[NT][2];
+    i32x4 a[MT][KS], b[NT][KS];
 };
 
-template <int MT, int NT, int NW>
+// bytes from a quantized row in LDS to the next: 16 rows start on 16 different 16-byte banks
+__device__ __host__ constexpr int lds_row(int64_t ld) { return (int) ((ld + 255) / 256 * 256 + 16); }
+
+// the activations into LDS, TPR threads a row (64: up to 2048 values, or all 256: up to 8192)
+template <int XT, int TPR>
+__device__ __forceinline__ void quantize_rows(const I8Gemm &p, int8_t *xs, float *xd, uint32_t *red) {
+    constexpr int PER = 4;                                       // vectors of 8 a thread
+    const int t = threadIdx.x % TPR, ld = (int) i8_ld(p.K), stride = lds_row(ld);
+    for (int n = threadIdx.x / TPR; n < p.N; n += NW * 64 / TPR) {
+        const char *row = (const char *) p.x + n * p.ld_x * (XT == X_F32 ? 4 : 2);
+        float v[PER][8];
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int c = (t + TPR * j) * 8;
+            if (c < p.K) i8_load8<XT == X_BF16, true>(row, c, p.K, v[j]);
+            else
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[j][e] = 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top = max(top, i8_abs_bits(v[j][e]));
+        for (int m = 1; m < 64; m *= 2) top = max(top, (uint32_t) __shfl_xor((int) top, m));
+        if constexpr (TPR > 64) {                                // (one row at a time: every thread comes here as often)
+            __syncthreads();
+            if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < TPR / 64; ++i) top = max(top, red[i]);
+        }
+        const I8Scale s = i8_scale(top);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int c = (t + TPR * j) * 8;
+            if (c < ld) *(u32x2 *) (xs + n * stride + c) = u32x2{i8_pack4(v[j], s), i8_pack4(v[j] + 4, s)};
+        }
+        if (t == 0) xd[n] = s.d;
+    }
+    __syncthreads();
+}
+
+template <int MT, int NT, int XT, int TPR>
 __global__ __launch_bounds__(NW * 64) void i8_gemm_rows_kernel(const I8Gemm p, int tiles_m) {
-    __shared__ __attribute__((aligned(16))) int red[NW > 1 ? NW * MT * NT * 256 : 4];
+    __shared__ __attribute__((aligned(16))) int red[NW * MT * NT * 256];
+    __shared__ float xds[16];
+    extern __shared__ __attribute__((aligned(16))) int8_t xs[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
     const int m0 = (int) (blockIdx.x % tiles_m) * (16 * MT), n0 = (int) (blockIdx.x / tiles_m) * (16 * NT);
     const int64_t ld = i8_ld(p.K);
-    const int nit = (int) ((ld + 127) / 128);
+    const int nit = (int) ((ld + 64 * KS - 1) / (64 * KS));
     // rows past M or N read the last one (their outputs are not stored)
     const int8_t *wq[MT], *xq[NT];
 #pragma unroll
     for (int i = 0; i < MT; ++i) wq[i] = p.wq + (int64_t) min(m0 + 16 * i + r, p.M - 1) * ld + 16 * g;
 #pragma unroll
-    for (int j = 0; j < NT; ++j) xq[j] = p.xq + (int64_t) min(n0 + 16 * j + r, p.N - 1) * ld + 16 * g;
-    auto load = [&](int it, RowFrags<MT, NT> &f) {
-        const int64_t k0 = (int64_t) it * 128;
-        const i32x4 zero = {0, 0, 0, 0};
+    for (int j = 0; j < NT; ++j) {
+        const int n = min(n0 + 16 * j + r, p.N - 1);
+        xq[j] = XT == X_I8 ? p.xq + (int64_t) n * ld + 16 * g : xs + n * lds_row(ld) + 16 * g;
+    }
+    typedef RowFrags<MT, NT> Frags;
+    const i32x4 zero = {0, 0, 0, 0};
+    auto load_w = [&](int it, Frags &f) {
+        const int64_t k0 = (int64_t) it * (64 * KS);
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            const bool in = k0 + 64 * ks + 16 * g < ld;      // (rows are whole pieces of 16)
+        for (int ks = 0; ks < KS; ++ks)                          // (rows are whole pieces of 16)
 #pragma unroll
-            for (int i = 0; i < MT; ++i) f.a[i][ks] = in ? *(const i32x4 *) (wq[i] + k0 + 64 * ks) : zero;
+            for (int i = 0; i < MT; ++i) f.a[i][ks] = k0 + 64 * ks + 16 * g < ld ? *(const i32x4 *) (wq[i] + k0 + 64 * ks) : zero;
+    };
+    auto load_x = [&](int it, Frags &f) {
+        const int64_t k0 = (int64_t) it * (64 * KS);
 #pragma unroll
-            for (int j = 0; j < NT; ++j) f.b[j][ks] = in ? *(const i32x4 *) (xq[j] + k0 + 64 * ks) : zero;
-        }
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) f.b[j][ks] = k0 + 64 * ks + 16 * g < ld ? *(const i32x4 *) (xq[j] + k0 + 64 * ks) : zero;
     };
     i32x4 acc[MT][NT];
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int j = 0; j < NT; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
-    auto product = [&](const RowFrags<MT, NT> &f) {
+        for (int j = 0; j < NT; ++j) acc[i][j] = zero;
+    auto product = [&](int it, Frags &f) {
+        if constexpr (XT != X_I8) load_x(it, f);
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
+        for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
             for (int i = 0; i < MT; ++i)
 #pragma unroll
                 for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f.a[i][ks], f.b[j][ks], acc[i][j], 0, 0, 0);
     };
+    auto load = [&](int it, Frags &f) {
+        load_w(it, f);
+        if constexpr (XT == X_I8) load_x(it, f);
+    };
+    Frags f0, f1;
+    if (wave < nit) load(wave, f0);
+    if constexpr (XT != X_I8) quantize_rows<XT, TPR>(p, xs, xds, (uint32_t *) red);
     if (wave < nit) {
-        RowFrags<MT, NT> f0, f1;
-        load(wave, f0);
         int it = wave;
         for (; it + NW < nit; it += 2 * NW) {
             load(it + NW, f1);
-            product(f0);
+            product(it, f0);
             if (it + 2 * NW < nit) load(it + 2 * NW, f0);
-            product(f1);
+            product(it + NW, f1);
         }
-        if (it < nit) product(f0);
+        if (it < nit) product(it, f0);
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i)
@@ -133,7 +201,7 @@ __global__ __launch_bounds__(NW * 64) void i8_gemm_rows_kernel(const I8Gemm p, i
             i32x4 v = *(const i32x4 *) (red + ((i * NT + j) * 64 + lane) * 4);
             for (int w = 1; w < NW; ++w) v += *(const i32x4 *) (red + ((w * MT * NT + i * NT + j) * 64 + lane) * 4);
             const int n = n0 + 16 * j + r, m = m0 + 16 * i + 4 * g;
-            if (n < p.N && m < p.M) store4(p, n, m, scaled(v, p.xd[n], channels(p, m)));
+            if (n < p.N && m < p.M) store4(p, n, m, scaled(v, XT == X_I8 ? p.xd[n] : xds[n], channels(p, m)));
         }
 }
 
@@ -152,12 +220,21 @@ hipError_t in_two(const I8Gemm &p, F launch) {
     return e == hipSuccess ? launch(b) : e;
 }
 
-template <int MT, int NT, int NW>
+template <int MT, int NT>
 hipError_t launch_rows(const I8Gemm &p, hipStream_t s) {
     const int tiles_m = (p.M + 16 * MT - 1) / (16 * MT), tiles_n = (p.N + 16 * NT - 1) / (16 * NT);
     const int64_t T = (int64_t) tiles_m * tiles_n;
-    if (T * NW * 64 >= MAX_THREADS) return in_two(p, [&](const I8Gemm &q) { return launch_rows<MT, NT, NW>(q, s); });
-    launch_kernel(i8_gemm_rows_kernel<MT, NT, NW>, dim3((unsigned) T), dim3(NW * 64), 0, s, p, tiles_m);
+    if (T * NW * 64 >= MAX_THREADS) return in_two(p, [&](const I8Gemm &q) { return launch_rows<MT, NT>(q, s); });
+    launch_kernel(i8_gemm_rows_kernel<MT, NT, X_I8, 64>, dim3((unsigned) T), dim3(NW * 64), 0, s, p, tiles_m);
+    return hipGetLastError();
+}
+// f32 / bf16 activations
+hipError_t launch_fused(const I8Gemm &p, hipStream_t s) {
+    const int tiles_m = (p.M + 15) / 16;                         // (M <= 2^26: 2^30 threads)
+    auto kern = p.x_f32 ? p.N == 1 ? i8_gemm_rows_kernel<1, 1, X_F32, 256> : i8_gemm_rows_kernel<1, 1, X_F32, 64>
+                        : p.N == 1 ? i8_gemm_rows_kernel<1, 1, X_BF16, 256> : i8_gemm_rows_kernel<1, 1, X_BF16, 64>;
+    const size_t lds = (size_t) p.N * lds_row(i8_ld(p.K));
+    launch_kernel(kern, dim3((unsigned) tiles_m), dim3(NW * 64), lds, s, p, tiles_m);
     return hipGetLastError();
 }
 
@@ -410,7 +487,15 @@ int shape_for(const I8Gemm &p) {
 
 }  // namespace
 
+// f32 / bf16 activations: a launch that quantizes them and the product's wait for it cost
+// 3 us; every workgroup's own quantization, of one row by all its threads or of up to
+// four by a wave each (us, inside / two launches; rows x M): 1 x 6144, K = 1024 5.2 /
+// 6.9; 1 x 8192, K = 8192 18.9 / 20.4; 3 x 6144, K = 1024 5.8 / 6.9; 4 x 2048, K = 2048
+// 6.9 / 7.2; 8 x 1024, K = 1024 6.6 / 6.4; 2 x 8192, K = 8192 22.6 / 20.4.
+bool gemm_i8_fused(int64_t N, int64_t K) { return N == 1 ? K <= 8192 : N <= 4 && K <= 2048 && N * K <= 4096; }
+
 hipError_t launch_gemm_i8(const I8Gemm &p, hipStream_t s) {
+    if (!p.xq) return launch_fused(p, s);
     switch (shape_for(p)) {
         case 1: return launch_tile<Cfg<2, 4, 4, 2, 2, true>>(p, s);
         case 2: return launch_tile<Cfg<2, 4, 2, 2, 3, true>>(p, s);
@@ -419,9 +504,9 @@ hipError_t launch_gemm_i8(const I8Gemm &p, hipStream_t s) {
         case 6: return launch_tile<Cfg<2, 4, 3, 1, 3, true>>(p, s);
         case 7: return launch_tile<Cfg<4, 2, 1, 3, 3, true>>(p, s);
         case 8: return launch_tile<Cfg<2, 4, 3, 2, 2, true>>(p, s);
-        case 11: return launch_rows<1, 1, 4>(p, s);
-        case 12: return launch_rows<2, 1, 4>(p, s);
-        case 13: return launch_rows<2, 2, 4>(p, s);
+        case 11: return launch_rows<1, 1>(p, s);
+        case 12: return launch_rows<2, 1>(p, s);
+        case 13: return launch_rows<2, 2>(p, s);
         default: return launch_tile<Cfg<2, 2, 1, 1, 4, false>>(p, s);
     }
 }

@@ -51,4 +51,29 @@ __device__ __forceinline__ uint32_t i8_pack4(const float *v, const I8Scale &s) {
     return w;
 }
 
+// 8 values of an f32 or bf16 row from column c on, those past K zeros; WIDE: the row starts on 16 bytes
+template <bool BF16, bool WIDE>
+__device__ __forceinline__ void i8_load8(const char *row, int c, int K, float *v) {
+    if (WIDE && c + 8 <= K) {
+        if constexpr (BF16) {
+            const u32x4 w = *(const u32x4 *) (row + (int64_t) c * 2);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                v[2 * q] = __uint_as_float(w[q] << 16);
+                v[2 * q + 1] = __uint_as_float(w[q] & 0xffff0000u);
+            }
+        } else {
+            const f32x4 a = ((const f32x4 *) (row + (int64_t) c * 4))[0], b = ((const f32x4 *) (row + (int64_t) c * 4))[1];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[e] = a[e];
+                v[4 + e] = b[e];
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = c + e < K ? load_as_f32<BF16 ? Elt::BF16 : Elt::F32>(row, c + e) : 0.0f;
+}
+
 }  // namespace tsk

@@ -21,31 +21,6 @@ __device__ __forceinline__ int64_t row_at(const Rows &t, int64_t r) {
     return i1 * t.nb1 + q % t.ne2 * t.nb2 + q / t.ne2 * t.nb3;
 }
 
-// 8 values from column c on, those past K zeros
-template <bool BF16, bool WIDE>
-__device__ __forceinline__ void load8(const char *row, int c, int K, float *v) {
-    if (WIDE && c + 8 <= K) {
-        if constexpr (BF16) {
-            const u32x4 w = *(const u32x4 *) (row + (int64_t) c * 2);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                v[2 * q] = __uint_as_float(w[q] << 16);
-                v[2 * q + 1] = __uint_as_float(w[q] & 0xffff0000u);
-            }
-        } else {
-            const f32x4 a = ((const f32x4 *) (row + (int64_t) c * 4))[0], b = ((const f32x4 *) (row + (int64_t) c * 4))[1];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                v[e] = a[e];
-                v[4 + e] = b[e];
-            }
-        }
-        return;
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = c + e < K ? load_as_f32<BF16 ? Elt::BF16 : Elt::F32>(row, c + e) : 0.0f;
-}
-
 // the largest of the NT threads of a row: 8 to 64 lanes of a wave, or NT / 64 waves
 template <int NT>
 __device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t *red) {
@@ -79,13 +54,13 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void i8_quantize_kernel(const 
         uint32_t top = 0;
         if constexpr (LONG) {
             for (int c = th * 8; c < K; c += NT * 8) {
-                load8<BF16, WIDE>(row, c, K, v[0]);
+                i8_load8<BF16, WIDE>(row, c, K, v[0]);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) top = max(top, i8_abs_bits(v[0][e]));
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < VN; ++j) load8<BF16, WIDE>(row, (th + NT * j) * 8, K, v[j]);
+            for (int j = 0; j < VN; ++j) i8_load8<BF16, WIDE>(row, (th + NT * j) * 8, K, v[j]);
 #pragma unroll
             for (int j = 0; j < VN; ++j)
 #pragma unroll
@@ -99,7 +74,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void i8_quantize_kernel(const 
         };
         if constexpr (LONG) {
             for (int c = th * 8; c < ld; c += NT * 8) {
-                load8<BF16, WIDE>(row, c, K, v[0]);
+                i8_load8<BF16, WIDE>(row, c, K, v[0]);
                 store(c, v[0]);
             }
         } else {

@@ -641,7 +641,8 @@ MulMatPlan plan_mul_mat(const tsk_tensor *a, const tsk_tensor *b, const tsk_tens
         pl.uni = row_stride(dst) != 0;
         pl.nslices = pl.uni ? 1 : b->ne[2] * b->ne[3];
         pl.Nslice = pl.uni ? row_count(b) : b->ne[1];
-        if (b->type != TSK_TYPE_I8_SPLIT) pl.act_bytes = align256(i8_bytes(K, row_count(b)));
+        if (b->type != TSK_TYPE_I8_SPLIT && !(row_stride(b) && gemm_i8_fused(pl.Nslice, K)))
+            pl.act_bytes = align256(i8_bytes(K, row_count(b)));
         pl.bytes = pl.act_bytes;
         return pl;
     }
@@ -735,7 +736,8 @@ int mul_mat_mx(const tsk_tensor *a, const tsk_tensor *b, const tsk_tensor *bias,
     return TSK_OK;
 }
 
-// I8_SPLIT weights (gemm_i8.hip); f32 / bf16 activations become planes in the scratch first
+// I8_SPLIT weights (gemm_i8.hip); f32 / bf16 activations become planes in the scratch first, few rows in the
+// product's own kernel
 int mul_mat_i8(const tsk_tensor *a, const tsk_tensor *b, const tsk_tensor *bias, tsk_tensor *dst, const MulMatPlan &pl,
                const Scratch &scr) {
     const int64_t K = a->ne[0], M = a->ne[1], ld = i8_ld(K);
@@ -760,10 +762,15 @@ int mul_mat_i8(const tsk_tensor *a, const tsk_tensor *b, const tsk_tensor *bias,
         xq = (const int8_t *) ws;
         xd = d;
     }
+    const bool fused = b->type != TSK_TYPE_I8_SPLIT && !pl.act_bytes;
+    const int64_t ld_b = fused ? (int64_t) row_stride(b) : 0;
+    p.x_f32 = b->type == TSK_TYPE_F32;
+    p.ld_x = fused ? ld_b / elt_size(b->type) : 0;
     for (int64_t sl = 0; sl < pl.nslices; ++sl) {
         p.y = (char *) dst->data + sl % b->ne[2] * dst->nb[2] + sl / b->ne[2] * dst->nb[3];
-        p.xq = xq + sl * pl.Nslice * ld;
-        p.xd = xd + sl * pl.Nslice;
+        p.xq = fused ? nullptr : xq + sl * pl.Nslice * ld;
+        p.xd = fused ? nullptr : xd + sl * pl.Nslice;
+        p.x = fused ? (const char *) b->data + sl * pl.Nslice * ld_b : nullptr;
         if ((e = launch_gemm_i8(p, scr.s)) != hipSuccess) return hip_fail(e, "mul_mat launch");
     }
     return TSK_OK;

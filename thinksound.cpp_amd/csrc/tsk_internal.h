@@ -385,8 +385,11 @@ hipError_t launch_i8_dequantize(const int8_t *q, const float *d, const View4 &y,
 struct I8Gemm {
     const int8_t *wq;              // [M][i8_ld(K)]
     const float *wd;               // [M]
-    const int8_t *xq;              // [N][i8_ld(K)]
+    const int8_t *xq;              // [N][i8_ld(K)]; null: x
     const float *xd;               // [N]
+    const void *x;                 // bf16 / f32 rows (16-byte aligned, ld_x elements apart), where gemm_i8_fused
+    int x_f32;
+    int64_t ld_x;
     const float *bias;             // [M], nullable, 16-byte aligned
     void *y;
     int y_bf16;
@@ -394,6 +397,8 @@ struct I8Gemm {
     int M, N, K;
 };
 hipError_t launch_gemm_i8(const I8Gemm &p, hipStream_t s);
+// whether N rows of K bf16 / f32 activations are quantized inside the product's kernel
+bool gemm_i8_fused(int64_t N, int64_t K);
 
 // ---------------------------------------------------------------- rotary positions over several axes
 // tsk_rope_axes' operands (rope_axes.hip): x and y [D, heads, S, B]
