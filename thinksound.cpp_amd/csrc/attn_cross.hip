@@ -29,12 +29,16 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
-constexpr int KT = 64;                  // states a tile
-
 // In each group of 16 lanes, lane i gets, as element j, element i % 4 of the 8
 // bytes that lane 4 j + i / 4 addresses: with lane s at row r0 + s / 4, columns c0 +
 // 4 (s % 4) .. + 3, lane i receives rows r0 .. r0 + 3 of column c0 + i
 __device__ __forceinline__ s16x4 read_turned(const uint16_t *p) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *) (p)); }
+
+// Piece c (16 bytes) of row t of a tile in LDS lies at slot c ^ key(t). K: a 16-byte read of a wave
+// takes one piece of 32 rows in turns of 16 lanes (0-3, 12-15, 20-27; 4-11, 16-19, 28-31; ...): the
+// keys send those to 16 places. V: the four rows of a transposing read, 64 bytes each
+template <int DP> __device__ __forceinline__ int k_key(int row) { return DP == 128 ? row & 15 : row >> 1 & 7; }
+template <int DP> __device__ __forceinline__ int v_key(int row) { return (DP == 128 ? 4 : 2) * (row & 3); }
 
 template <bool BF16> struct Half;
 template <> struct Half<true> {
@@ -78,67 +82,124 @@ __device__ __forceinline__ u32x4 load_q8(const char *row, int d, int type) {
     return o;
 }
 
-// DP: the head size rounded up to 64 or 128; the values past it are zeros
-template <int DP, bool BF16>
-__global__ __launch_bounds__(256) void cross_attn_kernel(const CrossAttn p, int qtiles) {
-    typedef Half<BF16> T;
-    typedef typename T::x8 x8;
-    constexpr int CH = DP / 8, RL = 64 / CH, NL = KT / RL, TILE = KT * DP;     // 16-byte pieces a row, rows and loads of 1 KB
-    constexpr int FAR = (int) 0x80000000u;
-    extern __shared__ __attribute__((aligned(1024))) uint16_t lds[];           // [2][K tile, V tile]
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int l32 = lane & 31, hi = lane >> 5;
-    const int qt = (int) (blockIdx.x % qtiles), hk = (int) (blockIdx.x / qtiles % p.Hkv), b = (int) (blockIdx.x / qtiles / p.Hkv);
-    const int G = p.H / p.Hkv;
-    const int64_t R = (int64_t) G * p.Nq;
-    const int nkv = p.kv_len ? max(0, min(p.kv_len[b], p.Nkv)) : p.Nkv;
-    const int nq = p.q_len ? max(0, min(p.q_len[b], p.Nq)) : p.Nq;
-    const int64_t r0 = (int64_t) qt * 128 + wave * 32;
-    if (nq == 0 || (G == 1 && (int64_t) qt * 128 >= nq)) return;
-    const int64_t row = std::min<int64_t>(r0 + l32, R - 1);
-    const int h = hk * G + (int) (row / p.Nq), iq = (int) (row % p.Nq);
+// A launch's unit: a tile of rows of one key and value head, and (splits > 1) one of the
+// ranges that its sequence's tiles of states are dealt to. The ranges go by the sequence's own
+// length, which the device alone knows: `per` tiles each, the last ones empty.
+struct Unit {
+    int b, hk, nkv, nq, tile0, tile1, split;
+    int64_t r0, R;
+    bool none;
+};
+template <int KT>
+__device__ __forceinline__ Unit unit_of(const CrossAttn &p, int qtiles, int rows) {
+    Unit u;
+    int64_t i = blockIdx.x;
+    u.split = (int) (i % p.splits);
+    i /= p.splits;
+    const int qt = (int) (i % qtiles);
+    u.hk = (int) (i / qtiles % p.Hkv);
+    u.b = (int) (i / qtiles / p.Hkv);
+    u.nkv = p.kv_len ? max(0, min(p.kv_len[u.b], p.Nkv)) : p.Nkv;
+    u.nq = p.q_len ? max(0, min(p.q_len[u.b], p.Nq)) : p.Nq;
+    const int G = p.H / p.Hkv, tiles = (u.nkv + KT - 1) / KT, per = (tiles + p.splits - 1) / p.splits;
+    u.R = (int64_t) G * p.Nq;
+    u.r0 = (int64_t) qt * rows;
+    u.tile0 = u.split * per;
+    u.tile1 = min(tiles, u.tile0 + per);
+    // (a first range without states writes its zeros)
+    u.none = u.nq == 0 || (G == 1 && u.r0 >= u.nq) || (u.split > 0 && u.tile0 >= u.tile1);
+    return u;
+}
+// ranges of a sequence that hold states (1 for one that has none)
+template <int KT>
+__device__ __forceinline__ int used_splits(const CrossAttn &p, int nkv) {
+    const int tiles = (nkv + KT - 1) / KT, per = (tiles + p.splits - 1) / p.splits;
+    return per ? (tiles + per - 1) / per : 1;
+}
 
-    const char *qrow = (const char *) p.q + iq * p.q_nb1 + h * p.q_nb2 + b * p.q_nb3;
-    x8 q[DP / 16];
+// head and token of row r of a key and value head's rows
+__device__ __forceinline__ void row_of(const CrossAttn &p, int hk, int64_t r, int &h, int &iq) {
+    const int g = (int) (r / p.Nq);
+    h = hk * (p.H / p.Hkv) + g;
+    iq = (int) (r - (int64_t) g * p.Nq);
+}
+template <int DP, bool BF16>
+__device__ __forceinline__ void load_q(const CrossAttn &p, int b, int h, int iq, int hi, typename Half<BF16>::x8 (&q)[DP / 16]) {
+    const char *row = (const char *) p.q + iq * p.q_nb1 + h * p.q_nb2 + b * p.q_nb3;
 #pragma unroll
     for (int ks = 0; ks < DP / 16; ++ks) {
         const int d = 16 * ks + 8 * hi;
         const u32x4 zero = {0, 0, 0, 0};
-        q[ks] = __builtin_bit_cast(x8, d < p.D ? load_q8<BF16>(qrow, d, p.q_type) : zero);
+        q[ks] = __builtin_bit_cast(typename Half<BF16>::x8, d < p.D ? load_q8<BF16>(row, d, p.q_type) : zero);
     }
+}
+// 1 / the sum of the weights; 0 where there are none, and a NaN stays
+__device__ __forceinline__ float inverse(float l) { return l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l; }
+// 4 values of an output row from dim d on
+__device__ __forceinline__ void store_o4(const CrossAttn &p, char *row, int d, f32x4 v) {
+    if (p.o_type == TSK_TYPE_F32) {
+        *(f32x4 *) (row + d * 4) = v;
+    } else if (p.o_type == TSK_TYPE_BF16) {
+        *(u32x2 *) (row + d * 2) = u32x2{f32_to_bf16_bits(v[0]) | (uint32_t) f32_to_bf16_bits(v[1]) << 16,
+                                        f32_to_bf16_bits(v[2]) | (uint32_t) f32_to_bf16_bits(v[3]) << 16};
+    } else {
+        *(u32x2 *) (row + d * 2) = u32x2{f32_to_f16_bits(v[0]) | (uint32_t) f32_to_f16_bits(v[1]) << 16,
+                                        f32_to_f16_bits(v[2]) | (uint32_t) f32_to_f16_bits(v[3]) << 16};
+    }
+}
+__device__ __forceinline__ char *o_row(const CrossAttn &p, int b, int h, int iq) {
+    return (char *) p.o + h * p.o_nb1 + iq * p.o_nb2 + b * p.o_nb3;
+}
+// Scratch of splits > 1: per range and row (i = (b * Hkv + hk) * R + r) D sums, then for all of
+// them the maximum and the sum of the weights
+__device__ __forceinline__ int64_t all_rows(const CrossAttn &p) { return (int64_t) p.B * p.H * p.Nq; }
+__device__ __forceinline__ float *part_o(const CrossAttn &p, int split, int64_t i) { return p.part + (split * all_rows(p) + i) * p.D; }
+__device__ __forceinline__ float *part_ml(const CrossAttn &p, int split, int64_t i) {
+    return p.part + (int64_t) p.splits * all_rows(p) * p.D + (split * all_rows(p) + i) * 2;
+}
 
-    const char *kp = (const char *) p.k + hk * p.k_nb2 + b * p.k_nb3, *vp = (const char *) p.v + hk * p.v_nb2 + b * p.v_nb3;
-    const uint8_t *flags = p.kv_valid ? p.kv_valid + b * p.kv_valid_nb : nullptr;
-    // Piece c of row t of a tile lies at slot c ^ key(t). K: 16 lanes of a 16-byte read take one piece
-    // of 16 rows: keys that send them to 16 places; V: the four rows of a transposing read
+// ---------------------------------------------------------------- few rows
+// A workgroup takes 32 rows, its four waves tiles of 32 states in turns, each through a ring
+// of its own in LDS: no barrier until their sums meet. Bound by the states' bytes.
+template <int DP, bool BF16>
+__global__ __launch_bounds__(256) void cross_attn_few_kernel(const CrossAttn p, int qtiles) {
+    typedef Half<BF16> T;
+    typedef typename T::x8 x8;
+    constexpr int KT = 32, CH = DP / 8, RL = 64 / CH, NL = KT / RL, TILE = KT * DP, NB = 2;
+    constexpr int FAR = (int) 0x80000000u, OS = DP + 4;
+    extern __shared__ __attribute__((aligned(1024))) uint16_t lds[];           // [wave][NB][K tile, V tile]
+    __shared__ float mls[4][2][32];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l32 = lane & 31, hi = lane >> 5;
+    const Unit u = unit_of<KT>(p, qtiles, 32);
+    if (u.none) return;
+    int h, iq;
+    row_of(p, u.hk, std::min<int64_t>(u.r0 + l32, u.R - 1), h, iq);
+    const char *kp = (const char *) p.k + u.hk * p.k_nb2 + u.b * p.k_nb3, *vp = (const char *) p.v + u.hk * p.v_nb2 + u.b * p.v_nb3;
+    const uint8_t *flags = p.kv_valid ? p.kv_valid + u.b * p.kv_valid_nb : nullptr;
     const int lr = lane / CH;
-    const int kc = (lane % CH) ^ (DP == 128 ? 4 * (wave & 3) + (lane >> 4) : (4 * (wave & 1) + (lane >> 4)) & 7);
-    const int vc = (lane % CH) ^ (DP == 128 ? 4 * (lr & 3) : 2 * (lr & 3));
-    const int koff = kc * 8 < p.D ? (int) (lr * p.k_nb1) + kc * 16 : FAR, voff = vc * 8 < p.D ? (int) (lr * p.v_nb1) + vc * 16 : FAR;
+    uint16_t *ring = lds + wave * NB * 2 * TILE;
     auto issue = [&](int tile, int buf) {
-        uint16_t *dst = lds + buf * 2 * TILE;
-        const int left = min(KT, nkv - tile * KT);
+        uint16_t *dst = ring + buf * 2 * TILE;
+        const int left = min(KT, u.nkv - tile * KT);
         const int64_t k0 = (int64_t) tile * KT;
-        // rows past the last state that counts read as zeros
         const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc((void *) (kp + k0 * p.k_nb1), (short) 0,
                                                                             (int) ((left - 1) * p.k_nb1) + 2 * p.D, 0x00020000);
         const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc((void *) (vp + k0 * p.v_nb1), (short) 0,
                                                                             (int) ((left - 1) * p.v_nb1) + 2 * p.D, 0x00020000);
 #pragma unroll
-        for (int i = 0; i < NL / 4; ++i) {
-            const int j = wave + 4 * i;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (lds_void *) (dst + j * 512), 16, koff, (int) (j * RL * p.k_nb1), 0, 0);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (lds_void *) (dst + TILE + j * 512), 16, voff, (int) (j * RL * p.v_nb1), 0, 0);
+        for (int j = 0; j < NL; ++j) {
+            const int kc = (lane % CH) ^ k_key<DP>(j * RL + lr), vc = (lane % CH) ^ v_key<DP>(lr);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (lds_void *) (dst + j * 512), 16, kc * 8 < p.D ? (int) (lr * p.k_nb1) + kc * 16 : FAR,
+                                                     (int) (j * RL * p.k_nb1), 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (lds_void *) (dst + TILE + j * 512), 16, vc * 8 < p.D ? (int) (lr * p.v_nb1) + vc * 16 : FAR,
+                                                     (int) (j * RL * p.v_nb1), 0, 0);
         }
     };
-    // bit s: state s of the tile counts
-    auto counted = [&](int tile) -> uint64_t {
-        const int left = nkv - tile * KT;
-        uint64_t m = left >= KT ? ~(uint64_t) 0 : ((uint64_t) 1 << left) - 1;
-        if (flags) m &= __ballot(lane < left && flags[(int64_t) tile * KT + lane]);
-        return m;
-    };
-
+    const int first = u.tile0 + wave;
+    if (first < u.tile1) issue(first, 0);
+    x8 q[DP / 16];
+    load_q<DP, BF16>(p, u.b, h, iq, hi, q);
     f32x16 o[DP / 32];
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db)
@@ -146,118 +207,430 @@ __global__ __launch_bounds__(256) void cross_attn_kernel(const CrossAttn p, int 
         for (int e = 0; e < 16; ++e) o[db][e] = 0.0f;
     float m_run = -__builtin_inff(), l_run = 0.0f;
     const float c = p.c;
-    const int l16 = lane & 15, grp = (lane >> 4) & 1, vrow = 4 * hi + (l16 >> 2), vkey = (DP == 128 ? 4 : 2) * (l16 >> 2);
-    const int tiles = (nkv + KT - 1) / KT;
-    if (tiles) issue(0, 0);
-    for (int t = 0; t < tiles; ++t) {
-        const uint64_t count = counted(t);
+    const int l16 = lane & 15, grp = (lane >> 4) & 1, vrow = 4 * hi + (l16 >> 2);
+    int buf = 0;
+    for (int t = first; t < u.tile1; t += 4, buf ^= 1) {
+        const int left = u.nkv - t * KT;
+        uint32_t count = left >= KT ? ~0u : (1u << left) - 1;
+        if (flags) count &= (uint32_t) __ballot(l32 < left && flags[(int64_t) t * KT + l32]);
+        // (the flags' loads are the wave's last: with them the tile has landed too)
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();                                     // tile t is in LDS, every wave is done with the one before
-        if (t + 1 < tiles) issue(t + 1, (t + 1) & 1);
-        const uint16_t *kb = lds + (t & 1) * 2 * TILE, *vb = kb + TILE;
+        if (t + 4 < u.tile1) issue(t + 4, buf ^ 1);
+        uint16_t *kb = ring + buf * 2 * TILE, *vb = kb + TILE;
         if (count == 0) continue;
-        const bool some = count != ~(uint64_t) 0;
-        if (some && flags) {
+        if (flags && count != ~0u) {
             // a state that does not count may hold anything: 0 times it may not be 0
-            const int s = tid >> 2;
-            if (!(count >> s & 1))
-                for (int i = 0; i < DP / 32; ++i) *(u32x4 *) (lds + (t & 1) * 2 * TILE + TILE + s * DP + (tid & 3) * (DP / 4) + i * 8) = u32x4{0, 0, 0, 0};
-            __syncthreads();
+            if (!(count >> l32 & 1))
+#pragma unroll
+                for (int i = 0; i < DP / 16; ++i) *(u32x4 *) (vb + l32 * DP + hi * (DP / 2) + i * 8) = u32x4{0, 0, 0, 0};
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
-        f32x16 s[2];
+        f32x16 s;
 #pragma unroll
-        for (int kb2 = 0; kb2 < 2; ++kb2) {
+        for (int e = 0; e < 16; ++e) s[e] = 0.0f;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) s[kb2][e] = 0.0f;
+        for (int ks = 0; ks < DP / 16; ++ks) s = T::mfma(*(const x8 *) (kb + l32 * DP + (((2 * ks + hi) ^ k_key<DP>(l32)) << 3)), q[ks], s);
+        if (count != ~0u) {
+            const uint32_t mine = count >> 4 * hi;
 #pragma unroll
-            for (int ks = 0; ks < DP / 16; ++ks) {
-                const int r = 32 * kb2 + l32, key = DP == 128 ? r & 15 : (r >> 1) & 7;
-                const x8 a = *(const x8 *) (kb + r * DP + (((2 * ks + hi) ^ key) << 3));
-                s[kb2] = T::mfma(a, q[ks], s[kb2]);
-            }
+            for (int e = 0; e < 16; ++e)
+                if (!(mine >> (8 * (e >> 2) + (e & 3)) & 1)) s[e] = -__builtin_inff();
         }
-        if (some) {
-            const uint64_t mine = count >> 4 * hi;
+        float top = s[0];
 #pragma unroll
-            for (int kb2 = 0; kb2 < 2; ++kb2)
-#pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    if (!(mine >> (32 * kb2 + 8 * (e >> 2) + (e & 3)) & 1)) s[kb2][e] = -__builtin_inff();
-        }
-        float top = s[0][0];
-#pragma unroll
-        for (int e = 1; e < 16; ++e) top = fmaxf(top, s[0][e]);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) top = fmaxf(top, s[1][e]);
+        for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
         const float m_new = fmaxf(m_run, half_pair_max(top) * c);
         const float sub = m_new == -__builtin_inff() ? 0.0f : m_new, alpha = __builtin_amdgcn_exp2f(m_run - sub);
+        if (__any(m_new > m_run)) {
+            l_run *= alpha;
+#pragma unroll
+            for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[db][e] *= alpha;
+        }
         m_run = m_new;
-        l_run *= alpha;
+        x8 pf[2];
 #pragma unroll
-        for (int db = 0; db < DP / 32; ++db)
+        for (int kg = 0; kg < 2; ++kg) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) o[db][e] *= alpha;
-        x8 pf[4];
-#pragma unroll
-        for (int kg = 0; kg < 4; ++kg) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) T::set(pf[kg], e, __builtin_amdgcn_exp2f(__builtin_fmaf(s[kg >> 1][8 * (kg & 1) + e], c, -sub)));
+            for (int e = 0; e < 8; ++e) T::set(pf[kg], e, __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * kg + e], c, -sub)));
 #pragma unroll
             for (int e = 0; e < 8; e += 2) l_run = T::sum2(pf[kg], e, l_run);
         }
 #pragma unroll
-        for (int kg = 0; kg < 4; ++kg)
+        for (int kg = 0; kg < 2; ++kg)
 #pragma unroll
             for (int db = 0; db < DP / 32; ++db) {
                 const int ch = 4 * db + 2 * grp + ((l16 & 3) >> 1);
-                const uint16_t *at = vb + (16 * kg + vrow) * DP + ((ch ^ vkey) << 3) + 4 * (l16 & 1);
+                const uint16_t *at = vb + (16 * kg + vrow) * DP + ((ch ^ v_key<DP>(l16 >> 2)) << 3) + 4 * (l16 & 1);
                 const s16x4 a = read_turned(at), a2 = read_turned(at + 8 * DP);
                 const s16x8 a8 = {a[0], a[1], a[2], a[3], a2[0], a2[1], a2[2], a2[3]};
                 o[db] = T::mfma(__builtin_bit_cast(x8, a8), pf[kg], o[db]);
             }
+        // (the next turn's loads land in the buffer read here: every read is done)
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
-    const float l = half_pair_sum(l_run), inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;   // (a NaN stays)
-    if (r0 + l32 >= R || iq >= nq) return;
-    char *orow = (char *) p.o + h * p.o_nb1 + iq * p.o_nb2 + b * p.o_nb3;
+    // the four waves' sums, brought to one maximum, meet in LDS: [wave][row][dim]
+    const float l_all = half_pair_sum(l_run);
+    if (hi == 0) {
+        mls[wave][0][l32] = m_run;
+        mls[wave][1][l32] = l_all;
+    }
+    __syncthreads();
+    float *os = (float *) lds;
+    float m = mls[0][0][l32];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) m = fmaxf(m, mls[w][0][l32]);
+    const float f = __builtin_amdgcn_exp2f(m_run - (m == -__builtin_inff() ? 0.0f : m));
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-            const int d = 32 * db + 2 * e + 4 * hi;
-            if (d >= p.D) continue;
-            const float v[4] = {o[db][e] * inv, o[db][e + 1] * inv, o[db][e + 2] * inv, o[db][e + 3] * inv};
-            if (p.o_type == TSK_TYPE_F32) {
-                *(f32x4 *) (orow + d * 4) = f32x4{v[0], v[1], v[2], v[3]};
-            } else if (p.o_type == TSK_TYPE_BF16) {
-                *(u32x2 *) (orow + d * 2) = u32x2{f32_to_bf16_bits(v[0]) | (uint32_t) f32_to_bf16_bits(v[1]) << 16,
-                                                 f32_to_bf16_bits(v[2]) | (uint32_t) f32_to_bf16_bits(v[3]) << 16};
-            } else {
-                *(u32x2 *) (orow + d * 2) = u32x2{f32_to_f16_bits(v[0]) | (uint32_t) f32_to_f16_bits(v[1]) << 16,
-                                                 f32_to_f16_bits(v[2]) | (uint32_t) f32_to_f16_bits(v[3]) << 16};
-            }
+        for (int e = 0; e < 16; e += 4)
+            *(f32x4 *) (os + (wave * 32 + l32) * OS + 32 * db + 2 * e + 4 * hi) = f32x4{o[db][e], o[db][e + 1], o[db][e + 2], o[db][e + 3]} * f;
+    __syncthreads();
+    const int64_t left = u.R - u.r0;
+    const int rows = left < 32 ? (int) left : 32, D4 = p.D / 4;
+    for (int i = tid; i < rows * D4; i += 256) {
+        const int r = i / D4, d = (i - r * D4) * 4;
+        float mr = mls[0][0][r], l = 0.0f;
+        for (int w = 1; w < 4; ++w) mr = fmaxf(mr, mls[w][0][r]);
+        const float sub = mr == -__builtin_inff() ? 0.0f : mr;
+        f32x4 v = {0, 0, 0, 0};
+        for (int w = 0; w < 4; ++w) {
+            l += mls[w][1][r] * __builtin_amdgcn_exp2f(mls[w][0][r] - sub);
+            v += *(const f32x4 *) (os + (w * 32 + r) * OS + d);
         }
+        int hr, iqr;
+        row_of(p, u.hk, u.r0 + r, hr, iqr);
+        if (iqr >= u.nq) continue;
+        if (p.splits > 1) {
+            const int64_t at = ((int64_t) u.b * p.Hkv + u.hk) * u.R + u.r0 + r;
+            *(f32x4 *) (part_o(p, u.split, at) + d) = v;
+            if (d == 0) {
+                float *ml = part_ml(p, u.split, at);
+                ml[0] = mr;
+                ml[1] = l;
+            }
+        } else {
+            store_o4(p, o_row(p, u.b, hr, iqr), d, v * inverse(l));
+        }
+    }
+}
+
+// the ranges of every row brought together, 4 dims a thread
+template <int KT>
+__global__ __launch_bounds__(256) void cross_attn_join_kernel(const CrossAttn p) {
+    const int D4 = p.D / 4;
+    const int64_t n = all_rows(p) * D4, R = (int64_t) (p.H / p.Hkv) * p.Nq;
+    for (int64_t i = (int64_t) blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t) gridDim.x * 256) {
+        const int64_t at = i / D4, unit = at / R;
+        const int d = (int) (i - at * D4) * 4, b = (int) (unit / p.Hkv), hk = (int) (unit % p.Hkv);
+        int h, iq;
+        row_of(p, hk, at - unit * R, h, iq);
+        if (p.q_len && iq >= p.q_len[b]) continue;
+        const int used = used_splits<KT>(p, p.kv_len ? max(0, min(p.kv_len[b], p.Nkv)) : p.Nkv);
+        float m = -__builtin_inff(), l = 0.0f;
+        for (int s = 0; s < used; ++s) m = fmaxf(m, part_ml(p, s, at)[0]);
+        const float sub = m == -__builtin_inff() ? 0.0f : m;
+        f32x4 v = {0, 0, 0, 0};
+        for (int s = 0; s < used; ++s) {
+            const float *ml = part_ml(p, s, at), f = __builtin_amdgcn_exp2f(ml[0] - sub);
+            l += ml[1] * f;
+            v += *(const f32x4 *) (part_o(p, s, at) + d) * f;
+        }
+        store_o4(p, o_row(p, b, h, iq), d, v * inverse(l));
+    }
+}
+
+// ---------------------------------------------------------------- many rows
+// A workgroup takes 128 QB rows, 32 QB a wave, and tiles of 64 states through a ring of three
+// in LDS. Half a tile (32 states) at a time, a wave multiplies the next half's K with Q and
+// the last half's V with P while it turns this half's logits into weights: three steps of
+// three halves without a dependence, so that the matrix unit and the rest of the SIMD work at
+// once. A wave with 64 rows (QB 2) uses every operand that it reads from LDS twice.
+//
+// The running maximum moves only when the logits pass it by more than 2^8, and then to a whole
+// number (log2 domain): sums and weights already rounded are scaled by a power of two, exactly.
+template <int DP, bool BF16, int QB>
+__global__ __launch_bounds__(256) void cross_attn_kernel(const CrossAttn p, int qtiles) {
+    typedef Half<BF16> T;
+    typedef typename T::x8 x8;
+    constexpr int KT = 64, CH = DP / 8, RL = 64 / CH, NL = KT / RL / 4, TILE = KT * DP;      // 16-byte pieces a row, rows a load, loads a wave
+    constexpr int FAR = (int) 0x80000000u;
+    extern __shared__ __attribute__((aligned(1024))) uint16_t lds[];           // [3][K tile, V tile]
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l32 = lane & 31, hi = lane >> 5;
+    const Unit u = unit_of<KT>(p, qtiles, 128 * QB);
+    if (u.none) return;
+    int h[QB], iq[QB];
+    x8 q[QB][DP / 16];
+#pragma unroll
+    for (int i = 0; i < QB; ++i) {
+        row_of(p, u.hk, std::min<int64_t>(u.r0 + (wave * QB + i) * 32 + l32, u.R - 1), h[i], iq[i]);
+        load_q<DP, BF16>(p, u.b, h[i], iq[i], hi, q[i]);
+    }
+    const char *kp = (const char *) p.k + u.hk * p.k_nb2 + u.b * p.k_nb3, *vp = (const char *) p.v + u.hk * p.v_nb2 + u.b * p.v_nb3;
+    const uint8_t *flags = p.kv_valid ? p.kv_valid + u.b * p.kv_valid_nb : nullptr;
+    // (a wave's loads are 4 * RL rows apart, which the keys do not see)
+    const int lr = lane / CH, kc = (lane % CH) ^ k_key<DP>(wave * RL + lr), vc = (lane % CH) ^ v_key<DP>(lr);
+    const int koff = kc * 8 < p.D ? (int) (lr * p.k_nb1) + kc * 16 : FAR, voff = vc * 8 < p.D ? (int) (lr * p.v_nb1) + vc * 16 : FAR;
+    // tile t into slot s; tiles past the last: zeros, so that every wait counts the same
+    auto issue = [&](int t, int s) {
+        uint16_t *dst = lds + s * 2 * TILE;
+        const int left = t < u.tile1 ? min(KT, u.nkv - t * KT) : 0;
+        const int64_t k0 = t < u.tile1 ? (int64_t) t * KT : 0;
+        // rows past the last state read as zeros
+        const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc((void *) (kp + k0 * p.k_nb1), (short) 0,
+                                                                            left ? (int) ((left - 1) * p.k_nb1) + 2 * p.D : 0, 0x00020000);
+        const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc((void *) (vp + k0 * p.v_nb1), (short) 0,
+                                                                            left ? (int) ((left - 1) * p.v_nb1) + 2 * p.D : 0, 0x00020000);
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            const int j = wave + 4 * i;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (lds_void *) (dst + j * 512), 16, koff, (int) (j * RL * p.k_nb1), 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (lds_void *) (dst + TILE + j * 512), 16, voff, (int) (j * RL * p.v_nb1), 0, 0);
+        }
+    };
+    // bit s: state s of tile t counts
+    auto counted = [&](int t) -> uint64_t {
+        const int left = u.nkv - t * KT;
+        if (t >= u.tile1) return 0;
+        uint64_t m = left >= KT ? ~(uint64_t) 0 : ((uint64_t) 1 << left) - 1;
+        if (flags) m &= __ballot(lane < left && flags[(int64_t) t * KT + lane]);
+        return m;
+    };
+    // a state that does not count may hold anything, and 0 times it may not be 0: its V becomes zeros
+    auto clear = [&](uint64_t count, int s) {
+        if (!flags || count == ~(uint64_t) 0) return;
+        const int r = tid >> 2;
+        if (!(count >> r & 1))
+#pragma unroll
+            for (int i = 0; i < DP / 32; ++i) *(u32x4 *) (lds + s * 2 * TILE + TILE + r * DP + (tid & 3) * (DP / 4) + i * 8) = u32x4{0, 0, 0, 0};
+        __syncthreads();
+    };
+    f32x16 o[QB][DP / 32];
+    float m[QB], sub[QB], l[QB];
+#pragma unroll
+    for (int i = 0; i < QB; ++i) {
+        m[i] = -__builtin_inff();
+        sub[i] = l[i] = 0.0f;
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[i][db][e] = 0.0f;
+    }
+    const float c = p.c;
+    const int l16 = lane & 15, grp = (lane >> 4) & 1, vrow = 4 * hi + (l16 >> 2);
+    struct Logits {
+        f32x16 s[QB];
+        float top[QB];
+    };
+    struct Weights {
+        x8 w[QB][2];
+    };
+    auto multiply_k = [&](int slot, int half, Logits &n) __attribute__((always_inline)) {
+        const uint16_t *kb = lds + slot * 2 * TILE + 32 * half * DP;
+#pragma unroll
+        for (int i = 0; i < QB; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) n.s[i][e] = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) {
+            const x8 a = *(const x8 *) (kb + l32 * DP + (((2 * ks + hi) ^ k_key<DP>(l32)) << 3));
+#pragma unroll
+            for (int i = 0; i < QB; ++i) n.s[i] = T::mfma(a, q[i][ks], n.s[i]);
+        }
+    };
+    auto largest = [&](Logits &n) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < QB; ++i) {
+            float t = n.s[i][0];
+#pragma unroll
+            for (int e = 1; e < 16; ++e) t = fmaxf(t, n.s[i][e]);
+            n.top[i] = t;
+        }
+    };
+    auto multiply_v = [&](int slot, int half, const Weights &w) __attribute__((always_inline)) {
+        const uint16_t *vb = lds + slot * 2 * TILE + TILE + 32 * half * DP;
+#pragma unroll
+        for (int kg = 0; kg < 2; ++kg)
+#pragma unroll
+            for (int db = 0; db < DP / 32; ++db) {
+                const int ch = 4 * db + 2 * grp + ((l16 & 3) >> 1);
+                const uint16_t *at = vb + (16 * kg + vrow) * DP + ((ch ^ v_key<DP>(l16 >> 2)) << 3) + 4 * (l16 & 1);
+                const s16x4 a = read_turned(at), a2 = read_turned(at + 8 * DP);
+                const s16x8 a8 = {a[0], a[1], a[2], a[3], a2[0], a2[1], a2[2], a2[3]};
+#pragma unroll
+                for (int i = 0; i < QB; ++i) o[i][db] = T::mfma(__builtin_bit_cast(x8, a8), w.w[i][kg], o[i][db]);
+            }
+    };
+    // logits to weights
+    auto weigh = [&](const Logits &n, Weights &w) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < QB; ++i)
+#pragma unroll
+            for (int kg = 0; kg < 2; ++kg) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) T::set(w.w[i][kg], e, __builtin_amdgcn_exp2f(__builtin_fmaf(n.s[i][8 * kg + e], c, -sub[i])));
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) l[i] = T::sum2(w.w[i][kg], e, l[i]);
+            }
+    };
+    // what the next weights go by: states that do not count leave, the maximum moves if it has to
+    auto settle = [&](Logits &n, uint64_t count, int half, Weights &before) __attribute__((always_inline)) {
+        const uint32_t part = (uint32_t) (count >> 32 * half);
+        if (part != ~0u) {
+            const uint32_t mine = part >> 4 * hi;
+#pragma unroll
+            for (int i = 0; i < QB; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (!(mine >> (8 * (e >> 2) + (e & 3)) & 1)) n.s[i][e] = -__builtin_inff();
+            largest(n);
+        }
+        float top[QB];
+        bool move = false;
+#pragma unroll
+        for (int i = 0; i < QB; ++i) {
+            top[i] = half_pair_max(n.top[i]) * c;
+            move = move || top[i] > m[i] + 8.0f;
+        }
+        if (!__any(move)) return;
+#pragma unroll
+        for (int i = 0; i < QB; ++i) {
+            const float to = top[i] > m[i] + 8.0f ? __builtin_ceilf(top[i]) : m[i];
+            const float s = to == -__builtin_inff() ? 0.0f : to, f = __builtin_amdgcn_exp2f(m[i] - s);
+            m[i] = to;
+            sub[i] = s;
+            l[i] *= f;
+#pragma unroll
+            for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[i][db][e] *= f;
+#pragma unroll
+            for (int kg = 0; kg < 2; ++kg)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) T::set(before.w[i][kg], e, (float) before.w[i][kg][e] * f);
+        }
+    };
+    constexpr int LOADS = 2 * NL;
+    if (u.tile0 < u.tile1) {
+        issue(u.tile0, 0);
+        issue(u.tile0 + 1, 1);
+        issue(u.tile0 + 2, 2);
+        Logits na, nb;
+        Weights wa, wb;
+#pragma unroll
+        for (int i = 0; i < QB; ++i)
+#pragma unroll
+            for (int kg = 0; kg < 2; ++kg)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) T::set(wa.w[i][kg], e, 0.0f), T::set(wb.w[i][kg], e, 0.0f);
+        uint64_t count = counted(u.tile0), next = counted(u.tile0 + 1);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");           // (tiles 0 and 1)
+        __syncthreads();
+        clear(count, 0);
+        clear(next, 1);
+        multiply_k(0, 0, na);
+        largest(na);
+        settle(na, count, 0, wb);
+        multiply_k(0, 1, nb);
+        weigh(na, wa);
+        largest(nb);
+        int slot = 0;
+        for (int t = u.tile0; t + 1 < u.tile1; ++t) {
+            const int s1 = slot == 2 ? 0 : slot + 1, s2 = s1 == 2 ? 0 : s1 + 1;
+            // second half of tile t
+            settle(nb, count, 1, wa);
+            multiply_k(s1, 0, na);
+            weigh(nb, wb);
+            multiply_v(slot, 0, wa);
+            largest(na);
+            // first half of tile t + 1
+            settle(na, next, 0, wb);
+            multiply_k(s1, 1, nb);
+            weigh(na, wa);
+            multiply_v(slot, 1, wb);
+            largest(nb);
+            count = next;
+            next = counted(t + 2);
+            // tile t + 2 has landed, every wave is done with tile t: its slot takes tile t + 3
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __syncthreads();
+            clear(next, s2);
+            issue(t + 3, slot);
+            slot = s1;
+        }
+        settle(nb, count, 1, wa);
+        weigh(nb, wb);
+        multiply_v(slot, 0, wa);
+        multiply_v(slot, 1, wb);
+    }
+#pragma unroll
+    for (int i = 0; i < QB; ++i) {
+        const int64_t r = u.r0 + (wave * QB + i) * 32 + l32;
+        const float la = half_pair_sum(l[i]), inv = inverse(la);
+        if (r >= u.R || iq[i] >= u.nq) continue;
+        char *row = o_row(p, u.b, h[i], iq[i]);
+        const int64_t at = ((int64_t) u.b * p.Hkv + u.hk) * u.R + r;
+        if (p.splits > 1 && hi == 0) {
+            float *ml = part_ml(p, u.split, at);
+            ml[0] = m[i];
+            ml[1] = la;
+        }
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const int d = 32 * db + 2 * e + 4 * hi;
+                if (d >= p.D) continue;
+                const f32x4 v = {o[i][db][e], o[i][db][e + 1], o[i][db][e + 2], o[i][db][e + 3]};
+                if (p.splits > 1) *(f32x4 *) (part_o(p, u.split, at) + d) = v;
+                else store_o4(p, row, d, v * inv);
+            }
+    }
+}
+
+template <class F>
+hipError_t launch_units(F kern, const CrossAttn &p, int rows, size_t lds, hipStream_t s) {
+    const int64_t R = (int64_t) (p.H / p.Hkv) * p.Nq, qtiles = (R + rows - 1) / rows, units = qtiles * p.Hkv * p.B * p.splits;
+    if (units >= (int64_t) 1 << 24) return hipErrorInvalidValue;
+    lds_opt_in((const void *) kern, lds);
+    launch_kernel(kern, dim3((unsigned) units), dim3(256), lds, s, p, (int) qtiles);
+    return hipGetLastError();
 }
 
 template <int DP, bool BF16>
-hipError_t launch_dp(const CrossAttn &p, hipStream_t s) {
-    const int64_t R = (int64_t) (p.H / p.Hkv) * p.Nq, qtiles = (R + 127) / 128, units = qtiles * p.Hkv * p.B;
-    constexpr size_t LDS = 2 * 2 * KT * DP * 2;
-    if (units * 256 >= (int64_t) 1 << 32 || units > 0x7fffffff) return hipErrorInvalidValue;
-    lds_opt_in((const void *) cross_attn_kernel<DP, BF16>, LDS);
-    launch_kernel(cross_attn_kernel<DP, BF16>, dim3((unsigned) units), dim3(256), LDS, s, p, (int) qtiles);
+hipError_t launch_dp(const CrossAttn &p, const CrossAttnPlan &plan, hipStream_t s) {
+    hipError_t e;
+    if (plan.rows == 32) e = launch_units(cross_attn_few_kernel<DP, BF16>, p, 32, 4 * 2 * 2 * 32 * DP * 2, s);
+    else if (plan.rows == 128) e = launch_units(cross_attn_kernel<DP, BF16, 1>, p, 128, 3 * 2 * 64 * DP * 2, s);
+    else e = launch_units(cross_attn_kernel<DP, BF16, 2>, p, 256, 3 * 2 * 64 * DP * 2, s);
+    if (e != hipSuccess || p.splits == 1) return e;
+    const int64_t n = (int64_t) p.B * p.H * p.Nq * (p.D / 4);
+    const dim3 grid((unsigned) std::min<int64_t>((n + 255) / 256, 1 << 20));
+    if (plan.rows == 32) launch_kernel(cross_attn_join_kernel<32>, grid, dim3(256), 0, s, p);
+    else launch_kernel(cross_attn_join_kernel<64>, grid, dim3(256), 0, s, p);
     return hipGetLastError();
 }
 
 }  // namespace
 
-int cross_attn_splits(int D, int64_t Nq, int64_t Nkv, int64_t H, int64_t Hkv, int64_t B, size_t *bytes) {
-    *bytes = 0;
-    return 1;
+CrossAttnPlan plan_cross_attn(int D, int64_t Nq, int64_t Nkv, int64_t H, int64_t Hkv, int64_t B) {
+    CrossAttnPlan c;
+    const int64_t R = H / Hkv * Nq;
+    auto units = [&](int rows) { return (R + rows - 1) / rows * Hkv * B; };
+    c.rows = tuning().cross_cfg ? tuning().cross_cfg / 100 : R <= 32 ? 32 : units(256) >= 256 ? 256 : 128;
+    const int64_t most = std::min<int64_t>((512 + units(c.rows) - 1) / units(c.rows), Nkv / (c.rows == 32 ? 512 : 256));
+    c.splits = tuning().cross_cfg ? tuning().cross_cfg % 100 : (int) std::max<int64_t>(1, std::min<int64_t>(most, 64));
+    c.bytes = c.splits > 1 ? (size_t) c.splits * (size_t) (B * H * Nq) * (size_t) (D + 2) * 4 : 0;
+    c.bytes = (c.bytes + 255) / 256 * 256;
+    return c;
 }
 
-hipError_t launch_cross_attn(const CrossAttn &p, hipStream_t s) {
-    if (p.D <= 64) return p.kv_bf16 ? launch_dp<64, true>(p, s) : launch_dp<64, false>(p, s);
-    return p.kv_bf16 ? launch_dp<128, true>(p, s) : launch_dp<128, false>(p, s);
+hipError_t launch_cross_attn(const CrossAttn &p, const CrossAttnPlan &plan, hipStream_t s) {
+    if (p.D <= 64) return p.kv_bf16 ? launch_dp<64, true>(p, plan, s) : launch_dp<64, false>(p, plan, s);
+    return p.kv_bf16 ? launch_dp<128, true>(p, plan, s) : launch_dp<128, false>(p, plan, s);
 }
 
 }  // namespace tsk

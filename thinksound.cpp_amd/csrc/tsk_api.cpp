@@ -67,6 +67,7 @@ void read_tuning() {
     t.coop_cfg = env_int("TSK_COOP_CFG", 0);
     t.mx_cfg = env_int("TSK_MX_CFG", 0);
     t.i8_cfg = env_int("TSK_I8_CFG", 0);
+    t.cross_cfg = env_int("TSK_CROSS_CFG", 0);
     t.attn_cfg = env_int("TSK_ATTN_CFG", 0);
     t.dit_sched = env_int("TSK_DIT_SCHED", 1) != 0;
     t.ln_block = env_int("TSK_LN_BLOCK", 0) != 0;
@@ -1528,12 +1529,12 @@ extern "C" int tsk_cross_attention(const tsk_tensor *q, const tsk_tensor *k, con
     a.q_len = p->q_len ? (const int32_t *) p->q_len->data : nullptr;
     a.kv_valid = p->kv_valid; a.kv_valid_nb = p->kv_valid_nb;
     a.c = p->scale * 1.4426950408889634f;
-    size_t bytes = 0;
+    const CrossAttnPlan plan = plan_cross_attn(a.D, a.Nq, a.Nkv, a.H, a.Hkv, a.B);
     void *ws = nullptr;
-    a.splits = cross_attn_splits(a.D, a.Nq, a.Nkv, a.H, a.Hkv, a.B, &bytes);
-    if (bytes && (rc = workspace((hipStream_t) stream, bytes, &ws))) return rc;
+    if (plan.bytes && (rc = workspace((hipStream_t) stream, plan.bytes, &ws))) return rc;
+    a.splits = plan.splits;
     a.part = (float *) ws;
-    const hipError_t e = launch_cross_attn(a, (hipStream_t) stream);
+    const hipError_t e = launch_cross_attn(a, plan, (hipStream_t) stream);
     return e == hipSuccess ? TSK_OK : hip_fail(e, "cross_attention launch");
 }
 
@@ -2223,7 +2224,7 @@ extern "C" int tsk_workspace_size(int op, const tsk_tensor *const *srcs, int n_s
             return TSK_OK;
         case TSK_OP_CROSS_ATTENTION:
             if ((rc = need(3)) || (rc = validate_cross_shapes(&t[0], &t[1], &t[2], &d))) return rc;
-            cross_attn_splits((int) t[0].ne[0], t[0].ne[1], t[1].ne[1], t[0].ne[2], t[1].ne[2], t[0].ne[3], bytes);
+            *bytes = plan_cross_attn((int) t[0].ne[0], t[0].ne[1], t[1].ne[1], t[0].ne[2], t[1].ne[2], t[0].ne[3]).bytes;
             return TSK_OK;
         case TSK_OP_RMS_NORM_MUL: case TSK_OP_ROPE_EXT: case TSK_OP_NORM: case TSK_OP_IM2COL:
             return TSK_OK;   // no scratch

@@ -432,9 +432,13 @@ struct CrossAttn {
     int splits;                    // key ranges, each a workgroup; > 1: part holds their sums
     float *part;
 };
-// key ranges for the node, and the scratch bytes they take
-int cross_attn_splits(int D, int64_t Nq, int64_t Nkv, int64_t H, int64_t Hkv, int64_t B, size_t *bytes);
-hipError_t launch_cross_attn(const CrossAttn &p, hipStream_t s);
+// rows of a workgroup, key ranges of the node and the scratch bytes that these take
+struct CrossAttnPlan {
+    int rows, splits;
+    size_t bytes;
+};
+CrossAttnPlan plan_cross_attn(int D, int64_t Nq, int64_t Nkv, int64_t H, int64_t Hkv, int64_t B);
+hipError_t launch_cross_attn(const CrossAttn &p, const CrossAttnPlan &plan, hipStream_t s);
 
 // ---------------------------------------------------------------- block norm
 // tsk_block_norm's operands; a stride of 0 broadcasts, data null: absent

@@ -32,6 +32,7 @@ bool workspace_can(hipStream_t s, size_t bytes);
 //   TSK_COOP_CFG  cooperative BF16 tile of the C-ABI GEMMs (0 = rule)
 //   TSK_MX_CFG    MXFP4 products: the tile or rows shape launch_gemm_mx's table numbers (0 = rule)
 //   TSK_I8_CFG    8-bit products: the tile or rows shape launch_gemm_i8's table numbers (0 = rule)
+//   TSK_CROSS_CFG cross attention: 100 * rows of a workgroup (32, 128, 256) + key ranges (0 = rule)
 //   TSK_GEMM_CFG  DiT block GEMM tiles, one character per projection
 //   TSK_ATTN_CFG  DiT attention launch shape (10 * key ranges + query blocks)
 //   TSK_DIT_SCHED 0: the sampler computes its conditioning inside every step
@@ -55,6 +56,7 @@ struct Tuning {
     int coop_cfg = 0;
     int mx_cfg = 0;
     int i8_cfg = 0;
+    int cross_cfg = 0;
     int gemm_cfg[4] = {0, 0, 0, 0};
     int attn_cfg = 0;
     bool dit_sched = true;
