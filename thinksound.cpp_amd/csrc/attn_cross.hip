@@ -13,7 +13,11 @@
 // P is rounded to K's type (bf16: half of 2^-8 a weight), its row sum adds the same rounded
 // values, so that the weights add up to 1.
 #include <algorithm>
+#include <utility>
 
+#ifndef PFD
+#define PFD 4
+#endif
 #include "tsk_common.h"
 #include "tsk_internal.h"
 #include "tsk_runtime.h"
@@ -40,26 +44,49 @@ __device__ __forceinline__ s16x4 read_turned(const uint16_t *p) { return __built
 template <int DP> __device__ __forceinline__ int k_key(int row) { return DP == 128 ? row & 15 : row >> 1 & 7; }
 template <int DP> __device__ __forceinline__ int v_key(int row) { return (DP == 128 ? 4 : 2) * (row & 3); }
 
+// 16 bytes a lane from base + off (the lane's) + at into LDS at byte dst + 16 * lane; zeros past
+// `bytes`. In assembly, since the compiler waits for every load into LDS before a transposing
+// read, whose address it does not see; it has no result register, and the waits for it are
+// written out where its bytes are read.
+__device__ __forceinline__ void load_lds(const void *base, int bytes, int off, int at, uint32_t dst) {
+    auto scalar = [](int v) { return __builtin_amdgcn_readfirstlane(v); };   // (all the same for every lane)
+    const i32x4 rs = {scalar((int) (uint32_t) (uintptr_t) base), scalar((int) ((uint32_t) ((uintptr_t) base >> 32) & 0xffffu)), scalar(bytes), 0x00020000};
+    const int m = scalar((int) dst);
+    uint32_t kept;                                             // (m0 is the compiler's; s_nop: scalars that a vector unit has just written)
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 4\n\tbuffer_load_dwordx4 %2, %3, %4 offen lds\n\ts_mov_b32 m0, %0"
+                 : "=&s"(kept) : "s"(m), "v"(off), "s"(rs), "s"(scalar(at)) : "memory");
+}
+
+__device__ __forceinline__ uint32_t lds_byte(uint16_t *p) { return (uint32_t) (uintptr_t) (lds_void *) p; }
+
 template <bool BF16> struct Half;
 template <> struct Half<true> {
     typedef bf16x8 x8;
+    typedef bf16x2 x2;
+    typedef __bf16 one;
     static __device__ __forceinline__ f32x16 mfma(x8 a, x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
-    static __device__ __forceinline__ uint16_t bits(float f) { return f32_to_bf16_bits(f); }
-    static __device__ __forceinline__ float sum2(x8 p, int i, float s) {
-        const bf16x2 v = {p[i], p[i + 1]}, one = {(__bf16) 1.0f, (__bf16) 1.0f};
-        return __builtin_amdgcn_fdot2_f32_bf16(v, one, s, false);
+    static __device__ __forceinline__ float add2(uint32_t p, float s) {
+        const x2 ones = {(one) 1.0f, (one) 1.0f};
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(x2, p), ones, s, false);
     }
-    static __device__ __forceinline__ void set(x8 &p, int i, float f) { p[i] = (__bf16) f; }
+    static __device__ __forceinline__ uint32_t pack2(float f, float g) {
+        const x2 v = {(one) f, (one) g};
+        return __builtin_bit_cast(uint32_t, v);
+    }
 };
 template <> struct Half<false> {
     typedef f16x8 x8;
+    typedef f16x2 x2;
+    typedef _Float16 one;
     static __device__ __forceinline__ f32x16 mfma(x8 a, x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
-    static __device__ __forceinline__ uint16_t bits(float f) { return f32_to_f16_bits(f); }
-    static __device__ __forceinline__ float sum2(x8 p, int i, float s) {
-        const f16x2 v = {p[i], p[i + 1]}, one = {(_Float16) 1.0f, (_Float16) 1.0f};
-        return __builtin_amdgcn_fdot2(v, one, s, false);
+    static __device__ __forceinline__ float add2(uint32_t p, float s) {
+        const x2 ones = {(one) 1.0f, (one) 1.0f};
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(x2, p), ones, s, false);
     }
-    static __device__ __forceinline__ void set(x8 &p, int i, float f) { p[i] = (_Float16) f; }
+    static __device__ __forceinline__ uint32_t pack2(float f, float g) {
+        const x2 v = {(one) f, (one) g};
+        return __builtin_bit_cast(uint32_t, v);
+    }
 };
 
 // 8 values of a query row in K's type
@@ -78,9 +105,14 @@ __device__ __forceinline__ u32x4 load_q8(const char *row, int d, int type) {
         }
     }
     u32x4 o;
-    for (int i = 0; i < 4; ++i) o[i] = Half<BF16>::bits(f[2 * i]) | (uint32_t) Half<BF16>::bits(f[2 * i + 1]) << 16;
+    for (int i = 0; i < 4; ++i) o[i] = Half<BF16>::pack2(f[2 * i], f[2 * i + 1]);
     return o;
 }
+
+// f(0), ..., f(N - 1), the arguments constants
+template <class F, int... I>
+__device__ __forceinline__ void each(F f, std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>{}), ...); }
+#define EACH(q, from, to, ...) each([&](auto q##_) __attribute__((always_inline)) { constexpr int q = decltype(q##_)::value + (from); __VA_ARGS__ }, std::make_integer_sequence<int, ((to) > (from) ? (to) - (from) : 0)>{})
 
 // A launch's unit: a tile of rows of one key and value head, and (splits > 1) one of the
 // ranges that its sequence's tiles of states are dealt to. The ranges go by the sequence's own
@@ -93,15 +125,20 @@ struct Unit {
 template <int KT>
 __device__ __forceinline__ Unit unit_of(const CrossAttn &p, int qtiles, int rows) {
     Unit u;
-    int64_t i = blockIdx.x;
-    u.split = (int) (i % p.splits);
-    i /= p.splits;
-    const int qt = (int) (i % qtiles);
-    u.hk = (int) (i / qtiles % p.Hkv);
-    u.b = (int) (i / qtiles / p.Hkv);
-    u.nkv = p.kv_len ? max(0, min(p.kv_len[u.b], p.Nkv)) : p.Nkv;
-    u.nq = p.q_len ? max(0, min(p.q_len[u.b], p.Nq)) : p.Nq;
-    const int G = p.H / p.Hkv, tiles = (u.nkv + KT - 1) / KT, per = (tiles + p.splits - 1) / p.splits;
+    // workgroup L runs on XCD L % 8: each XCD takes a run of the units, whose neighbours read the
+    // same states (the grid is a multiple of 8; the units past the last are none)
+    // (fewer than 2^23; the quotients come from vector units, and are the same for every lane)
+    auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+    const int i = (int) ((blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3));
+    const int unit = uniform(i / p.splits), head = uniform(unit / qtiles), qt = unit - head * qtiles;
+    u.split = i - unit * p.splits;
+    u.b = uniform(head / p.Hkv);
+    u.hk = head - u.b * p.Hkv;
+    u.none = u.b >= p.B;
+    if (u.none) return u;
+    u.nkv = uniform(p.kv_len ? max(0, min(p.kv_len[u.b], p.Nkv)) : p.Nkv);
+    u.nq = uniform(p.q_len ? max(0, min(p.q_len[u.b], p.Nq)) : p.Nq);
+    const int G = p.H / p.Hkv, tiles = (u.nkv + KT - 1) / KT, per = uniform((tiles + p.splits - 1) / p.splits);
     u.R = (int64_t) G * p.Nq;
     u.r0 = (int64_t) qt * rows;
     u.tile0 = u.split * per;
@@ -179,21 +216,19 @@ __global__ __launch_bounds__(256) void cross_attn_few_kernel(const CrossAttn p, 
     const uint8_t *flags = p.kv_valid ? p.kv_valid + u.b * p.kv_valid_nb : nullptr;
     const int lr = lane / CH;
     uint16_t *ring = lds + wave * NB * 2 * TILE;
+    const uint32_t ring0 = lds_byte(ring);
     auto issue = [&](int tile, int buf) {
-        uint16_t *dst = ring + buf * 2 * TILE;
+        const uint32_t dst = ring0 + buf * (4 * TILE);
         const int left = min(KT, u.nkv - tile * KT);
         const int64_t k0 = (int64_t) tile * KT;
-        const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc((void *) (kp + k0 * p.k_nb1), (short) 0,
-                                                                            (int) ((left - 1) * p.k_nb1) + 2 * p.D, 0x00020000);
-        const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc((void *) (vp + k0 * p.v_nb1), (short) 0,
-                                                                            (int) ((left - 1) * p.v_nb1) + 2 * p.D, 0x00020000);
+        const char *ks = kp + k0 * p.k_nb1, *vs = vp + k0 * p.v_nb1;
+        // rows past the last state read as zeros
+        const int k_bytes = (int) ((left - 1) * p.k_nb1) + 2 * p.D, v_bytes = (int) ((left - 1) * p.v_nb1) + 2 * p.D;
 #pragma unroll
         for (int j = 0; j < NL; ++j) {
             const int kc = (lane % CH) ^ k_key<DP>(j * RL + lr), vc = (lane % CH) ^ v_key<DP>(lr);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (lds_void *) (dst + j * 512), 16, kc * 8 < p.D ? (int) (lr * p.k_nb1) + kc * 16 : FAR,
-                                                     (int) (j * RL * p.k_nb1), 0, 0);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (lds_void *) (dst + TILE + j * 512), 16, vc * 8 < p.D ? (int) (lr * p.v_nb1) + vc * 16 : FAR,
-                                                     (int) (j * RL * p.v_nb1), 0, 0);
+            load_lds(ks, k_bytes, kc * 8 < p.D ? (int) (lr * p.k_nb1) + kc * 16 : FAR, (int) (j * RL * p.k_nb1), dst + j * 1024);
+            load_lds(vs, v_bytes, vc * 8 < p.D ? (int) (lr * p.v_nb1) + vc * 16 : FAR, (int) (j * RL * p.v_nb1), dst + 2 * TILE + j * 1024);
         }
     };
     const int first = u.tile0 + wave;
@@ -249,13 +284,12 @@ __global__ __launch_bounds__(256) void cross_attn_few_kernel(const CrossAttn p, 
                 for (int e = 0; e < 16; ++e) o[db][e] *= alpha;
         }
         m_run = m_new;
-        x8 pf[2];
+        u32x4 pf[2];
 #pragma unroll
-        for (int kg = 0; kg < 2; ++kg) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) T::set(pf[kg], e, __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * kg + e], c, -sub)));
-#pragma unroll
-            for (int e = 0; e < 8; e += 2) l_run = T::sum2(pf[kg], e, l_run);
+        for (int e = 0; e < 16; e += 2) {
+            const uint32_t two = T::pack2(__builtin_amdgcn_exp2f(__builtin_fmaf(s[e], c, -sub)), __builtin_amdgcn_exp2f(__builtin_fmaf(s[e + 1], c, -sub)));
+            l_run = T::add2(two, l_run);
+            pf[e / 8][e % 8 / 2] = two;
         }
 #pragma unroll
         for (int kg = 0; kg < 2; ++kg)
@@ -265,7 +299,7 @@ __global__ __launch_bounds__(256) void cross_attn_few_kernel(const CrossAttn p, 
                 const uint16_t *at = vb + (16 * kg + vrow) * DP + ((ch ^ v_key<DP>(l16 >> 2)) << 3) + 4 * (l16 & 1);
                 const s16x4 a = read_turned(at), a2 = read_turned(at + 8 * DP);
                 const s16x8 a8 = {a[0], a[1], a[2], a[3], a2[0], a2[1], a2[2], a2[3]};
-                o[db] = T::mfma(__builtin_bit_cast(x8, a8), pf[kg], o[db]);
+                o[db] = T::mfma(__builtin_bit_cast(x8, a8), __builtin_bit_cast(x8, pf[kg]), o[db]);
             }
         // (the next turn's loads land in the buffer read here: every read is done)
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -343,7 +377,7 @@ __global__ __launch_bounds__(256) void cross_attn_join_kernel(const CrossAttn p)
 }
 
 // ---------------------------------------------------------------- many rows
-// A workgroup takes 128 QB rows, 32 QB a wave, and tiles of 64 states through a ring of three
+// A workgroup takes 128 QB rows, 32 QB a wave, and tiles of 64 states through a ring of four
 // in LDS. Half a tile (32 states) at a time, a wave multiplies the next half's K with Q and
 // the last half's V with P while it turns this half's logits into weights: three steps of
 // three halves without a dependence, so that the matrix unit and the rest of the SIMD work at
@@ -351,16 +385,16 @@ __global__ __launch_bounds__(256) void cross_attn_join_kernel(const CrossAttn p)
 //
 // The running maximum moves only when the logits pass it by more than 2^8, and then to a whole
 // number (log2 domain): sums and weights already rounded are scaled by a power of two, exactly.
-template <int DP, bool BF16, int QB>
-__global__ __launch_bounds__(256) void cross_attn_kernel(const CrossAttn p, int qtiles) {
+template <int DP, bool BF16, int QB, int NW>
+__global__ __launch_bounds__(NW * 64) void cross_attn_kernel(const CrossAttn p, int qtiles) {
     typedef Half<BF16> T;
     typedef typename T::x8 x8;
-    constexpr int KT = 64, CH = DP / 8, RL = 64 / CH, NL = KT / RL / 4, TILE = KT * DP;      // 16-byte pieces a row, rows a load, loads a wave
+    constexpr int KT = 64, CH = DP / 8, RL = 64 / CH, NL = KT / RL / NW, TILE = KT * DP;     // 16-byte pieces a row, rows a load, loads a wave
     constexpr int FAR = (int) 0x80000000u;
-    extern __shared__ __attribute__((aligned(1024))) uint16_t lds[];           // [3][K tile, V tile]
+    extern __shared__ __attribute__((aligned(1024))) uint16_t lds[];           // [4][K tile, V tile]
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l32 = lane & 31, hi = lane >> 5;
-    const Unit u = unit_of<KT>(p, qtiles, 128 * QB);
+    const Unit u = unit_of<KT>(p, qtiles, 32 * QB * NW);
     if (u.none) return;
     int h[QB], iq[QB];
     x8 q[QB][DP / 16];
@@ -374,22 +408,24 @@ __global__ __launch_bounds__(256) void cross_attn_kernel(const CrossAttn p, int 
     // (a wave's loads are 4 * RL rows apart, which the keys do not see)
     const int lr = lane / CH, kc = (lane % CH) ^ k_key<DP>(wave * RL + lr), vc = (lane % CH) ^ v_key<DP>(lr);
     const int koff = kc * 8 < p.D ? (int) (lr * p.k_nb1) + kc * 16 : FAR, voff = vc * 8 < p.D ? (int) (lr * p.v_nb1) + vc * 16 : FAR;
-    // tile t into slot s; tiles past the last: zeros, so that every wait counts the same
-    auto issue = [&](int t, int s) {
-        uint16_t *dst = lds + s * 2 * TILE;
+    // tile t into slot s, a load at a time; tiles past the last: zeros, so that every wait counts the same
+    struct Source {
+        const char *k, *v;
+        int k_bytes, v_bytes;                                  // up to the last state that counts: rows past it read as zeros
+    };
+    auto source_of = [&](int t) {
         const int left = t < u.tile1 ? min(KT, u.nkv - t * KT) : 0;
         const int64_t k0 = t < u.tile1 ? (int64_t) t * KT : 0;
-        // rows past the last state read as zeros
-        const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc((void *) (kp + k0 * p.k_nb1), (short) 0,
-                                                                            left ? (int) ((left - 1) * p.k_nb1) + 2 * p.D : 0, 0x00020000);
-        const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc((void *) (vp + k0 * p.v_nb1), (short) 0,
-                                                                            left ? (int) ((left - 1) * p.v_nb1) + 2 * p.D : 0, 0x00020000);
-#pragma unroll
-        for (int i = 0; i < NL; ++i) {
-            const int j = wave + 4 * i;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (lds_void *) (dst + j * 512), 16, koff, (int) (j * RL * p.k_nb1), 0, 0);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (lds_void *) (dst + TILE + j * 512), 16, voff, (int) (j * RL * p.v_nb1), 0, 0);
-        }
+        return Source{kp + k0 * p.k_nb1, vp + k0 * p.v_nb1, left ? (int) ((left - 1) * p.k_nb1) + 2 * p.D : 0,
+                      left ? (int) ((left - 1) * p.v_nb1) + 2 * p.D : 0};
+    };
+    const uint32_t lds0 = lds_byte(lds);
+    constexpr int LOADS = 2 * NL;                              // of a wave and tile: K's and V's in turn
+    auto issue_one = [&](const Source &src, int s, int i) __attribute__((always_inline)) {
+        const int j = wave + NW * (i / 2);
+        const uint32_t dst = lds0 + s * (4 * TILE) + i % 2 * (2 * TILE) + j * 1024;
+        if (i % 2 == 0) load_lds(src.k, src.k_bytes, koff, (int) (j * RL * p.k_nb1), dst);
+        else load_lds(src.v, src.v_bytes, voff, (int) (j * RL * p.v_nb1), dst);
     };
     // bit s: state s of tile t counts
     auto counted = [&](int t) -> uint64_t {
@@ -402,10 +438,11 @@ __global__ __launch_bounds__(256) void cross_attn_kernel(const CrossAttn p, int 
     // a state that does not count may hold anything, and 0 times it may not be 0: its V becomes zeros
     auto clear = [&](uint64_t count, int s) {
         if (!flags || count == ~(uint64_t) 0) return;
-        const int r = tid >> 2;
+        constexpr int PER = NW;                                  // threads a row
+        const int r = tid / PER;
         if (!(count >> r & 1))
 #pragma unroll
-            for (int i = 0; i < DP / 32; ++i) *(u32x4 *) (lds + s * 2 * TILE + TILE + r * DP + (tid & 3) * (DP / 4) + i * 8) = u32x4{0, 0, 0, 0};
+            for (int i = 0; i < CH / PER; ++i) *(u32x4 *) (lds + s * 2 * TILE + TILE + r * DP + (tid % PER * (CH / PER) + i) * 8) = u32x4{0, 0, 0, 0};
         __syncthreads();
     };
     f32x16 o[QB][DP / 32];
@@ -426,61 +463,118 @@ __global__ __launch_bounds__(256) void cross_attn_kernel(const CrossAttn p, int 
         float top[QB];
     };
     struct Weights {
-        x8 w[QB][2];
+        u32x4 w[QB][2];                                          // pairs
     };
-    auto multiply_k = [&](int slot, int half, Logits &n) __attribute__((always_inline)) {
-        const uint16_t *kb = lds + slot * 2 * TILE + 32 * half * DP;
-#pragma unroll
-        for (int i = 0; i < QB; ++i)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) n.s[i][e] = 0.0f;
-#pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks) {
-            const x8 a = *(const x8 *) (kb + l32 * DP + (((2 * ks + hi) ^ k_key<DP>(l32)) << 3));
-#pragma unroll
-            for (int i = 0; i < QB; ++i) n.s[i] = T::mfma(a, q[i][ks], n.s[i]);
+    // A step's operands in LDS, K's of one half of a tile and V's of another, in the order of
+    // their products: two of K, one of V, ..., what is left of V; each read AHEAD products early
+    constexpr int NK = DP / 16, NF = 2 * NK, AHEAD = PFD, SLOTS = AHEAD + 1;
+    struct Pieces {
+        x8 f[SLOTS];
+    };
+    auto of_k = [](int f) { return f < NK / 2 * 3 && f % 3 != 2; };
+    auto index = [](int f) { return f >= NK / 2 * 3 ? f - NK : f % 3 == 2 ? f / 3 : f / 3 * 2 + f % 3; };
+    auto read_piece = [&](const uint16_t *kb, const uint16_t *vb, int f, Pieces &x) __attribute__((always_inline)) {
+        const int j = index(f);
+        if (of_k(f)) {
+            x.f[f % SLOTS] = *(const x8 *) (kb + l32 * DP + (((2 * j + hi) ^ k_key<DP>(l32)) << 3));
+        } else {
+            const int kg = j / (DP / 32), db = j % (DP / 32), ch = 4 * db + 2 * grp + ((l16 & 3) >> 1);
+            const uint16_t *at = vb + (16 * kg + vrow) * DP + ((ch ^ v_key<DP>(l16 >> 2)) << 3) + 4 * (l16 & 1);
+            const s16x4 a = read_turned(at), a2 = read_turned(at + 8 * DP);
+            const s16x8 a8 = {a[0], a[1], a[2], a[3], a2[0], a2[1], a2[2], a2[3]};
+            x.f[f % SLOTS] = __builtin_bit_cast(x8, a8);
         }
     };
+    auto k_at = [&](int slot, int half) { return lds + slot * 2 * TILE + 32 * half * DP; };
+    auto v_at = [&](int slot, int half) { return lds + slot * 2 * TILE + TILE + 32 * half * DP; };
     auto largest = [&](Logits &n) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < QB; ++i) {
             float t = n.s[i][0];
 #pragma unroll
             for (int e = 1; e < 16; ++e) t = fmaxf(t, n.s[i][e]);
+            asm volatile("" : "+v"(t));
             n.top[i] = t;
         }
     };
-    auto multiply_v = [&](int slot, int half, const Weights &w) __attribute__((always_inline)) {
-        const uint16_t *vb = lds + slot * 2 * TILE + TILE + 32 * half * DP;
-#pragma unroll
-        for (int kg = 0; kg < 2; ++kg)
-#pragma unroll
-            for (int db = 0; db < DP / 32; ++db) {
-                const int ch = 4 * db + 2 * grp + ((l16 & 3) >> 1);
-                const uint16_t *at = vb + (16 * kg + vrow) * DP + ((ch ^ v_key<DP>(l16 >> 2)) << 3) + 4 * (l16 & 1);
-                const s16x4 a = read_turned(at), a2 = read_turned(at + 8 * DP);
-                const s16x8 a8 = {a[0], a[1], a[2], a[3], a2[0], a2[1], a2[2], a2[3]};
-#pragma unroll
-                for (int i = 0; i < QB; ++i) o[i][db] = T::mfma(__builtin_bit_cast(x8, a8), w.w[i][kg], o[i][db]);
-            }
+    // A logit becomes a weight in three turns, each some products after the one before (a wave
+    // waits for its own results): the exponent, its power, and two of them rounded and added
+    auto turn1 = [&](Logits &n, int i, int e) __attribute__((always_inline)) {
+        float v = __builtin_fmaf(n.s[i][e], c, -sub[i]);
+        asm volatile("" : "+v"(v));                            // (worked out here and not where it is used)
+        n.s[i][e] = v;
     };
-    // logits to weights
-    auto weigh = [&](const Logits &n, Weights &w) __attribute__((always_inline)) {
+    auto turn2 = [&](Logits &n, int i, int e) __attribute__((always_inline)) {
+        float v = __builtin_amdgcn_exp2f(n.s[i][e]);
+        asm volatile("" : "+v"(v));
+        n.s[i][e] = v;
+    };
+    auto turn3 = [&](Logits &n, Weights &w, int i, int e) __attribute__((always_inline)) {
+        uint32_t two = T::pack2(n.s[i][e], n.s[i][e + 1]);
+        l[i] = T::add2(two, l[i]);
+        asm volatile("" : "+v"(two), "+v"(l[i]));
+        w.w[i][e / 8][e % 8 / 2] = two;
+    };
+    constexpr int PER = 16 / NF;                               // logits between two products
+    auto first_turns = [&](Logits &n) __attribute__((always_inline)) {
+        EACH(i, 0, QB, EACH(e, 0, 2 * PER, turn1(n, i, e);); EACH(e, 0, PER, turn2(n, i, e);););
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // the products of next (K . Q of a half) and of before (V of another), `now` weighed between them
+    auto step = [&](const uint16_t *kb, const uint16_t *vb, Pieces &x, Logits &now, Weights &w, Logits &next, const Weights &before,
+                    const Source &src, int to, auto part) __attribute__((always_inline)) {
+        constexpr int L0 = decltype(part)::value * LOADS / 2, L1 = LOADS / 2;  // half of the loads of a later tile
+        EACH(f, 0, NF,
+            constexpr int J = f >= NK / 2 * 3 ? f - NK : f % 3 == 2 ? f / 3 : f / 3 * 2 + f % 3;
+            constexpr bool K = f < NK / 2 * 3 && f % 3 != 2;
+            EACH(i, 0, QB,
+                if constexpr (K && J == 0) next.s[i] = f32x16{};
+                if constexpr (K) next.s[i] = T::mfma(x.f[f % SLOTS], q[i][J], next.s[i]);
+                else o[i][J % (DP / 32)] = T::mfma(x.f[f % SLOTS], __builtin_bit_cast(x8, before.w[i][J / (DP / 32)]), o[i][J % (DP / 32)]);
+                if constexpr (i == 0 && f + AHEAD < NF) read_piece(kb, vb, f + AHEAD, x);
+                if constexpr (i == QB - 1) {
+                    EACH(u, f * L1 / NF, (f + 1) * L1 / NF, issue_one(src, to, L0 + u););
+                }
+                EACH(u, 0, PER,
+                    if constexpr ((f + 2) * PER + u < 16) turn1(now, i, (f + 2) * PER + u);
+                    if constexpr ((f + 1) * PER + u < 16) turn2(now, i, (f + 1) * PER + u);
+                    if constexpr ((f * PER + u) % 2) turn3(now, w, i, f * PER + u - 1););
+                if constexpr (f == NF - 1 && i == QB - 1) largest(next);
+                __builtin_amdgcn_sched_barrier(0);););
+    };
+    auto first_pieces = [&](const uint16_t *kb, const uint16_t *vb, Pieces &x) __attribute__((always_inline)) {
+        EACH(f, 0, AHEAD, read_piece(kb, vb, f, x););
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto multiply_k = [&](const uint16_t *kb, Logits &n) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < QB; ++i)
 #pragma unroll
-            for (int kg = 0; kg < 2; ++kg) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) T::set(w.w[i][kg], e, __builtin_amdgcn_exp2f(__builtin_fmaf(n.s[i][8 * kg + e], c, -sub[i])));
-#pragma unroll
-                for (int e = 0; e < 8; e += 2) l[i] = T::sum2(w.w[i][kg], e, l[i]);
-            }
+            for (int e = 0; e < 16; ++e) n.s[i][e] = 0.0f;
+        EACH(f, 0, NF, if constexpr (f < NK / 2 * 3 && f % 3 != 2) {
+            Pieces x;
+            read_piece(kb, kb, f, x);
+            for (int i = 0; i < QB; ++i) n.s[i] = T::mfma(x.f[f % SLOTS], q[i][f / 3 * 2 + f % 3], n.s[i]);
+        });
+        largest(n);
+    };
+    auto multiply_v = [&](const uint16_t *vb, const Weights &w) __attribute__((always_inline)) {
+        EACH(f, 0, NF, if constexpr (!(f < NK / 2 * 3 && f % 3 != 2)) {
+            constexpr int J = f >= NK / 2 * 3 ? f - NK : f / 3;
+            Pieces x;
+            read_piece(vb, vb, f, x);
+            for (int i = 0; i < QB; ++i) o[i][J % (DP / 32)] = T::mfma(x.f[f % SLOTS], __builtin_bit_cast(x8, w.w[i][J / (DP / 32)]), o[i][J % (DP / 32)]);
+        });
+    };
+    auto weigh = [&](Logits &n, Weights &w) __attribute__((always_inline)) {
+        EACH(i, 0, QB, EACH(e, 0, 16, turn1(n, i, e); turn2(n, i, e);); EACH(e, 0, 8, turn3(n, w, i, 2 * e);););
     };
     // what the next weights go by: states that do not count leave, the maximum moves if it has to
     auto settle = [&](Logits &n, uint64_t count, int half, Weights &before) __attribute__((always_inline)) {
         const uint32_t part = (uint32_t) (count >> 32 * half);
         if (part != ~0u) {
-            const uint32_t mine = part >> 4 * hi;
+            uint32_t mine = part >> 4 * hi;
+            asm volatile("" : "+v"(mine));                     // (nothing of this is worked out ahead)
 #pragma unroll
             for (int i = 0; i < QB; ++i)
 #pragma unroll
@@ -498,6 +592,7 @@ __global__ __launch_bounds__(256) void cross_attn_kernel(const CrossAttn p, int 
         if (!__any(move)) return;
 #pragma unroll
         for (int i = 0; i < QB; ++i) {
+            asm volatile("" : "+v"(top[i]));
             const float to = top[i] > m[i] + 8.0f ? __builtin_ceilf(top[i]) : m[i];
             const float s = to == -__builtin_inff() ? 0.0f : to, f = __builtin_amdgcn_exp2f(m[i] - s);
             m[i] = to;
@@ -508,63 +603,61 @@ __global__ __launch_bounds__(256) void cross_attn_kernel(const CrossAttn p, int 
 #pragma unroll
                 for (int e = 0; e < 16; ++e) o[i][db][e] *= f;
 #pragma unroll
-            for (int kg = 0; kg < 2; ++kg)
+            for (int kg = 0; kg < 2; ++kg) {
+                const x8 w = __builtin_bit_cast(x8, before.w[i][kg]);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) T::set(before.w[i][kg], e, (float) before.w[i][kg][e] * f);
+                for (int e = 0; e < 4; ++e) before.w[i][kg][e] = T::pack2((float) w[2 * e] * f, (float) w[2 * e + 1] * f);
+            }
         }
     };
-    constexpr int LOADS = 2 * NL;
     if (u.tile0 < u.tile1) {
-        issue(u.tile0, 0);
-        issue(u.tile0 + 1, 1);
-        issue(u.tile0 + 2, 2);
+        for (int t = 0; t < 3; ++t) {
+            const Source src = source_of(u.tile0 + t);
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) issue_one(src, t, i);
+        }
         Logits na, nb;
         Weights wa, wb;
 #pragma unroll
         for (int i = 0; i < QB; ++i)
 #pragma unroll
-            for (int kg = 0; kg < 2; ++kg)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) T::set(wa.w[i][kg], e, 0.0f), T::set(wb.w[i][kg], e, 0.0f);
+            for (int kg = 0; kg < 2; ++kg) wa.w[i][kg] = wb.w[i][kg] = u32x4{0, 0, 0, 0};
         uint64_t count = counted(u.tile0), next = counted(u.tile0 + 1);
         asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");           // (tiles 0 and 1)
         __syncthreads();
         clear(count, 0);
         clear(next, 1);
-        multiply_k(0, 0, na);
-        largest(na);
+        multiply_k(k_at(0, 0), na);
         settle(na, count, 0, wb);
-        multiply_k(0, 1, nb);
+        multiply_k(k_at(0, 1), nb);
         weigh(na, wa);
-        largest(nb);
         int slot = 0;
+        Pieces x;
         for (int t = u.tile0; t + 1 < u.tile1; ++t) {
-            const int s1 = slot == 2 ? 0 : slot + 1, s2 = s1 == 2 ? 0 : s1 + 1;
-            // second half of tile t
+            const int s1 = (slot + 1) & 3, s2 = (slot + 2) & 3, s3 = (slot + 3) & 3;
+            // second half of tile t; tile t + 3 goes where tile t - 1 was, which every wave is done with
+            const Source src = source_of(t + 3);
+            first_pieces(k_at(s1, 0), v_at(slot, 0), x);
             settle(nb, count, 1, wa);
-            multiply_k(s1, 0, na);
-            weigh(nb, wb);
-            multiply_v(slot, 0, wa);
-            largest(na);
+            first_turns(nb);
+            step(k_at(s1, 0), v_at(slot, 0), x, nb, wb, na, wa, src, s3, std::integral_constant<int, 0>{});
             // first half of tile t + 1
+            first_pieces(k_at(s1, 1), v_at(slot, 1), x);
             settle(na, next, 0, wb);
-            multiply_k(s1, 1, nb);
-            weigh(na, wa);
-            multiply_v(slot, 1, wb);
-            largest(nb);
+            first_turns(na);
+            step(k_at(s1, 1), v_at(slot, 1), x, na, wa, nb, wb, src, s3, std::integral_constant<int, 1>{});
             count = next;
             next = counted(t + 2);
-            // tile t + 2 has landed, every wave is done with tile t: its slot takes tile t + 3
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            // tile t + 2 has landed
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS) : "memory");
             __syncthreads();
             clear(next, s2);
-            issue(t + 3, slot);
             slot = s1;
         }
         settle(nb, count, 1, wa);
         weigh(nb, wb);
-        multiply_v(slot, 0, wa);
-        multiply_v(slot, 1, wb);
+        multiply_v(v_at(slot, 0), wa);
+        multiply_v(v_at(slot, 1), wb);
     }
 #pragma unroll
     for (int i = 0; i < QB; ++i) {
@@ -592,20 +685,21 @@ __global__ __launch_bounds__(256) void cross_attn_kernel(const CrossAttn p, int 
 }
 
 template <class F>
-hipError_t launch_units(F kern, const CrossAttn &p, int rows, size_t lds, hipStream_t s) {
+hipError_t launch_units(F kern, const CrossAttn &p, int rows, int threads, size_t lds, hipStream_t s) {
     const int64_t R = (int64_t) (p.H / p.Hkv) * p.Nq, qtiles = (R + rows - 1) / rows, units = qtiles * p.Hkv * p.B * p.splits;
-    if (units >= (int64_t) 1 << 24) return hipErrorInvalidValue;
+    if (units >= (int64_t) 1 << 23) return hipErrorInvalidValue;
     lds_opt_in((const void *) kern, lds);
-    launch_kernel(kern, dim3((unsigned) units), dim3(256), lds, s, p, (int) qtiles);
+    launch_kernel(kern, dim3((unsigned) ((units + 7) / 8 * 8)), dim3(threads), lds, s, p, (int) qtiles);
     return hipGetLastError();
 }
 
 template <int DP, bool BF16>
 hipError_t launch_dp(const CrossAttn &p, const CrossAttnPlan &plan, hipStream_t s) {
     hipError_t e;
-    if (plan.rows == 32) e = launch_units(cross_attn_few_kernel<DP, BF16>, p, 32, 4 * 2 * 2 * 32 * DP * 2, s);
-    else if (plan.rows == 128) e = launch_units(cross_attn_kernel<DP, BF16, 1>, p, 128, 3 * 2 * 64 * DP * 2, s);
-    else e = launch_units(cross_attn_kernel<DP, BF16, 2>, p, 256, 3 * 2 * 64 * DP * 2, s);
+    if (plan.rows == 32) e = launch_units(cross_attn_few_kernel<DP, BF16>, p, 32, 256, 4 * 2 * 2 * 32 * DP * 2, s);
+    else if (plan.rows == 128) e = launch_units(cross_attn_kernel<DP, BF16, 1, 4>, p, 128, 256, 4 * 2 * 64 * DP * 2, s);
+    else if (plan.rows == 257) e = launch_units(cross_attn_kernel<DP, BF16, 1, 8>, p, 256, 512, 4 * 2 * 64 * DP * 2, s);
+    else e = launch_units(cross_attn_kernel<DP, BF16, 2, 4>, p, 256, 256, 4 * 2 * 64 * DP * 2, s);
     if (e != hipSuccess || p.splits == 1) return e;
     const int64_t n = (int64_t) p.B * p.H * p.Nq * (p.D / 4);
     const dim3 grid((unsigned) std::min<int64_t>((n + 255) / 256, 1 << 20));
@@ -621,7 +715,7 @@ CrossAttnPlan plan_cross_attn(int D, int64_t Nq, int64_t Nkv, int64_t H, int64_t
     const int64_t R = H / Hkv * Nq;
     auto units = [&](int rows) { return (R + rows - 1) / rows * Hkv * B; };
     c.rows = tuning().cross_cfg ? tuning().cross_cfg / 100 : R <= 32 ? 32 : units(256) >= 256 ? 256 : 128;
-    const int64_t most = std::min<int64_t>((512 + units(c.rows) - 1) / units(c.rows), Nkv / (c.rows == 32 ? 512 : 256));
+    const int64_t most = std::min<int64_t>(256 / units(c.rows), Nkv / (c.rows == 32 ? 512 : 256));
     c.splits = tuning().cross_cfg ? tuning().cross_cfg % 100 : (int) std::max<int64_t>(1, std::min<int64_t>(most, 64));
     c.bytes = c.splits > 1 ? (size_t) c.splits * (size_t) (B * H * Nq) * (size_t) (D + 2) * 4 : 0;
     c.bytes = (c.bytes + 255) / 256 * 256;
