@@ -446,11 +446,11 @@ __global__ __launch_bounds__(NW * 64) void cross_attn_kernel(const CrossAttn p, 
         __syncthreads();
     };
     f32x16 o[QB][DP / 32];
-    float m[QB], sub[QB], l[QB];
+    float m[QB], l[QB];
 #pragma unroll
     for (int i = 0; i < QB; ++i) {
-        m[i] = -__builtin_inff();
-        sub[i] = l[i] = 0.0f;
+        m[i] = -1e30f;                                         // (any logit is far above it)
+        l[i] = 0.0f;
 #pragma unroll
         for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
@@ -460,10 +460,10 @@ __global__ __launch_bounds__(NW * 64) void cross_attn_kernel(const CrossAttn p, 
     const int l16 = lane & 15, grp = (lane >> 4) & 1, vrow = 4 * hi + (l16 >> 2);
     struct Logits {
         f32x16 s[QB];
-        float top[QB];
     };
     struct Weights {
         u32x4 w[QB][2];                                          // pairs
+        float sum[QB];
     };
     // A step's operands in LDS, K's of one half of a tile and V's of another, in the order of
     // their products: two of K, one of V, ..., what is left of V; each read AHEAD products early
@@ -487,41 +487,35 @@ __global__ __launch_bounds__(NW * 64) void cross_attn_kernel(const CrossAttn p, 
     };
     auto k_at = [&](int slot, int half) { return lds + slot * 2 * TILE + 32 * half * DP; };
     auto v_at = [&](int slot, int half) { return lds + slot * 2 * TILE + TILE + 32 * half * DP; };
-    auto largest = [&](Logits &n) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < QB; ++i) {
-            float t = n.s[i][0];
-#pragma unroll
-            for (int e = 1; e < 16; ++e) t = fmaxf(t, n.s[i][e]);
-            asm volatile("" : "+v"(t));
-            n.top[i] = t;
-        }
-    };
     // A logit becomes a weight in three turns, each some products after the one before (a wave
     // waits for its own results): the exponent, its power, and two of them rounded and added
-    auto turn1 = [&](Logits &n, int i, int e) __attribute__((always_inline)) {
-        float v = __builtin_fmaf(n.s[i][e], c, -sub[i]);
+    struct Turns {
+        float v[QB][16];
+    };
+    auto turn1 = [&](const Logits &n, Turns &r, int i, int e) __attribute__((always_inline)) {
+        float v = __builtin_fmaf(n.s[i][e], c, -m[i]);
         asm volatile("" : "+v"(v));                            // (worked out here and not where it is used)
-        n.s[i][e] = v;
+        r.v[i][e] = v;
     };
-    auto turn2 = [&](Logits &n, int i, int e) __attribute__((always_inline)) {
-        float v = __builtin_amdgcn_exp2f(n.s[i][e]);
+    auto turn2 = [&](Turns &r, int i, int e) __attribute__((always_inline)) {
+        float v = __builtin_amdgcn_exp2f(r.v[i][e]);
         asm volatile("" : "+v"(v));
-        n.s[i][e] = v;
+        r.v[i][e] = v;
     };
-    auto turn3 = [&](Logits &n, Weights &w, int i, int e) __attribute__((always_inline)) {
-        uint32_t two = T::pack2(n.s[i][e], n.s[i][e + 1]);
-        l[i] = T::add2(two, l[i]);
-        asm volatile("" : "+v"(two), "+v"(l[i]));
+    auto turn3 = [&](const Turns &r, Weights &w, int i, int e) __attribute__((always_inline)) {
+        uint32_t two = T::pack2(r.v[i][e], r.v[i][e + 1]);
+        float sum = T::add2(two, e == 0 ? 0.0f : w.sum[i]);
+        asm volatile("" : "+v"(two), "+v"(sum));
+        w.sum[i] = sum;
         w.w[i][e / 8][e % 8 / 2] = two;
     };
     constexpr int PER = 16 / NF;                               // logits between two products
-    auto first_turns = [&](Logits &n) __attribute__((always_inline)) {
-        EACH(i, 0, QB, EACH(e, 0, 2 * PER, turn1(n, i, e);); EACH(e, 0, PER, turn2(n, i, e);););
+    auto first_turns = [&](const Logits &n, Turns &r) __attribute__((always_inline)) {
+        EACH(i, 0, QB, EACH(e, 0, 2 * PER, turn1(n, r, i, e);); EACH(e, 0, PER, turn2(r, i, e);););
         __builtin_amdgcn_sched_barrier(0);
     };
     // the products of next (K . Q of a half) and of before (V of another), `now` weighed between them
-    auto step = [&](const uint16_t *kb, const uint16_t *vb, Pieces &x, Logits &now, Weights &w, Logits &next, const Weights &before,
+    auto step = [&](const uint16_t *kb, const uint16_t *vb, Pieces &x, const Logits &now, Turns &r, Weights &w, Logits &next, const Weights &before,
                     const Source &src, int to, auto part) __attribute__((always_inline)) {
         constexpr int L0 = decltype(part)::value * LOADS / 2, L1 = LOADS / 2;  // half of the loads of a later tile
         EACH(f, 0, NF,
@@ -536,10 +530,9 @@ __global__ __launch_bounds__(NW * 64) void cross_attn_kernel(const CrossAttn p, 
                     EACH(u, f * L1 / NF, (f + 1) * L1 / NF, issue_one(src, to, L0 + u););
                 }
                 EACH(u, 0, PER,
-                    if constexpr ((f + 2) * PER + u < 16) turn1(now, i, (f + 2) * PER + u);
-                    if constexpr ((f + 1) * PER + u < 16) turn2(now, i, (f + 1) * PER + u);
-                    if constexpr ((f * PER + u) % 2) turn3(now, w, i, f * PER + u - 1););
-                if constexpr (f == NF - 1 && i == QB - 1) largest(next);
+                    if constexpr ((f + 2) * PER + u < 16) turn1(now, r, i, (f + 2) * PER + u);
+                    if constexpr ((f + 1) * PER + u < 16) turn2(r, i, (f + 1) * PER + u);
+                    if constexpr ((f * PER + u) % 2) turn3(r, w, i, f * PER + u - 1););
                 __builtin_amdgcn_sched_barrier(0);););
     };
     auto first_pieces = [&](const uint16_t *kb, const uint16_t *vb, Pieces &x) __attribute__((always_inline)) {
@@ -556,7 +549,6 @@ __global__ __launch_bounds__(NW * 64) void cross_attn_kernel(const CrossAttn p, 
             read_piece(kb, kb, f, x);
             for (int i = 0; i < QB; ++i) n.s[i] = T::mfma(x.f[f % SLOTS], q[i][f / 3 * 2 + f % 3], n.s[i]);
         });
-        largest(n);
     };
     auto multiply_v = [&](const uint16_t *vb, const Weights &w) __attribute__((always_inline)) {
         EACH(f, 0, NF, if constexpr (!(f < NK / 2 * 3 && f % 3 != 2)) {
@@ -566,49 +558,48 @@ __global__ __launch_bounds__(NW * 64) void cross_attn_kernel(const CrossAttn p, 
             for (int i = 0; i < QB; ++i) o[i][J % (DP / 32)] = T::mfma(x.f[f % SLOTS], __builtin_bit_cast(x8, w.w[i][J / (DP / 32)]), o[i][J % (DP / 32)]);
         });
     };
-    auto weigh = [&](Logits &n, Weights &w) __attribute__((always_inline)) {
-        EACH(i, 0, QB, EACH(e, 0, 16, turn1(n, i, e); turn2(n, i, e);); EACH(e, 0, 8, turn3(n, w, i, 2 * e);););
+    auto weigh = [&](const Logits &n, Weights &w) __attribute__((always_inline)) {
+        Turns r;
+        EACH(i, 0, QB, EACH(e, 0, 16, turn1(n, r, i, e); turn2(r, i, e);); EACH(e, 0, 8, turn3(r, w, i, 2 * e);););
     };
-    // what the next weights go by: states that do not count leave, the maximum moves if it has to
-    auto settle = [&](Logits &n, uint64_t count, int half, Weights &before) __attribute__((always_inline)) {
+    // states of a half that do not count leave before they are weighed
+    auto leave = [&](Logits &n, uint64_t count, int half) __attribute__((always_inline)) {
         const uint32_t part = (uint32_t) (count >> 32 * half);
-        if (part != ~0u) {
-            uint32_t mine = part >> 4 * hi;
-            asm volatile("" : "+v"(mine));                     // (nothing of this is worked out ahead)
+        if (part == ~0u) return;
+        uint32_t mine = part >> 4 * hi;
+        asm volatile("" : "+v"(mine));                         // (nothing of this is worked out ahead)
 #pragma unroll
-            for (int i = 0; i < QB; ++i)
+        for (int i = 0; i < QB; ++i)
 #pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    if (!(mine >> (8 * (e >> 2) + (e & 3)) & 1)) n.s[i][e] = -__builtin_inff();
-            largest(n);
-        }
-        float top[QB];
-        bool move = false;
+            for (int e = 0; e < 16; ++e)
+                if (!(mine >> (8 * (e >> 2) + (e & 3)) & 1)) n.s[i][e] = -__builtin_inff();
+    };
+    // Weights that have grown past 2^8 together (or are not finite): the maximum moves to a whole
+    // number, what has been summed shrinks by a power of two, and they are worked out again. The
+    // sums tell it, so the logits' own maximum is looked for only then
+    auto settle = [&](const Logits &n, Weights &w) __attribute__((always_inline)) {
+        bool far = false;
 #pragma unroll
-        for (int i = 0; i < QB; ++i) {
-            top[i] = half_pair_max(n.top[i]) * c;
-            move = move || top[i] > m[i] + 8.0f;
-        }
-        if (!__any(move)) return;
+        for (int i = 0; i < QB; ++i) far = far || !(w.sum[i] <= 256.0f);
+        if (__any(far)) {
 #pragma unroll
-        for (int i = 0; i < QB; ++i) {
-            asm volatile("" : "+v"(top[i]));
-            const float to = top[i] > m[i] + 8.0f ? __builtin_ceilf(top[i]) : m[i];
-            const float s = to == -__builtin_inff() ? 0.0f : to, f = __builtin_amdgcn_exp2f(m[i] - s);
-            m[i] = to;
-            sub[i] = s;
-            l[i] *= f;
+            for (int i = 0; i < QB; ++i) {
+                float top = n.s[i][0];
+                asm volatile("" : "+v"(top));
 #pragma unroll
-            for (int db = 0; db < DP / 32; ++db)
+                for (int e = 1; e < 16; ++e) top = fmaxf(top, n.s[i][e]);
+                const float to = fmaxf(m[i], __builtin_ceilf(half_pair_max(top) * c)), f = __builtin_amdgcn_exp2f(m[i] - to);
+                m[i] = to;
+                l[i] *= f;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) o[i][db][e] *= f;
+                for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
-            for (int kg = 0; kg < 2; ++kg) {
-                const x8 w = __builtin_bit_cast(x8, before.w[i][kg]);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) before.w[i][kg][e] = T::pack2((float) w[2 * e] * f, (float) w[2 * e + 1] * f);
+                    for (int e = 0; e < 16; ++e) o[i][db][e] *= f;
             }
+            weigh(n, w);
         }
+#pragma unroll
+        for (int i = 0; i < QB; ++i) l[i] += w.sum[i];
     };
     if (u.tile0 < u.tile1) {
         for (int t = 0; t < 3; ++t) {
@@ -628,24 +619,28 @@ __global__ __launch_bounds__(NW * 64) void cross_attn_kernel(const CrossAttn p, 
         clear(count, 0);
         clear(next, 1);
         multiply_k(k_at(0, 0), na);
-        settle(na, count, 0, wb);
-        multiply_k(k_at(0, 1), nb);
+        leave(na, count, 0);
         weigh(na, wa);
+        settle(na, wa);
+        multiply_k(k_at(0, 1), nb);
         int slot = 0;
         Pieces x;
+        Turns r;
         for (int t = u.tile0; t + 1 < u.tile1; ++t) {
             const int s1 = (slot + 1) & 3, s2 = (slot + 2) & 3, s3 = (slot + 3) & 3;
             // second half of tile t; tile t + 3 goes where tile t - 1 was, which every wave is done with
             const Source src = source_of(t + 3);
             first_pieces(k_at(s1, 0), v_at(slot, 0), x);
-            settle(nb, count, 1, wa);
-            first_turns(nb);
-            step(k_at(s1, 0), v_at(slot, 0), x, nb, wb, na, wa, src, s3, std::integral_constant<int, 0>{});
+            leave(nb, count, 1);
+            first_turns(nb, r);
+            step(k_at(s1, 0), v_at(slot, 0), x, nb, r, wb, na, wa, src, s3, std::integral_constant<int, 0>{});
             // first half of tile t + 1
             first_pieces(k_at(s1, 1), v_at(slot, 1), x);
-            settle(na, next, 0, wb);
-            first_turns(na);
-            step(k_at(s1, 1), v_at(slot, 1), x, na, wa, nb, wb, src, s3, std::integral_constant<int, 1>{});
+            settle(nb, wb);
+            leave(na, next, 0);
+            first_turns(na, r);
+            step(k_at(s1, 1), v_at(slot, 1), x, na, r, wa, nb, wb, src, s3, std::integral_constant<int, 1>{});
+            settle(na, wa);
             count = next;
             next = counted(t + 2);
             // tile t + 2 has landed
@@ -654,9 +649,10 @@ __global__ __launch_bounds__(NW * 64) void cross_attn_kernel(const CrossAttn p, 
             clear(next, s2);
             slot = s1;
         }
-        settle(nb, count, 1, wa);
+        leave(nb, count, 1);
         weigh(nb, wb);
         multiply_v(v_at(slot, 0), wa);
+        settle(nb, wb);
         multiply_v(v_at(slot, 1), wb);
     }
 #pragma unroll
