@@ -6,7 +6,7 @@
 // below its sequence's length and its flag is set; where none does, o is 0. The query heads that
 // share a key and value head stand below one another as rows of one problem.
 //
-// A wave holds 32 rows. Per tile of 64 states (v_mfma_f32_32x32x16, fp32 sums):
+// A wave holds 32 rows. Per tile of states (v_mfma_f32_32x32x16, fp32 sums):
 //   S^T = K Q^T      states x rows: lane l owns row l % 32 and half of the states,
 //   P^T = exp2(scale log2(e) S^T - m) in K's 16-bit type,
 //   O^T += V^T P^T   the sums of the first product lie as the second one's operand does.
@@ -15,9 +15,6 @@
 #include <algorithm>
 #include <utility>
 
-#ifndef PFD
-#define PFD 4
-#endif
 #include "tsk_common.h"
 #include "tsk_internal.h"
 #include "tsk_runtime.h"
@@ -114,6 +111,10 @@ template <class F, int... I>
 __device__ __forceinline__ void each(F f, std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>{}), ...); }
 #define EACH(q, from, to, ...) each([&](auto q##_) __attribute__((always_inline)) { constexpr int q = decltype(q##_)::value + (from); __VA_ARGS__ }, std::make_integer_sequence<int, ((to) > (from) ? (to) - (from) : 0)>{})
 
+// piece f of a step's 2 NK operands: two of K, one of V, ..., what is left of V
+__host__ __device__ constexpr bool piece_of_k(int NK, int f) { return f < NK / 2 * 3 && f % 3 != 2; }
+__host__ __device__ constexpr int piece_index(int NK, int f) { return f >= NK / 2 * 3 ? f - NK : f % 3 == 2 ? f / 3 : f / 3 * 2 + f % 3; }
+
 // A launch's unit: a tile of rows of one key and value head, and (splits > 1) one of the
 // ranges that its sequence's tiles of states are dealt to. The ranges go by the sequence's own
 // length, which the device alone knows: `per` tiles each, the last ones empty.
@@ -125,17 +126,28 @@ struct Unit {
 template <int KT>
 __device__ __forceinline__ Unit unit_of(const CrossAttn &p, int qtiles, int rows) {
     Unit u;
-    // workgroup L runs on XCD L % 8: each XCD takes a run of the units, whose neighbours read the
-    // same states (the grid is a multiple of 8; the units past the last are none)
+    // Workgroup L runs on XCD L % 8. From 8 key and value heads on (of all sequences), XCD x takes
+    // heads x, x + 8, ...: a head's states stay in one L2, neighbouring heads are read at the
+    // same time, and sequences of other lengths spread over all XCDs. Units are numbered with
+    // the ranges fastest, then the tiles of rows, then the heads
     // (fewer than 2^23; the quotients come from vector units, and are the same for every lane)
     auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
-    const int i = (int) ((blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3));
-    const int unit = uniform(i / p.splits), head = uniform(unit / qtiles), qt = unit - head * qtiles;
-    u.split = i - unit * p.splits;
+    const int per_head = qtiles * p.splits, heads = p.Hkv * p.B;
+    int head, in;
+    if (heads >= 8) {
+        const int j = (int) (blockIdx.x >> 3), g = uniform(j / per_head);
+        head = 8 * g + (int) (blockIdx.x & 7);
+        in = j - g * per_head;
+    } else {
+        head = uniform((int) blockIdx.x / per_head);
+        in = (int) blockIdx.x - head * per_head;
+    }
+    u.none = head >= heads;
+    if (u.none) return u;
+    const int qt = uniform(in / p.splits);
+    u.split = in - qt * p.splits;
     u.b = uniform(head / p.Hkv);
     u.hk = head - u.b * p.Hkv;
-    u.none = u.b >= p.B;
-    if (u.none) return u;
     u.nkv = uniform(p.kv_len ? max(0, min(p.kv_len[u.b], p.Nkv)) : p.Nkv);
     u.nq = uniform(p.q_len ? max(0, min(p.q_len[u.b], p.Nq)) : p.Nq);
     const int G = p.H / p.Hkv, tiles = (u.nkv + KT - 1) / KT, per = uniform((tiles + p.splits - 1) / p.splits);
@@ -351,41 +363,69 @@ __global__ __launch_bounds__(256) void cross_attn_few_kernel(const CrossAttn p, 
     }
 }
 
-// the ranges of every row brought together, 4 dims a thread
-template <int KT>
-__global__ __launch_bounds__(256) void cross_attn_join_kernel(const CrossAttn p) {
-    const int D4 = p.D / 4;
-    const int64_t n = all_rows(p) * D4, R = (int64_t) (p.H / p.Hkv) * p.Nq;
-    for (int64_t i = (int64_t) blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t) gridDim.x * 256) {
-        const int64_t at = i / D4, unit = at / R;
-        const int d = (int) (i - at * D4) * 4, b = (int) (unit / p.Hkv), hk = (int) (unit % p.Hkv);
-        int h, iq;
-        row_of(p, hk, at - unit * R, h, iq);
-        if (p.q_len && iq >= p.q_len[b]) continue;
-        const int used = used_splits<KT>(p, p.kv_len ? max(0, min(p.kv_len[b], p.Nkv)) : p.Nkv);
-        float m = -__builtin_inff(), l = 0.0f;
-        for (int s = 0; s < used; ++s) m = fmaxf(m, part_ml(p, s, at)[0]);
-        const float sub = m == -__builtin_inff() ? 0.0f : m;
-        f32x4 v = {0, 0, 0, 0};
-        for (int s = 0; s < used; ++s) {
-            const float *ml = part_ml(p, s, at), f = __builtin_amdgcn_exp2f(ml[0] - sub);
-            l += ml[1] * f;
-            v += *(const f32x4 *) (part_o(p, s, at) + d) * f;
-        }
-        store_o4(p, o_row(p, b, h, iq), d, v * inverse(l));
+// The ranges of a row brought together: a thread takes 4 dims and every G-th range, all of
+// whose reads are on their way at once; G threads' sums meet in LDS (G a power of two, ranges
+// up to 256 / (DP / 4))
+template <int KT, int DP>
+__global__ __launch_bounds__(256) void cross_attn_join_kernel(const CrossAttn p, int G) {
+    constexpr int T4 = DP / 4, NG = 256 / T4, MOST = CROSS_ATTN_SPLITS / NG;
+    __shared__ float ms[NG], ls[NG];
+    __shared__ __attribute__((aligned(16))) f32x4 vs[256];
+    const int seat = threadIdx.x / T4, g = seat % G, d = threadIdx.x % T4 * 4;
+    const int64_t mine = (int64_t) blockIdx.x * (NG / G) + seat / G, rows = all_rows(p), at = std::min<int64_t>(mine, rows - 1);
+    const int64_t R = (int64_t) (p.H / p.Hkv) * p.Nq, unit = at / R;
+    const int b = (int) (unit / p.Hkv), hk = (int) (unit % p.Hkv);
+    int h, iq;
+    row_of(p, hk, at - unit * R, h, iq);
+    // (rows of tokens past the last are in no range, and are not stored)
+    const bool there = mine < rows && !(p.q_len && iq >= p.q_len[b]);
+    const int used = there ? used_splits<KT>(p, p.kv_len ? max(0, min(p.kv_len[b], p.Nkv)) : p.Nkv) : 0;
+    float mv[MOST], lv[MOST], m = -__builtin_inff(), l = 0.0f;
+    f32x4 ov[MOST], v = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < MOST; ++i) {
+        const int s = g + G * i;
+        const bool in = s < used;
+        mv[i] = in ? part_ml(p, s, at)[0] : -__builtin_inff();
+        lv[i] = in ? part_ml(p, s, at)[1] : 0.0f;
+        ov[i] = in && d < p.D ? *(const f32x4 *) (part_o(p, s, at) + d) : v;
     }
+#pragma unroll
+    for (int i = 0; i < MOST; ++i) m = fmaxf(m, mv[i]);
+    const float sub = m == -__builtin_inff() ? 0.0f : m;
+#pragma unroll
+    for (int i = 0; i < MOST; ++i) {
+        const float f = __builtin_amdgcn_exp2f(mv[i] - sub);
+        l += lv[i] * f;
+        v += ov[i] * f;
+    }
+    if (d == 0) {
+        ms[seat] = m;
+        ls[seat] = l;
+    }
+    vs[threadIdx.x] = v;
+    __syncthreads();
+    if (g > 0 || d >= p.D || !there) return;
+    for (int i = 1; i < G; ++i) m = fmaxf(m, ms[seat + i]);
+    const float all = m == -__builtin_inff() ? 0.0f : m;
+    l = 0.0f;
+    v = f32x4{0, 0, 0, 0};
+    for (int i = 0; i < G; ++i) {
+        const float f = __builtin_amdgcn_exp2f(ms[seat + i] - all);
+        l += ls[seat + i] * f;
+        v += vs[threadIdx.x + i * T4] * f;
+    }
+    store_o4(p, o_row(p, b, h, iq), d, v * inverse(l));
 }
 
 // ---------------------------------------------------------------- many rows
-// A workgroup takes 128 QB rows, 32 QB a wave, and tiles of 64 states through a ring of four
-// in LDS. Half a tile (32 states) at a time, a wave multiplies the next half's K with Q and
-// the last half's V with P while it turns this half's logits into weights: three steps of
-// three halves without a dependence, so that the matrix unit and the rest of the SIMD work at
-// once. A wave with 64 rows (QB 2) uses every operand that it reads from LDS twice.
-//
-// The running maximum moves only when the logits pass it by more than 2^8, and then to a whole
-// number (log2 domain): sums and weights already rounded are scaled by a power of two, exactly.
-template <int DP, bool BF16, int QB, int NW>
+// A workgroup takes 32 NW rows, 32 a wave, and tiles of 64 states through a ring of four in
+// LDS. Half a tile (32 states) at a time, a wave multiplies the next half's K with Q and the
+// last half's V with P while it turns this half's logits into weights: three steps of three
+// halves without a dependence, so that the matrix unit and the rest of the SIMD work at once.
+// Products, LDS reads, loads and the softmax's operations are in the program's order
+// (sched_barrier).
+template <int DP, bool BF16, int NW>
 __global__ __launch_bounds__(NW * 64) void cross_attn_kernel(const CrossAttn p, int qtiles) {
     typedef Half<BF16> T;
     typedef typename T::x8 x8;
@@ -394,18 +434,16 @@ __global__ __launch_bounds__(NW * 64) void cross_attn_kernel(const CrossAttn p, 
     extern __shared__ __attribute__((aligned(1024))) uint16_t lds[];           // [4][K tile, V tile]
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l32 = lane & 31, hi = lane >> 5;
-    const Unit u = unit_of<KT>(p, qtiles, 32 * QB * NW);
+    const Unit u = unit_of<KT>(p, qtiles, 32 * NW);
     if (u.none) return;
-    int h[QB], iq[QB];
-    x8 q[QB][DP / 16];
-#pragma unroll
-    for (int i = 0; i < QB; ++i) {
-        row_of(p, u.hk, std::min<int64_t>(u.r0 + (wave * QB + i) * 32 + l32, u.R - 1), h[i], iq[i]);
-        load_q<DP, BF16>(p, u.b, h[i], iq[i], hi, q[i]);
-    }
+    const int64_t row = u.r0 + wave * 32 + l32;
+    int h, iq;
+    row_of(p, u.hk, std::min<int64_t>(row, u.R - 1), h, iq);
+    x8 q[DP / 16];
+    load_q<DP, BF16>(p, u.b, h, iq, hi, q);
     const char *kp = (const char *) p.k + u.hk * p.k_nb2 + u.b * p.k_nb3, *vp = (const char *) p.v + u.hk * p.v_nb2 + u.b * p.v_nb3;
     const uint8_t *flags = p.kv_valid ? p.kv_valid + u.b * p.kv_valid_nb : nullptr;
-    // (a wave's loads are 4 * RL rows apart, which the keys do not see)
+    // (a wave's loads are NW * RL rows apart, which the keys do not see)
     const int lr = lane / CH, kc = (lane % CH) ^ k_key<DP>(wave * RL + lr), vc = (lane % CH) ^ v_key<DP>(lr);
     const int koff = kc * 8 < p.D ? (int) (lr * p.k_nb1) + kc * 16 : FAR, voff = vc * 8 < p.D ? (int) (lr * p.v_nb1) + vc * 16 : FAR;
     // tile t into slot s, a load at a time; tiles past the last: zeros, so that every wait counts the same
@@ -438,44 +476,31 @@ __global__ __launch_bounds__(NW * 64) void cross_attn_kernel(const CrossAttn p, 
     // a state that does not count may hold anything, and 0 times it may not be 0: its V becomes zeros
     auto clear = [&](uint64_t count, int s) {
         if (!flags || count == ~(uint64_t) 0) return;
-        constexpr int PER = NW;                                  // threads a row
-        const int r = tid / PER;
+        const int r = tid / NW;                                  // NW threads a row
         if (!(count >> r & 1))
 #pragma unroll
-            for (int i = 0; i < CH / PER; ++i) *(u32x4 *) (lds + s * 2 * TILE + TILE + r * DP + (tid % PER * (CH / PER) + i) * 8) = u32x4{0, 0, 0, 0};
+            for (int i = 0; i < CH / NW; ++i) *(u32x4 *) (lds + s * 2 * TILE + TILE + r * DP + (tid % NW * (CH / NW) + i) * 8) = u32x4{0, 0, 0, 0};
         __syncthreads();
     };
-    f32x16 o[QB][DP / 32];
-    float m[QB], l[QB];
+    f32x16 o[DP / 32];
 #pragma unroll
-    for (int i = 0; i < QB; ++i) {
-        m[i] = -1e30f;                                         // (any logit is far above it)
-        l[i] = 0.0f;
-#pragma unroll
-        for (int db = 0; db < DP / 32; ++db)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o[i][db][e] = 0.0f;
-    }
+    for (int db = 0; db < DP / 32; ++db) o[db] = f32x16{};
+    float m = -1e30f, l = 0.0f;                                  // (any logit is far above it)
     const float c = p.c;
     const int l16 = lane & 15, grp = (lane >> 4) & 1, vrow = 4 * hi + (l16 >> 2);
-    struct Logits {
-        f32x16 s[QB];
-    };
     struct Weights {
-        u32x4 w[QB][2];                                          // pairs
-        float sum[QB];
+        u32x4 w[2];                                              // pairs
+        float sum;
     };
     // A step's operands in LDS, K's of one half of a tile and V's of another, in the order of
     // their products: two of K, one of V, ..., what is left of V; each read AHEAD products early
-    constexpr int NK = DP / 16, NF = 2 * NK, AHEAD = PFD, SLOTS = AHEAD + 1;
+    constexpr int NK = DP / 16, NF = 2 * NK, AHEAD = 4, SLOTS = AHEAD + 1;
     struct Pieces {
         x8 f[SLOTS];
     };
-    auto of_k = [](int f) { return f < NK / 2 * 3 && f % 3 != 2; };
-    auto index = [](int f) { return f >= NK / 2 * 3 ? f - NK : f % 3 == 2 ? f / 3 : f / 3 * 2 + f % 3; };
     auto read_piece = [&](const uint16_t *kb, const uint16_t *vb, int f, Pieces &x) __attribute__((always_inline)) {
-        const int j = index(f);
-        if (of_k(f)) {
+        const int j = piece_index(NK, f);
+        if (piece_of_k(NK, f)) {
             x.f[f % SLOTS] = *(const x8 *) (kb + l32 * DP + (((2 * j + hi) ^ k_key<DP>(l32)) << 3));
         } else {
             const int kg = j / (DP / 32), db = j % (DP / 32), ch = 4 * db + 2 * grp + ((l16 & 3) >> 1);
@@ -490,116 +515,101 @@ __global__ __launch_bounds__(NW * 64) void cross_attn_kernel(const CrossAttn p, 
     // A logit becomes a weight in three turns, each some products after the one before (a wave
     // waits for its own results): the exponent, its power, and two of them rounded and added
     struct Turns {
-        float v[QB][16];
+        float v[16];
     };
-    auto turn1 = [&](const Logits &n, Turns &r, int i, int e) __attribute__((always_inline)) {
-        float v = __builtin_fmaf(n.s[i][e], c, -m[i]);
-        asm volatile("" : "+v"(v));                            // (worked out here and not where it is used)
-        r.v[i][e] = v;
+    auto turn1 = [&](const f32x16 &n, Turns &r, int e) __attribute__((always_inline)) {
+        float v = __builtin_fmaf(n[e], c, -m);
+        asm volatile("" : "+v"(v));                              // (worked out here and not where it is used)
+        r.v[e] = v;
     };
-    auto turn2 = [&](Turns &r, int i, int e) __attribute__((always_inline)) {
-        float v = __builtin_amdgcn_exp2f(r.v[i][e]);
+    auto turn2 = [&](Turns &r, int e) __attribute__((always_inline)) {
+        float v = __builtin_amdgcn_exp2f(r.v[e]);
         asm volatile("" : "+v"(v));
-        r.v[i][e] = v;
+        r.v[e] = v;
     };
-    auto turn3 = [&](const Turns &r, Weights &w, int i, int e) __attribute__((always_inline)) {
-        uint32_t two = T::pack2(r.v[i][e], r.v[i][e + 1]);
-        float sum = T::add2(two, e == 0 ? 0.0f : w.sum[i]);
+    auto turn3 = [&](const Turns &r, Weights &w, int e) __attribute__((always_inline)) {
+        uint32_t two = T::pack2(r.v[e], r.v[e + 1]);
+        float sum = T::add2(two, e == 0 ? 0.0f : w.sum);
         asm volatile("" : "+v"(two), "+v"(sum));
-        w.sum[i] = sum;
-        w.w[i][e / 8][e % 8 / 2] = two;
+        w.sum = sum;
+        w.w[e / 8][e % 8 / 2] = two;
     };
-    constexpr int PER = 16 / NF;                               // logits between two products
-    auto first_turns = [&](const Logits &n, Turns &r) __attribute__((always_inline)) {
-        EACH(i, 0, QB, EACH(e, 0, 2 * PER, turn1(n, r, i, e);); EACH(e, 0, PER, turn2(r, i, e);););
+    constexpr int PER = 16 / NF;                                 // logits between two products
+    auto first_turns = [&](const f32x16 &n, Turns &r) __attribute__((always_inline)) {
+        EACH(e, 0, 2 * PER, turn1(n, r, e););
+        EACH(e, 0, PER, turn2(r, e););
         __builtin_amdgcn_sched_barrier(0);
-    };
-    // the products of next (K . Q of a half) and of before (V of another), `now` weighed between them
-    auto step = [&](const uint16_t *kb, const uint16_t *vb, Pieces &x, const Logits &now, Turns &r, Weights &w, Logits &next, const Weights &before,
-                    const Source &src, int to, auto part) __attribute__((always_inline)) {
-        constexpr int L0 = decltype(part)::value * LOADS / 2, L1 = LOADS / 2;  // half of the loads of a later tile
-        EACH(f, 0, NF,
-            constexpr int J = f >= NK / 2 * 3 ? f - NK : f % 3 == 2 ? f / 3 : f / 3 * 2 + f % 3;
-            constexpr bool K = f < NK / 2 * 3 && f % 3 != 2;
-            EACH(i, 0, QB,
-                if constexpr (K && J == 0) next.s[i] = f32x16{};
-                if constexpr (K) next.s[i] = T::mfma(x.f[f % SLOTS], q[i][J], next.s[i]);
-                else o[i][J % (DP / 32)] = T::mfma(x.f[f % SLOTS], __builtin_bit_cast(x8, before.w[i][J / (DP / 32)]), o[i][J % (DP / 32)]);
-                if constexpr (i == 0 && f + AHEAD < NF) read_piece(kb, vb, f + AHEAD, x);
-                if constexpr (i == QB - 1) {
-                    EACH(u, f * L1 / NF, (f + 1) * L1 / NF, issue_one(src, to, L0 + u););
-                }
-                EACH(u, 0, PER,
-                    if constexpr ((f + 2) * PER + u < 16) turn1(now, r, i, (f + 2) * PER + u);
-                    if constexpr ((f + 1) * PER + u < 16) turn2(r, i, (f + 1) * PER + u);
-                    if constexpr ((f * PER + u) % 2) turn3(r, w, i, f * PER + u - 1););
-                __builtin_amdgcn_sched_barrier(0);););
     };
     auto first_pieces = [&](const uint16_t *kb, const uint16_t *vb, Pieces &x) __attribute__((always_inline)) {
         EACH(f, 0, AHEAD, read_piece(kb, vb, f, x););
         __builtin_amdgcn_sched_barrier(0);
     };
-    auto multiply_k = [&](const uint16_t *kb, Logits &n) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < QB; ++i)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) n.s[i][e] = 0.0f;
-        EACH(f, 0, NF, if constexpr (f < NK / 2 * 3 && f % 3 != 2) {
+    // the products of next (K . Q of a half) and of before (V of another), `now` weighed between
+    // them, and one half (part) of the loads of a later tile
+    auto step = [&](const uint16_t *kb, const uint16_t *vb, Pieces &x, const f32x16 &now, Turns &r, Weights &w, f32x16 &next,
+                    const Weights &before, const Source &src, int to, auto part) __attribute__((always_inline)) {
+        constexpr int L0 = decltype(part)::value * LOADS / 2, L1 = LOADS / 2;
+        EACH(f, 0, NF,
+            constexpr int J = piece_index(NK, f);
+            if constexpr (piece_of_k(NK, f)) next = T::mfma(x.f[f % SLOTS], q[J], J == 0 ? f32x16{} : next);
+            else o[J % (DP / 32)] = T::mfma(x.f[f % SLOTS], __builtin_bit_cast(x8, before.w[J / (DP / 32)]), o[J % (DP / 32)]);
+            if constexpr (f + AHEAD < NF) read_piece(kb, vb, f + AHEAD, x);
+            EACH(i, f * L1 / NF, (f + 1) * L1 / NF, issue_one(src, to, L0 + i););
+            EACH(i, 0, PER,
+                if constexpr ((f + 2) * PER + i < 16) turn1(now, r, (f + 2) * PER + i);
+                if constexpr ((f + 1) * PER + i < 16) turn2(r, (f + 1) * PER + i);
+                if constexpr ((f * PER + i) % 2) turn3(r, w, f * PER + i - 1););
+            __builtin_amdgcn_sched_barrier(0););
+    };
+    // the same alone, before the first step and after the last
+    auto multiply_k = [&](const uint16_t *kb, f32x16 &n) __attribute__((always_inline)) {
+        n = f32x16{};
+        EACH(f, 0, NF, if constexpr (piece_of_k(NK, f)) {
             Pieces x;
             read_piece(kb, kb, f, x);
-            for (int i = 0; i < QB; ++i) n.s[i] = T::mfma(x.f[f % SLOTS], q[i][f / 3 * 2 + f % 3], n.s[i]);
+            n = T::mfma(x.f[f % SLOTS], q[piece_index(NK, f)], n);
         });
     };
     auto multiply_v = [&](const uint16_t *vb, const Weights &w) __attribute__((always_inline)) {
-        EACH(f, 0, NF, if constexpr (!(f < NK / 2 * 3 && f % 3 != 2)) {
-            constexpr int J = f >= NK / 2 * 3 ? f - NK : f / 3;
+        EACH(f, 0, NF, if constexpr (!piece_of_k(NK, f)) {
+            constexpr int J = piece_index(NK, f);
             Pieces x;
             read_piece(vb, vb, f, x);
-            for (int i = 0; i < QB; ++i) o[i][J % (DP / 32)] = T::mfma(x.f[f % SLOTS], __builtin_bit_cast(x8, w.w[i][J / (DP / 32)]), o[i][J % (DP / 32)]);
+            o[J % (DP / 32)] = T::mfma(x.f[f % SLOTS], __builtin_bit_cast(x8, w.w[J / (DP / 32)]), o[J % (DP / 32)]);
         });
     };
-    auto weigh = [&](const Logits &n, Weights &w) __attribute__((always_inline)) {
+    auto weigh = [&](const f32x16 &n, Weights &w) __attribute__((always_inline)) {
         Turns r;
-        EACH(i, 0, QB, EACH(e, 0, 16, turn1(n, r, i, e); turn2(r, i, e);); EACH(e, 0, 8, turn3(r, w, i, 2 * e);););
+        EACH(e, 0, 16, turn1(n, r, e); turn2(r, e););
+        EACH(e, 0, 8, turn3(r, w, 2 * e););
     };
     // states of a half that do not count leave before they are weighed
-    auto leave = [&](Logits &n, uint64_t count, int half) __attribute__((always_inline)) {
+    auto leave = [&](f32x16 &n, uint64_t count, int half) __attribute__((always_inline)) {
         const uint32_t part = (uint32_t) (count >> 32 * half);
         if (part == ~0u) return;
         uint32_t mine = part >> 4 * hi;
-        asm volatile("" : "+v"(mine));                         // (nothing of this is worked out ahead)
+        asm volatile("" : "+v"(mine));                           // (nothing of this is worked out ahead)
 #pragma unroll
-        for (int i = 0; i < QB; ++i)
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-                if (!(mine >> (8 * (e >> 2) + (e & 3)) & 1)) n.s[i][e] = -__builtin_inff();
+        for (int e = 0; e < 16; ++e)
+            if (!(mine >> (8 * (e >> 2) + (e & 3)) & 1)) n[e] = -__builtin_inff();
     };
     // Weights that have grown past 2^8 together (or are not finite): the maximum moves to a whole
-    // number, what has been summed shrinks by a power of two, and they are worked out again. The
-    // sums tell it, so the logits' own maximum is looked for only then
-    auto settle = [&](const Logits &n, Weights &w) __attribute__((always_inline)) {
-        bool far = false;
+    // number (log2 domain), what has been summed shrinks by a power of two, exactly, and they are
+    // worked out again. The sums tell it, so the logits' maximum is looked for only then
+    auto settle = [&](const f32x16 &n, Weights &w) __attribute__((always_inline)) {
+        if (__any(!(w.sum <= 256.0f))) {
+            float top = n[0];
+            asm volatile("" : "+v"(top));
 #pragma unroll
-        for (int i = 0; i < QB; ++i) far = far || !(w.sum[i] <= 256.0f);
-        if (__any(far)) {
+            for (int e = 1; e < 16; ++e) top = fmaxf(top, n[e]);
+            const float to = fmaxf(m, __builtin_ceilf(half_pair_max(top) * c)), f = __builtin_amdgcn_exp2f(m - to);
+            m = to;
+            l *= f;
 #pragma unroll
-            for (int i = 0; i < QB; ++i) {
-                float top = n.s[i][0];
-                asm volatile("" : "+v"(top));
-#pragma unroll
-                for (int e = 1; e < 16; ++e) top = fmaxf(top, n.s[i][e]);
-                const float to = fmaxf(m[i], __builtin_ceilf(half_pair_max(top) * c)), f = __builtin_amdgcn_exp2f(m[i] - to);
-                m[i] = to;
-                l[i] *= f;
-#pragma unroll
-                for (int db = 0; db < DP / 32; ++db)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) o[i][db][e] *= f;
-            }
+            for (int db = 0; db < DP / 32; ++db) o[db] *= f;
             weigh(n, w);
         }
-#pragma unroll
-        for (int i = 0; i < QB; ++i) l[i] += w.sum[i];
+        l += w.sum;
     };
     if (u.tile0 < u.tile1) {
         for (int t = 0; t < 3; ++t) {
@@ -607,12 +617,8 @@ __global__ __launch_bounds__(NW * 64) void cross_attn_kernel(const CrossAttn p, 
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) issue_one(src, t, i);
         }
-        Logits na, nb;
+        f32x16 na, nb;
         Weights wa, wb;
-#pragma unroll
-        for (int i = 0; i < QB; ++i)
-#pragma unroll
-            for (int kg = 0; kg < 2; ++kg) wa.w[i][kg] = wb.w[i][kg] = u32x4{0, 0, 0, 0};
         uint64_t count = counted(u.tile0), next = counted(u.tile0 + 1);
         asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");           // (tiles 0 and 1)
         __syncthreads();
@@ -643,7 +649,7 @@ __global__ __launch_bounds__(NW * 64) void cross_attn_kernel(const CrossAttn p, 
             settle(na, wa);
             count = next;
             next = counted(t + 2);
-            // tile t + 2 has landed
+            // tile t + 2 has landed (t + 3 may be on its way)
             asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS) : "memory");
             __syncthreads();
             clear(next, s2);
@@ -654,38 +660,36 @@ __global__ __launch_bounds__(NW * 64) void cross_attn_kernel(const CrossAttn p, 
         multiply_v(v_at(slot, 0), wa);
         settle(nb, wb);
         multiply_v(v_at(slot, 1), wb);
+        // (no load may land in an LDS that is another workgroup's by then)
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    const float la = half_pair_sum(l), inv = inverse(la);
+    if (row >= u.R || iq >= u.nq) return;
+    const int64_t at = ((int64_t) u.b * p.Hkv + u.hk) * u.R + row;
+    if (p.splits > 1 && hi == 0) {
+        float *ml = part_ml(p, u.split, at);
+        ml[0] = m;
+        ml[1] = la;
     }
 #pragma unroll
-    for (int i = 0; i < QB; ++i) {
-        const int64_t r = u.r0 + (wave * QB + i) * 32 + l32;
-        const float la = half_pair_sum(l[i]), inv = inverse(la);
-        if (r >= u.R || iq[i] >= u.nq) continue;
-        char *row = o_row(p, u.b, h[i], iq[i]);
-        const int64_t at = ((int64_t) u.b * p.Hkv + u.hk) * u.R + r;
-        if (p.splits > 1 && hi == 0) {
-            float *ml = part_ml(p, u.split, at);
-            ml[0] = m[i];
-            ml[1] = la;
+    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const int d = 32 * db + 2 * e + 4 * hi;
+            if (d >= p.D) continue;
+            const f32x4 v = {o[db][e], o[db][e + 1], o[db][e + 2], o[db][e + 3]};
+            if (p.splits > 1) *(f32x4 *) (part_o(p, u.split, at) + d) = v;
+            else store_o4(p, o_row(p, u.b, h, iq), d, v * inv);
         }
-#pragma unroll
-        for (int db = 0; db < DP / 32; ++db)
-#pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-                const int d = 32 * db + 2 * e + 4 * hi;
-                if (d >= p.D) continue;
-                const f32x4 v = {o[i][db][e], o[i][db][e + 1], o[i][db][e + 2], o[i][db][e + 3]};
-                if (p.splits > 1) *(f32x4 *) (part_o(p, u.split, at) + d) = v;
-                else store_o4(p, row, d, v * inv);
-            }
-    }
 }
 
 template <class F>
 hipError_t launch_units(F kern, const CrossAttn &p, int rows, int threads, size_t lds, hipStream_t s) {
-    const int64_t R = (int64_t) (p.H / p.Hkv) * p.Nq, qtiles = (R + rows - 1) / rows, units = qtiles * p.Hkv * p.B * p.splits;
+    const int64_t R = (int64_t) (p.H / p.Hkv) * p.Nq, qtiles = (R + rows - 1) / rows, heads = (int64_t) p.Hkv * p.B;
+    const int64_t units = (heads >= 8 ? (heads + 7) / 8 * 8 : heads) * qtiles * p.splits;
     if (units >= (int64_t) 1 << 23) return hipErrorInvalidValue;
     lds_opt_in((const void *) kern, lds);
-    launch_kernel(kern, dim3((unsigned) ((units + 7) / 8 * 8)), dim3(threads), lds, s, p, (int) qtiles);
+    launch_kernel(kern, dim3((unsigned) units), dim3(threads), lds, s, p, (int) qtiles);
     return hipGetLastError();
 }
 
@@ -693,26 +697,49 @@ template <int DP, bool BF16>
 hipError_t launch_dp(const CrossAttn &p, const CrossAttnPlan &plan, hipStream_t s) {
     hipError_t e;
     if (plan.rows == 32) e = launch_units(cross_attn_few_kernel<DP, BF16>, p, 32, 256, 4 * 2 * 2 * 32 * DP * 2, s);
-    else if (plan.rows == 128) e = launch_units(cross_attn_kernel<DP, BF16, 1, 4>, p, 128, 256, 4 * 2 * 64 * DP * 2, s);
-    else if (plan.rows == 257) e = launch_units(cross_attn_kernel<DP, BF16, 1, 8>, p, 256, 512, 4 * 2 * 64 * DP * 2, s);
-    else e = launch_units(cross_attn_kernel<DP, BF16, 2, 4>, p, 256, 256, 4 * 2 * 64 * DP * 2, s);
+    else if (plan.rows == 128) e = launch_units(cross_attn_kernel<DP, BF16, 4>, p, 128, 256, 4 * 2 * 64 * DP * 2, s);
+    else e = launch_units(cross_attn_kernel<DP, BF16, 8>, p, 256, 512, 4 * 2 * 64 * DP * 2, s);
     if (e != hipSuccess || p.splits == 1) return e;
-    const int64_t n = (int64_t) p.B * p.H * p.Nq * (p.D / 4);
-    const dim3 grid((unsigned) std::min<int64_t>((n + 255) / 256, 1 << 20));
-    if (plan.rows == 32) launch_kernel(cross_attn_join_kernel<32>, grid, dim3(256), 0, s, p);
-    else launch_kernel(cross_attn_join_kernel<64>, grid, dim3(256), 0, s, p);
+    constexpr int NG = 256 / (DP / 4);
+    int G = 1;
+    while (G < p.splits && G < NG) G *= 2;
+    // (fewer than 2^24 rows, plan_cross_attn)
+    const dim3 grid((unsigned) (((int64_t) p.B * p.H * p.Nq + NG / G - 1) / (NG / G)));
+    if (plan.rows == 32) launch_kernel(cross_attn_join_kernel<32, DP>, grid, dim3(256), 0, s, p, G);
+    else launch_kernel(cross_attn_join_kernel<64, DP>, grid, dim3(256), 0, s, p, G);
     return hipGetLastError();
 }
 
 }  // namespace
 
 CrossAttnPlan plan_cross_attn(int D, int64_t Nq, int64_t Nkv, int64_t H, int64_t Hkv, int64_t B) {
-    CrossAttnPlan c;
+    CrossAttnPlan c = {128, 1, 0};
     const int64_t R = H / Hkv * Nq;
-    auto units = [&](int rows) { return (R + rows - 1) / rows * Hkv * B; };
-    c.rows = tuning().cross_cfg ? tuning().cross_cfg / 100 : R <= 32 ? 32 : units(256) >= 256 ? 256 : 128;
-    const int64_t most = std::min<int64_t>(256 / units(c.rows), Nkv / (c.rows == 32 ? 512 : 256));
-    c.splits = tuning().cross_cfg ? tuning().cross_cfg % 100 : (int) std::max<int64_t>(1, std::min<int64_t>(most, 64));
+    const bool wide = D > 64;
+    double least = 0;
+    for (int kind = 0; kind < 3; ++kind) {
+        const int rows = kind == 0 ? 32 : kind == 1 ? 128 : 256;
+        const double units = (double) ((R + rows - 1) / rows) * (double) (Hkv * B);
+        const double tiles = kind == 0 ? (double) ((Nkv + 127) / 128) : (double) ((Nkv + 63) / 64);     // of a wave
+        const int on_a_cu = wide || kind == 2 ? 1 : 2;
+        const double fixed = kind == 0 ? 3 : 2.5, alone = wide ? kind == 0 ? 1.12 : kind == 1 ? 1.2 : 1.93 : kind == 0 ? 0.55 : kind == 1 ? 0.84 : 1.17,
+                     full = wide ? alone : kind == 0 ? 0.9 : kind == 1 ? 1.28 : 1.17;
+        for (int s = 1; s <= CROSS_ATTN_SPLITS; s *= 2) {
+            if (s > 1 && (s > (int) tiles || B * H * Nq >= (int64_t) 1 << 24)) break;
+            const double on = units * s / 256, turns = std::ceil(on / on_a_cu), each = on <= 1 ? alone : full;
+            double cost = turns * (fixed + std::ceil(tiles / s) * each);
+            if (s > 1) cost += 3 + (double) (B * H * Nq) * s * D * 8 / 3e6;
+            if (!least || cost < least) {
+                least = cost;
+                c.rows = rows;
+                c.splits = s;
+            }
+        }
+    }
+    if (tuning().cross_cfg) {
+        c.rows = tuning().cross_cfg / 100;
+        c.splits = std::min(tuning().cross_cfg % 100, CROSS_ATTN_SPLITS);
+    }
     c.bytes = c.splits > 1 ? (size_t) c.splits * (size_t) (B * H * Nq) * (size_t) (D + 2) * 4 : 0;
     c.bytes = (c.bytes + 255) / 256 * 256;
     return c;

@@ -432,6 +432,7 @@ struct CrossAttn {
     int splits;                    // key ranges, each a workgroup; > 1: part holds their sums
     float *part;
 };
+constexpr int CROSS_ATTN_SPLITS = 64;     // most key ranges
 // rows of a workgroup, key ranges of the node and the scratch bytes that these take
 struct CrossAttnPlan {
     int rows, splits;
