@@ -188,7 +188,7 @@ __device__ __forceinline__ void store_row(void *row, int bf16, int C, int t, con
 // NT threads a row (fewer than 256: 256 / NT rows a workgroup), its values in
 // registers. What a pass needs beside them (WTS: weights, MOD: gate, scale and
 // shift) is loaded before the statistics that it waits for.
-template <int V, int VN, int NT, bool WTS, bool MOD>
+template <int V, int VN, int NT, bool WTS, bool MOD, bool I8>
 __global__ __launch_bounds__(NT < 256 ? 256 : NT) void block_norm_kernel(const BlockNorm p) {
     __shared__ float red[NT > 64 ? (NT < 256 ? 256 / NT : 1) * 2 * (NT / 64) : 1];
     constexpr int RW = NT < 256 ? 256 / NT : 1;                      // rows of a workgroup
@@ -203,7 +203,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void block_norm_kernel(const B
         const int i1 = (int) (r % p.n1), i2 = (int) (r / p.n1 % p.n2), i3 = (int) (r / p.n1 / p.n2);
         const bool has_y = p.y.data, has_gate = MOD && p.gate.data, has_scale = MOD && p.scale.data, has_shift = MOD && p.shift.data;
         const bool has_post_w = WTS && p.post_w, has_pre_w = WTS && p.pre_w;
-        const bool has_out = p.dst.data || p.scales || p.i8;
+        const bool has_out = I8 || p.dst.data || p.scales;
         float x[VN][V], y[VN][V], w[VN][V] = {}, f[VN][V] = {}, h[VN][V] = {}, mean, inv;
         load_row<V, VN, NT>(row_of(p.x, i1, i2, i3), p.x_bf16, C, t, x);
         if (has_y) {
@@ -237,9 +237,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void block_norm_kernel(const B
 #pragma unroll
             for (int e = 0; e < V; ++e)
                 x[j][e] = modulated(x[j][e], p.pre_norm, mean, inv, has_pre_w, w[j][e], has_scale, f[j][e], has_shift, h[j][e]);
-        if (p.dst.data) {
-            if (mine) store_row<V, VN, NT>(row_of(p.dst, i1, i2, i3), p.dst_bf16, C, t, x);
-        } else if (p.i8) {
+        if constexpr (I8) {
             const int ld = (int) i8_ld(C);
             uint32_t top = 0;
 #pragma unroll
@@ -259,6 +257,8 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void block_norm_kernel(const B
             }
             if (t < ld - C) q[C + t] = 0;                        // (at most 15: a row has 16 threads at least)
             if (t == 0) p.i8_d[r] = s.d;
+        } else if (p.dst.data) {
+            if (mine) store_row<V, VN, NT>(row_of(p.dst, i1, i2, i3), p.dst_bf16, C, t, x);
         } else if constexpr (V == 8) {
             // a block of 32 is four threads' vectors (C % 32 == 0: all four hold one, or none)
 #pragma unroll
@@ -375,8 +375,10 @@ template <int V, int VN, int NT>
 hipError_t launch_bn(const BlockNorm &p, int64_t rows, hipStream_t s) {
     constexpr int RW = NT < 256 ? 256 / NT : 1;
     const bool wts = p.post_w || p.pre_w, mod = p.gate.data || p.scale.data || p.shift.data;
-    launch_kernel(wts ? mod ? block_norm_kernel<V, VN, NT, true, true> : block_norm_kernel<V, VN, NT, true, false>
-                      : mod ? block_norm_kernel<V, VN, NT, false, true> : block_norm_kernel<V, VN, NT, false, false>,
+    // (8-bit rows have one kernel for all: in the others their code costs up to nine registers)
+    launch_kernel(p.i8 ? block_norm_kernel<V, VN, NT, true, true, true>
+                  : wts ? mod ? block_norm_kernel<V, VN, NT, true, true, false> : block_norm_kernel<V, VN, NT, true, false, false>
+                        : mod ? block_norm_kernel<V, VN, NT, false, true, false> : block_norm_kernel<V, VN, NT, false, false, false>,
                   dim3((unsigned) std::min<int64_t>((rows + RW - 1) / RW, 1 << 20)), dim3(NT < 256 ? 256 : NT), 0, s, p);
     return hipGetLastError();
 }

@@ -43,12 +43,25 @@ __device__ __forceinline__ int i8_code(float x, const I8Scale &s) {
     const bool off = a > lim || (a == lim && (i & 1));
     return off ? i + (r > 0.0f ? 1 : -1) : i;
 }
+// The codes of four values. x / d and x * (1 / d) are at most 127 and 2^-16 apart, so that the
+// integer nearest to the product is that of the quotient, but where the product is within
+// 2^-16 of a half: there i8_code decides. The sum with 1.5 * 2^23 rounds to an integer, whose
+// low byte is the sum's. (8192 x 8192 bf16: 48.3 us; with i8_code for every value 52.4.)
 __device__ __forceinline__ uint32_t i8_pack4(const float *v, const I8Scale &s) {
     if (s.inv == 0.0f) return 0u;
-    uint32_t w = 0;
+    uint32_t b[4];
+    float off = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) w |= ((uint32_t) i8_code(v[e], s) & 255u) << 8 * e;
-    return w;
+    for (int e = 0; e < 4; ++e) {
+        const float m = __builtin_fmaf(v[e], s.inv, 12582912.0f);
+        off = fmaxf(off, __builtin_fabsf(__builtin_fmaf(v[e], s.inv, 12582912.0f - m)));
+        b[e] = __float_as_uint(m);
+    }
+    if (off > 0.5f - 0x1p-16f) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) b[e] = (uint32_t) i8_code(v[e], s);
+    }
+    return __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u) | __builtin_amdgcn_perm(b[3], b[2], 0x04000c0cu);
 }
 
 // 8 values of an f32 or bf16 row from column c on, those past K zeros; WIDE: the row starts on 16 bytes

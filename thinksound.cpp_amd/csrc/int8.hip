@@ -2,7 +2,9 @@
 //
 // d = max(amax, 2^-100) / 127, q = the integer nearest to x / d (i8.h). Bound by memory:
 // a row is read once into the registers of the threads that share it, whose largest
-// magnitude is found between the load and the store.
+// magnitude is found between the load and the store. A vector instruction takes a wave four
+// cycles, so a value's few count: 8192 x 8192 bf16 48.3 us (4.2 TB/s, of a copy's 5.1), f32
+// 59.7 (5.6).
 #include <algorithm>
 
 #include "i8.h"
@@ -12,11 +14,14 @@ namespace tsk {
 
 namespace {
 
+// flat: rows nb1 apart throughout
 struct Rows {
     int64_t nb1, nb2, nb3;
     int ne1, ne2;
+    bool flat;
 };
 __device__ __forceinline__ int64_t row_at(const Rows &t, int64_t r) {
+    if (t.flat) return r * t.nb1;
     const int64_t i1 = r % t.ne1, q = r / t.ne1;
     return i1 * t.nb1 + q % t.ne2 * t.nb2 + q / t.ne2 * t.nb3;
 }
@@ -39,7 +44,9 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t *red) {
 }
 
 // NT threads a row, VN vectors of 8 values each in registers; rows longer than that
-// (LONG) are read a second time.
+// (LONG) are read a second time. Up to 2048 values a row is a wave's or less, without LDS or
+// barriers (32768 rows of 2000, bf16: 45.5 us, with 256 threads a row 73), and rows of up to
+// 256 have lanes for their own vectors only (100000 of 192: 20.1 us, with 64 lanes each 44.5).
 template <bool BF16, bool WIDE, int VN, int NT, bool LONG>
 __global__ __launch_bounds__(NT < 256 ? 256 : NT) void i8_quantize_kernel(const void *x, const Rows t, int64_t rows, int K, int64_t ld,
                                                                           int8_t *q, float *d) {
@@ -89,46 +96,63 @@ template <bool BF16, bool WIDE>
 hipError_t launch_quantize(const void *x, const Rows &t, int64_t rows, int K, int64_t ld, int8_t *q, float *d, hipStream_t s) {
     auto go = [&](auto kern, int nt) {
         const int rw = nt < 256 ? 256 / nt : 1;
-        launch_kernel(kern, dim3((unsigned) std::min<int64_t>((rows + rw - 1) / rw, 1 << 20)), dim3(nt < 256 ? 256 : nt), 0, s, x, t,
+        launch_kernel(kern, dim3((unsigned) std::min<int64_t>((rows + rw - 1) / rw, 1 << 22)), dim3(nt < 256 ? 256 : nt), 0, s, x, t,
                       rows, K, ld, q, d);
         return hipGetLastError();
     };
+    if (ld <= 8 * 8) return go(i8_quantize_kernel<BF16, WIDE, 1, 8, false>, 8);
     if (ld <= 16 * 8) return go(i8_quantize_kernel<BF16, WIDE, 1, 16, false>, 16);
+    if (ld <= 32 * 8) return go(i8_quantize_kernel<BF16, WIDE, 1, 32, false>, 32);
     if (ld <= 64 * 8) return go(i8_quantize_kernel<BF16, WIDE, 1, 64, false>, 64);
-    if (ld <= 128 * 8) return go(i8_quantize_kernel<BF16, WIDE, 1, 128, false>, 128);
+    if (ld <= 64 * 16) return go(i8_quantize_kernel<BF16, WIDE, 2, 64, false>, 64);
+    if (ld <= 64 * 32) return go(i8_quantize_kernel<BF16, WIDE, 4, 64, false>, 64);
     if (ld <= 256 * 16) return go(i8_quantize_kernel<BF16, WIDE, 2, 256, false>, 256);
     if (ld <= 512 * 16) return go(i8_quantize_kernel<BF16, WIDE, 2, 512, false>, 512);
     if (ld <= 1024 * 16) return go(i8_quantize_kernel<BF16, WIDE, 2, 1024, false>, 1024);
     return go(i8_quantize_kernel<BF16, WIDE, 1, 1024, true>, 1024);
 }
 
-// One thread per 8 values
+// A thread takes V values, and others a grid of threads on: step_r rows and step_c times V
+// values, P times V a row. (8192 x 8192 to f32 60.7 us, with 4 values a thread 64.4; 1000 rows of
+// 20001 with 8 57.9, with 4 38.5.)
 template <bool BF16, bool WIDE>
-__global__ void i8_dequantize_kernel(const int8_t *q, const float *d, int64_t rows, int K, int P, void *y, const Rows t) {
-    const int64_t n = rows * P, ld = i8_ld(K);
-    for (int64_t i = (int64_t) blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t) gridDim.x * blockDim.x) {
-        const int64_t r = i / P;
-        const int c = (int) (i - r * P) * 8;
-        const u32x2 w = *(const u32x2 *) (q + r * ld + c);
+__global__ void i8_dequantize_kernel(const int8_t *q, const float *d, int64_t rows, int K, int P, int64_t step_r, int step_c, void *y,
+                                     const Rows t) {
+    constexpr int V = WIDE ? 8 : 4;
+    const int64_t ld = i8_ld(K);
+    const unsigned first = blockIdx.x * blockDim.x + threadIdx.x;
+    int p = (int) (first % (unsigned) P);
+    for (int64_t r = first / (unsigned) P; r < rows; r += step_r, p += step_c) {
+        if (p >= P) {
+            p -= P;
+            if (++r >= rows) break;
+        }
+        const int c = p * V;
+        const char *codes = (const char *) q + r * ld + c;
+        uint32_t w[V / 4];
+        if constexpr (V == 8) {
+            const u32x2 two = *(const u32x2 *) codes;
+            w[0] = two[0];
+            w[1] = two[1];
+        } else w[0] = *(const uint32_t *) codes;
         const float s = d[r];
-        float v[8];
+        float v[V];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = s * (float) (int8_t) (w[e >> 2] >> 8 * (e & 3));
+        for (int e = 0; e < V; ++e) v[e] = s * (float) (int8_t) (w[e >> 2] >> 8 * (e & 3));
         char *row = (char *) y + row_at(t, r);
-        if (WIDE && c + 8 <= K) {
-            if constexpr (BF16) {
-                u32x4 h;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) h[e] = f32_to_bf16_bits(v[2 * e]) | (uint32_t) f32_to_bf16_bits(v[2 * e + 1]) << 16;
-                *(u32x4 *) (row + (int64_t) c * 2) = h;
-            } else {
-                ((f32x4 *) (row + (int64_t) c * 4))[0] = f32x4{v[0], v[1], v[2], v[3]};
-                ((f32x4 *) (row + (int64_t) c * 4))[1] = f32x4{v[4], v[5], v[6], v[7]};
+        if constexpr (WIDE) {
+            if (c + V <= K) {
+                if constexpr (BF16) *(bf16x8 *) (row + (int64_t) c * 2) = bf16x8{(__bf16) v[0], (__bf16) v[1], (__bf16) v[2], (__bf16) v[3],
+                                                                                 (__bf16) v[4], (__bf16) v[5], (__bf16) v[6], (__bf16) v[7]};
+                else {
+                    ((f32x4 *) (row + (int64_t) c * 4))[0] = f32x4{v[0], v[1], v[2], v[3]};
+                    ((f32x4 *) (row + (int64_t) c * 4))[1] = f32x4{v[4], v[5], v[6], v[7]};
+                }
+                continue;
             }
-            continue;
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
+        for (int e = 0; e < V; ++e)
             if (c + e < K) store_from_f32<BF16 ? Elt::BF16 : Elt::F32>(row, c + e, v[e]);
     }
 }
@@ -137,6 +161,7 @@ Rows rows_of(const View4 &t) {
     Rows r;
     r.nb1 = t.nb[1]; r.nb2 = t.nb[2]; r.nb3 = t.nb[3];
     r.ne1 = (int) t.ne[1]; r.ne2 = (int) t.ne[2];
+    r.flat = (t.ne[2] == 1 || t.nb[2] == t.nb[1] * t.ne[1]) && (t.ne[3] == 1 || t.nb[3] == t.nb[1] * t.ne[1] * t.ne[2]);
     return r;
 }
 bool on_16(const View4 &t) {
@@ -159,11 +184,12 @@ hipError_t launch_i8_quantize(const View4 &x, int8_t *q, float *d, hipStream_t s
 
 hipError_t launch_i8_dequantize(const int8_t *q, const float *d, const View4 &y, hipStream_t s) {
     const int64_t rows = y.ne[1] * y.ne[2] * y.ne[3];
-    const int K = (int) y.ne[0], P = (K + 7) / 8;
     const bool bf16 = y.type == TSK_TYPE_BF16, wide = on_16(y);
+    const int K = (int) y.ne[0], P = wide ? (K + 7) / 8 : (K + 3) / 4;
+    const int64_t threads = std::min<int64_t>((rows * P + 255) / 256, 1 << 20) * 256;
     launch_kernel(bf16 ? wide ? i8_dequantize_kernel<true, true> : i8_dequantize_kernel<true, false>
                        : wide ? i8_dequantize_kernel<false, true> : i8_dequantize_kernel<false, false>,
-                  dim3((unsigned) std::min<int64_t>((rows * P + 255) / 256, 1 << 20)), dim3(256), 0, s, q, d, rows, K, P, (void *) y.data,
+                  dim3((unsigned) (threads / 256)), dim3(256), 0, s, q, d, rows, K, P, threads / P, (int) (threads % P), (void *) y.data,
                   rows_of(y));
     return hipGetLastError();
 }
