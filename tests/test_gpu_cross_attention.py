@@ -262,3 +262,78 @@ def test_two_streams(T, Nkv):  # noqa: F811
         assert np.array_equal(o.numpy(), w)
     for s in st:
         s.destroy()
+
+
+@pytest.fixture
+def shape(T, monkeypatch):  # noqa: F811
+    """every call with one shape: rows of a workgroup and ranges of the states"""
+    def use(rows, ranges):
+        monkeypatch.setenv("TSK_CROSS_CFG", str(100 * rows + ranges))
+        T.init(0, reread=True)
+    yield use
+    monkeypatch.delenv("TSK_CROSS_CFG", raising=False)
+    T.init(0, reread=True)
+
+
+SHAPES = [(r, n) for r in (32, 128, 256) for n in (1, 2, 16, 64)]
+
+
+@pytest.mark.parametrize("D", [40, 64, 96, 128])
+@pytest.mark.parametrize("rows,ranges", SHAPES)
+def test_each_shape(T, shape, rows, ranges, D):  # noqa: F811
+    """shared heads whose number is no multiple of 8, few heads, ragged rows and tiles, lengths that leave ranges empty"""
+    shape(rows, ranges)
+    rng = np.random.default_rng(rows + D)
+    check(T, rng, 3, 6, 3, 37, 1000, D, kv_len=[1000, 129, 0], spread=3.0)
+    check(T, rng, 1, 10, 10, 33, 130, D, kv="f16", out="f32", spread=3.0)
+    check(T, rng, 1, 2, 2, 300, 777, D, valid=(rng.random((1, 777)) < 0.7), q_len=[290])
+    check(T, rng, 2, 1, 1, 1, 64 * ranges + 1, D, kv="f16", kv_len=[64 * ranges + 1, 1], valid=np.arange(64 * ranges + 1) != 5)
+
+
+@pytest.mark.parametrize("rows,ranges", SHAPES)
+def test_maximum_that_moves_in_each_shape(T, shape, rows, ranges):  # noqa: F811
+    """logits that rise, fall and jump past every threshold between and within ranges"""
+    shape(rows, ranges)
+    n, d, rng = 1500, 128, np.random.default_rng(3)
+    jump = np.zeros(n)
+    jump[::97] = np.linspace(10, 60, len(jump[::97]))
+    for ramp in (np.linspace(0, 60, n), np.linspace(60, 0, n), jump, np.linspace(-60, -50, n)):
+        q = np.zeros((1, 1, 50, d), np.float32)
+        q[..., 0] = 8.0 * np.linspace(-1, 1, 50)
+        k = rng.standard_normal((1, 1, n, d)).astype(np.float32) * 0.1
+        k[..., 0] = ramp
+        v = rng.standard_normal((1, 1, n, d)).astype(np.float32)
+        for kv in ("bf16", "f16"):
+            (Q, q2), (K, k2), (V, v2) = (to(T, t, kv) for t in (q, k, v))
+            got = T.cross_attention(Q, K, V, scale=0.125).numpy()
+            want, size, big = crossref.attention(q2, k2, v2, 0.125)
+            assert (np.abs(got - want) - tolerance(want, size, big, d, n, kv, "f32", np.abs(v2).max())).max() <= 0
+
+
+@pytest.mark.parametrize("rows,ranges", SHAPES)
+def test_states_that_do_not_count_in_each_shape(T, shape, rows, ranges):  # noqa: F811
+    """NaN and infinities where no state counts; a NaN that counts reaches its rows and no others"""
+    shape(rows, ranges)
+    rng = np.random.default_rng(9)
+    B, Nq, n, d = 2, 40, 400, 64
+    q, k, v = (rng.standard_normal((B, 1, m, d)).astype(np.float32) for m in (Nq, n, n))
+    lens = np.array([333, 150], np.int32)
+    for b in range(B):
+        k[b, 0, lens[b]:] = np.nan
+        v[b, 0, lens[b]:] = np.inf
+    flags = np.ones((B, n), np.uint8)
+    flags[:, 7::11] = 0
+    k[:, :, 7::11], v[:, :, 7::11] = np.inf, np.nan
+    Q, K, V = (to(T, t, "bf16")[0] for t in (q, k, v))
+    kw = dict(kv_len=T.to_device(lens), kv_valid=T.to_device(flags))
+    got = T.cross_attention(Q, K, V, **kw).numpy()
+    count = (np.arange(n) < lens[:, None]) & (flags != 0)
+    k2, v2 = (np.where(count[:, None, :, None], mxref.bf16_values(mxref.bf16_bits(t)), 0.0) for t in (k, v))
+    want, size, big = crossref.attention(mxref.bf16_values(mxref.bf16_bits(q)), k2, v2, 0.125, count)
+    assert (np.abs(got - want) - tolerance(want, size, big, d, n, "bf16", "f32", np.abs(v2).max())).max() <= 0
+    v[1, 0, 40, 3] = np.nan                                    # (its flag is 0: 40 = 7 + 3 * 11)
+    assert np.array_equal(T.cross_attention(Q, K, to(T, v, "bf16")[0], **kw).numpy(), got)
+    v[1, 0, 41, 3] = np.nan
+    got2 = T.cross_attention(Q, K, to(T, v, "bf16")[0], **kw).numpy()
+    assert np.array_equal(got2[0], got[0]) and np.isnan(got2[1, :, 0, 3]).all()
+    assert np.array_equal(np.delete(got2[1, :, 0], 3, 1), np.delete(got[1, :, 0], 3, 1))

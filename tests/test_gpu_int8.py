@@ -255,3 +255,63 @@ def test_block_norm_of_rows_that_are_not_finite(T):
     sp = T.SplitI8(T.to_device(np.full(6 * 100, 99, np.uint8)), 96, 6)
     T.block_norm(T.to_device(x), pre=T.NORM_NONE, dst=sp)
     check_planes(sp, x, 96)
+
+
+@pytest.mark.parametrize("cfg", [1, 2, 3, 4, 5, 6, 7, 8, 11, 12, 13])
+def test_each_shape(T, monkeypatch, cfg):
+    """every kernel's tiles over ragged rows, outputs and depths; what lies behind the outputs stays"""
+    rng = np.random.default_rng(cfg)
+    monkeypatch.setenv("TSK_I8_CFG", str(cfg))
+    T.init(0, reread=True)
+    try:
+        for n, k, m in ((5, 33, 20), (300, 1000, 515), (1, 1, 1), (270, 64, 258), (257, 129, 1), (33, 4100, 300), (1, 300, 260)):
+            x = crossref.i8_quantize((rng.standard_normal((n, k)) * np.exp(rng.standard_normal((n, 1)))).astype(np.float32))
+            w = crossref.i8_quantize(rng.standard_normal((m, k)).astype(np.float32))
+            bias = rng.standard_normal(m).astype(np.float32)
+            for b, dtype in ((None, "bf16"), (bias, "f32")):
+                ldy = (m + 7) // 8 * 8
+                out = dev(T, np.full((n, ldy), 9.0, np.float32), dtype)
+                T.mul_mat(planes(T, *w), planes(T, *x), bias=None if b is None else T.to_device(b), out=out.view(0, (n, m), out.strides))
+                got = host(out)
+                y, tol = want_linear(x, w, b, dtype)
+                assert off(got[:, :m], y, tol) <= 0, (n, k, m, dtype)
+                assert (got[:, m:] == 9.0).all()
+    finally:
+        monkeypatch.delenv("TSK_I8_CFG")
+        T.init(0, reread=True)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("amax", [127.0, 254.0, 1.0, 127.0 * 2.0 ** -90, 126.99999])
+def test_codes_next_to_a_half(T, dtype, amax):
+    """every half between two integers, exact and one step of the type to either side, in rows of a known scale"""
+    d = np.float32(amax) / np.float32(127.0)
+    halves = (np.arange(-127, 127) + 0.5).astype(np.float64) * np.float64(d)
+    x = typed(halves.astype(np.float32), dtype)
+    if dtype == "f32":
+        near = [x, np.nextafter(x, np.float32(np.inf)), np.nextafter(x, np.float32(-np.inf))]
+    else:
+        step = np.abs(x) * np.float32(2.0 ** -7)
+        near = [x, typed(x + step, dtype), typed(x - step, dtype)]
+    rows = np.stack([np.concatenate([[np.float32(amax)], np.clip(t, -np.float32(amax), np.float32(amax))]).astype(np.float32) for t in near])
+    rows = typed(rows, dtype)
+    check_planes(T.i8_quantize(dev(T, rows, dtype)), rows, rows.shape[1])
+
+
+def test_two_streams(T):
+    """products on two streams keep their quantized activations apart"""
+    rng = np.random.default_rng(2)
+    W = T.i8_quantize(T.to_device(rng.standard_normal((260, 1030)).astype(np.float32)))
+    xs = [T.to_device(rng.standard_normal((n, 1032)).astype(np.float32)).view(0, (n, 1030), (1032, 1)) for n in (90, 400)]
+    want = [T.mul_mat(W, x).numpy() for x in xs]
+    st, outs = [T.Stream(), T.Stream()], [T.empty(w.shape) for w in want]
+    T.synchronize()
+    for _ in range(20):
+        for s, x, o in zip(st, xs, outs):
+            T.mul_mat(W, x, out=o, stream=s)
+    for s in st:
+        s.synchronize()
+    for o, w in zip(outs, want):
+        assert np.array_equal(o.numpy(), w)
+    for s in st:
+        s.destroy()

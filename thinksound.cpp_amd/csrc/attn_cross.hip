@@ -209,7 +209,9 @@ __device__ __forceinline__ float *part_ml(const CrossAttn &p, int split, int64_t
 
 // ---------------------------------------------------------------- few rows
 // A workgroup takes 32 rows, its four waves tiles of 32 states in turns, each through a ring
-// of its own in LDS: no barrier until their sums meet. Bound by the states' bytes.
+// of its own in LDS: no barrier until their sums meet. Bound by the states' bytes: one token of
+// 4 sequences of 32 heads to 16384 states of 8 heads of 128, bf16, in 16 ranges: 57.5 us, 4.7 TB/s
+// (a copy 5.1); with the kernel for many rows 62.
 template <int DP, bool BF16>
 __global__ __launch_bounds__(256) void cross_attn_few_kernel(const CrossAttn p, int qtiles) {
     typedef Half<BF16> T;
@@ -424,7 +426,10 @@ __global__ __launch_bounds__(256) void cross_attn_join_kernel(const CrossAttn p,
 // last half's V with P while it turns this half's logits into weights: three steps of three
 // halves without a dependence, so that the matrix unit and the rest of the SIMD work at once.
 // Products, LDS reads, loads and the softmax's operations are in the program's order
-// (sched_barrier).
+// (sched_barrier). 4096 tokens to 8192 states of 16 heads of 128, bf16: 243 us, 1130 TF/s (a
+// library's matrix product of 8192^3 1390); the matrix unit is busy for 52 % of the cycles and
+// the vector unit's exponentials, sums and roundings for most of the others. One half a step, each
+// after the other, took 325 us, a largest logit found before each weight 251.
 template <int DP, bool BF16, int NW>
 __global__ __launch_bounds__(NW * 64) void cross_attn_kernel(const CrossAttn p, int qtiles) {
     typedef Half<BF16> T;
@@ -712,6 +717,18 @@ hipError_t launch_dp(const CrossAttn &p, const CrossAttnPlan &plan, hipStream_t 
 
 }  // namespace
 
+// Rows of a workgroup (32: cross_attn_few_kernel; 128, 256) and ranges of the states, by what
+// each is estimated to take: turns of the workgroups that 256 CUs hold (two a CU of small ones),
+// a turn's fixed part and tiles in us (alone on a CU, or sharing it), and the join of the ranges. The
+// constants were fitted to such pairs (us, bf16; rows x ranges, the rule's first):
+//   B 2, 646 tokens,   77 states, 16 heads of  64: 128 x 1   7.2, 32 x 1  10.2, 256 x 1   8.6
+//   B 1, 4096,       8192,        16 heads of 128: 256 x 1 243.5, 128 x 1 308.9, 256 x 4 333.5
+//   B 1, 4096,       8192,         2 heads of 128: 128 x 4  58.3, 256 x 4  70.9, 128 x 1 149.7
+//   B 1, 300,        3000,         4 heads of 128:  32 x 4  18.4, 128 x 16 20.1, 32 x 1   32.2
+//   B 4, 1000,       1000,         4 heads of 128: 128 x 1  25.3, 32 x 1  29.3, 256 x 1   32.7
+//   B 4, 1,  16384, 32 heads on 8 of 128:           32 x 16 57.5, 128 x 16 61.9, 32 x 1  179.6
+//   B 1, 1,   8192,        16 heads of  64:         32 x 16 13.4, 128 x 16 16.7, 32 x 1   46.3
+// Lengths that are shorter than the states are not known here; then it may be some 20 % off.
 CrossAttnPlan plan_cross_attn(int D, int64_t Nq, int64_t Nkv, int64_t H, int64_t Hkv, int64_t B) {
     CrossAttnPlan c = {128, 1, 0};
     const int64_t R = H / Hkv * Nq;
@@ -736,9 +753,10 @@ CrossAttnPlan plan_cross_attn(int D, int64_t Nq, int64_t Nkv, int64_t H, int64_t
             }
         }
     }
-    if (tuning().cross_cfg) {
-        c.rows = tuning().cross_cfg / 100;
-        c.splits = std::min(tuning().cross_cfg % 100, CROSS_ATTN_SPLITS);
+    const int cfg = tuning().cross_cfg, forced = cfg / 100;
+    if (forced == 32 || forced == 128 || forced == 256) {
+        c.rows = forced;
+        c.splits = std::max(1, std::min(cfg % 100, CROSS_ATTN_SPLITS));
     }
     c.bytes = c.splits > 1 ? (size_t) c.splits * (size_t) (B * H * Nq) * (size_t) (D + 2) * 4 : 0;
     c.bytes = (c.bytes + 255) / 256 * 256;
