@@ -337,3 +337,28 @@ def test_states_that_do_not_count_in_each_shape(T, shape, rows, ranges):  # noqa
     got2 = T.cross_attention(Q, K, to(T, v, "bf16")[0], **kw).numpy()
     assert np.array_equal(got2[0], got[0]) and np.isnan(got2[1, :, 0, 3]).all()
     assert np.array_equal(np.delete(got2[1, :, 0], 3, 1), np.delete(got[1, :, 0], 3, 1))
+
+
+@pytest.mark.parametrize("kv,size", [("bf16", 2.0 ** 8), ("bf16", 2.0 ** 20), ("bf16", 2.0 ** 55), ("f16", 2.0 ** 8), ("f16", 2.0 ** 14)])   # (f16 holds less than 2^16)
+@pytest.mark.parametrize("rows,ranges", SHAPES)
+def test_huge_logits(T, shape, rows, ranges, kv, size):  # noqa: F811
+    """logits of 2^16 to 2^110 of either sign: all equal ones weigh the same (exactly: their products are powers of two), and where
+    one stands above the others it takes all"""
+    shape(rows, ranges)
+    rng = np.random.default_rng(1)
+    n, d = 300, 64
+    v = rng.standard_normal((1, 1, n, d)).astype(np.float32)
+    for sign in (1.0, -1.0):
+        q = np.zeros((1, 1, 40, d), np.float32)
+        q[..., 0] = size * 2.0 ** (np.arange(40) % 4 / 2 // 1)
+        k = np.zeros((1, 1, n, d), np.float32)
+        k[..., 0] = sign * size
+        (Q, _), (K, _), (V, v2) = (to(T, t, kv) for t in (q, k, v))
+        got = T.cross_attention(Q, K, V, scale=0.7).numpy()
+        mean = v2[0, 0].astype(np.float64).mean(0)
+        tol = (2 * U[kv] + 2 * (n + 64) * 2.0 ** -23) * np.abs(v2[0, 0]).mean(0) + 2.0 ** -24 * np.abs(mean)
+        assert np.isfinite(got).all() and (np.abs(got[0, :, 0] - mean) <= tol).all()
+        k[0, 0, 123, 0] *= 2.0 if sign > 0 else 0.5
+        got = T.cross_attention(Q, to(T, k, kv)[0], V, scale=0.7).numpy()
+        # one weight w: w v is exact (8 and 11 bits each), 1 / w and its product with w v round once each: 2 * 2^-24 of v
+        assert (np.abs(got[0, :, 0] - v2[0, 0, 123]) <= 2.0 ** -23 * np.abs(v2[0, 0, 123])).all()

@@ -182,6 +182,12 @@ __device__ __forceinline__ void load_q(const CrossAttn &p, int b, int h, int iq,
         q[ks] = __builtin_bit_cast(typename Half<BF16>::x8, d < p.D ? load_q8<BF16>(row, d, p.q_type) : zero);
     }
 }
+// a rounded product, whatever is added to it
+__device__ __forceinline__ float times(float a, float b) {
+    float v = a * b;
+    asm volatile("" : "+v"(v));
+    return v;
+}
 // 1 / the sum of the weights; 0 where there are none, and a NaN stays
 __device__ __forceinline__ float inverse(float l) { return l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l; }
 // 4 values of an output row from dim d on
@@ -288,7 +294,7 @@ __global__ __launch_bounds__(256) void cross_attn_few_kernel(const CrossAttn p, 
         float top = s[0];
 #pragma unroll
         for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
-        const float m_new = fmaxf(m_run, half_pair_max(top) * c);
+        const float m_new = fmaxf(m_run, times(half_pair_max(top), c));
         const float sub = m_new == -__builtin_inff() ? 0.0f : m_new, alpha = __builtin_amdgcn_exp2f(m_run - sub);
         if (__any(m_new > m_run)) {
             l_run *= alpha;
@@ -301,7 +307,8 @@ __global__ __launch_bounds__(256) void cross_attn_few_kernel(const CrossAttn p, 
         u32x4 pf[2];
 #pragma unroll
         for (int e = 0; e < 16; e += 2) {
-            const uint32_t two = T::pack2(__builtin_amdgcn_exp2f(__builtin_fmaf(s[e], c, -sub)), __builtin_amdgcn_exp2f(__builtin_fmaf(s[e + 1], c, -sub)));
+            // (logits times c are rounded as the maximum was: no weight is above 1)
+            const uint32_t two = T::pack2(__builtin_amdgcn_exp2f(times(s[e], c) - sub), __builtin_amdgcn_exp2f(times(s[e + 1], c) - sub));
             l_run = T::add2(two, l_run);
             pf[e / 8][e % 8 / 2] = two;
         }
@@ -490,7 +497,8 @@ __global__ __launch_bounds__(NW * 64) void cross_attn_kernel(const CrossAttn p, 
     f32x16 o[DP / 32];
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db) o[db] = f32x16{};
-    float m = -1e30f, l = 0.0f;                                  // (any logit is far above it)
+    float m = -3.40282347e38f, l = 0.0f;                         // (below any logit; -inf would be no number less itself)
+    float most = 256.0f;                                         // sum of a half's weights that stay as they are
     const float c = p.c;
     const int l16 = lane & 15, grp = (lane >> 4) & 1, vrow = 4 * hi + (l16 >> 2);
     struct Weights {
@@ -585,7 +593,7 @@ __global__ __launch_bounds__(NW * 64) void cross_attn_kernel(const CrossAttn p, 
     };
     auto weigh = [&](const f32x16 &n, Weights &w) __attribute__((always_inline)) {
         Turns r;
-        EACH(e, 0, 16, turn1(n, r, e); turn2(r, e););
+        EACH(e, 0, 16, r.v[e] = times(n[e], c) - m; turn2(r, e););
         EACH(e, 0, 8, turn3(r, w, 2 * e););
     };
     // states of a half that do not count leave before they are weighed
@@ -600,15 +608,19 @@ __global__ __launch_bounds__(NW * 64) void cross_attn_kernel(const CrossAttn p, 
     };
     // Weights that have grown past 2^8 together (or are not finite): the maximum moves to a whole
     // number (log2 domain), what has been summed shrinks by a power of two, exactly, and they are
-    // worked out again. The sums tell it, so the logits' maximum is looked for only then
+    // worked out again, from logits rounded as the maximum was, which leaves no weight above 1. The
+    // sums tell it, so the logits' maximum is looked for only then. Past 2^22 the steps' unrounded
+    // products with c differ from the rounded maximum by halves and more: there, all are
+    // worked out again
     auto settle = [&](const f32x16 &n, Weights &w) __attribute__((always_inline)) {
-        if (__any(!(w.sum <= 256.0f))) {
+        if (__any(!(w.sum <= most))) {
             float top = n[0];
             asm volatile("" : "+v"(top));
 #pragma unroll
             for (int e = 1; e < 16; ++e) top = fmaxf(top, n[e]);
-            const float to = fmaxf(m, __builtin_ceilf(half_pair_max(top) * c)), f = __builtin_amdgcn_exp2f(m - to);
+            const float to = fmaxf(m, __builtin_ceilf(times(half_pair_max(top), c))), f = __builtin_amdgcn_exp2f(m - to);
             m = to;
+            most = __builtin_fabsf(to) < 0x1p22f ? 256.0f : -1.0f;
             l *= f;
 #pragma unroll
             for (int db = 0; db < DP / 32; ++db) o[db] *= f;
