@@ -219,6 +219,10 @@ def test_cross_attention_refusals(uninit):  # noqa: F811
         assert go(q, bad, v, P(), y) == STRIDE
     assert go(q, k, v, P(), at(fake(T, T.BF16, (B, N, H, D), 2), q.data)) == ARG
     assert go(q, k, v, P(kv_len=at(lens, y.data)), y) == ARG
+    span = B * N * H * D * 4
+    assert go(q, k, v, P(kv_valid=y.data - M - 1, kv_valid_nb=M), y) == ARG            # (the second sequence's flags)
+    assert go(q, k, v, P(kv_valid=y.data + span - 1), y) == ARG
+    assert go(q, k, v, P(kv_valid=y.data - 2 * M, kv_valid_nb=M), y) == NOT_INIT and go(q, k, v, P(kv_valid=y.data + span), y) == NOT_INIT
     rows = at(fake(T, T.F32, (B, N, H, D), 4), 0x3000000)
     rows.nb[2] = 16
     assert go(q, k, v, P(), rows) == STRIDE

@@ -1504,6 +1504,9 @@ int validate_cross(const tsk_tensor *q, const tsk_tensor *k, const tsk_tensor *v
     if (p->kv_valid && p->kv_valid_nb < 0) return fail(TSK_ERR_INVALID_ARG, "kv_valid_nb");
     for (const tsk_tensor *t : {q, k, v, p->kv_len, p->q_len})
         if (t && may_overlap(t, dst)) return fail(TSK_ERR_INVALID_ARG, "dst overlaps an input");
+    const uintptr_t f0 = (uintptr_t) p->kv_valid, f1 = f0 + (size_t) (B - 1) * (size_t) p->kv_valid_nb + (size_t) k->ne[1];
+    if (p->kv_valid && f0 < (uintptr_t) dst->data + span_bytes(dst) && (uintptr_t) dst->data < f1)
+        return fail(TSK_ERR_INVALID_ARG, "dst overlaps kv_valid");
     return TSK_OK;
 }
 
