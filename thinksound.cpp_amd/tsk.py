@@ -10,6 +10,7 @@ TskError with the library's status and message; nothing falls back to a CPU
 path: if libtsk.so is missing, load() raises.
 """
 import ctypes
+import gc
 import os
 
 import numpy as np
@@ -444,16 +445,24 @@ class Stream:
 class Graph:
     """The work a function enqueues on `stream`, captured into a HIP graph
     (hipStreamCaptureModeGlobal: a call that is not allowed under capture,
-    hipMalloc among them, fails the capture) and replayed with launch()."""
+    hipMalloc among them, fails the capture) and replayed with launch().
+    The garbage collector waits meanwhile: an array that it frees would fail
+    the capture too."""
 
     def __init__(self, stream, fn):
         H = hip()
-        _hipcheck(H.hipStreamBeginCapture(stream.h, 0), "hipStreamBeginCapture")
+        collects = gc.isenabled()
+        gc.disable()
         try:
-            fn()
+            _hipcheck(H.hipStreamBeginCapture(stream.h, 0), "hipStreamBeginCapture")
+            try:
+                fn()
+            finally:
+                g = ctypes.c_void_p()
+                rc = H.hipStreamEndCapture(stream.h, ctypes.byref(g))
         finally:
-            g = ctypes.c_void_p()
-            rc = H.hipStreamEndCapture(stream.h, ctypes.byref(g))
+            if collects:
+                gc.enable()
         _hipcheck(rc, "hipStreamEndCapture")
         self.graph = g
         e = ctypes.c_void_p()
