@@ -3,8 +3,8 @@
 // d = max(amax, 2^-100) / 127, q = the integer nearest to x / d (i8.h). Bound by memory:
 // a row is read once into the registers of the threads that share it, whose largest
 // magnitude is found between the load and the store. A vector instruction takes a wave four
-// cycles, so a value's few count: 8192 x 8192 bf16 48.3 us (4.2 TB/s, of a copy's 5.1), f32
-// 59.7 (5.6).
+// cycles, so a value's few count: 8192 x 8192 bf16 37.7 us (5.3 TB/s; a copy 5.1; with magnitudes
+// of 32 bits and i8_code for every value 52.4), f32 60.0 (5.6).
 #include <algorithm>
 
 #include "i8.h"
@@ -29,8 +29,19 @@ __device__ __forceinline__ int64_t row_at(const Rows &t, int64_t r) {
 // the largest of the NT threads of a row: 8 to 64 lanes of a wave, or NT / 64 waves
 template <int NT>
 __device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t *red) {
-    // (magnitudes' bits order like unsigned integers, NaNs on top)
-    for (int m = 1; m < (NT < 64 ? NT : 64); m *= 2) v = max(v, (uint32_t) __shfl_xor((int) v, m));
+    // (magnitudes' bits order like unsigned integers, NaNs on top; DPP: swaps within quads, then mirrors of 8 and 16)
+    v = max(v, (uint32_t) __builtin_amdgcn_update_dpp(0, (int) v, 0xB1, 0xF, 0xF, false));
+    v = max(v, (uint32_t) __builtin_amdgcn_update_dpp(0, (int) v, 0x4E, 0xF, 0xF, false));
+    v = max(v, (uint32_t) __builtin_amdgcn_update_dpp(0, (int) v, 0x141, 0xF, 0xF, false));
+    if constexpr (NT > 8) v = max(v, (uint32_t) __builtin_amdgcn_update_dpp(0, (int) v, 0x140, 0xF, 0xF, false));
+    if constexpr (NT > 16) {
+        const auto s16 = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        v = max(s16[0], s16[1]);
+    }
+    if constexpr (NT > 32) {
+        const auto s32 = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        v = max(s32[0], s32[1]);
+    }
     if constexpr (NT > 64) {
         uint32_t *own = red + threadIdx.x / NT * (NT / 64);
         __syncthreads();                                     // (the row before may still be read)
@@ -43,10 +54,53 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t *red) {
     return v;
 }
 
+// 8 values as they are kept until their row's largest is known: bf16 ones in pairs, whose
+// magnitudes are compared two at a time
+template <bool BF16, bool WIDE> struct Vec8 {
+    float v[8];
+    __device__ __forceinline__ void load(const char *row, int c, int K) { i8_load8<BF16, WIDE>(row, c, K, v); }
+    __device__ __forceinline__ uint32_t top() const {
+        uint32_t t = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) t = max(t, i8_abs_bits(v[e]));
+        return t;
+    }
+    __device__ __forceinline__ void values(float *w) const {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = v[e];
+    }
+};
+typedef __attribute__((__vector_size__(2 * sizeof(uint16_t)))) uint16_t u16x2;
+template <> struct Vec8<true, true> {
+    u32x4 w;
+    __device__ __forceinline__ void load(const char *row, int c, int K) {
+        if (c + 8 <= K) {
+            w = *(const u32x4 *) (row + (int64_t) c * 2);
+            return;
+        }
+        const uint16_t *h = (const uint16_t *) row;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = (c + 2 * e < K ? h[c + 2 * e] : 0u) | (c + 2 * e + 1 < K ? (uint32_t) h[c + 2 * e + 1] << 16 : 0u);
+    }
+    __device__ __forceinline__ uint32_t top() const {
+        u16x2 t = {0, 0};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t = __builtin_elementwise_max(t, __builtin_bit_cast(u16x2, w[e] & 0x7fff7fffu));
+        return (uint32_t) max(t[0], t[1]) << 16;
+    }
+    __device__ __forceinline__ void values(float *v) const {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+    }
+};
+
 // NT threads a row, VN vectors of 8 values each in registers; rows longer than that
 // (LONG) are read a second time. Up to 2048 values a row is a wave's or less, without LDS or
-// barriers (32768 rows of 2000, bf16: 45.5 us, with 256 threads a row 73), and rows of up to
-// 256 have lanes for their own vectors only (100000 of 192: 20.1 us, with 64 lanes each 44.5).
+// barriers (32768 rows of 2000, bf16, on 256 threads each 73 us, on a wave 45.5, and 37.5 with
+// bf16 in pairs), and rows of up to 256 have lanes for their own vectors only (100000 of 192: 44.5
+// us with 64 lanes each, 19.2). Longer ones: 8192 rows of 4096 on 256 threads 21.9, on a wave
+// 26.9; of 5120 on 256 threads 31.7, on 512 41.4; 8192 bf16 ones of 8192 on 256 threads 37.7, on 512
+// 41.3, but 8 of them 4.3 and 3.6, and f32 ones 61.0 and 60.0.
 template <bool BF16, bool WIDE, int VN, int NT, bool LONG>
 __global__ __launch_bounds__(NT < 256 ? 256 : NT) void i8_quantize_kernel(const void *x, const Rows t, int64_t rows, int K, int64_t ld,
                                                                           int8_t *q, float *d) {
@@ -57,31 +111,30 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void i8_quantize_kernel(const 
         const bool mine = r0 + threadIdx.x / NT < rows;
         const int64_t r = mine ? r0 + threadIdx.x / NT : rows - 1;
         const char *row = (const char *) x + row_at(t, r);
-        float v[VN][8];
+        Vec8<BF16, WIDE> v[VN];
         uint32_t top = 0;
         if constexpr (LONG) {
             for (int c = th * 8; c < K; c += NT * 8) {
-                i8_load8<BF16, WIDE>(row, c, K, v[0]);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) top = max(top, i8_abs_bits(v[0][e]));
+                v[0].load(row, c, K);
+                top = max(top, v[0].top());
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < VN; ++j) i8_load8<BF16, WIDE>(row, (th + NT * j) * 8, K, v[j]);
+            for (int j = 0; j < VN; ++j) v[j].load(row, (th + NT * j) * 8, K);
 #pragma unroll
-            for (int j = 0; j < VN; ++j)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) top = max(top, i8_abs_bits(v[j][e]));
+            for (int j = 0; j < VN; ++j) top = max(top, v[j].top());
         }
         top = row_max<NT>(top, red);
         const I8Scale s = i8_scale(top);
         if (!mine) continue;
-        auto store = [&](int c, const float *w) {
+        auto store = [&](int c, const Vec8<BF16, WIDE> &x) {
+            float w[8];
+            x.values(w);
             if (c < ld) *(u32x2 *) (q + r * ld + c) = u32x2{i8_pack4(w, s), i8_pack4(w + 4, s)};
         };
         if constexpr (LONG) {
             for (int c = th * 8; c < ld; c += NT * 8) {
-                i8_load8<BF16, WIDE>(row, c, K, v[0]);
+                v[0].load(row, c, K);
                 store(c, v[0]);
             }
         } else {
@@ -107,6 +160,8 @@ hipError_t launch_quantize(const void *x, const Rows &t, int64_t rows, int K, in
     if (ld <= 64 * 16) return go(i8_quantize_kernel<BF16, WIDE, 2, 64, false>, 64);
     if (ld <= 64 * 32) return go(i8_quantize_kernel<BF16, WIDE, 4, 64, false>, 64);
     if (ld <= 256 * 16) return go(i8_quantize_kernel<BF16, WIDE, 2, 256, false>, 256);
+    if (ld <= 256 * 24) return go(i8_quantize_kernel<BF16, WIDE, 3, 256, false>, 256);
+    if (BF16 && ld <= 256 * 32 && rows > 256) return go(i8_quantize_kernel<BF16, WIDE, 4, 256, false>, 256);
     if (ld <= 512 * 16) return go(i8_quantize_kernel<BF16, WIDE, 2, 512, false>, 512);
     if (ld <= 1024 * 16) return go(i8_quantize_kernel<BF16, WIDE, 2, 1024, false>, 1024);
     return go(i8_quantize_kernel<BF16, WIDE, 1, 1024, true>, 1024);
