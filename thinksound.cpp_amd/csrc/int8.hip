@@ -6,6 +6,7 @@
 // cycles, so a value's few count: 8192 x 8192 bf16 37.7 us (5.3 TB/s; a copy 5.1; with magnitudes
 // of 32 bits and i8_code for every value 52.4), f32 60.0 (5.6).
 #include <algorithm>
+#include <type_traits>
 
 #include "i8.h"
 #include "tsk_internal.h"
@@ -71,11 +72,12 @@ template <bool BF16, bool WIDE> struct Vec8 {
     }
 };
 typedef __attribute__((__vector_size__(2 * sizeof(uint16_t)))) uint16_t u16x2;
-template <> struct Vec8<true, true> {
+template <bool WIDE> struct Vec8<true, WIDE> {
     u32x4 w;
     __device__ __forceinline__ void load(const char *row, int c, int K) {
         if (c + 8 <= K) {
-            w = *(const u32x4 *) (row + (int64_t) c * 2);
+            if constexpr (WIDE) w = *(const u32x4 *) (row + (int64_t) c * 2);
+            else w = *(const u32x4_any2 *) (row + (int64_t) c * 2);
             return;
         }
         const uint16_t *h = (const uint16_t *) row;
@@ -167,13 +169,11 @@ hipError_t launch_quantize(const void *x, const Rows &t, int64_t rows, int K, in
     return go(i8_quantize_kernel<BF16, WIDE, 1, 1024, true>, 1024);
 }
 
-// A thread takes V values, and others a grid of threads on: step_r rows and step_c times V
-// values, P times V a row. (8192 x 8192 to f32 60.7 us, with 4 values a thread 64.4; 1000 rows of
-// 20001 with 8 57.9, with 4 38.5.)
+// A thread takes 8 values, and others a grid of threads on: step_r rows and step_c times 8
+// values, P times 8 a row.
 template <bool BF16, bool WIDE>
 __global__ void i8_dequantize_kernel(const int8_t *q, const float *d, int64_t rows, int K, int P, int64_t step_r, int step_c, void *y,
                                      const Rows t) {
-    constexpr int V = WIDE ? 8 : 4;
     const int64_t ld = i8_ld(K);
     const unsigned first = blockIdx.x * blockDim.x + threadIdx.x;
     int p = (int) (first % (unsigned) P);
@@ -182,32 +182,28 @@ __global__ void i8_dequantize_kernel(const int8_t *q, const float *d, int64_t ro
             p -= P;
             if (++r >= rows) break;
         }
-        const int c = p * V;
-        const char *codes = (const char *) q + r * ld + c;
-        uint32_t w[V / 4];
-        if constexpr (V == 8) {
-            const u32x2 two = *(const u32x2 *) codes;
-            w[0] = two[0];
-            w[1] = two[1];
-        } else w[0] = *(const uint32_t *) codes;
+        const int c = p * 8;
+        const u32x2 w = *(const u32x2 *) (q + r * ld + c);
         const float s = d[r];
-        float v[V];
+        float v[8];
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[e] = s * (float) (int8_t) (w[e >> 2] >> 8 * (e & 3));
+        for (int e = 0; e < 8; ++e) v[e] = s * (float) (int8_t) (w[e >> 2] >> 8 * (e & 3));
         char *row = (char *) y + row_at(t, r);
-        if constexpr (WIDE) {
-            if (c + V <= K) {
-                if constexpr (BF16) *(bf16x8 *) (row + (int64_t) c * 2) = bf16x8{(__bf16) v[0], (__bf16) v[1], (__bf16) v[2], (__bf16) v[3],
-                                                                                 (__bf16) v[4], (__bf16) v[5], (__bf16) v[6], (__bf16) v[7]};
-                else {
-                    ((f32x4 *) (row + (int64_t) c * 4))[0] = f32x4{v[0], v[1], v[2], v[3]};
-                    ((f32x4 *) (row + (int64_t) c * 4))[1] = f32x4{v[4], v[5], v[6], v[7]};
-                }
-                continue;
+        if (c + 8 <= K) {
+            if constexpr (BF16) {
+                const bf16x8 h = {(__bf16) v[0], (__bf16) v[1], (__bf16) v[2], (__bf16) v[3], (__bf16) v[4], (__bf16) v[5], (__bf16) v[6], (__bf16) v[7]};
+                if constexpr (WIDE) *(bf16x8 *) (row + (int64_t) c * 2) = h;
+                else *(u32x4_any2 *) (row + (int64_t) c * 2) = __builtin_bit_cast(u32x4, h);
+            } else {
+                const f32x4 a = {v[0], v[1], v[2], v[3]}, b = {v[4], v[5], v[6], v[7]};
+                typedef typename std::conditional<WIDE, f32x4, f32x4_any4>::type T;
+                ((T *) (row + (int64_t) c * 4))[0] = a;
+                ((T *) (row + (int64_t) c * 4))[1] = b;
             }
+            continue;
         }
 #pragma unroll
-        for (int e = 0; e < V; ++e)
+        for (int e = 0; e < 8; ++e)
             if (c + e < K) store_from_f32<BF16 ? Elt::BF16 : Elt::F32>(row, c + e, v[e]);
     }
 }
@@ -240,7 +236,7 @@ hipError_t launch_i8_quantize(const View4 &x, int8_t *q, float *d, hipStream_t s
 hipError_t launch_i8_dequantize(const int8_t *q, const float *d, const View4 &y, hipStream_t s) {
     const int64_t rows = y.ne[1] * y.ne[2] * y.ne[3];
     const bool bf16 = y.type == TSK_TYPE_BF16, wide = on_16(y);
-    const int K = (int) y.ne[0], P = wide ? (K + 7) / 8 : (K + 3) / 4;
+    const int K = (int) y.ne[0], P = (K + 7) / 8;
     const int64_t threads = std::min<int64_t>((rows * P + 255) / 256, 1 << 20) * 256;
     launch_kernel(bf16 ? wide ? i8_dequantize_kernel<true, true> : i8_dequantize_kernel<true, false>
                        : wide ? i8_dequantize_kernel<false, true> : i8_dequantize_kernel<false, false>,
