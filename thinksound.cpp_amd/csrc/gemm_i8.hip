@@ -4,7 +4,7 @@
 //   Y[n, m] = (sum_k XQ[n, k] WQ[m, k]) * XD[n] * WD[m] + bias[m].
 //
 // Sums are int32 and exact (K below 2^17: 2^14 K stays below 2^31); they are
-// rounded once to fp32, then scaled. v_mfma_i32_16x16x64_i8 multiplies.
+// rounded once to fp32, then scaled (few rows: v_mfma_i32_16x16x64_i8, tiles: v_mfma_i32_32x32x32_i8).
 #include <algorithm>
 #include <cmath>
 #include <utility>
