@@ -41,7 +41,7 @@ __device__ __forceinline__ s16x4 read_turned(const uint16_t *p) { return __built
 template <int DP> __device__ __forceinline__ int k_key(int row) { return DP == 128 ? row & 15 : row >> 1 & 7; }
 template <int DP> __device__ __forceinline__ int v_key(int row) { return (DP == 128 ? 4 : 2) * (row & 3); }
 
-// 16 bytes a lane from base + off (the lane's) + at into LDS at byte dst + 16 * lane; zeros past
+// 16 bytes a lane from base + off (the lane's) + at into LDS at byte dst + 16 * lane; zeros where off + at (it does not wrap) passes
 // `bytes`. In assembly, since the compiler waits for every load into LDS before a transposing
 // read, whose address it does not see; it has no result register, and the waits for it are
 // written out where its bytes are read.
