@@ -362,3 +362,11 @@ def test_huge_logits(T, shape, rows, ranges, kv, size):  # noqa: F811
         got = T.cross_attention(Q, to(T, k, kv)[0], V, scale=0.7).numpy()
         # one weight w: w v is exact (8 and 11 bits each), 1 / w and its product with w v round once each: 2 * 2^-24 of v
         assert (np.abs(got[0, :, 0] - v2[0, 0, 123]) <= 2.0 ** -23 * np.abs(v2[0, 0, 123])).all()
+
+
+def test_flags_of_another_kind_are_refused(T):  # noqa: F811
+    rng = np.random.default_rng(0)
+    q, k = (to(T, rng.standard_normal((2, 1, n, 64)), "bf16")[0] for n in (3, 9))
+    for flags in (np.ones((2, 9), np.float32), np.ones((2, 8), np.uint8), np.ones((1, 9), np.uint8)):
+        with pytest.raises(ValueError):
+            T.cross_attention(q, k, k, kv_valid=T.to_device(flags))

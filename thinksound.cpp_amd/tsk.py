@@ -794,6 +794,8 @@ def cross_attention(q, k, v, scale=None, kv_len=None, q_len=None, kv_valid=None,
     if kv_valid is not None:
         if tuple(kv_valid.shape) not in ((B, k.shape[2]), (k.shape[2],)) or kv_valid.stride(-1) != 1:
             raise ValueError("kv_valid of %s for k of %s" % (tuple(kv_valid.shape), tuple(k.shape)))
+        if kv_valid.element_size() != 1:
+            raise ValueError("kv_valid of %s: a byte a state" % kv_valid.dtype)
         p.kv_valid, p.kv_valid_nb = kv_valid.data_ptr(), kv_valid.stride(0) if len(kv_valid.shape) == 2 else 0
     dq, dk, dv, dd = desc(q), desc(k), desc(v), desc(out)
     check(load().tsk_cross_attention(ctypes.byref(dq), ctypes.byref(dk), ctypes.byref(dv), ctypes.byref(p), ctypes.byref(dd),
