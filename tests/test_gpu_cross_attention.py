@@ -278,7 +278,7 @@ def shape(T, monkeypatch):  # noqa: F811
 SHAPES = [(r, n) for r in (32, 128, 256) for n in (1, 2, 16, 64)]
 
 
-@pytest.mark.parametrize("D", [40, 64, 96, 128])
+@pytest.mark.parametrize("D", [24, 32, 40, 64, 72, 96, 104, 128])
 @pytest.mark.parametrize("rows,ranges", SHAPES)
 def test_each_shape(T, shape, rows, ranges, D):  # noqa: F811
     """shared heads whose number is no multiple of 8, few heads, ragged rows and tiles, lengths that leave ranges empty"""

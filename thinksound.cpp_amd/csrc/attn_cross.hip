@@ -38,6 +38,10 @@ __device__ __forceinline__ s16x4 read_turned(const uint16_t *p) { return __built
 // Piece c (16 bytes) of row t of a tile in LDS lies at slot c ^ key(t). K: a 16-byte read of a wave
 // takes one piece of 32 rows in turns of 16 lanes (0-3, 12-15, 20-27; 4-11, 16-19, 28-31; ...): the
 // keys send those to 16 places. V: the four rows of a transposing read, 64 bytes each
+// Values of a state's row in LDS (64 or 128, which the keys below need), of which the first DQ, D
+// rounded up to 32, are multiplied: 4096 tokens to 8192 states of 16 heads of 72 195 us (all 128
+// 219), of 96 208 (231), of 32 127 (64: 136)
+constexpr int row_of_lds(int DQ) { return DQ <= 64 ? 64 : 128; }
 template <int DP> __device__ __forceinline__ int k_key(int row) { return DP == 128 ? row & 15 : row >> 1 & 7; }
 template <int DP> __device__ __forceinline__ int v_key(int row) { return (DP == 128 ? 4 : 2) * (row & 3); }
 
@@ -172,11 +176,11 @@ __device__ __forceinline__ void row_of(const CrossAttn &p, int hk, int64_t r, in
     h = hk * (p.H / p.Hkv) + g;
     iq = (int) (r - (int64_t) g * p.Nq);
 }
-template <int DP, bool BF16>
-__device__ __forceinline__ void load_q(const CrossAttn &p, int b, int h, int iq, int hi, typename Half<BF16>::x8 (&q)[DP / 16]) {
+template <int DQ, bool BF16>
+__device__ __forceinline__ void load_q(const CrossAttn &p, int b, int h, int iq, int hi, typename Half<BF16>::x8 (&q)[DQ / 16]) {
     const char *row = (const char *) p.q + iq * p.q_nb1 + h * p.q_nb2 + b * p.q_nb3;
 #pragma unroll
-    for (int ks = 0; ks < DP / 16; ++ks) {
+    for (int ks = 0; ks < DQ / 16; ++ks) {
         const int d = 16 * ks + 8 * hi;
         const u32x4 zero = {0, 0, 0, 0};
         q[ks] = __builtin_bit_cast(typename Half<BF16>::x8, d < p.D ? load_q8<BF16>(row, d, p.q_type) : zero);
@@ -218,11 +222,11 @@ __device__ __forceinline__ float *part_ml(const CrossAttn &p, int split, int64_t
 // of its own in LDS: no barrier until their sums meet. Bound by the states' bytes: one token of
 // 4 sequences of 32 heads to 16384 states of 8 heads of 128, bf16, in 16 ranges: 57.5 us, 4.7 TB/s
 // (a copy 5.1); with the kernel for many rows 62.
-template <int DP, bool BF16>
+template <int DQ, bool BF16>
 __global__ __launch_bounds__(256) void cross_attn_few_kernel(const CrossAttn p, int qtiles) {
     typedef Half<BF16> T;
     typedef typename T::x8 x8;
-    constexpr int KT = 32, CH = DP / 8, RL = 64 / CH, NL = KT / RL, TILE = KT * DP, NB = 2;
+    constexpr int DP = row_of_lds(DQ), KT = 32, CH = DP / 8, RL = 64 / CH, NL = KT / RL, TILE = KT * DP, NB = 2;
     constexpr int FAR = (int) 0x80000000u, OS = DP + 4;
     extern __shared__ __attribute__((aligned(1024))) uint16_t lds[];           // [wave][NB][K tile, V tile]
     __shared__ float mls[4][2][32];
@@ -253,11 +257,11 @@ __global__ __launch_bounds__(256) void cross_attn_few_kernel(const CrossAttn p, 
     };
     const int first = u.tile0 + wave;
     if (first < u.tile1) issue(first, 0);
-    x8 q[DP / 16];
-    load_q<DP, BF16>(p, u.b, h, iq, hi, q);
-    f32x16 o[DP / 32];
+    x8 q[DQ / 16];
+    load_q<DQ, BF16>(p, u.b, h, iq, hi, q);
+    f32x16 o[DQ / 32];
 #pragma unroll
-    for (int db = 0; db < DP / 32; ++db)
+    for (int db = 0; db < DQ / 32; ++db)
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[db][e] = 0.0f;
     float m_run = -__builtin_inff(), l_run = 0.0f;
@@ -284,7 +288,7 @@ __global__ __launch_bounds__(256) void cross_attn_few_kernel(const CrossAttn p, 
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[e] = 0.0f;
 #pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks) s = T::mfma(*(const x8 *) (kb + l32 * DP + (((2 * ks + hi) ^ k_key<DP>(l32)) << 3)), q[ks], s);
+        for (int ks = 0; ks < DQ / 16; ++ks) s = T::mfma(*(const x8 *) (kb + l32 * DP + (((2 * ks + hi) ^ k_key<DP>(l32)) << 3)), q[ks], s);
         if (count != ~0u) {
             const uint32_t mine = count >> 4 * hi;
 #pragma unroll
@@ -299,7 +303,7 @@ __global__ __launch_bounds__(256) void cross_attn_few_kernel(const CrossAttn p, 
         if (__any(m_new > m_run)) {
             l_run *= alpha;
 #pragma unroll
-            for (int db = 0; db < DP / 32; ++db)
+            for (int db = 0; db < DQ / 32; ++db)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) o[db][e] *= alpha;
         }
@@ -315,7 +319,7 @@ __global__ __launch_bounds__(256) void cross_attn_few_kernel(const CrossAttn p, 
 #pragma unroll
         for (int kg = 0; kg < 2; ++kg)
 #pragma unroll
-            for (int db = 0; db < DP / 32; ++db) {
+            for (int db = 0; db < DQ / 32; ++db) {
                 const int ch = 4 * db + 2 * grp + ((l16 & 3) >> 1);
                 const uint16_t *at = vb + (16 * kg + vrow) * DP + ((ch ^ v_key<DP>(l16 >> 2)) << 3) + 4 * (l16 & 1);
                 const s16x4 a = read_turned(at), a2 = read_turned(at + 8 * DP);
@@ -338,7 +342,7 @@ __global__ __launch_bounds__(256) void cross_attn_few_kernel(const CrossAttn p, 
     for (int w = 1; w < 4; ++w) m = fmaxf(m, mls[w][0][l32]);
     const float f = __builtin_amdgcn_exp2f(m_run - (m == -__builtin_inff() ? 0.0f : m));
 #pragma unroll
-    for (int db = 0; db < DP / 32; ++db)
+    for (int db = 0; db < DQ / 32; ++db)
 #pragma unroll
         for (int e = 0; e < 16; e += 4)
             *(f32x4 *) (os + (wave * 32 + l32) * OS + 32 * db + 2 * e + 4 * hi) = f32x4{o[db][e], o[db][e + 1], o[db][e + 2], o[db][e + 3]} * f;
@@ -437,11 +441,11 @@ __global__ __launch_bounds__(256) void cross_attn_join_kernel(const CrossAttn p,
 // library's matrix product of 8192^3 1390); the matrix unit is busy for 52 % of the cycles and
 // the vector unit's exponentials, sums and roundings for most of the others. One half a step, each
 // after the other, took 325 us, a largest logit found before each weight 251.
-template <int DP, bool BF16, int NW>
+template <int DQ, bool BF16, int NW>
 __global__ __launch_bounds__(NW * 64) void cross_attn_kernel(const CrossAttn p, int qtiles) {
     typedef Half<BF16> T;
     typedef typename T::x8 x8;
-    constexpr int KT = 64, CH = DP / 8, RL = 64 / CH, NL = KT / RL / NW, TILE = KT * DP;     // 16-byte pieces a row, rows a load, loads a wave
+    constexpr int DP = row_of_lds(DQ), KT = 64, CH = DP / 8, RL = 64 / CH, NL = KT / RL / NW, TILE = KT * DP;     // 16-byte pieces a row, rows a load, loads a wave
     constexpr int FAR = (int) 0x80000000u;
     extern __shared__ __attribute__((aligned(1024))) uint16_t lds[];           // [4][K tile, V tile]
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -451,8 +455,8 @@ __global__ __launch_bounds__(NW * 64) void cross_attn_kernel(const CrossAttn p, 
     const int64_t row = u.r0 + wave * 32 + l32;
     int h, iq;
     row_of(p, u.hk, std::min<int64_t>(row, u.R - 1), h, iq);
-    x8 q[DP / 16];
-    load_q<DP, BF16>(p, u.b, h, iq, hi, q);
+    x8 q[DQ / 16];
+    load_q<DQ, BF16>(p, u.b, h, iq, hi, q);
     const char *kp = (const char *) p.k + u.hk * p.k_nb2 + u.b * p.k_nb3, *vp = (const char *) p.v + u.hk * p.v_nb2 + u.b * p.v_nb3;
     const uint8_t *flags = p.kv_valid ? p.kv_valid + u.b * p.kv_valid_nb : nullptr;
     // (a wave's loads are NW * RL rows apart, which the keys do not see)
@@ -494,9 +498,9 @@ __global__ __launch_bounds__(NW * 64) void cross_attn_kernel(const CrossAttn p, 
             for (int i = 0; i < CH / NW; ++i) *(u32x4 *) (lds + s * 2 * TILE + TILE + r * DP + (tid % NW * (CH / NW) + i) * 8) = u32x4{0, 0, 0, 0};
         __syncthreads();
     };
-    f32x16 o[DP / 32];
+    f32x16 o[DQ / 32];
 #pragma unroll
-    for (int db = 0; db < DP / 32; ++db) o[db] = f32x16{};
+    for (int db = 0; db < DQ / 32; ++db) o[db] = f32x16{};
     float m = -3.40282347e38f, l = 0.0f;                         // (below any logit; -inf would be no number less itself)
     float most = 256.0f;                                         // sum of a half's weights that stay as they are
     const float c = p.c;
@@ -507,7 +511,7 @@ __global__ __launch_bounds__(NW * 64) void cross_attn_kernel(const CrossAttn p, 
     };
     // A step's operands in LDS, K's of one half of a tile and V's of another, in the order of
     // their products: two of K, one of V, ..., what is left of V; each read AHEAD products early
-    constexpr int NK = DP / 16, NF = 2 * NK, AHEAD = 4, SLOTS = AHEAD + 1;
+    constexpr int NK = DQ / 16, NF = 2 * NK, AHEAD = 4, SLOTS = AHEAD + 1;
     struct Pieces {
         x8 f[SLOTS];
     };
@@ -516,7 +520,7 @@ __global__ __launch_bounds__(NW * 64) void cross_attn_kernel(const CrossAttn p, 
         if (piece_of_k(NK, f)) {
             x.f[f % SLOTS] = *(const x8 *) (kb + l32 * DP + (((2 * j + hi) ^ k_key<DP>(l32)) << 3));
         } else {
-            const int kg = j / (DP / 32), db = j % (DP / 32), ch = 4 * db + 2 * grp + ((l16 & 3) >> 1);
+            const int kg = j / (DQ / 32), db = j % (DQ / 32), ch = 4 * db + 2 * grp + ((l16 & 3) >> 1);
             const uint16_t *at = vb + (16 * kg + vrow) * DP + ((ch ^ v_key<DP>(l16 >> 2)) << 3) + 4 * (l16 & 1);
             const s16x4 a = read_turned(at), a2 = read_turned(at + 8 * DP);
             const s16x8 a8 = {a[0], a[1], a[2], a[3], a2[0], a2[1], a2[2], a2[3]};
@@ -547,7 +551,7 @@ __global__ __launch_bounds__(NW * 64) void cross_attn_kernel(const CrossAttn p, 
         w.sum = sum;
         w.w[e / 8][e % 8 / 2] = two;
     };
-    constexpr int PER = 16 / NF;                                 // logits between two products
+    constexpr int PER = (16 + NF - 1) / NF;                      // logits between two products
     auto first_turns = [&](const f32x16 &n, Turns &r) __attribute__((always_inline)) {
         EACH(e, 0, 2 * PER, turn1(n, r, e););
         EACH(e, 0, PER, turn2(r, e););
@@ -565,13 +569,13 @@ __global__ __launch_bounds__(NW * 64) void cross_attn_kernel(const CrossAttn p, 
         EACH(f, 0, NF,
             constexpr int J = piece_index(NK, f);
             if constexpr (piece_of_k(NK, f)) next = T::mfma(x.f[f % SLOTS], q[J], J == 0 ? f32x16{} : next);
-            else o[J % (DP / 32)] = T::mfma(x.f[f % SLOTS], __builtin_bit_cast(x8, before.w[J / (DP / 32)]), o[J % (DP / 32)]);
+            else o[J % (DQ / 32)] = T::mfma(x.f[f % SLOTS], __builtin_bit_cast(x8, before.w[J / (DQ / 32)]), o[J % (DQ / 32)]);
             if constexpr (f + AHEAD < NF) read_piece(kb, vb, f + AHEAD, x);
             EACH(i, f * L1 / NF, (f + 1) * L1 / NF, issue_one(src, to, L0 + i););
             EACH(i, 0, PER,
                 if constexpr ((f + 2) * PER + i < 16) turn1(now, r, (f + 2) * PER + i);
                 if constexpr ((f + 1) * PER + i < 16) turn2(r, (f + 1) * PER + i);
-                if constexpr ((f * PER + i) % 2) turn3(r, w, f * PER + i - 1););
+                if constexpr ((f * PER + i) % 2 && f * PER + i < 16) turn3(r, w, f * PER + i - 1););
             __builtin_amdgcn_sched_barrier(0););
     };
     // the same alone, before the first step and after the last
@@ -588,7 +592,7 @@ __global__ __launch_bounds__(NW * 64) void cross_attn_kernel(const CrossAttn p, 
             constexpr int J = piece_index(NK, f);
             Pieces x;
             read_piece(vb, vb, f, x);
-            o[J % (DP / 32)] = T::mfma(x.f[f % SLOTS], __builtin_bit_cast(x8, w.w[J / (DP / 32)]), o[J % (DP / 32)]);
+            o[J % (DQ / 32)] = T::mfma(x.f[f % SLOTS], __builtin_bit_cast(x8, w.w[J / (DQ / 32)]), o[J % (DQ / 32)]);
         });
     };
     auto weigh = [&](const f32x16 &n, Weights &w) __attribute__((always_inline)) {
@@ -623,7 +627,7 @@ __global__ __launch_bounds__(NW * 64) void cross_attn_kernel(const CrossAttn p, 
             most = __builtin_fabsf(to) < 0x1p22f ? 256.0f : -1.0f;
             l *= f;
 #pragma unroll
-            for (int db = 0; db < DP / 32; ++db) o[db] *= f;
+            for (int db = 0; db < DQ / 32; ++db) o[db] *= f;
             weigh(n, w);
         }
         l += w.sum;
@@ -689,7 +693,7 @@ __global__ __launch_bounds__(NW * 64) void cross_attn_kernel(const CrossAttn p, 
         ml[1] = la;
     }
 #pragma unroll
-    for (int db = 0; db < DP / 32; ++db)
+    for (int db = 0; db < DQ / 32; ++db)
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
             const int d = 32 * db + 2 * e + 4 * hi;
@@ -710,12 +714,13 @@ hipError_t launch_units(F kern, const CrossAttn &p, int rows, int threads, size_
     return hipGetLastError();
 }
 
-template <int DP, bool BF16>
+template <int DQ, bool BF16>
 hipError_t launch_dp(const CrossAttn &p, const CrossAttnPlan &plan, hipStream_t s) {
+    constexpr int DP = row_of_lds(DQ);
     hipError_t e;
-    if (plan.rows == 32) e = launch_units(cross_attn_few_kernel<DP, BF16>, p, 32, 256, 4 * 2 * 2 * 32 * DP * 2, s);
-    else if (plan.rows == 128) e = launch_units(cross_attn_kernel<DP, BF16, 4>, p, 128, 256, 4 * 2 * 64 * DP * 2, s);
-    else e = launch_units(cross_attn_kernel<DP, BF16, 8>, p, 256, 512, 4 * 2 * 64 * DP * 2, s);
+    if (plan.rows == 32) e = launch_units(cross_attn_few_kernel<DQ, BF16>, p, 32, 256, 4 * 2 * 2 * 32 * DP * 2, s);
+    else if (plan.rows == 128) e = launch_units(cross_attn_kernel<DQ, BF16, 4>, p, 128, 256, 4 * 2 * 64 * DP * 2, s);
+    else e = launch_units(cross_attn_kernel<DQ, BF16, 8>, p, 256, 512, 4 * 2 * 64 * DP * 2, s);
     if (e != hipSuccess || p.splits == 1) return e;
     constexpr int NG = 256 / (DP / 4);
     int G = 1;
@@ -776,8 +781,14 @@ CrossAttnPlan plan_cross_attn(int D, int64_t Nq, int64_t Nkv, int64_t H, int64_t
 }
 
 hipError_t launch_cross_attn(const CrossAttn &p, const CrossAttnPlan &plan, hipStream_t s) {
-    if (p.D <= 64) return p.kv_bf16 ? launch_dp<64, true>(p, plan, s) : launch_dp<64, false>(p, plan, s);
-    return p.kv_bf16 ? launch_dp<128, true>(p, plan, s) : launch_dp<128, false>(p, plan, s);
+    auto go = [&](auto bf16) {
+        constexpr bool BF16 = decltype(bf16)::value;
+        if (p.D <= 32) return launch_dp<32, BF16>(p, plan, s);
+        if (p.D <= 64) return launch_dp<64, BF16>(p, plan, s);
+        if (p.D <= 96) return launch_dp<96, BF16>(p, plan, s);
+        return launch_dp<128, BF16>(p, plan, s);
+    };
+    return p.kv_bf16 ? go(std::true_type()) : go(std::false_type());
 }
 
 }  // namespace tsk
