@@ -315,3 +315,23 @@ def test_two_streams(T):
         assert np.array_equal(o.numpy(), w)
     for s in st:
         s.destroy()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,k", [(70, 40), (30, 500), (20, 1500), (9, 2048), (15, 6001), (300, 8185), (300, 8192), (5, 8000), (1030, 24)])
+def test_rows_of_each_width(T, dtype, rows, k):
+    """rows of every number of threads, few and many, on 16 bytes and not"""
+    x = typed(hard_rows(np.random.default_rng(rows + k), rows, k), dtype)
+    for first in (0, 1):                                       # (1: every row starts off 16 bytes)
+        ld = (k + 7) // 8 * 8 + 8
+        pad = np.full((rows, ld), 1e30, np.float32)
+        pad[:, first:first + k] = x
+        P = dev(T, pad, dtype)
+        sp = T.i8_quantize(P.view(first, (rows, k), P.strides))
+        check_planes(sp, x, k)
+        q, d = crossref.i8_quantize(x)
+        out = dev(T, np.full((rows, ld), 7.0, np.float32), dtype)
+        T.i8_dequantize(sp, out=out.view(first, (rows, k), out.strides))
+        got = host(out)
+        assert np.array_equal(got[:, first:first + k], typed(q.astype(np.float32) * d[:, None], dtype), equal_nan=True)
+        assert (got[:, :first] == 7.0).all() and (got[:, first + k:] == 7.0).all()

@@ -148,3 +148,14 @@ def test_replayed_from_a_graph(T):  # noqa: F811
         assert np.array_equal(out.numpy(), want[i])
     g.destroy()
     st.destroy()
+
+
+@pytest.mark.parametrize("b,s,h", [(1, 2100, 70), (1, 9001, 3), (300, 10, 2), (1, 40, 200)])
+@pytest.mark.parametrize("d,dims", [(64, (40, 24)), (65, (64,)), (20, (8, 6))])
+@pytest.mark.parametrize("halves", [False, True])
+def test_many(T, b, s, h, d, dims, halves):  # noqa: F811
+    """more heads than are in flight at once, more tokens and sequences than waves, heads of a token over several waves"""
+    rng = np.random.default_rng(h)
+    x = rng.standard_normal((b, s, h, d)).astype(np.float32)
+    w = (1 + 0.1 * rng.standard_normal(d)).astype(np.float32)
+    check(T, x, rng.integers(0, 3000, (b, len(dims), s)).astype(np.int32), dims, halves, w=w, dtype="bf16" if s > 2000 else "f32")
