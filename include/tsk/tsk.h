@@ -384,7 +384,7 @@ typedef struct tsk_cross_attn_params {
  * D is a multiple of 8, at most 128; rows are contiguous on 16-byte starts, and their
  * strides any (k and v: at most 2^24 bytes from a state to the next). A token that no
  * state counts for gets 0; what the states that do not count hold, infinities and NaNs
- * too, has no effect. Tokens from q_len on are not written.
+ * too, has no effect. Tokens from q_len on are neither read nor written.
  * Products are exact and logits, softmax and sums fp32; the weights are rounded to k's
  * type before they multiply v (bf16: within 2^-8, f16: 2^-11) and are divided by
  * the sum of what they were rounded to. dst must not overlap an input. Scratch: long

@@ -176,14 +176,15 @@ __device__ __forceinline__ void row_of(const CrossAttn &p, int hk, int64_t r, in
     h = hk * (p.H / p.Hkv) + g;
     iq = (int) (r - (int64_t) g * p.Nq);
 }
+// (tokens past the sequence's last may hold anything, and a wave's rows decide together when their maxima move: they are zeros)
 template <int DQ, bool BF16>
-__device__ __forceinline__ void load_q(const CrossAttn &p, int b, int h, int iq, int hi, typename Half<BF16>::x8 (&q)[DQ / 16]) {
-    const char *row = (const char *) p.q + iq * p.q_nb1 + h * p.q_nb2 + b * p.q_nb3;
+__device__ __forceinline__ void load_q(const CrossAttn &p, const Unit &u, int h, int iq, int hi, typename Half<BF16>::x8 (&q)[DQ / 16]) {
+    const char *row = (const char *) p.q + iq * p.q_nb1 + h * p.q_nb2 + u.b * p.q_nb3;
 #pragma unroll
     for (int ks = 0; ks < DQ / 16; ++ks) {
         const int d = 16 * ks + 8 * hi;
         const u32x4 zero = {0, 0, 0, 0};
-        q[ks] = __builtin_bit_cast(typename Half<BF16>::x8, d < p.D ? load_q8<BF16>(row, d, p.q_type) : zero);
+        q[ks] = __builtin_bit_cast(typename Half<BF16>::x8, iq < u.nq && d < p.D ? load_q8<BF16>(row, d, p.q_type) : zero);
     }
 }
 // a rounded product, whatever is added to it
@@ -258,7 +259,7 @@ __global__ __launch_bounds__(256) void cross_attn_few_kernel(const CrossAttn p, 
     const int first = u.tile0 + wave;
     if (first < u.tile1) issue(first, 0);
     x8 q[DQ / 16];
-    load_q<DQ, BF16>(p, u.b, h, iq, hi, q);
+    load_q<DQ, BF16>(p, u, h, iq, hi, q);
     f32x16 o[DQ / 32];
 #pragma unroll
     for (int db = 0; db < DQ / 32; ++db)
@@ -456,7 +457,7 @@ __global__ __launch_bounds__(NW * 64) void cross_attn_kernel(const CrossAttn p, 
     int h, iq;
     row_of(p, u.hk, std::min<int64_t>(row, u.R - 1), h, iq);
     x8 q[DQ / 16];
-    load_q<DQ, BF16>(p, u.b, h, iq, hi, q);
+    load_q<DQ, BF16>(p, u, h, iq, hi, q);
     const char *kp = (const char *) p.k + u.hk * p.k_nb2 + u.b * p.k_nb3, *vp = (const char *) p.v + u.hk * p.v_nb2 + u.b * p.v_nb3;
     const uint8_t *flags = p.kv_valid ? p.kv_valid + u.b * p.kv_valid_nb : nullptr;
     // (a wave's loads are NW * RL rows apart, which the keys do not see)
