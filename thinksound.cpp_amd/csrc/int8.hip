@@ -150,9 +150,10 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void i8_quantize_kernel(const 
 template <bool BF16, bool WIDE>
 hipError_t launch_quantize(const void *x, const Rows &t, int64_t rows, int K, int64_t ld, int8_t *q, float *d, hipStream_t s) {
     auto go = [&](auto kern, int nt) {
-        const int rw = nt < 256 ? 256 / nt : 1;
-        launch_kernel(kern, dim3((unsigned) std::min<int64_t>((rows + rw - 1) / rw, 1 << 22)), dim3(nt < 256 ? 256 : nt), 0, s, x, t,
-                      rows, K, ld, q, d);
+        const int rw = nt < 256 ? 256 / nt : 1, threads = nt < 256 ? 256 : nt;
+        // (a launch holds fewer than 2^32 threads; the rows left are taken in turns)
+        launch_kernel(kern, dim3((unsigned) std::min<int64_t>((rows + rw - 1) / rw, (1 << 30) / threads)), dim3(threads), 0, s, x, t, rows, K,
+                      ld, q, d);
         return hipGetLastError();
     };
     if (ld <= 8 * 8) return go(i8_quantize_kernel<BF16, WIDE, 1, 8, false>, 8);
