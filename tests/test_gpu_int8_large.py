@@ -1,9 +1,12 @@
-"""8-bit rows of more threads than one launch holds: 2^22 rows and more, of 1024 threads each. The rows overlap, each four (f32)
-or eight (bf16) values on."""
+"""8-bit rows of the largest sizes: more threads than one launch holds (2^22 rows and more, of 1024 threads each; they overlap, each four
+(f32) or eight (bf16) values on), and rows of nearly 2^31 values."""
+import ctypes
+
 import numpy as np
 import pytest
 
 import crossref
+import mxref
 from test_gpu_int8 import T, dev, off, planes, typed, want_linear  # noqa: F401  (T: fixture)
 from test_gpu_mxfp4_ends import fetch
 
@@ -45,3 +48,29 @@ def test_product(T):  # noqa: F811
     for i in ROWS:
         want, tol = want_linear(crossref.i8_quantize(row(i)), w, None, "f32")
         assert off(y[i:i + 1], want, tol) <= 0, i
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_the_longest_row(T, dtype):  # noqa: F811
+    """2^31 - 256 values, zeros but for runs at its start, past 2^30 and at its end, and back"""
+    k, n, size = (1 << 31) - 256, 50000, 4 if dtype == "f32" else 2
+    rng = np.random.default_rng(5)
+    x = T.empty((1, k), dtype)
+    T._hipcheck(T.hip().hipMemset(ctypes.c_void_p(x.ptr), 0, ctypes.c_size_t(x.nbytes)), "hipMemset")
+    runs = [(at, typed(rng.standard_normal(n).astype(np.float32), dtype)) for at in (0, (1 << 30) - 17, k - n)]
+    for at, v in runs:
+        src = np.ascontiguousarray(v if dtype == "f32" else mxref.bf16_bits(v))
+        T._hipcheck(T.hip().hipMemcpy(ctypes.c_void_p(x.ptr + at * size), ctypes.c_void_p(src.ctypes.data), ctypes.c_size_t(src.nbytes), 1),
+                    "hipMemcpy H2D")
+    sp = T.i8_quantize(x)
+    q, d = crossref.i8_quantize(np.concatenate([v for _, v in runs])[None])
+    assert fetch(T, sp.buf, k, (1,), np.float32) == d
+    back = T.i8_dequantize(sp, dtype, out=x)
+    for i, (at, _) in enumerate(runs):
+        want = q[0, i * n:(i + 1) * n]
+        assert np.array_equal(fetch(T, sp.buf, at, (n,), np.int8), want), at
+        got = fetch(T, back, at * size, (n,), np.float32 if dtype == "f32" else np.uint16)
+        value = want.astype(np.float32) * d
+        assert np.array_equal(got, value if dtype == "f32" else mxref.bf16_bits(value).reshape(-1)), at
+        if at:
+            assert not fetch(T, sp.buf, at - n, (n,), np.int8).any(), at

@@ -116,8 +116,9 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void i8_quantize_kernel(const 
         Vec8<BF16, WIDE> v[VN];
         uint32_t top = 0;
         if constexpr (LONG) {
-            for (int c = th * 8; c < K; c += NT * 8) {
-                v[0].load(row, c, K);
+            // (64 bits: a step past a row of nearly 2^31 values is not below it)
+            for (int64_t c = th * 8; c < K; c += NT * 8) {
+                v[0].load(row, (int) c, K);
                 top = max(top, v[0].top());
             }
         } else {
@@ -135,9 +136,9 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void i8_quantize_kernel(const 
             if (c < ld) *(u32x2 *) (q + r * ld + c) = u32x2{i8_pack4(w, s), i8_pack4(w + 4, s)};
         };
         if constexpr (LONG) {
-            for (int c = th * 8; c < ld; c += NT * 8) {
-                v[0].load(row, c, K);
-                store(c, v[0]);
+            for (int64_t c = th * 8; c < ld; c += NT * 8) {
+                v[0].load(row, (int) c, K);
+                store((int) c, v[0]);
             }
         } else {
 #pragma unroll
