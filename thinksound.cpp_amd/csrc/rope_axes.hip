@@ -125,7 +125,7 @@ __global__ __launch_bounds__(64) void rope_axes_kernel(const RopeAxes p, int hea
     constexpr int HPW = 64 / LPH;
     const int lane = threadIdx.x, hl = lane / LPH, D = (int) p.x.ne[0], H = (int) p.x.ne[1];
     const Lane l = lane_of<HALVES>(p, D, lane % LPH);
-    const int h0 = (int) blockIdx.y * heads_a_wave, h1 = min(H, h0 + heads_a_wave);
+    const int h0 = (int) blockIdx.y * heads_a_wave, h1 = h0 + min(heads_a_wave, H - h0);   // (their sum may pass 2^31)
     const float over_D = 1.0f / (float) D;
     float w[8] = {};
     if (p.w) {
@@ -221,7 +221,7 @@ hipError_t launch_lph(const RopeAxes &p, hipStream_t s) {
     const int64_t tokens = p.x.ne[2] * p.x.ne[3];
     const int want = (int) std::min<int64_t>(passes, std::max<int64_t>(1, WAVES / tokens));
     const int heads = (passes + want - 1) / want * hpw;
-    const dim3 grid((unsigned) std::min(p.x.ne[2], MOST), (unsigned) ((H + heads - 1) / heads),
+    const dim3 grid((unsigned) std::min(p.x.ne[2], MOST), (unsigned) (((int64_t) H + heads - 1) / heads),
                     (unsigned) std::min<int64_t>(p.x.ne[3], 1 << 8));
     auto go = [&](auto kern) {
         launch_kernel(kern, grid, dim3(64), 0, s, p, heads);
