@@ -9,9 +9,11 @@ ggml's ne[] (a ggml [D, N, H, B] tensor has shape (B, H, N, D)). Errors raise
 TskError with the library's status and message; nothing falls back to a CPU
 path: if libtsk.so is missing, load() raises.
 """
+import contextlib
 import ctypes
 import gc
 import os
+import threading
 
 import numpy as np
 
@@ -442,27 +444,43 @@ class Stream:
             self.h = None
 
 
+# captures that are on, in any thread, and whether the collector ran before the first of them
+_captures, _collects, _captures_lock = 0, False, threading.Lock()
+
+
+@contextlib.contextmanager
+def _collector_waits():
+    global _captures, _collects
+    with _captures_lock:
+        if _captures == 0:
+            _collects = gc.isenabled()
+            gc.disable()
+        _captures += 1
+    try:
+        yield
+    finally:
+        with _captures_lock:
+            _captures -= 1
+            if _captures == 0 and _collects:
+                gc.enable()
+
+
 class Graph:
     """The work a function enqueues on `stream`, captured into a HIP graph
     (hipStreamCaptureModeGlobal: a call that is not allowed under capture,
     hipMalloc among them, fails the capture) and replayed with launch().
-    The garbage collector waits meanwhile: an array that it frees would fail
-    the capture too."""
+    The garbage collector waits until no capture is on: an array that it frees
+    would fail the capture too."""
 
     def __init__(self, stream, fn):
         H = hip()
-        collects = gc.isenabled()
-        gc.disable()
-        try:
+        with _collector_waits():
             _hipcheck(H.hipStreamBeginCapture(stream.h, 0), "hipStreamBeginCapture")
             try:
                 fn()
             finally:
                 g = ctypes.c_void_p()
                 rc = H.hipStreamEndCapture(stream.h, ctypes.byref(g))
-        finally:
-            if collects:
-                gc.enable()
         _hipcheck(rc, "hipStreamEndCapture")
         self.graph = g
         e = ctypes.c_void_p()
