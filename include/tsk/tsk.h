@@ -374,6 +374,7 @@ typedef struct tsk_cross_attn_params {
     const tsk_tensor *q_len;     /* nullable, I32 [B]: tokens of each sequence (clamped)  */
     const uint8_t *kv_valid;     /* nullable, DEVICE [B][Nkv]: 0 marks a state that does not count */
     int64_t kv_valid_nb;         /* bytes between two sequences' flags; 0 shares one       */
+    int prec;                    /* enum tsk_prec: how the weights meet v                  */
 } tsk_cross_attn_params;
 /*
  * Attention of tokens to states of another number (a text's or a video's), softmax over
@@ -385,9 +386,11 @@ typedef struct tsk_cross_attn_params {
  * strides any (k and v: at most 2^24 bytes from a state to the next). A token that no
  * state counts for gets 0; what the states that do not count hold, infinities and NaNs
  * too, has no effect. Tokens from q_len on are neither read nor written.
- * Products are exact and logits, softmax and sums fp32; the weights are rounded to k's
- * type before they multiply v (bf16: within 2^-8, f16: 2^-11) and are divided by
- * the sum of what they were rounded to. dst must not overlap an input. Scratch: long
+ * Products are exact and logits, softmax and sums fp32. TSK_PREC_DEFAULT: the weights are
+ * rounded to k's type before they multiply v (bf16: within 2^-8, f16: 2^-11, or 2^-24 of
+ * the largest weight where that is more) and are divided by the sum of what they were
+ * rounded to; TSK_PREC_F32: two parts of k's type (bf16: within 2^-16, f16: 2^-22, or 2^-24 of
+ * the largest), half as many products again. dst must not overlap an input. Scratch: long
  * states of few tokens are dealt to several workgroups, whose sums meet in the stream's
  * workspace (tsk_workspace_size, TSK_OP_CROSS_ATTENTION).
  */

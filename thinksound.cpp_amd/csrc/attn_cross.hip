@@ -10,8 +10,12 @@
 //   S^T = K Q^T      states x rows: lane l owns row l % 32 and half of the states,
 //   P^T = exp2(scale log2(e) S^T - m) in K's 16-bit type,
 //   O^T += V^T P^T   the sums of the first product lie as the second one's operand does.
-// P is rounded to K's type (bf16: half of 2^-8 a weight), its row sum adds the same rounded
-// values, so that the weights add up to 1.
+// P is rounded to K's type (bf16 within 2^-8, f16 2^-11), its row sum adds the same rounded
+// values, so that the weights add up to 1. With TWO (the caller's choice), what that rounding loses is a
+// second part of K's type, which multiplies V as well, and the sum adds the weights as they are. Error of the
+// norm into f32, 512 tokens to 4096 states of heads of 128, and us of 4096 tokens to 8192 states of 16 heads of 128 / of one
+// token of 4 x 32 heads to 16384 states of 8: bf16 one part 1.4e-3, 267 / 57.9, two 2.0e-6, 358 / 58.3; f16 one 1.7e-4, 270,
+// two 2.8e-7, 368. (Rounding an output to bf16 alone is 1.7e-3, to f16 2.1e-4.)
 #include <algorithm>
 #include <utility>
 
@@ -74,6 +78,11 @@ template <> struct Half<true> {
         const x2 v = {(one) f, (one) g};
         return __builtin_bit_cast(uint32_t, v);
     }
+    // what f and g lose in pack2
+    static __device__ __forceinline__ uint32_t rest2(float f, float g, uint32_t two) {
+        const float a = __uint_as_float(two << 16), b = __uint_as_float(two & 0xffff0000u);
+        return pack2(f - a, g - b);
+    }
 };
 template <> struct Half<false> {
     typedef f16x8 x8;
@@ -87,6 +96,12 @@ template <> struct Half<false> {
     static __device__ __forceinline__ uint32_t pack2(float f, float g) {
         const x2 v = {(one) f, (one) g};
         return __builtin_bit_cast(uint32_t, v);
+    }
+    // what f and g lose in pack2
+    static __device__ __forceinline__ uint32_t rest2(float f, float g, uint32_t two) {
+        const x2 h = __builtin_bit_cast(x2, two);
+        const float a = (float) h[0], b = (float) h[1];
+        return pack2(f - a, g - b);
     }
 };
 
@@ -223,7 +238,7 @@ __device__ __forceinline__ float *part_ml(const CrossAttn &p, int split, int64_t
 // of its own in LDS: no barrier until their sums meet. Bound by the states' bytes: one token of
 // 4 sequences of 32 heads to 16384 states of 8 heads of 128, bf16, in 16 ranges: 57.5 us, 4.7 TB/s
 // (a copy 5.1); with the kernel for many rows 62.
-template <int DQ, bool BF16>
+template <int DQ, bool BF16, bool TWO>
 __global__ __launch_bounds__(256) void cross_attn_few_kernel(const CrossAttn p, int qtiles) {
     typedef Half<BF16> T;
     typedef typename T::x8 x8;
@@ -309,13 +324,17 @@ __global__ __launch_bounds__(256) void cross_attn_few_kernel(const CrossAttn p, 
                 for (int e = 0; e < 16; ++e) o[db][e] *= alpha;
         }
         m_run = m_new;
-        u32x4 pf[2];
+        u32x4 pf[TWO ? 2 : 1][2];
 #pragma unroll
         for (int e = 0; e < 16; e += 2) {
             // (logits times c are rounded as the maximum was: no weight is above 1)
-            const uint32_t two = T::pack2(__builtin_amdgcn_exp2f(times(s[e], c) - sub), __builtin_amdgcn_exp2f(times(s[e + 1], c) - sub));
-            l_run = T::add2(two, l_run);
-            pf[e / 8][e % 8 / 2] = two;
+            const float w0 = __builtin_amdgcn_exp2f(times(s[e], c) - sub), w1 = __builtin_amdgcn_exp2f(times(s[e + 1], c) - sub);
+            const uint32_t two = T::pack2(w0, w1);
+            pf[0][e / 8][e % 8 / 2] = two;
+            if constexpr (TWO) {
+                pf[1][e / 8][e % 8 / 2] = T::rest2(w0, w1, two);
+                l_run += w0 + w1;
+            } else l_run = T::add2(two, l_run);
         }
 #pragma unroll
         for (int kg = 0; kg < 2; ++kg)
@@ -325,7 +344,8 @@ __global__ __launch_bounds__(256) void cross_attn_few_kernel(const CrossAttn p, 
                 const uint16_t *at = vb + (16 * kg + vrow) * DP + ((ch ^ v_key<DP>(l16 >> 2)) << 3) + 4 * (l16 & 1);
                 const s16x4 a = read_turned(at), a2 = read_turned(at + 8 * DP);
                 const s16x8 a8 = {a[0], a[1], a[2], a[3], a2[0], a2[1], a2[2], a2[3]};
-                o[db] = T::mfma(__builtin_bit_cast(x8, a8), __builtin_bit_cast(x8, pf[kg]), o[db]);
+#pragma unroll
+                for (auto &part : pf) o[db] = T::mfma(__builtin_bit_cast(x8, a8), __builtin_bit_cast(x8, part[kg]), o[db]);
             }
         // (the next turn's loads land in the buffer read here: every read is done)
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -442,7 +462,7 @@ __global__ __launch_bounds__(256) void cross_attn_join_kernel(const CrossAttn p,
 // library's matrix product of 8192^3 1390); the matrix unit is busy for 52 % of the cycles and
 // the vector unit's exponentials, sums and roundings for most of the others. One half a step, each
 // after the other, took 325 us, a largest logit found before each weight 251.
-template <int DQ, bool BF16, int NW>
+template <int DQ, bool BF16, int NW, bool TWO>
 __global__ __launch_bounds__(NW * 64) void cross_attn_kernel(const CrossAttn p, int qtiles) {
     typedef Half<BF16> T;
     typedef typename T::x8 x8;
@@ -507,7 +527,7 @@ __global__ __launch_bounds__(NW * 64) void cross_attn_kernel(const CrossAttn p, 
     const float c = p.c;
     const int l16 = lane & 15, grp = (lane >> 4) & 1, vrow = 4 * hi + (l16 >> 2);
     struct Weights {
-        u32x4 w[2];                                              // pairs
+        u32x4 w[TWO ? 2 : 1][2];                                 // pairs, of each part
         float sum;
     };
     // A step's operands in LDS, K's of one half of a tile and V's of another, in the order of
@@ -547,10 +567,16 @@ __global__ __launch_bounds__(NW * 64) void cross_attn_kernel(const CrossAttn p, 
     };
     auto turn3 = [&](const Turns &r, Weights &w, int e) __attribute__((always_inline)) {
         uint32_t two = T::pack2(r.v[e], r.v[e + 1]);
-        float sum = T::add2(two, e == 0 ? 0.0f : w.sum);
+        float sum = e == 0 ? 0.0f : w.sum;
+        if constexpr (TWO) {
+            uint32_t rest = T::rest2(r.v[e], r.v[e + 1], two);
+            sum += r.v[e] + r.v[e + 1];
+            asm volatile("" : "+v"(rest));
+            w.w[1][e / 8][e % 8 / 2] = rest;
+        } else sum = T::add2(two, sum);
         asm volatile("" : "+v"(two), "+v"(sum));
         w.sum = sum;
-        w.w[e / 8][e % 8 / 2] = two;
+        w.w[0][e / 8][e % 8 / 2] = two;
     };
     constexpr int PER = (16 + NF - 1) / NF;                      // logits between two products
     auto first_turns = [&](const f32x16 &n, Turns &r) __attribute__((always_inline)) {
@@ -562,6 +588,12 @@ __global__ __launch_bounds__(NW * 64) void cross_attn_kernel(const CrossAttn p, 
         EACH(f, 0, AHEAD, read_piece(kb, vb, f, x););
         __builtin_amdgcn_sched_barrier(0);
     };
+    // piece j of V times its weights
+    auto add_v = [&](const x8 &v, const Weights &w, auto j) __attribute__((always_inline)) {
+        constexpr int KG = decltype(j)::value / (DQ / 32), DB = decltype(j)::value % (DQ / 32);
+        o[DB] = T::mfma(v, __builtin_bit_cast(x8, w.w[0][KG]), o[DB]);
+        if constexpr (TWO) o[DB] = T::mfma(v, __builtin_bit_cast(x8, w.w[1][KG]), o[DB]);
+    };
     // the products of next (K . Q of a half) and of before (V of another), `now` weighed between
     // them, and one half (part) of the loads of a later tile
     auto step = [&](const uint16_t *kb, const uint16_t *vb, Pieces &x, const f32x16 &now, Turns &r, Weights &w, f32x16 &next,
@@ -570,7 +602,7 @@ __global__ __launch_bounds__(NW * 64) void cross_attn_kernel(const CrossAttn p, 
         EACH(f, 0, NF,
             constexpr int J = piece_index(NK, f);
             if constexpr (piece_of_k(NK, f)) next = T::mfma(x.f[f % SLOTS], q[J], J == 0 ? f32x16{} : next);
-            else o[J % (DQ / 32)] = T::mfma(x.f[f % SLOTS], __builtin_bit_cast(x8, before.w[J / (DQ / 32)]), o[J % (DQ / 32)]);
+            else add_v(x.f[f % SLOTS], before, std::integral_constant<int, J>{});
             if constexpr (f + AHEAD < NF) read_piece(kb, vb, f + AHEAD, x);
             EACH(i, f * L1 / NF, (f + 1) * L1 / NF, issue_one(src, to, L0 + i););
             EACH(i, 0, PER,
@@ -593,7 +625,7 @@ __global__ __launch_bounds__(NW * 64) void cross_attn_kernel(const CrossAttn p, 
             constexpr int J = piece_index(NK, f);
             Pieces x;
             read_piece(vb, vb, f, x);
-            o[J % (DQ / 32)] = T::mfma(x.f[f % SLOTS], __builtin_bit_cast(x8, w.w[J / (DQ / 32)]), o[J % (DQ / 32)]);
+            add_v(x.f[f % SLOTS], w, std::integral_constant<int, J>{});
         });
     };
     auto weigh = [&](const f32x16 &n, Weights &w) __attribute__((always_inline)) {
@@ -715,13 +747,13 @@ hipError_t launch_units(F kern, const CrossAttn &p, int rows, int threads, size_
     return hipGetLastError();
 }
 
-template <int DQ, bool BF16>
+template <int DQ, bool BF16, bool TWO>
 hipError_t launch_dp(const CrossAttn &p, const CrossAttnPlan &plan, hipStream_t s) {
     constexpr int DP = row_of_lds(DQ);
     hipError_t e;
-    if (plan.rows == 32) e = launch_units(cross_attn_few_kernel<DQ, BF16>, p, 32, 256, 4 * 2 * 2 * 32 * DP * 2, s);
-    else if (plan.rows == 128) e = launch_units(cross_attn_kernel<DQ, BF16, 4>, p, 128, 256, 4 * 2 * 64 * DP * 2, s);
-    else e = launch_units(cross_attn_kernel<DQ, BF16, 8>, p, 256, 512, 4 * 2 * 64 * DP * 2, s);
+    if (plan.rows == 32) e = launch_units(cross_attn_few_kernel<DQ, BF16, TWO>, p, 32, 256, 4 * 2 * 2 * 32 * DP * 2, s);
+    else if (plan.rows == 128) e = launch_units(cross_attn_kernel<DQ, BF16, 4, TWO>, p, 128, 256, 4 * 2 * 64 * DP * 2, s);
+    else e = launch_units(cross_attn_kernel<DQ, BF16, 8, TWO>, p, 256, 512, 4 * 2 * 64 * DP * 2, s);
     if (e != hipSuccess || p.splits == 1) return e;
     constexpr int NG = 256 / (DP / 4);
     int G = 1;
@@ -782,14 +814,16 @@ CrossAttnPlan plan_cross_attn(int D, int64_t Nq, int64_t Nkv, int64_t H, int64_t
 }
 
 hipError_t launch_cross_attn(const CrossAttn &p, const CrossAttnPlan &plan, hipStream_t s) {
-    auto go = [&](auto bf16) {
-        constexpr bool BF16 = decltype(bf16)::value;
-        if (p.D <= 32) return launch_dp<32, BF16>(p, plan, s);
-        if (p.D <= 64) return launch_dp<64, BF16>(p, plan, s);
-        if (p.D <= 96) return launch_dp<96, BF16>(p, plan, s);
-        return launch_dp<128, BF16>(p, plan, s);
+    auto go = [&](auto bf16, auto two) {
+        constexpr bool BF16 = decltype(bf16)::value, TWO = decltype(two)::value;
+        if (p.D <= 32) return launch_dp<32, BF16, TWO>(p, plan, s);
+        if (p.D <= 64) return launch_dp<64, BF16, TWO>(p, plan, s);
+        if (p.D <= 96) return launch_dp<96, BF16, TWO>(p, plan, s);
+        return launch_dp<128, BF16, TWO>(p, plan, s);
     };
-    return p.kv_bf16 ? go(std::true_type()) : go(std::false_type());
+    std::true_type t;
+    std::false_type f;
+    return p.kv_bf16 ? p.two_parts ? go(t, t) : go(t, f) : p.two_parts ? go(f, t) : go(f, f);
 }
 
 }  // namespace tsk

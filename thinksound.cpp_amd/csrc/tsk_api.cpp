@@ -1500,6 +1500,7 @@ int validate_cross(const tsk_tensor *q, const tsk_tensor *k, const tsk_tensor *v
     if ((rc = validate_cross_shapes(q, k, v, dst))) return rc;
     const int64_t B = q->ne[3];
     if (!(p->scale > 0.0f) || !std::isfinite(p->scale)) return fail(TSK_ERR_INVALID_ARG, "scale");
+    if (p->prec != TSK_PREC_DEFAULT && p->prec != TSK_PREC_F32) return fail(TSK_ERR_INVALID_ARG, "prec %d", p->prec);
     if ((rc = check_lengths(p->kv_len, "kv_len", B)) || (rc = check_lengths(p->q_len, "q_len", B))) return rc;
     if (p->kv_valid && p->kv_valid_nb < 0) return fail(TSK_ERR_INVALID_ARG, "kv_valid_nb");
     for (const tsk_tensor *t : {q, k, v, p->kv_len, p->q_len})
@@ -1532,6 +1533,7 @@ extern "C" int tsk_cross_attention(const tsk_tensor *q, const tsk_tensor *k, con
     a.q_len = p->q_len ? (const int32_t *) p->q_len->data : nullptr;
     a.kv_valid = p->kv_valid; a.kv_valid_nb = p->kv_valid_nb;
     a.c = p->scale * 1.4426950408889634f;
+    a.two_parts = p->prec == TSK_PREC_F32;
     const CrossAttnPlan plan = plan_cross_attn(a.D, a.Nq, a.Nkv, a.H, a.Hkv, a.B);
     void *ws = nullptr;
     if (plan.bytes && (rc = workspace((hipStream_t) stream, plan.bytes, &ws))) return rc;

@@ -429,6 +429,7 @@ struct CrossAttn {
     const uint8_t *kv_valid;       // [B][kv_valid_nb], nullable
     int64_t kv_valid_nb;
     float c;                       // scale * log2(e)
+    int two_parts;                 // weights in two parts of k's type (TSK_PREC_F32)
     int splits;                    // key ranges, each a workgroup; > 1: part holds their sums
     float *part;
 };

@@ -58,7 +58,7 @@ class RopeAxesParams(ctypes.Structure):
 
 class CrossAttnParams(ctypes.Structure):
     _fields_ = [("scale", ctypes.c_float), ("kv_len", ctypes.POINTER(TskTensor)), ("q_len", ctypes.POINTER(TskTensor)),
-                ("kv_valid", ctypes.c_void_p), ("kv_valid_nb", ctypes.c_int64)]
+                ("kv_valid", ctypes.c_void_p), ("kv_valid_nb", ctypes.c_int64), ("prec", ctypes.c_int)]
 
 
 class T5Config(ctypes.Structure):
@@ -798,14 +798,16 @@ def rope_axes(x, pos, dims, pairs=ROPE_ADJACENT, shared_freqs=False, freq_base=1
     return out
 
 
-def cross_attention(q, k, v, scale=None, kv_len=None, q_len=None, kv_valid=None, out=None, out_dtype="f32", stream=None):
+def cross_attention(q, k, v, scale=None, kv_len=None, q_len=None, kv_valid=None, out=None, out_dtype="f32", stream=None,
+                    prec=PREC_DEFAULT):
     """Attention to states of another number (tsk_cross_attention): q (B, H, Nq, D), k / v (B, Hkv, Nkv, D) f16 / bf16 ->
-    (B, Nq, H, D). kv_len, q_len (B,) i32; kv_valid u8 (B, Nkv), or (Nkv,) for all; scale None: D ** -0.5."""
+    (B, Nq, H, D). kv_len, q_len (B,) i32; kv_valid u8 (B, Nkv), or (Nkv,) for all; scale None: D ** -0.5;
+    prec PREC_F32: weights in two parts of k's type."""
     init()
     B, H, Nq, D = q.shape
     out = DeviceArray((B, Nq, H, D), out_dtype) if out is None else out
     p = CrossAttnParams()
-    p.scale = D ** -0.5 if scale is None else scale
+    p.scale, p.prec = D ** -0.5 if scale is None else scale, prec
     for name, t in (("kv_len", kv_len), ("q_len", q_len)):
         if t is not None:
             setattr(p, name, ctypes.pointer(desc(t)))
