@@ -359,8 +359,9 @@ typedef struct tsk_rope_axes_params {
  *   x   : F32 or BF16, ne = [D, n_head, S, B], D <= 384, rows contiguous
  *   pos : I32 or F32, ne = [S, n_axes, B or 1], rows contiguous; fractions are taken
  *   dst : F32 or BF16 of x's shape; may be x itself, no other overlap
- * Angles are formed in 64 bits (tsk_rope_ext: as ggml's running fp32 product), sines and
- * cosines are within 2^-22; a position that is infinite or NaN gives NaN.
+ * Angles are formed in 64 bits (tsk_rope_ext: as ggml's running fp32 product): sines and
+ * cosines are within 2^-22 + 2^-50 |freq_scale * position| (freq_base below 1, whose frequencies
+ * pass 1: 2^-22 + 2^-46 |angle|). A position that is infinite or NaN gives NaN.
  */
 int tsk_rope_axes(const tsk_tensor *x, const tsk_tensor *pos, const tsk_rope_axes_params *p, tsk_tensor *dst,
                   tsk_stream stream);
@@ -382,8 +383,10 @@ typedef struct tsk_cross_attn_params {
  *   q    : ne = [D, Nq, H, B]    F32, F16 or BF16, converted to k's type
  *   k, v : ne = [D, Nkv, Hkv, B] F16 or BF16, H % Hkv == 0 (head h reads h / (H / Hkv))
  *   dst  : ne = [D, H, Nq, B]    F32, F16 or BF16 (ggml's permuted result)
- * D is a multiple of 8, at most 128; rows are contiguous on 16-byte starts, and their
- * strides any (k and v: at most 2^24 bytes from a state to the next). A token that no
+ * D is a multiple of 8, at most 128; rows are contiguous on 16-byte starts. Strides of q and
+ * of the heads and sequences of k and v are any (0: shared), from a state to the next a row
+ * at least and 2^24 bytes at most; dst's rows share no bytes. The H / Hkv * Nq rows of a
+ * key and value head, in groups of 32, are at most 2^22 over all of them. A token that no
  * state counts for gets 0; what the states that do not count hold, infinities and NaNs
  * too, has no effect. Tokens from q_len on are neither read nor written.
  * Products are exact and logits, softmax and sums fp32. TSK_PREC_DEFAULT: the weights are
