@@ -27,11 +27,12 @@ typedef __attribute__((__vector_size__(8), aligned(2))) uint32_t u32x2_any2;
 typedef __attribute__((__vector_size__(8), aligned(2))) __bf16 bf16x4_any2;
 typedef __attribute__((__vector_size__(16), aligned(4))) float f32x4_any4;
 
-// cos and sin of q quarter turns: the nearest whole quarter apart, Taylor's series of the
-// rest, at most an eighth of a turn (the first terms left out: 1.2e-10 and 1.8e-9)
-__device__ __forceinline__ void cos_sin(double q, float &c, float &s) {
-    const double n = __builtin_rint(q);
-    const float f = (float) (q - n) * 1.57079632679489662f, f2 = f * f;
+// cos and sin of pos * freq quarter turns: the nearest whole quarter apart, Taylor's series of the
+// rest, at most an eighth of a turn (the first terms left out: 1.2e-10 and 1.8e-9). The rest is the exact
+// product's; where the rounded one is off by a quarter and more itself, from 2^51 on, the rounded one's
+__device__ __forceinline__ void cos_sin(double pos, double freq, float &c, float &s) {
+    const double q = pos * freq, n = __builtin_rint(q), rest = __builtin_fabs(q) < 0x1p51 ? __builtin_fma(pos, freq, -n) : 0.0;
+    const float f = (float) rest * 1.57079632679489662f, f2 = f * f;
     const float sn = f + f * f2 * (-1.0f / 6 + f2 * (1.0f / 120 + f2 * (-1.0f / 5040 + f2 * (1.0f / 362880))));
     const float cn = 1.0f + f2 * (-0.5f + f2 * (1.0f / 24 + f2 * (-1.0f / 720 + f2 * (1.0f / 40320 + f2 * (-1.0f / 3628800)))));
     // n modulo 4 (n is whole; of 2^53 and more it is a multiple of 4 or may as well be one)
@@ -188,7 +189,7 @@ __global__ __launch_bounds__(64) void rope_axes_kernel(const RopeAxes p, int hea
                 const int a = (i >= p.first[1]) + (i >= p.first[2]) + (i >= p.first[3]);
                 const char *at = (const char *) p.pos + a * p.pos_nb1 + b * p.pos_nb2 + s * 4;
                 const int word = *(const int *) at;
-                cos_sin((p.pos_f32 ? (double) __int_as_float(word) : (double) word) * p.quarters[i], cosines[i], sines[i]);
+                cos_sin(p.pos_f32 ? (double) __int_as_float(word) : (double) word, p.quarters[i], cosines[i], sines[i]);
             }
             __syncthreads();
             // (of a run's pairs past the last nothing is used)
