@@ -70,7 +70,7 @@ __device__ __forceinline__ void store4(const I8Gemm &p, int n, int m, f32x4 v) {
 // few, by the launch; turns of 256 or 512 k and 8 waves are no faster (16.4 to 18.3).
 //
 // XT: f32 or bf16 activations, quantized by every workgroup into LDS while its first
-// weights are on their way (gemm_i8_fused).
+// weights are on their way (gemm_i8_fits).
 enum : int { X_I8 = 0, X_BF16 = 1, X_F32 = 2 };
 
 constexpr int NW = 4, KS = 2;
@@ -492,7 +492,13 @@ int shape_for(const I8Gemm &p) {
 // four by a wave each (us, inside / two launches; rows x M): 1 x 6144, K = 1024 5.2 /
 // 6.9; 1 x 8192, K = 8192 18.9 / 20.4; 3 x 6144, K = 1024 5.8 / 6.9; 4 x 2048, K = 2048
 // 6.9 / 7.2; 8 x 1024, K = 1024 6.6 / 6.4; 2 x 8192, K = 8192 22.6 / 20.4.
-bool gemm_i8_fused(int64_t N, int64_t K) { return N == 1 ? K <= 8192 : N <= 4 && K <= 2048 && N * K <= 4096; }
+bool gemm_i8_fits(int64_t N, int64_t K) { return N == 1 ? K <= 8192 : N <= 4 && K <= 2048 && N * K <= 4096; }
+// Each workgroup of 16 channels does so, and from some 32768 channels on they cost more than the launch
+// (weights that are in no cache): 1 x 32768, K = 1024 10.8 / 11.5, x 65536 16.9 / 16.5, x 152064 32.7 / 29.7; K = 256
+// 7.4 / 6.6, 11.5 / 8.0, 22.1 / 12.5; 2 x 32768, K = 2048 18.2 / 17.7, x 152064 63.5 / 55.4; 4 x 32768, K = 1024 11.9 / 12.0,
+// x 152064 40.9 / 33.7. One row of 2048 and more hides behind its weights: K = 2048 x 152064 50.6 / 53.3, K = 4096 111.6 / 119.9,
+// K = 8192 210.8 / 212.5.
+bool gemm_i8_fused(int64_t N, int64_t K, int64_t M) { return gemm_i8_fits(N, K) && (M <= 32768 || (N == 1 && K >= 2048)); }
 
 hipError_t launch_gemm_i8(const I8Gemm &p, hipStream_t s) {
     if (!p.xq) return launch_fused(p, s);

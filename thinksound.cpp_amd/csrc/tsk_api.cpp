@@ -642,7 +642,7 @@ MulMatPlan plan_mul_mat(const tsk_tensor *a, const tsk_tensor *b, const tsk_tens
         pl.uni = row_stride(dst) != 0;
         pl.nslices = pl.uni ? 1 : b->ne[2] * b->ne[3];
         pl.Nslice = pl.uni ? row_count(b) : b->ne[1];
-        if (b->type != TSK_TYPE_I8_SPLIT && !(row_stride(b) && gemm_i8_fused(pl.Nslice, K)))
+        if (b->type != TSK_TYPE_I8_SPLIT && !(row_stride(b) && gemm_i8_fused(pl.Nslice, K, M)))
             pl.act_bytes = align256(i8_bytes(K, row_count(b)));
         pl.bytes = pl.act_bytes;
         return pl;
@@ -754,16 +754,21 @@ int mul_mat_i8(const tsk_tensor *a, const tsk_tensor *b, const tsk_tensor *bias,
     const int8_t *xq = i8_codes(b);
     const float *xd = i8_scales(b);
     hipError_t e;
-    if (pl.act_bytes) {
-        void *ws = nullptr;
+    void *ws = nullptr;
+    // (rows that fit in the product's kernel can do without)
+    if (pl.act_bytes && row_stride(b) && gemm_i8_fits(pl.Nslice, K)) {
+        ws = scr.optional(pl.bytes);
+    } else if (pl.act_bytes) {
         int rc;
         if ((rc = scr.get(pl.bytes, &ws))) return rc;
+    }
+    if (ws) {
         float *d = (float *) ((char *) ws + (size_t) row_count(b) * (size_t) ld);
         if ((e = launch_i8_quantize(view(b), (int8_t *) ws, d, scr.s)) != hipSuccess) return hip_fail(e, "mul_mat input quantize");
         xq = (const int8_t *) ws;
         xd = d;
     }
-    const bool fused = b->type != TSK_TYPE_I8_SPLIT && !pl.act_bytes;
+    const bool fused = b->type != TSK_TYPE_I8_SPLIT && !ws;
     const int64_t ld_b = fused ? (int64_t) row_stride(b) : 0;
     p.x_f32 = b->type == TSK_TYPE_F32;
     p.ld_x = fused ? ld_b / elt_size(b->type) : 0;

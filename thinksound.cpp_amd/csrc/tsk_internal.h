@@ -387,7 +387,7 @@ struct I8Gemm {
     const float *wd;               // [M]
     const int8_t *xq;              // [N][i8_ld(K)]; null: x
     const float *xd;               // [N]
-    const void *x;                 // bf16 / f32 rows (16-byte aligned, ld_x elements apart), where gemm_i8_fused
+    const void *x;                 // bf16 / f32 rows (16-byte aligned, ld_x elements apart), where gemm_i8_fits
     int x_f32;
     int64_t ld_x;
     const float *bias;             // [M], nullable, 16-byte aligned
@@ -397,8 +397,10 @@ struct I8Gemm {
     int M, N, K;
 };
 hipError_t launch_gemm_i8(const I8Gemm &p, hipStream_t s);
-// whether N rows of K bf16 / f32 activations are quantized inside the product's kernel
-bool gemm_i8_fused(int64_t N, int64_t K);
+// whether N rows of K bf16 / f32 activations can be quantized inside the product's kernel, and whether
+// it then is the faster of the two (the same bits)
+bool gemm_i8_fits(int64_t N, int64_t K);
+bool gemm_i8_fused(int64_t N, int64_t K, int64_t M);
 
 // ---------------------------------------------------------------- rotary positions over several axes
 // tsk_rope_axes' operands (rope_axes.hip): x and y [D, heads, S, B]
