@@ -52,7 +52,11 @@
  *     tsk_workspace_size; the library then never allocates), or else one the
  *     library owns per (device, stream) and grows on first need (that growth
  *     waits for the stream and reallocates; once every shape has been seen
- *     no operator allocates or synchronises).
+ *     no operator allocates or synchronises). A captured graph keeps using the
+ *     buffer of its capture, which must be large enough before the capture begins:
+ *     the library's own stays until tsk_release_workspace or tsk_shutdown, also
+ *     where a larger one has taken its place. Graphs captured on one stream, and its
+ *     eager calls, share that buffer: one runs after the other.
  */
 #ifndef TSK_TSK_H
 #define TSK_TSK_H

@@ -12,6 +12,7 @@
 #include <map>
 #include <mutex>
 #include <utility>
+#include <vector>
 
 #include "../../include/tsk/tsk.h"
 #include "i8.h"
@@ -51,6 +52,8 @@ struct Workspace {
     void *ptr = nullptr;
     size_t size = 0;
     bool external = false;
+    bool recorded = false;        // a captured graph reads and writes ptr
+    std::vector<void *> kept;     // earlier library-owned buffers that captured graphs use
 };
 std::map<std::pair<int, hipStream_t>, Workspace> g_ws;
 
@@ -185,6 +188,21 @@ bool workspace_can(hipStream_t s, size_t bytes) {
     return c == hipStreamCaptureStatusNone;
 }
 
+namespace {
+// another buffer takes the place of w's own: a graph that was captured with it may still be launched
+void drop_owned(Workspace &w) {
+    if (w.ptr && !w.external) {
+        if (w.recorded) w.kept.push_back(w.ptr);
+        else (void) hipFree(w.ptr);
+    }
+    w.recorded = false;
+}
+void free_all(Workspace &w) {
+    if (w.ptr && !w.external) (void) hipFree(w.ptr);
+    for (void *p : w.kept) (void) hipFree(p);
+}
+}  // namespace
+
 int workspace(hipStream_t s, size_t bytes, void **out) {
     *out = nullptr;
     if (!bytes) return TSK_OK;
@@ -193,6 +211,8 @@ int workspace(hipStream_t s, size_t bytes, void **out) {
     if (e != hipSuccess) return hip_fail(e, "hipGetDevice");
     std::lock_guard<std::mutex> lk(g_mu);
     Workspace &w = g_ws[std::make_pair(dev, s)];
+    hipStreamCaptureStatus c = hipStreamCaptureStatusNone;
+    if (s && hipStreamIsCapturing(s, &c) != hipSuccess) (void) hipGetLastError();
     if (w.size < bytes) {
         if (w.external)
             return fail(TSK_ERR_NOMEM, "the workspace bound to this stream holds %zu bytes, the call needs %zu", w.size,
@@ -200,7 +220,7 @@ int workspace(hipStream_t s, size_t bytes, void **out) {
         // only work queued on s reads this stream's buffer
         e = hipStreamSynchronize(s);
         if (e != hipSuccess) return hip_fail(e, "hipStreamSynchronize");
-        if (w.ptr) (void) hipFree(w.ptr);
+        drop_owned(w);
         w.ptr = nullptr;
         w.size = 0;
         const size_t sz = (bytes + 0xfffff) & ~(size_t) 0xfffff;
@@ -208,6 +228,7 @@ int workspace(hipStream_t s, size_t bytes, void **out) {
         if (e != hipSuccess) return fail(TSK_ERR_NOMEM, "hipMalloc(%zu): %s", sz, hipGetErrorString(e));
         w.size = sz;
     }
+    if (c != hipStreamCaptureStatusNone) w.recorded = true;
     *out = w.ptr;
     return TSK_OK;
 }
@@ -404,8 +425,7 @@ extern "C" int tsk_shutdown(void) {
     std::lock_guard<std::mutex> lk(g_mu);
     if (g_device < 0) return TSK_OK;
     (void) hipDeviceSynchronize();
-    for (auto &kv : g_ws)
-        if (kv.second.ptr && !kv.second.external) (void) hipFree(kv.second.ptr);
+    for (auto &kv : g_ws) free_all(kv.second);
     g_ws.clear();
     g_device = -1;
     return TSK_OK;
@@ -426,7 +446,7 @@ extern "C" int tsk_set_workspace(tsk_stream stream, void *ptr, size_t bytes) {
         // the library-owned buffer may still be read by work queued on s
         e = hipStreamSynchronize(s);
         if (e != hipSuccess) return hip_fail(e, "hipStreamSynchronize");
-        (void) hipFree(w.ptr);
+        drop_owned(w);
     }
     w.ptr = ptr;
     w.size = bytes;
@@ -444,10 +464,10 @@ extern "C" int tsk_release_workspace(tsk_stream stream) {
     std::lock_guard<std::mutex> lk(g_mu);
     auto it = g_ws.find(std::make_pair(dev, s));
     if (it == g_ws.end()) return TSK_OK;
-    if (it->second.ptr && !it->second.external) {
+    if ((it->second.ptr && !it->second.external) || !it->second.kept.empty()) {
         e = hipStreamSynchronize(s);
         if (e != hipSuccess) return hip_fail(e, "hipStreamSynchronize");
-        (void) hipFree(it->second.ptr);
+        free_all(it->second);
     }
     g_ws.erase(it);
     return TSK_OK;
