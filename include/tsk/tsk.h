@@ -334,7 +334,8 @@ size_t tsk_mxfp4_split_nbytes(int64_t K, int64_t M);
  * x and dst must not overlap.
  */
 int tsk_i8_quantize(const tsk_tensor *x, tsk_tensor *dst, tsk_stream stream);
-/* d * q of an I8_SPLIT tensor, an fp32 product, as F32 rows or rounded to BF16 rows. */
+/* d * q of an I8_SPLIT tensor, an fp32 product, as F32 rows or rounded to BF16 rows. (Of a row
+ * whose largest value is fp32's largest, that one comes back infinite: 127 d is past it.) */
 int tsk_i8_dequantize(const tsk_tensor *x, tsk_tensor *dst, tsk_stream stream);
 /* Bytes an I8_SPLIT tensor of `rows` rows of K values occupies. */
 size_t tsk_i8_split_nbytes(int64_t K, int64_t rows);
@@ -373,7 +374,7 @@ int tsk_rope_axes(const tsk_tensor *x, const tsk_tensor *pos, const tsk_rope_axe
 /* ---- attention to an encoder's states ---------------------------------------- */
 
 typedef struct tsk_cross_attn_params {
-    float scale;                 /* factor of q . k, > 0                                 */
+    float scale;                 /* factor of q . k, > 0 and below 2^127                 */
     const tsk_tensor *kv_len;    /* nullable, I32 [B]: states of each sequence, those from
                                   * there on do not count (clamped to 0 .. Nkv)          */
     const tsk_tensor *q_len;     /* nullable, I32 [B]: tokens of each sequence (clamped)  */
@@ -393,7 +394,8 @@ typedef struct tsk_cross_attn_params {
  * key and value head, in groups of 32, are at most 2^22 over all of them. A token that no
  * state counts for gets 0; what the states that do not count hold, infinities and NaNs
  * too, has no effect. Tokens from q_len on are neither read nor written.
- * Products are exact and logits, softmax and sums fp32. TSK_PREC_DEFAULT: the weights are
+ * Products are exact and logits, softmax and sums fp32 (logits of 2^127 and more are
+ * infinite, of either sign). TSK_PREC_DEFAULT: the weights are
  * rounded to k's type before they multiply v (bf16: within 2^-8, f16: 2^-11, or 2^-24 of
  * the largest weight where that is more) and are divided by the sum of what they were
  * rounded to; TSK_PREC_F32: two parts of k's type (bf16: within 2^-16, f16: 2^-22, or 2^-24 of

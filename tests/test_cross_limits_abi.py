@@ -2,7 +2,7 @@
 import pytest
 
 from test_abi import fake, tsk, uninit  # noqa: F401  (fixtures)
-from test_cross_ops_abi import ALIGN, NOT_INIT, SHAPE, STRIDE, at, cross_params
+from test_cross_ops_abi import ALIGN, ARG, NOT_INIT, SHAPE, STRIDE, at, cross_params
 from test_mxfp4_abi import call
 
 
@@ -37,3 +37,12 @@ def test_strides_of_states(uninit):  # noqa: F811
         k.nb[2] = k.nb[3] = q.nb[1] = q.nb[2] = q.nb[3] = 0
 
     assert go(uninit, 2, 4, 2, 5, edit=shared) == NOT_INIT
+
+
+def test_scale(uninit):  # noqa: F811
+    """a scale whose product with log2 e is no fp32 number would make every logit infinite or NaN"""
+    T = uninit
+    q, k = at(fake(T, T.BF16, (1, 2, 5, 64), 2), 0x100000), at(fake(T, T.BF16, (1, 2, 9, 64), 2), 0x200000)
+    y = at(fake(T, T.F32, (1, 5, 2, 64), 4), 0x300000)
+    for scale, rc in ((1e-45, NOT_INIT), (1.7e38, NOT_INIT), (2.0 ** 127, ARG), (3.4e38, ARG), (float("inf"), ARG), (-1.0, ARG)):
+        assert call(T, "tsk_cross_attention", q, k, k, cross_params(T, scale=scale), y) == rc

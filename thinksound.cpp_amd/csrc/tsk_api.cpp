@@ -1524,7 +1524,8 @@ int validate_cross(const tsk_tensor *q, const tsk_tensor *k, const tsk_tensor *v
     if (!p) return fail(TSK_ERR_INVALID_ARG, "params is NULL");
     if ((rc = validate_cross_shapes(q, k, v, dst))) return rc;
     const int64_t B = q->ne[3];
-    if (!(p->scale > 0.0f) || !std::isfinite(p->scale)) return fail(TSK_ERR_INVALID_ARG, "scale");
+    // (times log2 e it is an fp32 number too)
+    if (!(p->scale > 0.0f) || !(p->scale < 0x1p127f)) return fail(TSK_ERR_INVALID_ARG, "scale");
     if (p->prec != TSK_PREC_DEFAULT && p->prec != TSK_PREC_F32) return fail(TSK_ERR_INVALID_ARG, "prec %d", p->prec);
     if ((rc = check_lengths(p->kv_len, "kv_len", B)) || (rc = check_lengths(p->q_len, "q_len", B))) return rc;
     if (p->kv_valid && p->kv_valid_nb < 0) return fail(TSK_ERR_INVALID_ARG, "kv_valid_nb");
