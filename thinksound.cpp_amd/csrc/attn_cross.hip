@@ -43,8 +43,8 @@ __device__ __forceinline__ s16x4 read_turned(const uint16_t *p) { return __built
 // takes one piece of 32 rows in turns of 16 lanes (0-3, 12-15, 20-27; 4-11, 16-19, 28-31; ...): the
 // keys send those to 16 places. V: the four rows of a transposing read, 64 bytes each
 // Values of a state's row in LDS (64 or 128, which the keys below need), of which the first DQ, D
-// rounded up to 32, are multiplied: 4096 tokens to 8192 states of 16 heads of 72 195 us (all 128
-// 219), of 96 208 (231), of 32 127 (64: 136)
+// rounded up to 32, are multiplied: 4096 tokens to 8192 states of 16 heads of 72 217 us (all 128
+// 240), of 96 216 (238), of 32 132 (64: 140)
 constexpr int row_of_lds(int DQ) { return DQ <= 64 ? 64 : 128; }
 template <int DP> __device__ __forceinline__ int k_key(int row) { return DP == 128 ? row & 15 : row >> 1 & 7; }
 template <int DP> __device__ __forceinline__ int v_key(int row) { return (DP == 128 ? 4 : 2) * (row & 3); }
@@ -459,7 +459,7 @@ __global__ __launch_bounds__(256) void cross_attn_join_kernel(const CrossAttn p,
 // halves without a dependence, so that the matrix unit and the rest of the SIMD work at once.
 // Products, LDS reads, loads and the softmax's operations are in the program's order
 // (sched_barrier). 4096 tokens to 8192 states of 16 heads of 128, bf16: 243 us, 1130 TF/s (a
-// library's matrix product of 8192^3 1390); the matrix unit is busy for 52 % of the cycles and
+// library's matrix product of 8192^3 1390; 249 to 267 on other cards); the matrix unit is busy for 54 % of the cycles and
 // the vector unit's exponentials, sums and roundings for most of the others. One half a step, each
 // after the other, took 325 us, a largest logit found before each weight 251.
 template <int DQ, bool BF16, int NW, bool TWO>
@@ -778,7 +778,8 @@ hipError_t launch_dp(const CrossAttn &p, const CrossAttnPlan &plan, hipStream_t 
 //   B 4, 1000,       1000,         4 heads of 128: 128 x 1  25.3, 32 x 1  29.3, 256 x 1   32.7
 //   B 4, 1,  16384, 32 heads on 8 of 128:           32 x 16 57.5, 128 x 16 61.9, 32 x 1  179.6
 //   B 1, 1,   8192,        16 heads of  64:         32 x 16 13.4, 128 x 16 16.7, 32 x 1   46.3
-// Lengths that are shorter than the states are not known here; then it may be some 20 % off.
+// Lengths that are shorter than the states are not known here; then it may be some 20 % off. The constants are those of
+// heads of 64 and of 128, which smaller heads of either kind take too.
 CrossAttnPlan plan_cross_attn(int D, int64_t Nq, int64_t Nkv, int64_t H, int64_t Hkv, int64_t B) {
     CrossAttnPlan c = {128, 1, 0};
     const int64_t R = H / Hkv * Nq;

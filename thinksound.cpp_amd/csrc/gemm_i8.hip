@@ -66,8 +66,9 @@ __device__ __forceinline__ void store4(const I8Gemm &p, int n, int m, f32x4 v) {
 // deal the K range among them in turns of 64 KS k; their sums meet in LDS.
 // Lane l holds row l % 16 of either operand and of each 64 k the 16 bytes l / 16.
 //
-// Bound by the weights' bytes (8 x 8192, K = 8192 15.4 us, 4.4 TB/s) and, where they are
-// few, by the launch; turns of 256 or 512 k and 8 waves are no faster (16.4 to 18.3).
+// Bound by the weights' bytes (8 x 8192, K = 8192, 48 matrices in turn so that none is in a cache: 15.7 us, 4.3 TB/s;
+// one again and again 14.3) and, where they are few, by the launch; turns of 256 or 512 k and 8 waves are no
+// faster (16.4 to 18.3, 8 matrices in turn).
 //
 // XT: f32 or bf16 activations, quantized by every workgroup into LDS while its first
 // weights are on their way (gemm_i8_fits).

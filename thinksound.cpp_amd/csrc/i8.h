@@ -46,8 +46,7 @@ __device__ __forceinline__ int i8_code(float x, const I8Scale &s) {
 // The codes of four values. x / d and x * (1 / d) are at most 127 and 2^-16 apart, so that the
 // integer nearest to the product is that of the quotient, but where the product is within
 // 2^-16 of a half: there i8_code decides. The sum with 1.5 * 2^23 rounds to an integer, whose
-// low byte is the sum's. (8192 x 8192 bf16: 48.3 us where
-// i8_code for every value took 52.4.)
+// low byte is the sum's. (8192 x 8192 bf16: 37.7 us, with i8_code for every value 40.2.)
 __device__ __forceinline__ uint32_t i8_pack4(const float *v, const I8Scale &s) {
     if (s.inv == 0.0f) return 0u;
     uint32_t b[4];

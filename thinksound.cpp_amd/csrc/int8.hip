@@ -3,8 +3,9 @@
 // d = max(amax, 2^-100) / 127, q = the integer nearest to x / d (i8.h). Bound by memory:
 // a row is read once into the registers of the threads that share it, whose largest
 // magnitude is found between the load and the store. A vector instruction takes a wave four
-// cycles, so a value's few count: 8192 x 8192 bf16 37.7 us (5.3 TB/s; a copy 5.1; with magnitudes
-// of 32 bits and i8_code for every value 52.4), f32 60.0 (5.6).
+// cycles, so a value's few count: 8192 x 8192 bf16, 16 arrays in turn so that none is in a cache, 37.7 us
+// (5.3 TB/s; a copy 5.1; with magnitudes of 32 bits and i8_code for every value 52.4; one array again and again
+// 32), f32 60.0 (5.6).
 #include <algorithm>
 #include <type_traits>
 

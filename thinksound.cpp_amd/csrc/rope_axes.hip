@@ -8,9 +8,9 @@
 // few. Bound by memory: x is read and y written once. A vector instruction of a wave takes
 // four cycles, so that some 500 of them a token are as long as its memory: each angle is formed
 // by one lane of the wave and used for all heads, the values stay as loaded until their turn,
-// and a wave goes on to other tokens. 16384 tokens of 16 heads of 128, bf16: 26.0 us, 5.16 TB/s
-// (angles formed by each lane for its own pairs 35.8, and one pass of heads in flight 42);
-// 8192 tokens of 32 heads of 64, f32: 25.3 us, 5.3 TB/s.
+// and a wave goes on to other tokens. 16384 tokens of 16 heads of 128, bf16, x in no cache: 26.3 us, 5.1 TB/s (calls that
+// follow one another 27.8, copies as long 26.3; angles formed by each lane for its own pairs 35.8, and one pass of heads
+// in flight 42).
 #include <algorithm>
 
 #include "tsk_common.h"
