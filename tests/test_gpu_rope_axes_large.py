@@ -1,4 +1,4 @@
-"""Rotary positions of one token of nearly 2^31 heads, dealt to waves of which the last has fewer."""
+"""Rotary positions of one token of nearly 2^31 heads, dealt to waves of which the last has fewer, and of very many sequences."""
 import numpy as np
 import pytest
 
@@ -6,7 +6,7 @@ import crossref
 import mxref
 from test_gpu_int8 import T  # noqa: F401  (fixture)
 from test_gpu_mxfp4_ends import fetch
-from test_gpu_rope_axes import tolerance
+from test_gpu_rope_axes import check, tolerance
 
 pytestmark = pytest.mark.gpu
 
@@ -25,3 +25,13 @@ def test_the_most_heads(T):  # noqa: F811
     for at in places:
         got = mxref.bf16_values(fetch(T, x, 4 * at, (2 * n,), np.uint16)).reshape(1, 1, n, 2)
         assert (np.abs(got - want) - tolerance(a, size, want, 2.0, False, "bf16")).max() <= 0, at
+
+
+@pytest.mark.parametrize("b,s,h,d", [(9001, 1, 3, 32), (4096, 1, 16, 128), (700, 13, 2, 20), (3000, 4, 1, 64)])
+@pytest.mark.parametrize("shared", [False, True])
+def test_many_short_sequences(T, b, s, h, d, shared):  # noqa: F811
+    """more sequences than waves, and fewer; positions of their own and one array for all"""
+    rng = np.random.default_rng(b)
+    x = rng.standard_normal((b, s, h, d)).astype(np.float32)
+    pos = rng.integers(0, 3000, (1 if shared else b, 2, s)).astype(np.int32)
+    check(T, x, pos, (d - 8, 8), w=(1 + 0.1 * rng.standard_normal(d)).astype(np.float32), dtype="bf16" if d == 128 else "f32")
