@@ -446,8 +446,8 @@ extern "C" int tsk_set_workspace(tsk_stream stream, void *ptr, size_t bytes) {
         // the library-owned buffer may still be read by work queued on s
         e = hipStreamSynchronize(s);
         if (e != hipSuccess) return hip_fail(e, "hipStreamSynchronize");
-        drop_owned(w);
     }
+    drop_owned(w);
     w.ptr = ptr;
     w.size = bytes;
     w.external = ptr != nullptr;
